@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_PKG, "libhp_rms_norm_b200.so")
 
 DTYPE_BF16 = 0
 DTYPE_FP16 = 1
+DTYPE_FP32 = 2  # gradients of grad_norm / grad_clip only
 
 OK = 0
 ERR_INVALID_ARGUMENT = -1
@@ -24,6 +25,7 @@ ERR_CUDA = -4
 
 LAUNCH_PDL = 1
 LAUNCH_DEFAULT = LAUNCH_PDL
+WORKSPACE_QUERY = 2
 
 ACT_SILU = 0
 ACT_GELU = 1
@@ -52,7 +54,23 @@ EXPORTED = (
     "hprn_wait_timeouts",
     "hprn_rms_norm_fp8_group",
     "hprn_test_stall_bulk_copy",
+    "hprn_gated_linear",
+    "hprn_gated_linear_backward",
+    "hprn_linear_cross_entropy",
+    "hprn_linear_cross_entropy_backward",
+    "hprn_rms_norm_backward",
+    "hprn_grad_norm",
+    "hprn_grad_clip",
 )
+
+
+class Grad(ctypes.Structure):
+    """hprn_grad: one tensor of grad_norm / grad_clip."""
+    _fields_ = [("grad", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32)]
+
 
 
 class HprnError(RuntimeError):
@@ -109,6 +127,19 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.hprn_rms_norm_fp8_group.argtypes = [vp, vp, i64, i64, vp, vp, vp, i64, i64, i64, i64, i64,
                                             ctypes.c_double, c_int, c_int, c_int, vp, u32]
     lib.hprn_rms_norm_fp8_group.restype = c_int
+    wsp = ctypes.POINTER(i64)
+    lib.hprn_gated_linear.argtypes = [vp] * 4 + [i64] * 7 + [c_int, c_int, vp, wsp, vp, u32]
+    lib.hprn_gated_linear_backward.argtypes = [vp] * 6 + [i64] * 9 + [c_int, c_int, vp, wsp, vp, u32]
+    lib.hprn_linear_cross_entropy.argtypes = [vp] * 5 + [i64] * 6 + [c_int, vp, wsp, vp, u32]
+    lib.hprn_linear_cross_entropy_backward.argtypes = [vp] * 7 + [i64] * 8 + [c_int, vp, wsp, vp, u32]
+    lib.hprn_rms_norm_backward.argtypes = [vp] * 6 + [i64] * 6 + [ctypes.c_double, c_int, vp, wsp,
+                                                                vp, u32]
+    lib.hprn_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, vp, wsp, vp, u32]
+    lib.hprn_grad_clip.argtypes = [ctypes.POINTER(Grad), i64, vp, ctypes.c_double, vp, u32]
+    for fn in (lib.hprn_gated_linear, lib.hprn_gated_linear_backward, lib.hprn_linear_cross_entropy,
+               lib.hprn_linear_cross_entropy_backward, lib.hprn_rms_norm_backward,
+               lib.hprn_grad_norm, lib.hprn_grad_clip):
+        fn.restype = c_int
     _lib = lib
     return lib
 
@@ -315,3 +346,26 @@ def rms_norm_nvfp4_tensors(out, block_scales, inp, weight, res, eps: float, glob
                    res.data_ptr() if res is not None else None, rows, hidden, out.stride(0) * 2,
                    inp.stride(0), res.stride(0) if res is not None else hidden, eps,
                    dtype_code(inp), global_scale.data_ptr(), stream, flags)
+
+
+def workspace_bytes(entry: str, *args) -> int:
+    """Bytes of workspace that the training entry point `entry` (an exported name) needs for
+    the arguments before ``workspace``."""
+    need = ctypes.c_int64(0)
+    _check(getattr(load(), entry)(*args, None, ctypes.byref(need), None, WORKSPACE_QUERY))
+    return need.value
+
+
+def call_with_workspace(entry: str, *args, workspace: int = 0, workspace_size: int = 0,
+                        stream: int = 0, flags: int = LAUNCH_DEFAULT) -> None:
+    """Calls a training entry point with the arguments before ``workspace`` and a workspace of
+    at least ``workspace_bytes(entry, *args)`` bytes."""
+    size = ctypes.c_int64(workspace_size)
+    _check(getattr(load(), entry)(*args, workspace, ctypes.byref(size), stream, flags))
+
+
+def grad_clip(grads, norm_ptr: int, max_norm: float, stream: int = 0,
+              flags: int = LAUNCH_DEFAULT) -> None:
+    """hprn_grad_clip over a list of ``Grad``."""
+    table = (Grad * max(1, len(grads)))(*grads)
+    _check(load().hprn_grad_clip(table, len(grads), norm_ptr, max_norm, stream, flags))

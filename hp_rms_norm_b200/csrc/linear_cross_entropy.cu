@@ -1,0 +1,355 @@
+// Softmax cross entropy of a linear layer over a vocabulary, without keeping
+// the logits L = X W^T (X [rows, hidden], W [vocab, hidden]):
+//   lse_i  = log sum_j exp(L_ij),  loss_i = lse_i - L_{i, t_i}
+// and 0 for rows whose target t_i is `ignore_index`.
+//
+// Forward: each tile of L leaves, per row, its largest value and the sum of
+// exponentials relative to it (8 bytes for a tile's columns instead of 4 per
+// logit), and the logit of the row's target; a second kernel joins a row's
+// tiles:  lse = M + log sum_t s_t exp(m_t - M),  M = max_t m_t.
+//
+// Backward, c_i the gradient of loss_i:
+//   S_ij = c_i (exp(L_ij - lse_i) - [j == t_i]),  dX = S W,  dW = S^T X
+// one piece of the vocabulary at a time: the piece's logits are computed again
+// and leave as S (16-bit, the tensor cores' operand), dW's rows of that piece
+// are complete, and dX is summed over the pieces in fp32 and rounded once.
+//
+// S in fp16: softmax values of a large vocabulary times a mean's 1/rows fall
+// below fp16's smallest normal (6e-5), so S is held times a power of two that
+// puts the largest |c_i| between 2^14 and 2^15, and the sums are divided by it.
+// bf16 has fp32's range and needs none.
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "matmul.cuh"
+#include "runtime.cuh"
+
+namespace hprn {
+
+// A row's target: its column, or kIgnored, or kInvalid (outside the vocabulary).
+constexpr int64_t kIgnored = -1, kInvalid = -2;
+__device__ __forceinline__ int64_t target_of(const int64_t* target, int64_t i, int64_t ignore,
+                                             int64_t vocab) {
+  const int64_t t = target[i];
+  return t == ignore ? kIgnored : (t < 0 || t >= vocab) ? kInvalid : t;
+}
+
+struct LossEpilogue {
+  static constexpr bool kPaired = false;
+  float2* partial = nullptr;  // [tiles, rows]: {max, sum of exp(l - max)}
+  float* target_logit = nullptr;
+  const int64_t* target = nullptr;
+  int64_t ignore = 0;
+  int64_t rows = 0;
+  int64_t vocab = 0;
+
+  struct Row {
+    float m, s;
+    int64_t t;
+  };
+  __device__ __forceinline__ Row begin(int64_t i) const {
+    return Row{-INFINITY, 0.f, target_of(target, i, ignore, vocab)};
+  }
+  __device__ __forceinline__ void chunk(Row& r, int64_t i, int64_t j, const float (&v)[kChunk]) const {
+    const int64_t left = vocab - j;
+    float m = r.m;
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k)
+      if (k < left) m = fmaxf(m, v[k]);
+    // All so far -inf (or NaN, which fmaxf skips and the sum keeps): exp(-inf - 0) = 0.
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = r.s * expf(r.m - ref);
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k)
+      if (k < left) s += expf(v[k] - ref);
+    r.m = m, r.s = s;
+    if (r.t >= j && r.t < j + kChunk) {
+      float x = 0.f;
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) x = r.t == j + k ? v[k] : x;
+      target_logit[i] = x;
+    }
+  }
+  __device__ __forceinline__ void end(Row& r, int64_t i, int64_t tile) const {
+    partial[tile * rows + i] = make_float2(r.m, r.s);
+  }
+};
+
+// Joins a row's tiles: one warp-sized group of threads per row would read the
+// partials of a row `rows` apart, so threads of a CTA take neighbouring rows
+// and the CTA's y groups take tiles in turn.
+constexpr int kJoinRows = 32;
+constexpr int kJoinGroups = 8;
+
+__global__ void __launch_bounds__(kJoinRows* kJoinGroups)
+    loss_join(const float2* partial, const float* target_logit, const int64_t* target,
+              int64_t ignore, int64_t rows, int64_t vocab, int64_t tiles, float* loss, float* lse) {
+  __shared__ float2 part[kJoinGroups][kJoinRows];
+  pdl_wait();
+  const int tx = threadIdx.x, ty = threadIdx.y;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kJoinRows + tx;
+  float m = -INFINITY, s = 0.f;
+  auto join = [](float& m, float& s, float2 p) {
+    const float top = fmaxf(m, p.x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    s = s * expf(m - ref) + p.y * expf(p.x - ref);
+    m = top;
+  };
+  if (i < rows)
+    for (int64_t t = ty; t < tiles; t += kJoinGroups) join(m, s, partial[t * rows + i]);
+  part[ty][tx] = make_float2(m, s);
+  __syncthreads();
+  if (ty != 0 || i >= rows) return;
+  for (int g = 1; g < kJoinGroups; ++g) join(m, s, part[g][tx]);
+  const float l = (m == -INFINITY ? 0.f : m) + logf(s);
+  lse[i] = l;
+  const int64_t t = target_of(target, i, ignore, vocab);
+  loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - target_logit[i];
+}
+
+// {factor, 1 / factor}: the power of two S is held times.
+__global__ void __launch_bounds__(1024) loss_grad_scale(const float* grad_loss, const int64_t* target,
+                                                        int64_t ignore, int64_t rows, float* out) {
+  __shared__ float part[32];
+  pdl_wait();
+  float m = 0.f;
+  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+    if (target[i] != ignore) m = fmaxf(m, fabsf(grad_loss[i]));
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  m = part[threadIdx.x];
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (threadIdx.x == 0) {
+    // m in [2^e, 2^(e+1)): times 2^(14 - e).  Exponents are kept where both
+    // factors are normal; 0, infinities and NaN take 1.
+    int e = 14;
+    if (m > 0.f && m <= 3.402823466e38f) e = max(-100, min(100, ilogbf(m)));
+    out[0] = ldexpf(1.f, 14 - e);
+    out[1] = ldexpf(1.f, e - 14);
+  }
+}
+
+template <typename T>
+struct LossGradEpilogue {
+  static constexpr bool kPaired = false;
+  uint16_t* s = nullptr;
+  int64_t ld = 0;
+  const float* lse = nullptr;
+  const float* grad_loss = nullptr;
+  const float* factor = nullptr;  // or null for 1
+  const int64_t* target = nullptr;
+  int64_t ignore = 0;
+  int64_t vocab = 0;
+  int64_t first = 0;  // the piece's first column
+  int64_t cols = 0;   // the piece's columns
+
+  struct Row {
+    float c, lse;
+    int64_t t;  // within the piece (or past its end); kInvalid before it
+  };
+  __device__ __forceinline__ Row begin(int64_t i) const {
+    const int64_t t = target_of(target, i, ignore, vocab);
+    float c = grad_loss[i] * (factor ? *factor : 1.f);
+    // A target outside the vocabulary has no loss: NaN, like the loss itself.
+    c = t == kInvalid ? __int_as_float(0x7fc00000) : c;
+    return Row{c, lse[i], t == kIgnored ? kIgnored : t >= first ? t - first : kInvalid};
+  }
+  __device__ __forceinline__ void chunk(Row& r, int64_t i, int64_t j, const float (&v)[kChunk]) const {
+    float g[kChunk];
+    if (r.t == kIgnored) {
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) g[k] = 0.f;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+        g[k] = r.c * (expf(v[k] - r.lse) - (r.t == j + k ? 1.f : 0.f));
+    }
+    store_chunk<T>(s + i * ld, j, cols, g);
+  }
+  __device__ __forceinline__ void end(Row&, int64_t, int64_t) const {}
+};
+
+namespace {
+
+// S's share of the workspace: pieces of the vocabulary of equal length such
+// that a piece's S takes at most this much.
+constexpr int64_t kPieceBytes = int64_t{512} << 20;
+
+struct Pieces {
+  int64_t count, cols;
+};
+Pieces pieces_of(int64_t rows, int64_t vocab) {
+  int64_t most = kPieceBytes / 2 / (rows > 0 ? rows : 1) / 256 * 256;
+  if (most < 256) most = 256;
+  const int64_t count = vocab > 0 ? (vocab + most - 1) / most : 0;
+  const int64_t cols = count > 0 ? round_up((vocab + count - 1) / count, 256) : 0;
+  return Pieces{cols > 0 ? (vocab + cols - 1) / cols : 0, cols};
+}
+
+int check_common(int64_t rows, int64_t hidden, int64_t vocab, int dtype, unsigned flags,
+                 const int64_t* workspace_bytes) {
+  if (flags & ~static_cast<unsigned>(HPRN_LAUNCH_PDL | HPRN_WORKSPACE_QUERY))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "unknown launch flags");
+  if (dtype != HPRN_DTYPE_BF16 && dtype != HPRN_DTYPE_FP16)
+    return fail(HPRN_ERR_UNSUPPORTED_DTYPE, "dtype must be kFloat16 or kBFloat16");
+  if (rows < 0 || hidden < 0 || vocab < 0) return fail(HPRN_ERR_INVALID_ARGUMENT, "sizes must be >= 0");
+  if (rows > kMaxExtent || hidden > kMaxExtent || vocab > kMaxExtent)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "rows, hidden and vocab must be at most 2^30");
+  if (!workspace_bytes) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace_bytes pointer required");
+  return HPRN_OK;
+}
+
+}  // namespace
+}  // namespace hprn
+
+extern "C" {
+
+int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const void* weight,
+                              const int64_t* target, int64_t ignore_index, int64_t rows,
+                              int64_t hidden, int64_t vocab, int64_t input_row_stride,
+                              int64_t weight_row_stride, int dtype, void* workspace,
+                              int64_t* workspace_bytes, void* stream, unsigned flags) {
+  using namespace hprn;
+  int st = check_common(rows, hidden, vocab, dtype, flags, workspace_bytes);
+  if (st != HPRN_OK) return st;
+  if ((rows > 1 && input_row_stride < hidden) || (vocab > 1 && weight_row_stride < hidden))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  Workspace ws(workspace, *workspace_bytes);
+  const int64_t tiles = product_tiles<LossEpilogue>(vocab);
+  float2* partial = ws.take<float2>(tiles * rows);
+  float* target_logit = ws.take<float>(rows);
+  if (flags & HPRN_WORKSPACE_QUERY) {
+    *workspace_bytes = ws.needed();
+    return ok();
+  }
+  if (rows == 0) return ok();
+  if (!loss || !lse || !target || (hidden > 0 && (!input || (vocab > 0 && !weight))))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(loss, 4) || !aligned(lse, 4) || !aligned(target, 8) || !aligned(input, 2) ||
+      !aligned(weight, 2))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  const Extent outs[] = {extent32(loss, 1, rows, rows), extent32(lse, 1, rows, rows)};
+  const Extent ins[] = {extent16(input, rows, hidden, input_row_stride),
+                      extent16(weight, vocab, hidden, weight_row_stride),
+                      extent_of(target, 1, rows, rows, 8)};
+  if (!disjoint(outs, ins)) return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors");
+  if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
+  const DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (vocab > 0) {
+    Product q;
+    q.a = {static_cast<const uint16_t*>(input), input_row_stride, true};
+    q.b = {static_cast<const uint16_t*>(weight), weight_row_stride, true};
+    q.m = rows, q.n = vocab, q.depth = hidden;
+    LossEpilogue e;
+    e.partial = partial, e.target_logit = target_logit, e.target = target;
+    e.ignore = ignore_index, e.rows = rows, e.vocab = vocab;
+    st = dtype == HPRN_DTYPE_BF16 ? launch_product<__nv_bfloat16>(q, e, cs, "linear_cross_entropy")
+                                  : launch_product<__half>(q, e, cs, "linear_cross_entropy");
+    if (st != HPRN_OK) return st;
+  }
+  loss_join<<<static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), dim3(kJoinRows, kJoinGroups), 0, cs>>>(
+      partial, target_logit, target, ignore_index, rows, vocab, tiles, loss, lse);
+  return check_launch("linear_cross_entropy");
+}
+
+int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, const float* grad_loss,
+                                       const void* input, const void* weight, const int64_t* target,
+                                       const float* lse, int64_t ignore_index, int64_t rows,
+                                       int64_t hidden, int64_t vocab, int64_t grad_input_row_stride,
+                                       int64_t grad_weight_row_stride, int64_t input_row_stride,
+                                       int64_t weight_row_stride, int dtype, void* workspace,
+                                       int64_t* workspace_bytes, void* stream, unsigned flags) {
+  using namespace hprn;
+  int st = check_common(rows, hidden, vocab, dtype, flags, workspace_bytes);
+  if (st != HPRN_OK) return st;
+  if ((rows > 1 && (input_row_stride < hidden || grad_input_row_stride < hidden)) ||
+      (vocab > 1 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  Workspace ws(workspace, *workspace_bytes);
+  const Pieces pieces = pieces_of(rows, vocab);
+  uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
+  float* sum = pieces.count > 1 ? ws.take<float>(rows * hidden) : nullptr;
+  float* factor = dtype == HPRN_DTYPE_FP16 ? ws.take<float>(2) : nullptr;
+  if (flags & HPRN_WORKSPACE_QUERY) {
+    *workspace_bytes = ws.needed();
+    return ok();
+  }
+  if (hidden == 0) return ok();
+  if ((rows > 0 && (!grad_input || !grad_loss || !input || !target || !lse)) ||
+      (vocab > 0 && (!grad_weight || !weight)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(grad_input, 2) || !aligned(grad_weight, 2) || !aligned(grad_loss, 4) ||
+      !aligned(input, 2) || !aligned(weight, 2) || !aligned(target, 8) || !aligned(lse, 4))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  const Extent outs[] = {extent16(grad_input, rows, hidden, grad_input_row_stride),
+                       extent16(grad_weight, vocab, hidden, grad_weight_row_stride)};
+  const Extent ins[] = {extent32(grad_loss, 1, rows, rows),
+                      extent16(input, rows, hidden, input_row_stride),
+                      extent16(weight, vocab, hidden, weight_row_stride),
+                      extent_of(target, 1, rows, rows, 8), extent32(lse, 1, rows, rows)};
+  if (!disjoint(outs, ins)) return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors");
+  if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
+  const DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (factor && rows > 0) {
+    loss_grad_scale<<<1, 1024, 0, cs>>>(grad_loss, target, ignore_index, rows, factor);
+    if ((st = check_launch("linear_cross_entropy_backward")) != HPRN_OK) return st;
+  }
+  const uint16_t* x = static_cast<const uint16_t*>(input);
+  const uint16_t* w = static_cast<const uint16_t*>(weight);
+  const char* what = "linear_cross_entropy_backward";
+  auto all = [&](auto t) {
+    using T = decltype(t);
+    int r = HPRN_OK;
+    // Without a vocabulary the input's gradient is an empty sum: zero.
+    const int64_t count = pieces.count > 0 ? pieces.count : 1;
+    for (int64_t p = 0; p < count && r == HPRN_OK; ++p) {
+      const int64_t first = p * pieces.cols;
+      const int64_t cols = vocab - first < pieces.cols ? vocab - first : pieces.cols;
+      if (rows > 0 && cols > 0) {
+        Product q;
+        q.a = {x, input_row_stride, true};
+        q.b = {w + first * weight_row_stride, weight_row_stride, true};
+        q.m = rows, q.n = cols, q.depth = hidden;
+        LossGradEpilogue<T> e;
+        e.s = s, e.ld = pieces.cols, e.lse = lse, e.grad_loss = grad_loss, e.factor = factor;
+        e.target = target, e.ignore = ignore_index, e.vocab = vocab, e.first = first, e.cols = cols;
+        if ((r = launch_product<T>(q, e, cs, what)) != HPRN_OK) break;
+      }
+      if (rows > 0) {
+        Product q;
+        q.a = {s, pieces.cols, true};
+        q.b = {w + first * weight_row_stride, weight_row_stride, false};
+        q.m = rows, q.n = hidden, q.depth = cols;
+        StoreEpilogue<T> e;
+        e.out = static_cast<uint16_t*>(grad_input), e.ld = grad_input_row_stride, e.n = hidden;
+        e.sum = sum, e.first = p == 0, e.last = p == count - 1;
+        e.scale = factor ? factor + 1 : nullptr;
+        if ((r = launch_product<T>(q, e, cs, what)) != HPRN_OK) break;
+      }
+      if (cols > 0) {
+        Product q;
+        q.a = {s, pieces.cols, false};
+        q.b = {x, input_row_stride, false};
+        q.m = cols, q.n = hidden, q.depth = rows;
+        StoreEpilogue<T> e;
+        e.out = static_cast<uint16_t*>(grad_weight) + first * grad_weight_row_stride;
+        e.ld = grad_weight_row_stride, e.n = hidden;
+        e.scale = factor && rows > 0 ? factor + 1 : nullptr;
+        r = launch_product<T>(q, e, cs, what);
+      }
+    }
+    return r;
+  };
+  return dtype == HPRN_DTYPE_BF16 ? all(__nv_bfloat16{}) : all(__half{});
+}
+
+}  // extern "C"

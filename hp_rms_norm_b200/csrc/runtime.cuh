@@ -53,6 +53,68 @@ inline bool aligned(const void* p, int bytes) {
   return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0;
 }
 
+// The largest rows / hidden / vocabulary the matrix-product entry points take.
+constexpr int64_t kMaxExtent = int64_t{1} << 30;
+
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// A caller's workspace, handed out in 256-byte aligned pieces.  Taking pieces
+// only adds up sizes, so the same code answers how much a call needs.
+class Workspace {
+ public:
+  Workspace(void* base, int64_t bytes) : base_(static_cast<char*>(base)), bytes_(bytes) {}
+  template <typename T>
+  T* take(int64_t count) {
+    const int64_t at = round_up(used_, 256);
+    used_ = at + count * static_cast<int64_t>(sizeof(T));
+    return base_ ? reinterpret_cast<T*>(base_ + at) : nullptr;
+  }
+  int64_t needed() const { return used_; }
+  bool fits() const { return used_ == 0 || (base_ && aligned(base_, 256) && used_ <= bytes_); }
+
+ private:
+  char* base_;
+  int64_t bytes_;
+  int64_t used_ = 0;
+};
+
+// The bytes a [rows, cols] tensor covers; null pointers cover none.
+struct Extent {
+  const char* lo;
+  const char* hi;
+  int64_t row_stride, row_bytes;
+};
+inline Extent extent_of(const void* p, int64_t rows, int64_t cols, int64_t row_stride, int64_t elem) {
+  const char* b = static_cast<const char*>(p);
+  if (!b || rows <= 0 || cols <= 0) return Extent{nullptr, nullptr, 0, 0};
+  return Extent{b, b + elem * ((rows - 1) * row_stride + cols), elem * row_stride, elem * cols};
+}
+inline Extent extent16(const void* p, int64_t rows, int64_t cols, int64_t row_stride) {
+  return extent_of(p, rows, cols, row_stride, 2);
+}
+inline Extent extent32(const void* p, int64_t rows, int64_t cols, int64_t row_stride) {
+  return extent_of(p, rows, cols, row_stride, 4);
+}
+// Two tensors that share a byte.  Ranges that overlap share none where their
+// rows have one stride and interleave (column slices of one buffer).
+inline bool extents_overlap(const Extent& a, const Extent& b) {
+  if (!(a.lo < b.hi && b.lo < a.hi)) return false;
+  if (a.row_stride != b.row_stride || a.row_stride <= 0) return true;
+  const int64_t m = (((b.lo - a.lo) % a.row_stride) + a.row_stride) % a.row_stride;
+  return !(m >= a.row_bytes && a.row_stride - m >= b.row_bytes);
+}
+// No output overlaps an input or another output.
+template <size_t NO, size_t NI>
+bool disjoint(const Extent (&outs)[NO], const Extent (&ins)[NI]) {
+  for (size_t i = 0; i < NO; ++i) {
+    for (size_t j = 0; j < NI; ++j)
+      if (extents_overlap(outs[i], ins[j])) return false;
+    for (size_t j = 0; j < i; ++j)
+      if (extents_overlap(outs[i], outs[j])) return false;
+  }
+  return true;
+}
+
 // Reports a failed launch (cudaGetLastError after the launch) as HPRN_ERR_CUDA.
 int check_launch(const char* what);
 

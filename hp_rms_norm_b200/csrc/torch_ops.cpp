@@ -15,7 +15,10 @@
 #include <ATen/core/Tensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/Functions.h>
 #include <torch/library.h>
+
+#include <vector>
 
 #include "hp_rms_norm_b200.h"
 
@@ -322,6 +325,312 @@ void gelu_tanh_and_mul(at::Tensor& out, const at::Tensor& input) {
   act_and_mul(out, input, HPRN_ACT_GELU_TANH);
 }
 
+// ---------------------------------------------------------------------------
+// Training operators (extensions past the reference).
+
+// A [..., cols] tensor as rows of one stride on `like`'s device.
+struct Rows {
+  void* p = nullptr;
+  int64_t rows = 0, stride = 0;
+};
+
+Rows rows_arg(const at::Tensor& t, const char* name, int64_t cols, const at::Tensor& like,
+              at::ScalarType type) {
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) == cols, name, ".size(-1) must be ", cols);
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be a CUDA tensor on the same device as the others");
+  TORCH_CHECK(t.scalar_type() == type, name, " must be of dtype ", type);
+  TORCH_CHECK(cols <= 1 || t.numel() == 0 || t.stride(-1) == 1, name, ".stride(-1) == 1");
+  Rows r;
+  if (t.numel() > 0 || cols == 0) {
+    rows_of(t, name, &r.rows, &r.stride);
+  } else {
+    r.rows = 0, r.stride = cols;
+  }
+  if (r.rows <= 1) r.stride = cols;  // never stepped over
+  r.p = t.data_ptr();
+  return r;
+}
+
+// Same rows as `like` (the leading dimensions, not just their product).
+void check_leading(const at::Tensor& t, const char* name, const at::Tensor& like) {
+  TORCH_CHECK(t.dim() == like.dim(), name, " must have as many dimensions as input");
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    TORCH_CHECK(t.size(i) == like.size(i), name, " and input must agree on leading dimensions");
+}
+
+const float* float_rows(const at::Tensor& t, const char* name, int64_t rows, const at::Tensor& like) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == rows && t.is_contiguous() &&
+                  t.is_cuda() && t.device() == like.device(),
+              name, " must be a contiguous float32 tensor with one entry per row");
+  return t.data_ptr<float>();
+}
+
+const int64_t* target_rows(const at::Tensor& t, int64_t rows, const at::Tensor& like) {
+  TORCH_CHECK(t.scalar_type() == at::kLong && t.numel() == rows && t.is_contiguous() &&
+                  t.is_cuda() && t.device() == like.device(),
+              "target must be a contiguous int64 tensor with one entry per row");
+  return t.data_ptr<int64_t>();
+}
+
+// Runs an entry point twice: once for the size of its workspace, once with a
+// workspace from torch's allocator (which keeps the memory for this stream).
+template <typename F>
+void with_workspace(const at::Tensor& like, F&& call) {
+  const c10::cuda::CUDAGuard guard(like.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(like.device().index()).stream();
+  int64_t bytes = 0;
+  check_status(call(nullptr, &bytes, stream, HPRN_WORKSPACE_QUERY));
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, like.options().dtype(at::kByte));
+  check_status(call(bytes > 0 ? ws.data_ptr() : nullptr, &bytes, stream, HPRN_LAUNCH_DEFAULT));
+}
+
+int act_code(c10::string_view act) {
+  if (act == "silu") return HPRN_ACT_SILU;
+  if (act == "gelu") return HPRN_ACT_GELU;
+  if (act == "gelu_tanh") return HPRN_ACT_GELU_TANH;
+  TORCH_CHECK(false, "act must be 'silu', 'gelu' or 'gelu_tanh'");
+}
+
+struct GatedCall {
+  int act, dtype;
+  int64_t hidden, d;
+  Rows x, w;
+};
+
+GatedCall check_gated(const at::Tensor& input, const at::Tensor& weight, c10::string_view act) {
+  GatedCall c;
+  c.act = act_code(act);
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(weight.dim() == 2 && weight.size(0) % 2 == 0, "weight must be [2 * d, hidden]");
+  c.dtype = dtype_code(input);
+  c.hidden = input.size(-1);
+  c.d = weight.size(0) / 2;
+  c.x = rows_arg(input, "input", c.hidden, input, input.scalar_type());
+  c.w = rows_arg(weight, "weight", c.hidden, input, input.scalar_type());
+  return c;
+}
+
+// rows of a [..., cols] tensor, its last dimension included when that is 0.
+int64_t leading(const at::Tensor& t) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
+  return n;
+}
+
+void gated_linear(at::Tensor& out, c10::optional<at::Tensor> gate_up, const at::Tensor& input,
+                  const at::Tensor& weight, c10::string_view act) {
+  const GatedCall c = check_gated(input, weight, act);
+  const int64_t rows = leading(input);
+  check_leading(out, "out", input);
+  const Rows o = rows_arg(out, "out", c.d, input, input.scalar_type());
+  Rows g;
+  if (gate_up.has_value()) {
+    check_leading(*gate_up, "gate_up", input);
+    g = rows_arg(*gate_up, "gate_up", 2 * c.d, input, at::kFloat);
+  }
+  if (rows == 0 || c.d == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_gated_linear(o.p, static_cast<float*>(g.p), c.x.p, c.w.p, rows, c.hidden, c.d,
+                             o.stride, g.stride, c.x.stride, c.w.stride, c.act, c.dtype, ws, bytes,
+                             s, flags);
+  });
+}
+
+void gated_linear_backward(at::Tensor& grad_input, at::Tensor& grad_weight,
+                           const at::Tensor& grad_out, const at::Tensor& input,
+                           const at::Tensor& weight, c10::optional<at::Tensor> gate_up,
+                           c10::string_view act) {
+  const GatedCall c = check_gated(input, weight, act);
+  const int64_t rows = leading(input);
+  check_leading(grad_out, "grad_out", input);
+  check_leading(grad_input, "grad_input", input);
+  TORCH_CHECK(grad_weight.sizes() == weight.sizes(), "grad_weight must have the weight's shape");
+  const Rows d = rows_arg(grad_out, "grad_out", c.d, input, input.scalar_type());
+  const Rows gi = rows_arg(grad_input, "grad_input", c.hidden, input, input.scalar_type());
+  const Rows gw = rows_arg(grad_weight, "grad_weight", c.hidden, input, input.scalar_type());
+  Rows g;
+  if (gate_up.has_value()) {
+    check_leading(*gate_up, "gate_up", input);
+    g = rows_arg(*gate_up, "gate_up", 2 * c.d, input, at::kFloat);
+  }
+  if (c.hidden == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_gated_linear_backward(gi.p, gw.p, d.p, static_cast<const float*>(g.p), c.x.p, c.w.p,
+                                      rows, c.hidden, c.d, gi.stride, gw.stride, d.stride, g.stride,
+                                      c.x.stride, c.w.stride, c.act, c.dtype, ws, bytes, s, flags);
+  });
+}
+
+struct LossCall {
+  int dtype;
+  int64_t rows, hidden, vocab;
+  Rows x, w;
+  const int64_t* target;
+};
+
+LossCall check_loss(const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target) {
+  LossCall c;
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(weight.dim() == 2, "weight must be [vocab, hidden]");
+  c.dtype = dtype_code(input);
+  c.rows = leading(input);
+  c.hidden = input.size(-1);
+  c.vocab = weight.size(0);
+  c.x = rows_arg(input, "input", c.hidden, input, input.scalar_type());
+  c.w = rows_arg(weight, "weight", c.hidden, input, input.scalar_type());
+  c.target = target_rows(target, c.rows, input);
+  return c;
+}
+
+void linear_cross_entropy(at::Tensor& loss, at::Tensor& lse, const at::Tensor& input,
+                          const at::Tensor& weight, const at::Tensor& target, int64_t ignore_index) {
+  const LossCall c = check_loss(input, weight, target);
+  float* lp = const_cast<float*>(float_rows(loss, "loss", c.rows, input));
+  float* ep = const_cast<float*>(float_rows(lse, "lse", c.rows, input));
+  if (c.rows == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_linear_cross_entropy(lp, ep, c.x.p, c.w.p, c.target, ignore_index, c.rows, c.hidden,
+                                     c.vocab, c.x.stride, c.w.stride, c.dtype, ws, bytes, s, flags);
+  });
+}
+
+void linear_cross_entropy_backward(at::Tensor& grad_input, at::Tensor& grad_weight,
+                                   const at::Tensor& grad_loss, const at::Tensor& input,
+                                   const at::Tensor& weight, const at::Tensor& target,
+                                   const at::Tensor& lse, int64_t ignore_index) {
+  const LossCall c = check_loss(input, weight, target);
+  TORCH_CHECK(grad_input.sizes() == input.sizes(), "grad_input must have the input's shape");
+  TORCH_CHECK(grad_weight.sizes() == weight.sizes(), "grad_weight must have the weight's shape");
+  const Rows gi = rows_arg(grad_input, "grad_input", c.hidden, input, input.scalar_type());
+  const Rows gw = rows_arg(grad_weight, "grad_weight", c.hidden, input, input.scalar_type());
+  const float* gl = float_rows(grad_loss, "grad_loss", c.rows, input);
+  const float* ep = float_rows(lse, "lse", c.rows, input);
+  if (c.hidden == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_linear_cross_entropy_backward(gi.p, gw.p, gl, c.x.p, c.w.p, c.target, ep,
+                                              ignore_index, c.rows, c.hidden, c.vocab, gi.stride,
+                                              gw.stride, c.x.stride, c.w.stride, c.dtype, ws, bytes,
+                                              s, flags);
+  });
+}
+
+void rms_norm_backward(at::Tensor& grad_input, at::Tensor& grad_weight, const at::Tensor& grad_out,
+                       const at::Tensor& input, const at::Tensor& weight,
+                       c10::optional<at::Tensor> grad_residual, double eps) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(weight.dim() == 1, "weight.dim() == 1");
+  const int64_t hidden = weight.size(0);
+  TORCH_CHECK(input.size(-1) == hidden, "input.size(-1) == hidden_dim");
+  const int dtype = dtype_code(input);
+  const at::ScalarType type = input.scalar_type();
+  const int64_t rows = leading(input);
+  TORCH_CHECK(grad_out.sizes() == input.sizes(), "grad_out must have the input's shape");
+  TORCH_CHECK(grad_input.sizes() == input.sizes(), "grad_input must have the input's shape");
+  TORCH_CHECK(grad_weight.dim() == 1, "grad_weight.dim() == 1");
+  const Rows x = rows_arg(input, "input", hidden, input, type);
+  const Rows w = rows_arg(weight, "weight", hidden, input, type);
+  const Rows d = rows_arg(grad_out, "grad_out", hidden, input, type);
+  const Rows gi = rows_arg(grad_input, "grad_input", hidden, input, type);
+  const Rows gw = rows_arg(grad_weight, "grad_weight", hidden, input, type);
+  Rows r;
+  if (grad_residual.has_value()) {
+    TORCH_CHECK(grad_residual->sizes() == input.sizes(), "grad_residual must have the input's shape");
+    r = rows_arg(*grad_residual, "grad_residual", hidden, input, type);
+  }
+  if (hidden == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_rms_norm_backward(gi.p, gw.p, d.p, x.p, w.p, r.p, rows, hidden, gi.stride, d.stride,
+                                  x.stride, r.stride, eps, dtype, ws, bytes, s, flags);
+  });
+}
+
+int32_t grad_dtype(const at::Tensor& t) {
+  if (t.scalar_type() == at::kBFloat16) return HPRN_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return HPRN_DTYPE_FP16;
+  if (t.scalar_type() == at::kFloat) return HPRN_DTYPE_FP32;
+  TORCH_CHECK(false, "gradients must be kFloat16, kBFloat16 or kFloat");
+}
+
+// rows, cols and row stride of a tensor whose elements are taken in order.
+void grad_layout(const at::Tensor& t, const char* name, int64_t* rows, int64_t* cols, int64_t* stride) {
+  if (t.is_contiguous()) {
+    *rows = 1, *cols = t.numel(), *stride = t.numel();
+    return;
+  }
+  *cols = t.size(-1);
+  TORCH_CHECK(t.size(-1) == 1 || t.stride(-1) == 1, name,
+              " must be contiguous in its last dimension");
+  rows_of(t, name, rows, stride);
+}
+
+std::vector<hprn_grad> grad_table(at::TensorList grads, const at::TensorList* outs,
+                                  const at::Tensor& norm) {
+  TORCH_CHECK(norm.is_cuda() && norm.scalar_type() == at::kFloat && norm.numel() == 1,
+              "norm must be one float32 on the gradients' device");
+  std::vector<hprn_grad> table(grads.size());
+  for (size_t k = 0; k < grads.size(); ++k) {
+    const at::Tensor& t = grads[k];
+    hprn_grad& e = table[k];
+    TORCH_CHECK(t.is_cuda() && t.device() == norm.device(),
+                "gradients must be CUDA tensors on one device");
+    e.dtype = e.out_dtype = grad_dtype(t);
+    grad_layout(t, "gradients", &e.rows, &e.cols, &e.row_stride);
+    e.grad = t.data_ptr(), e.out = nullptr, e.out_row_stride = e.row_stride;
+    if (!outs) continue;
+    const at::Tensor& o = (*outs)[k];
+    TORCH_CHECK(o.is_cuda() && o.device() == norm.device(), "out must be on the gradients' device");
+    TORCH_CHECK(o.sizes() == t.sizes(), "out must have the gradients' shapes");
+    e.out_dtype = grad_dtype(o);
+    e.out = o.data_ptr();
+    int64_t orows = 0, ocols = 0;
+    grad_layout(o, "out", &orows, &ocols, &e.out_row_stride);
+    if (orows == e.rows && ocols == e.cols) continue;
+    // One of the two is contiguous, the other has rows: walk both by its rows.
+    if (e.rows == 1) {
+      e.rows = orows, e.cols = ocols, e.row_stride = ocols;
+    } else if (orows == 1) {
+      e.out_row_stride = e.cols;
+    }
+  }
+  return table;
+}
+
+void grad_norm(at::Tensor& norm, at::TensorList grads) {
+  const std::vector<hprn_grad> table = grad_table(grads, nullptr, norm);
+  with_workspace(norm, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_grad_norm(norm.data_ptr<float>(), table.data(), static_cast<int64_t>(table.size()),
+                          ws, bytes, s, flags);
+  });
+}
+
+void grad_clip(at::TensorList out, at::TensorList grads, const at::Tensor& norm, double max_norm) {
+  TORCH_CHECK(out.size() == grads.size(), "out must have one tensor per gradient");
+  const std::vector<hprn_grad> table = grad_table(grads, &out, norm);
+  const c10::cuda::CUDAGuard guard(norm.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(norm.device().index()).stream();
+  check_status(hprn_grad_clip(table.data(), static_cast<int64_t>(table.size()),
+                              norm.data_ptr<float>(), max_norm, stream, HPRN_LAUNCH_DEFAULT));
+}
+
+void gated_linear_meta(at::Tensor&, c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
+                       c10::string_view) {}
+void gated_linear_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                const at::Tensor&, c10::optional<at::Tensor>, c10::string_view) {}
+void linear_cross_entropy_meta(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
+                               const at::Tensor&, int64_t) {}
+void linear_cross_entropy_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&,
+                                        const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                        const at::Tensor&, int64_t) {}
+void rms_norm_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const at::Tensor&, c10::optional<at::Tensor>, double) {}
+void grad_norm_meta(at::Tensor&, at::TensorList) {}
+void grad_clip_meta(at::TensorList, at::TensorList, const at::Tensor&, double) {}
+
 // Shape-only kernels for tracing (torch.compile / FakeTensor): the ops return
 // nothing and only mutate their annotated arguments.
 void rms_norm_meta(at::Tensor&, const at::Tensor&, at::Tensor&, double) {}
@@ -356,6 +665,20 @@ TORCH_LIBRARY(hp_rms_norm, m) {
   m.def("silu_and_mul(Tensor(a!) out, Tensor input) -> ()");
   m.def("gelu_and_mul(Tensor(a!) out, Tensor input) -> ()");
   m.def("gelu_tanh_and_mul(Tensor(a!) out, Tensor input) -> ()");
+  // Extensions: training operators.
+  m.def("gated_linear(Tensor(a!) out, Tensor(b!)? gate_up, Tensor input, Tensor weight, "
+        "str act) -> ()");
+  m.def("gated_linear_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, Tensor grad_out, "
+        "Tensor input, Tensor weight, Tensor? gate_up, str act) -> ()");
+  m.def("linear_cross_entropy(Tensor(a!) loss, Tensor(b!) lse, Tensor input, Tensor weight, "
+        "Tensor target, int ignore_index) -> ()");
+  m.def("linear_cross_entropy_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, "
+        "Tensor grad_loss, Tensor input, Tensor weight, Tensor target, Tensor lse, "
+        "int ignore_index) -> ()");
+  m.def("rms_norm_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, Tensor grad_out, "
+        "Tensor input, Tensor weight, Tensor? grad_residual, float eps) -> ()");
+  m.def("grad_norm(Tensor(a!) norm, Tensor[] grads) -> ()");
+  m.def("grad_clip(Tensor(a!)[] out, Tensor[] grads, Tensor norm, float max_norm) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
@@ -368,6 +691,13 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("silu_and_mul", &silu_and_mul);
   m.impl("gelu_and_mul", &gelu_and_mul);
   m.impl("gelu_tanh_and_mul", &gelu_tanh_and_mul);
+  m.impl("gated_linear", &gated_linear);
+  m.impl("gated_linear_backward", &gated_linear_backward);
+  m.impl("linear_cross_entropy", &linear_cross_entropy);
+  m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward);
+  m.impl("rms_norm_backward", &rms_norm_backward);
+  m.impl("grad_norm", &grad_norm);
+  m.impl("grad_clip", &grad_clip);
 }
 
 TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
@@ -380,4 +710,11 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("silu_and_mul", &act_and_mul_meta);
   m.impl("gelu_and_mul", &act_and_mul_meta);
   m.impl("gelu_tanh_and_mul", &act_and_mul_meta);
+  m.impl("gated_linear", &gated_linear_meta);
+  m.impl("gated_linear_backward", &gated_linear_backward_meta);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_meta);
+  m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_meta);
+  m.impl("rms_norm_backward", &rms_norm_backward_meta);
+  m.impl("grad_norm", &grad_norm_meta);
+  m.impl("grad_clip", &grad_clip_meta);
 }

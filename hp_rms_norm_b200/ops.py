@@ -10,7 +10,10 @@ Extensions (not in the reference): ``rms_norm`` (plain RMSNorm),
 ``fused_add_rms_norm`` (the fused op into a separate output) and
 ``rms_norm_fp8`` (either form with an fp8 e4m3 output, static or per-row
 scale), ``rms_norm_nvfp4`` (NVFP4 output), and the gated activations ``silu_and_mul``, ``gelu_and_mul`` and
-``gelu_tanh_and_mul``.  Everything dispatches through ``torch.ops.hp_rms_norm``, registered
+``gelu_tanh_and_mul``; and for training ``gated_linear`` (a feed-forward block's gate and up
+products with the activation), ``linear_cross_entropy`` (the loss of a linear layer over a
+vocabulary, without its logits), their backward passes, ``rms_norm_backward``, and
+``grad_norm`` / ``clip_grad_norm``.  Everything dispatches through ``torch.ops.hp_rms_norm``, registered
 by this package's compiled ``_C`` extension.
 """
 import torch
@@ -126,5 +129,90 @@ def gelu_tanh_and_mul(input, out=None):
     return _act_and_mul(torch.ops.hp_rms_norm.gelu_tanh_and_mul.default, input, out)
 
 
+def gated_linear(input, weight, act="silu", out=None, gate_up=None):
+    """out = act(input Wg^T) * (input Wu^T), the first half of a SwiGLU / GeGLU feed-forward
+    block in one kernel.  ``input`` [..., hidden], ``weight`` [2 d, hidden] holding Wg's rows,
+    then Wu's (the order ``silu_and_mul`` reads its halves in); ``act`` 'silu', 'gelu' or
+    'gelu_tanh'.  ``gate_up``, a float32 [..., 2 d] tensor, receives the two products for
+    ``gated_linear_backward``.  Returns ``out`` [..., d]."""
+    if out is None:
+        out = torch.empty(input.shape[:-1] + (weight.shape[0] // 2,), dtype=input.dtype,
+                          device=input.device)
+    torch.ops.hp_rms_norm.gated_linear.default(out, gate_up, input, weight, act)
+    return out
+
+
+def gated_linear_backward(grad_out, input, weight, act="silu", gate_up=None):
+    """Gradients (grad_input, grad_weight) of ``gated_linear`` for a gradient of its output.
+    With the ``gate_up`` that the forward call wrote the two products are read from it, without
+    it they are computed again."""
+    grad_input = torch.empty(input.shape, dtype=input.dtype, device=input.device)
+    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    torch.ops.hp_rms_norm.gated_linear_backward.default(grad_input, grad_weight, grad_out, input,
+                                                        weight, gate_up, act)
+    return grad_input, grad_weight
+
+
+def linear_cross_entropy(input, weight, target, ignore_index=-100):
+    """Per-row cross entropy of softmax(input weight^T) against ``target``, without holding the
+    logits: ``input`` [..., hidden], ``weight`` [vocab, hidden], ``target`` int64 [...].
+    Returns (loss, lse), float32 [...]: the loss (0 where the target is ``ignore_index``, NaN
+    where it is otherwise outside the vocabulary) and the logits' log-sum-exp, which
+    ``linear_cross_entropy_backward`` takes."""
+    loss = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
+    lse = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
+    torch.ops.hp_rms_norm.linear_cross_entropy.default(loss, lse, input, weight, target,
+                                                       ignore_index)
+    return loss, lse
+
+
+def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, ignore_index=-100):
+    """Gradients (grad_input, grad_weight) of ``linear_cross_entropy`` for the gradients of the
+    rows' losses, ``grad_loss`` float32 [...]; the logits are computed again, one piece of the
+    vocabulary at a time."""
+    grad_input = torch.empty(input.shape, dtype=input.dtype, device=input.device)
+    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    torch.ops.hp_rms_norm.linear_cross_entropy_backward.default(
+        grad_input, grad_weight, grad_loss, input, weight, target, lse, ignore_index)
+    return grad_input, grad_weight
+
+
+def rms_norm_backward(grad_out, input, weight, eps, grad_residual=None):
+    """Gradients (grad_input, grad_weight) of RMSNorm for a gradient of its output.  For the
+    fused forms ``input`` is the updated residual, and ``grad_residual`` the gradient that
+    reaches it from its other uses, which is added: grad_input is then the gradient of both
+    addends."""
+    grad_input = torch.empty(input.shape, dtype=input.dtype, device=input.device)
+    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    torch.ops.hp_rms_norm.rms_norm_backward.default(grad_input, grad_weight, grad_out, input,
+                                                    weight, grad_residual, eps)
+    return grad_input, grad_weight
+
+
+def grad_norm(grads):
+    """The 2-norm over all elements of all tensors of ``grads`` (float32, bfloat16 or float16,
+    mixed as they come), a float32 scalar tensor."""
+    if not len(grads):
+        return torch.zeros((), dtype=torch.float32)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    torch.ops.hp_rms_norm.grad_norm.default(norm, grads)
+    return norm
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """Scales every gradient by min(1, max_norm / (norm + 1e-6)), norm the 2-norm over all of
+    them, in place or into the tensors of ``out`` (of any of the three types: 16-bit gradients
+    into an optimiser's float32 buffers, say).  Returns the norm before clipping, a float32
+    scalar tensor; nothing waits for the GPU."""
+    norm = grad_norm(grads)
+    if len(grads):
+        torch.ops.hp_rms_norm.grad_clip.default(grads if out is None else out, grads, norm,
+                                                max_norm)
+    return norm
+
+
 __all__ = ["hp_rms_norm", "relu", "rms_norm", "fused_add_rms_norm", "rms_norm_fp8", "rms_norm_nvfp4",
-           "rms_norm_fp8_group", "silu_and_mul", "gelu_and_mul", "gelu_tanh_and_mul", "torch"]
+           "rms_norm_fp8_group", "silu_and_mul", "gelu_and_mul", "gelu_tanh_and_mul",
+           "gated_linear", "gated_linear_backward", "linear_cross_entropy",
+           "linear_cross_entropy_backward", "rms_norm_backward", "grad_norm", "clip_grad_norm",
+           "torch"]

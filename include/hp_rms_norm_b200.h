@@ -37,7 +37,8 @@ extern "C" {
 
 typedef enum hprn_dtype {
   HPRN_DTYPE_BF16 = 0, /* torch.bfloat16 / __nv_bfloat16 */
-  HPRN_DTYPE_FP16 = 1  /* torch.float16  / __half        */
+  HPRN_DTYPE_FP16 = 1, /* torch.float16  / __half        */
+  HPRN_DTYPE_FP32 = 2  /* torch.float32 / float: gradients of hprn_grad_* only */
 } hprn_dtype;
 
 /*
@@ -206,6 +207,126 @@ HPRN_API int hprn_rms_norm_fp8_group(void* out, float* scales, int64_t scale_row
                                      int64_t input_row_stride, int64_t residual_row_stride,
                                      double eps, int dtype, int group_size, int scale_pow2,
                                      void* stream, unsigned flags);
+
+/*
+ * Training operators (extensions past the reference).
+ *
+ * Workspaces: these calls allocate nothing, so a call that needs scratch
+ * memory takes it from the caller.  With HPRN_WORKSPACE_QUERY in `flags` a call
+ * launches nothing and writes the bytes it would need to *workspace_bytes
+ * (sizes, strides and pointers as in the call to come; no tensor is read).
+ * Without it, *workspace_bytes is the size of `workspace` (device memory,
+ * 256-byte aligned; may be NULL when the call needs none).  The workspace is
+ * free again once the call's work on the stream is done; it carries nothing
+ * from one call to the next.
+ */
+#define HPRN_WORKSPACE_QUERY 2u
+
+/*
+ * Gated linear layer, the first half of a SwiGLU / GeGLU feed-forward block:
+ *   G = input Wg^T, U = input Wu^T   (fp32 sums of 16-bit products)
+ *   out[i, j] = round_T(act(G_ij) * U_ij),  j < d
+ * input [rows, hidden], weight [2d, hidden] holding Wg's d rows, then Wu's.
+ * gate_up (NULL, or fp32 [rows, 2d]) receives G in its first d columns and U
+ * in the others, unrounded, for hprn_gated_linear_backward.  hidden == 0 gives
+ * sums of nothing: 0.  Outputs must not overlap inputs or each other.
+ */
+HPRN_API int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* weight,
+                               int64_t rows, int64_t hidden, int64_t d, int64_t out_row_stride,
+                               int64_t gate_up_row_stride, int64_t input_row_stride,
+                               int64_t weight_row_stride, int act, int dtype, void* workspace,
+                               int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Gradients of hprn_gated_linear for a gradient D of its output:
+ *   S = round_T([D U act'(G) | D act(G)])
+ *   grad_input [rows, hidden] = round_T(S weight)
+ *   grad_weight [2d, hidden]  = round_T(S^T input)
+ * gate_up: what the forward call wrote (it is not changed), or NULL to compute
+ * the two products again.
+ */
+HPRN_API int hprn_gated_linear_backward(
+    void* grad_input, void* grad_weight, const void* grad_out, const float* gate_up,
+    const void* input, const void* weight, int64_t rows, int64_t hidden, int64_t d,
+    int64_t grad_input_row_stride, int64_t grad_weight_row_stride, int64_t grad_out_row_stride,
+    int64_t gate_up_row_stride, int64_t input_row_stride, int64_t weight_row_stride, int act,
+    int dtype, void* workspace, int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Softmax cross entropy of a linear layer over a vocabulary, the logits never
+ * held: with L = input weight^T (fp32 sums), t = target[i],
+ *   lse[i]  = log sum_j exp(L_ij)
+ *   loss[i] = lse[i] - L_{i, t}; 0 where t == ignore_index; NaN where t is
+ *             otherwise outside [0, vocab)
+ * input [rows, hidden], weight [vocab, hidden], target int64 [rows], loss and
+ * lse fp32 [rows].
+ */
+HPRN_API int hprn_linear_cross_entropy(float* loss, float* lse, const void* input,
+                                       const void* weight, const int64_t* target,
+                                       int64_t ignore_index, int64_t rows, int64_t hidden,
+                                       int64_t vocab, int64_t input_row_stride,
+                                       int64_t weight_row_stride, int dtype, void* workspace,
+                                       int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Gradients of hprn_linear_cross_entropy for gradients c[i] = grad_loss[i] of
+ * the rows' losses (fp32), lse from the forward call:
+ *   S_ij = round_T(c_i (exp(L_ij - lse_i) - [j == target_i])); 0 in rows with
+ *          target_i == ignore_index, NaN in rows with any other invalid target
+ *   grad_input [rows, hidden]  = round_T(S weight)
+ *   grad_weight [vocab, hidden] = round_T(S^T input)
+ * In fp16, S is held times a power of two (the largest |c_i| brought to
+ * [2^14, 2^15)), so small probabilities do not underflow.
+ */
+HPRN_API int hprn_linear_cross_entropy_backward(
+    void* grad_input, void* grad_weight, const float* grad_loss, const void* input,
+    const void* weight, const int64_t* target, const float* lse, int64_t ignore_index,
+    int64_t rows, int64_t hidden, int64_t vocab, int64_t grad_input_row_stride,
+    int64_t grad_weight_row_stride, int64_t input_row_stride, int64_t weight_row_stride, int dtype,
+    void* workspace, int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Gradients of RMSNorm, y = x w inv, inv = rsqrt(mean(x^2) + eps), for a
+ * gradient D of y:
+ *   grad_input  = round_T(inv (w D - x inv mean(w D x inv)) + grad_residual)
+ *   grad_weight = round_T(sum over rows of D x inv)
+ * For the fused add + RMSNorm `input` is the updated residual, and grad_input
+ * the gradient of both its addends.  grad_residual (NULL for none): the
+ * gradient that reaches `input` through the residual branch.
+ */
+HPRN_API int hprn_rms_norm_backward(void* grad_input, void* grad_weight, const void* grad_out,
+                                    const void* input, const void* weight,
+                                    const void* grad_residual, int64_t rows, int64_t hidden,
+                                    int64_t grad_input_row_stride, int64_t grad_out_row_stride,
+                                    int64_t input_row_stride, int64_t grad_residual_row_stride,
+                                    double eps, int dtype, void* workspace,
+                                    int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/* One gradient tensor of hprn_grad_norm / hprn_grad_clip: rows x cols elements
+ * of an hprn_dtype; `out` is read by hprn_grad_clip only. */
+typedef struct hprn_grad {
+  const void* grad;
+  void* out;
+  int64_t rows, cols;
+  int64_t row_stride, out_row_stride;
+  int32_t dtype, out_dtype;
+} hprn_grad;
+
+/*
+ * *norm = sqrt(sum of the squares of all elements of all tensors) (fp32 on the
+ * device; 0 for no elements).  `grads` is a host array, read during the call.
+ * The same tensors give the same bits on every call.
+ */
+HPRN_API int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* workspace,
+                            int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * out = round(grad * min(1, max_norm / (*norm + 1e-6))) for every tensor; a NaN
+ * norm makes every output NaN.  `out` may be the gradient itself (same type and
+ * stride), which is then left unwritten where the factor is 1; otherwise it must not overlap it.
+ */
+HPRN_API int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm,
+                            double max_norm, void* stream, unsigned flags);
 
 /* Message for the last non-OK status returned on this thread ("" if none). */
 HPRN_API const char* hprn_last_error(void);

@@ -1,0 +1,206 @@
+"""linear_cross_entropy and its backward pass on the GPU against the 64-bit formulas."""
+import pytest
+import torch
+
+import hp_rms_norm_b200 as hp
+from tests import training_reference as R
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+IGNORE = -100
+SHAPES = [(1, 64, 256), (1, 1001, 1), (2, 8, 3), (7, 1, 31), (9, 264, 1000), (33, 40, 513),
+          (64, 512, 2048), (100, 1000, 333), (129, 136, 4097), (300, 520, 1500), (513, 264, 777)]
+
+
+def make(rows, hidden, vocab, dtype, device, ignored=0.2, scale=2.0, seed=0):
+    g = torch.Generator(device=device).manual_seed(seed + rows * 7 + hidden * 3 + vocab)
+    x = torch.randn(rows, hidden, generator=g, device=device).to(dtype)
+    w = (torch.randn(vocab, hidden, generator=g, device=device) * scale * hidden ** -0.5).to(dtype)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=device)
+    t[torch.rand(rows, generator=g, device=device) < ignored] = IGNORE
+    c = torch.rand(rows, generator=g, device=device) + 0.5
+    return x, w, t, c
+
+
+def logit_error(x, w):
+    return x.shape[1] * R.F32 * (x.double().abs() @ w.double().abs().T)
+
+
+def check_loss(loss, lse, x, w, t, label):
+    want, want_lse, logits = R.linear_cross_entropy(x, w, t, IGNORE)
+    e = logit_error(x, w).max(-1).values if w.shape[0] else torch.zeros_like(want)
+    # lse moves by at most the logits' error; its own arithmetic is an fp32 sum of V
+    # exponentials, each off by 2^-22 (2 + |l - max|) at most, and a logarithm.
+    spread = (logits.max(-1).values - logits.min(-1).values).clamp(min=1)
+    el = e + w.shape[0] * R.F32 + 4 * R.F32 * (2 + spread) + 2 * R.F32 * want_lse.abs()
+    R.assert_within(lse, want_lse, el, label + " lse")
+    counts = (t != IGNORE).double()
+    R.assert_within(loss, want, (el + e + 2 * R.F32 * (want.abs() + want_lse.abs())) * counts, label)
+
+
+def check_backward(dx, dw, c, x, w, t, label):
+    want_x, want_w, s = R.linear_cross_entropy_backward(c, x, w, t, IGNORE)
+    _, lse, logits = R.linear_cross_entropy(x, w, t, IGNORE)
+    le = logit_error(x, w)
+    spread = (logits.max(-1).values - logits.min(-1).values).clamp(min=1)
+    el = le.max(-1).values + w.shape[0] * R.F32 + 4 * R.F32 * (2 + spread) + 2 * R.F32 * lse.abs()
+    p = torch.exp(logits - lse[:, None])
+    rel = 2 * (le + el[:, None] + 4 * R.F32 * (2 + (logits - lse[:, None]).abs()))
+    e = c.double()[:, None] * (p * rel + R.F32) * (t != IGNORE)[:, None]
+    # fp16 holds S times a power of two that brings the largest |c| to 2^14 or more.
+    tiny = R.TINY[dx.dtype] * (c.max().item() * 2.0 ** -14 if dx.dtype == torch.float16 else 1.0)
+    e = e + R.U[dx.dtype] * (s.abs() + e) + tiny
+    bx = R.product_bound(s, w.double(), e, w.shape[0])
+    R.assert_within(dx, want_x, R.rounded(bx, want_x, dx.dtype), label + " dx")
+    bw = R.product_bound(s.T, x.double(), e.T, x.shape[0])
+    R.assert_within(dw, want_w, R.rounded(bw, want_w, dw.dtype), label + " dw")
+    R.assert_near(dx, want_x, R.rounding_noise(s, w.double(), dx.dtype), label + " dx")
+    R.assert_near(dw, want_w, R.rounding_noise(s.T, x.double(), dx.dtype), label + " dw")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_forward_and_backward(cuda, shape, dt):
+    x, w, t, c = make(*shape, DTYPES[dt], cuda)
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    check_loss(loss, lse, x, w, t, f"{shape} {dt}")
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    check_backward(dx, dw, c, x, w, t, f"{shape} {dt}")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_sharp_logits(cuda, dt):
+    """Logits of several hundred: exponentials that overflow and underflow fp32 by themselves."""
+    x, w, t, c = make(70, 128, 600, DTYPES[dt], cuda, scale=60.0)
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    check_loss(loss, lse, x, w, t, "sharp")
+    assert torch.isfinite(loss).all() and loss.max() > 100
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1.0, 1e4])
+def test_gradient_range_in_fp16(cuda, scale):
+    """A mean's small factors times small probabilities, and large ones, keep their precision:
+    relative to 16-bit outputs that hold them, here checked on rows rescaled by the caller."""
+    x, w, t, c = make(64, 64, 4000, torch.float16, cuda, ignored=0.0)
+    w[:, :] = (w.float() * 0.05).half()  # nearly uniform probabilities: 1 / 4000 each
+    _, lse = hp.linear_cross_entropy(x, w, t)
+    c = torch.full_like(c, scale)
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    check = [(dx, R.linear_cross_entropy_backward(c, x, w, t, IGNORE)[0]),
+             (dw, R.linear_cross_entropy_backward(c, x, w, t, IGNORE)[1])]
+    for got, want in check:
+        # u for S, u for the output, and half a subnormal step of the output
+        step = 2.0 ** -25 * want.numel() ** 0.5
+        assert (got.double() - want).norm() <= 2 * R.U[torch.float16] * want.norm() + step
+
+
+def test_ignored_and_invalid_rows(cuda):
+    x, w, t, c = make(130, 64, 300, torch.bfloat16, cuda, ignored=0.0)
+    t[:] = IGNORE
+    c[3] = float("inf")  # an ignored row's gradient does not matter
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    assert not loss.any()
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    assert not dx.any() and not dw.any()
+    t[:] = 5
+    t[0], t[129], t[7], t[8] = 299, 0, 300, -1
+    c[:] = 1
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    assert loss[[7, 8]].isnan().all() and torch.isfinite(loss).sum() == 128
+    dx, _ = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    assert dx[[7, 8]].isnan().all() and torch.isfinite(dx).all(-1).sum() == 128
+    # another ignore_index, inside the vocabulary
+    loss, _ = hp.linear_cross_entropy(x, w, t, ignore_index=5)
+    assert (loss == 0).sum() == 126
+
+
+def test_pieces_of_the_vocabulary(cuda):
+    """Enough rows for the vocabulary to be taken in several pieces (512 MiB of 16-bit logit
+    gradients each): the input's gradient is summed over them."""
+    rows, vocab = 40000, 9001
+    x, w, t, c = make(rows, 16, vocab, torch.bfloat16, cuda)
+    t[0], t[1], t[2] = 0, vocab - 1, 6400
+    _, lse = hp.linear_cross_entropy(x, w, t)
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    want = R.linear_cross_entropy_backward(c, x, w, t, IGNORE)
+    R.assert_near(dx, want[0], R.rounding_noise(want[2], w.double(), w.dtype), "dx")
+    R.assert_near(dw, want[1], R.rounding_noise(want[2].T, x.double(), w.dtype), "dw")
+
+
+def test_empty(cuda):
+    x, w, t, c = make(12, 64, 48, torch.float16, cuda)
+    loss, lse = hp.linear_cross_entropy(x[:0], w, t[:0])
+    assert loss.shape == (0,)
+    dx, dw = hp.linear_cross_entropy_backward(c[:0], x[:0], w, t[:0], lse)
+    assert dx.shape == (0, 64) and not dw.any()
+    loss, lse = hp.linear_cross_entropy(x, w[:0], torch.full_like(t, IGNORE))
+    assert not loss.any() and (lse == float("-inf")).all()
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w[:0], torch.full_like(t, IGNORE), lse)
+    assert not dx.any() and dw.shape == (0, 64)
+    loss, lse = hp.linear_cross_entropy(x[:, :0], w[:, :0], t)
+    torch.testing.assert_close(lse, torch.full_like(lse, 48.0).log())
+
+
+def test_differences(cuda):
+    """The loss's own differences in random directions.  Inputs are multiples of 2^-4 and the
+    step 2^-5 a element, so x + h v is exact in bf16."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    rows, hidden, vocab = 48, 64, 400
+    x = (torch.randint(-12, 13, (rows, hidden), generator=g, device=cuda) / 16).bfloat16()
+    w = (torch.randint(-12, 13, (vocab, hidden), generator=g, device=cuda) / 32).bfloat16()
+    t = torch.randint(0, vocab, (rows,), generator=g, device=cuda)
+    _, lse = hp.linear_cross_entropy(x, w, t)
+    dx, _ = hp.linear_cross_entropy_backward(torch.ones(rows, device=cuda), x, w, t, lse)
+    h = 2.0 ** -5
+    for _ in range(4):
+        v = (torch.randint(0, 2, x.shape, generator=g, device=cuda) * 2 - 1).double()
+        hi = hp.linear_cross_entropy((x.double() + h * v).bfloat16(), w, t)[0].double()
+        lo = hp.linear_cross_entropy((x.double() - h * v).bfloat16(), w, t)[0].double()
+        diff = (hi - lo) / (2 * h)
+        along = (dx.double() * v).sum(-1)
+        # third derivatives of lse along v: the third central moment of (W v), at most
+        # max|W v| var; fp32 losses of about 7; bf16 gradients.
+        wv = (w.double() @ v.T)
+        third = h * h / 6 * 2 * wv.abs().max(0).values ** 3
+        bound = third + 2 * 7 * 8 * R.F32 / h + 3 * R.U[torch.bfloat16] * dx.double().abs().sum(-1)
+        assert ((diff - along).abs() <= bound).all()
+
+
+def test_streams_graphs_and_shapes(cuda):
+    x, w, t, c = make(66, 256, 500, torch.bfloat16, cuda)
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    want = (loss, lse, *hp.linear_cross_entropy_backward(c, x, w, t, lse))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a, b = hp.linear_cross_entropy(x, w, t)
+        got = (a, b, *hp.linear_cross_entropy_backward(c, x, w, t, b))
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a, b = hp.linear_cross_entropy(x, w, t)
+        kept = (a, b, *hp.linear_cross_entropy_backward(c, x, w, t, b))
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for p, q, r in zip(want, got, kept):
+        assert torch.equal(p, q) and torch.equal(p, r)
+    loss3, _ = hp.linear_cross_entropy(x.view(6, 11, 256), w, t.view(6, 11))
+    assert loss3.shape == (6, 11) and torch.equal(loss3.view(-1), loss)
+
+
+def test_refusals(cuda):
+    x, w, t, c = make(4, 32, 16, torch.bfloat16, cuda)
+    lse = torch.zeros(4, device=cuda)
+    for bad in (lambda: hp.linear_cross_entropy(x.cpu(), w, t),
+                lambda: hp.linear_cross_entropy(x, w.half(), t),
+                lambda: hp.linear_cross_entropy(x, w, t.int()),
+                lambda: hp.linear_cross_entropy(x, w, t[:3]),
+                lambda: hp.linear_cross_entropy(x, w, t.cpu()),
+                lambda: hp.linear_cross_entropy(x, w[:, :-1], t),
+                lambda: hp.linear_cross_entropy_backward(c.double(), x, w, t, lse),
+                lambda: hp.linear_cross_entropy_backward(c, x, w, t, lse[:2]),
+                lambda: hp.linear_cross_entropy_backward(c[:2], x, w, t, lse)):
+        with pytest.raises(RuntimeError):
+            bad()
