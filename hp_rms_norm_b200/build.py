@@ -27,9 +27,10 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB_NAME = "libhp_rms_norm_b200.so"
 LIB = os.path.join(PKG, LIB_NAME)
-CUDA_SOURCES = ["rms_norm.cu", "relu.cu", "act_and_mul.cu", "gated_linear.cu",
+CUDA_SOURCES = ["rms_norm.cu", "relu.cu", "act_and_mul.cu", "matmul.cu", "gated_linear.cu",
                 "linear_cross_entropy.cu", "rms_norm_backward.cu", "grad_clip.cu", "runtime.cu"]
-HEADERS = ["vec.cuh", "bulk.cuh", "runtime.cuh", "rms_norm_kernels.cuh", "matmul.cuh", "gated.cuh"]
+HEADERS = ["vec.cuh", "bulk.cuh", "runtime.cuh", "rms_norm_kernels.cuh", "tcgen05.cuh", "matmul.cuh",
+           "gated.cuh"]
 
 # HPRN_DEBUG=1 (or the reference's own DEBUG=1, setup.py:23-28 there) builds
 # host code without optimisation and with debug symbols (device code keeps -O3

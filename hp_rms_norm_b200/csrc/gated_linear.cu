@@ -180,13 +180,14 @@ int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* 
                     (gate_up && gate_up_row_stride < 2 * d))) ||
       (d > 0 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
-  const bool empty = rows == 0 || d == 0;
   Workspace ws(workspace, *workspace_bytes);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
+  const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
   }
-  if (empty) return ok();
+  if (rows == 0 || d == 0) return ok();
   if (!out || (hidden > 0 && (!input || !weight)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
   if (!aligned(out, 2) || !aligned(input, 2) || !aligned(weight, 2) || !aligned(gate_up, 4))
@@ -199,16 +200,18 @@ int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* 
   if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
   Product q;
-  q.a = {static_cast<const uint16_t*>(input), input_row_stride, true};
-  q.b = {static_cast<const uint16_t*>(weight), weight_row_stride, true};
+  q.a = {x.data(), x.ld()};
+  q.b = {w.data(), w.ld()};
   q.m = rows, q.n = d, q.depth = hidden, q.pair_offset = d;
   return with_type_and_act(dtype, act, [&](auto t, auto a) {
     using T = decltype(t);
     GatedEpilogue<T, decltype(a)::value> e;
     e.out = static_cast<uint16_t*>(out), e.ld = out_row_stride, e.d = d;
     e.gate_up = gate_up, e.gate_up_ld = gate_up_row_stride;
-    return launch_product<T>(q, e, static_cast<cudaStream_t>(stream), "gated_linear");
+    return launch_product<T, true, true>(q, e, cs, flags, "gated_linear");
   });
 }
 
@@ -228,6 +231,8 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
       (d > 0 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
+  const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride);
   const int64_t s_ld = round_up(2 * d, 16);
   uint16_t* s = ws.take<uint16_t>(rows * s_ld);
   if (flags & HPRN_WORKSPACE_QUERY) {
@@ -252,8 +257,7 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  const uint16_t* x = static_cast<const uint16_t*>(input);
-  const uint16_t* w = static_cast<const uint16_t*>(weight);
+  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
   if (rows > 0 && d > 0) {
     st = with_type_and_act(dtype, act, [&](auto t, auto a) {
       using T = decltype(t);
@@ -262,18 +266,18 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
         GatedGradArgs g{static_cast<const uint16_t*>(grad_out), grad_out_row_stride, gate_up,
                         gate_up_row_stride, s, s_ld, rows, d};
         const int64_t ctas = (rows * d + 1023) / 1024;
-        gated_grad_rows<T, kAct><<<static_cast<unsigned>(ctas < 16 * dev->sm_count ? ctas : 16 * dev->sm_count),
-                                   256, 0, cs>>>(g);
-        return check_launch("gated_linear_backward");
+        const int64_t most = 16 * dev->sm_count;
+        return launch_rows(gated_grad_rows<T, kAct>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
+                           dim3(256), cs, flags, "gated_linear_backward", g);
       }
       Product q;
-      q.a = {x, input_row_stride, true};
-      q.b = {w, weight_row_stride, true};
+      q.a = {x.data(), x.ld()};
+      q.b = {w.data(), w.ld()};
       q.m = rows, q.n = d, q.depth = hidden, q.pair_offset = d;
       GatedGradEpilogue<T, kAct> e;
       e.dout = static_cast<const uint16_t*>(grad_out), e.dout_ld = grad_out_row_stride;
       e.s = s, e.s_ld = s_ld, e.d = d;
-      return launch_product<T>(q, e, cs, "gated_linear_backward");
+      return launch_product<T, true, true>(q, e, cs, flags, "gated_linear_backward");
     });
     if (st != HPRN_OK) return st;
   }
@@ -284,21 +288,21 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
     int r = HPRN_OK;
     if (rows > 0) {
       Product q;
-      q.a = {s, s_ld, true};
-      q.b = {w, weight_row_stride, false};
+      q.a = {s, s_ld};
+      q.b = {w.data(), w.ld()};
       q.m = rows, q.n = hidden, q.depth = 2 * d;
       StoreEpilogue<T> e;
       e.out = static_cast<uint16_t*>(grad_input), e.ld = grad_input_row_stride, e.n = hidden;
-      r = launch_product<T>(q, e, cs, "gated_linear_backward");
+      r = launch_product<T, true, false>(q, e, cs, flags, "gated_linear_backward");
     }
     if (r == HPRN_OK && d > 0) {
       Product q;
-      q.a = {s, s_ld, false};
-      q.b = {x, input_row_stride, false};
+      q.a = {s, s_ld};
+      q.b = {x.data(), x.ld()};
       q.m = 2 * d, q.n = hidden, q.depth = rows;
       StoreEpilogue<T> e;
       e.out = static_cast<uint16_t*>(grad_weight), e.ld = grad_weight_row_stride, e.n = hidden;
-      r = launch_product<T>(q, e, cs, "gated_linear_backward");
+      r = launch_product<T, false, false>(q, e, cs, flags, "gated_linear_backward");
     }
     return r;
   };

@@ -207,13 +207,13 @@ int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* wor
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   int64_t at = 0;
   st = for_tables(grads, count, [&](const GradTable& t, int64_t chunks) {
-    grad_square_sums<<<static_cast<unsigned>(chunks), kClipThreads, 0, cs>>>(t, partial + at);
+    float* part = partial + at;
     at += chunks;
-    return check_launch("grad_norm");
+    return launch_rows(grad_square_sums, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
+                       "grad_norm", t, part);
   });
   if (st != HPRN_OK) return st;
-  grad_norm_join<<<1, 1024, 0, cs>>>(partial, total, norm);
-  return check_launch("grad_norm");
+  return launch_rows(grad_norm_join, dim3(1), dim3(1024), cs, flags, "grad_norm", partial, total, norm);
 }
 
 int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm, double max_norm,
@@ -231,8 +231,8 @@ int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm, dou
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   st = for_tables(grads, count, [&](const GradTable& t, int64_t chunks) {
-    grad_scale<<<static_cast<unsigned>(chunks), kClipThreads, 0, cs>>>(t, norm, static_cast<float>(max_norm));
-    return check_launch("grad_clip");
+    return launch_rows(grad_scale, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
+                       "grad_clip", t, norm, static_cast<float>(max_norm));
   });
   return st == HPRN_OK ? ok() : st;
 }

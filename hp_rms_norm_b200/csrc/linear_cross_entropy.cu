@@ -220,7 +220,13 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   if ((rows > 1 && input_row_stride < hidden) || (vocab > 1 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
-  const int64_t tiles = product_tiles<LossEpilogue>(vocab);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
+  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride);
+  Product q;
+  q.a = {x.data(), x.ld()};
+  q.b = {w.data(), w.ld()};
+  q.m = rows, q.n = vocab, q.depth = hidden;
+  const int64_t tiles = product_tiles<LossEpilogue>(q);
   float2* partial = ws.take<float2>(tiles * rows);
   float* target_logit = ws.take<float>(rows);
   if (flags & HPRN_WORKSPACE_QUERY) {
@@ -242,21 +248,19 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const char* what = "linear_cross_entropy";
+  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
   if (vocab > 0) {
-    Product q;
-    q.a = {static_cast<const uint16_t*>(input), input_row_stride, true};
-    q.b = {static_cast<const uint16_t*>(weight), weight_row_stride, true};
-    q.m = rows, q.n = vocab, q.depth = hidden;
     LossEpilogue e;
     e.partial = partial, e.target_logit = target_logit, e.target = target;
     e.ignore = ignore_index, e.rows = rows, e.vocab = vocab;
-    st = dtype == HPRN_DTYPE_BF16 ? launch_product<__nv_bfloat16>(q, e, cs, "linear_cross_entropy")
-                                  : launch_product<__half>(q, e, cs, "linear_cross_entropy");
+    st = dtype == HPRN_DTYPE_BF16 ? launch_product<__nv_bfloat16, true, true>(q, e, cs, flags, what)
+                                  : launch_product<__half, true, true>(q, e, cs, flags, what);
     if (st != HPRN_OK) return st;
   }
-  loss_join<<<static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), dim3(kJoinRows, kJoinGroups), 0, cs>>>(
-      partial, target_logit, target, ignore_index, rows, vocab, tiles, loss, lse);
-  return check_launch("linear_cross_entropy");
+  return launch_rows(loss_join, dim3(static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows)),
+                     dim3(kJoinRows, kJoinGroups), cs, flags, what, partial, target_logit, target,
+                     ignore_index, rows, vocab, vocab > 0 ? tiles : 0, loss, lse);
 }
 
 int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, const float* grad_loss,
@@ -273,6 +277,8 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       (vocab > 1 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
+  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride);
   const Pieces pieces = pieces_of(rows, vocab);
   uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
   float* sum = pieces.count > 1 ? ws.take<float>(rows * hidden) : nullptr;
@@ -299,13 +305,13 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (factor && rows > 0) {
-    loss_grad_scale<<<1, 1024, 0, cs>>>(grad_loss, target, ignore_index, rows, factor);
-    if ((st = check_launch("linear_cross_entropy_backward")) != HPRN_OK) return st;
-  }
-  const uint16_t* x = static_cast<const uint16_t*>(input);
-  const uint16_t* w = static_cast<const uint16_t*>(weight);
   const char* what = "linear_cross_entropy_backward";
+  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  if (factor && rows > 0) {
+    st = launch_rows(loss_grad_scale, dim3(1), dim3(1024), cs, flags, what, grad_loss, target, ignore_index,
+                     rows, factor);
+    if (st != HPRN_OK) return st;
+  }
   auto all = [&](auto t) {
     using T = decltype(t);
     int r = HPRN_OK;
@@ -316,35 +322,35 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       const int64_t cols = vocab - first < pieces.cols ? vocab - first : pieces.cols;
       if (rows > 0 && cols > 0) {
         Product q;
-        q.a = {x, input_row_stride, true};
-        q.b = {w + first * weight_row_stride, weight_row_stride, true};
+        q.a = {x.data(), x.ld()};
+        q.b = {w.data() + first * w.ld(), w.ld()};
         q.m = rows, q.n = cols, q.depth = hidden;
         LossGradEpilogue<T> e;
         e.s = s, e.ld = pieces.cols, e.lse = lse, e.grad_loss = grad_loss, e.factor = factor;
         e.target = target, e.ignore = ignore_index, e.vocab = vocab, e.first = first, e.cols = cols;
-        if ((r = launch_product<T>(q, e, cs, what)) != HPRN_OK) break;
+        if ((r = launch_product<T, true, true>(q, e, cs, flags, what)) != HPRN_OK) break;
       }
       if (rows > 0) {
         Product q;
-        q.a = {s, pieces.cols, true};
-        q.b = {w + first * weight_row_stride, weight_row_stride, false};
+        q.a = {s, pieces.cols};
+        q.b = {w.data() + first * w.ld(), w.ld()};
         q.m = rows, q.n = hidden, q.depth = cols;
         StoreEpilogue<T> e;
         e.out = static_cast<uint16_t*>(grad_input), e.ld = grad_input_row_stride, e.n = hidden;
         e.sum = sum, e.first = p == 0, e.last = p == count - 1;
         e.scale = factor ? factor + 1 : nullptr;
-        if ((r = launch_product<T>(q, e, cs, what)) != HPRN_OK) break;
+        if ((r = launch_product<T, true, false>(q, e, cs, flags, what)) != HPRN_OK) break;
       }
       if (cols > 0) {
         Product q;
-        q.a = {s, pieces.cols, false};
-        q.b = {x, input_row_stride, false};
+        q.a = {s, pieces.cols};
+        q.b = {x.data(), x.ld()};
         q.m = cols, q.n = hidden, q.depth = rows;
         StoreEpilogue<T> e;
         e.out = static_cast<uint16_t*>(grad_weight) + first * grad_weight_row_stride;
         e.ld = grad_weight_row_stride, e.n = hidden;
         e.scale = factor && rows > 0 ? factor + 1 : nullptr;
-        r = launch_product<T>(q, e, cs, what);
+        r = launch_product<T, false, false>(q, e, cs, flags, what);
       }
     }
     return r;

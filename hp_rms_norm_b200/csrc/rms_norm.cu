@@ -963,6 +963,17 @@ int run(const Problem& q, void* stream, unsigned flags) {
   return ok();
 }
 
+// The wait counter's address on the current device, for the kernels of other
+// files.
+int timeout_counter(unsigned** out) {
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, g_wait_timeouts);
+  if (e != cudaSuccess)
+    return fail(HPRN_ERR_CUDA, std::string("the wait-timeout count: ") + cudaGetErrorString(e));
+  *out = static_cast<unsigned*>(p);
+  return HPRN_OK;
+}
+
 }  // namespace hprn
 
 extern "C" {

@@ -98,18 +98,18 @@ __global__ void __launch_bounds__(256) norm_grad_weight(NormGradArgs a) {
 }
 
 template <typename T>
-int launch_norm_grad(const NormGradArgs& a, cudaStream_t stream) {
+int launch_norm_grad(const NormGradArgs& a, cudaStream_t stream, unsigned flags) {
   const char* what = "rms_norm_backward";
   const unsigned cols = static_cast<unsigned>((a.hidden + 255) / 256);
   if (a.rows > 0) {
-    norm_grad_stats<T><<<static_cast<unsigned>(a.rows), 256, 0, stream>>>(a);
-    int st = check_launch(what);
+    int st = launch_rows(norm_grad_stats<T>, dim3(static_cast<unsigned>(a.rows)), dim3(256), stream, flags,
+                         what, a);
     if (st != HPRN_OK) return st;
-    norm_grad_columns<T><<<dim3(cols, static_cast<unsigned>(a.groups)), 256, 0, stream>>>(a);
-    if ((st = check_launch(what)) != HPRN_OK) return st;
+    st = launch_rows(norm_grad_columns<T>, dim3(cols, static_cast<unsigned>(a.groups)), dim3(256), stream,
+                     flags, what, a);
+    if (st != HPRN_OK) return st;
   }
-  norm_grad_weight<T><<<cols, 256, 0, stream>>>(a);
-  return check_launch(what);
+  return launch_rows(norm_grad_weight<T>, dim3(cols), dim3(256), stream, flags, what, a);
 }
 
 }  // namespace hprn
@@ -166,6 +166,6 @@ extern "C" int hprn_rms_norm_backward(void* grad_input, void* grad_weight, const
   a.x_stride = input_row_stride, a.extra_stride = grad_residual_row_stride;
   a.eps = static_cast<float>(eps);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  return dtype == HPRN_DTYPE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, cs)
-                                  : launch_norm_grad<__half>(a, cs);
+  return dtype == HPRN_DTYPE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, cs, flags)
+                                  : launch_norm_grad<__half>(a, cs, flags);
 }

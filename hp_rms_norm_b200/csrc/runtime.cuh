@@ -115,6 +115,28 @@ bool disjoint(const Extent (&outs)[NO], const Extent (&ins)[NI]) {
   return true;
 }
 
+// Launches a kernel that begins with pdl_wait(), with programmatic stream
+// serialization where `flags` ask for it.
+template <typename... P, typename... A>
+int launch_rows(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, unsigned flags,
+                const char* what, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if (flags & HPRN_LAUNCH_PDL) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...);
+  if (e != cudaSuccess)
+    return fail(HPRN_ERR_CUDA, std::string(what) + " launch failed: " + cudaGetErrorString(e));
+  return ok();
+}
+
 // Reports a failed launch (cudaGetLastError after the launch) as HPRN_ERR_CUDA.
 int check_launch(const char* what);
 
