@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
     mbar_init_fence();
     if (args.depth_blocks > 0) prefetch_tensor_map(&map_a), prefetch_tensor_map(&map_b);
   }
+  __syncwarp();
   if (warp == 2) tmem_alloc<kGroup>(smem_u32(&tmem_base), L::kTmemColumns);
   tmem_fence_before();
   __syncthreads();
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
       }
     }
   }
+  __syncwarp();
   tmem_fence_before();
   __syncthreads();
   if constexpr (kGroup == 2) cluster_sync_all();
@@ -401,7 +403,7 @@ struct Tiling {
 
 template <typename E>
 inline Tiling tiling_of(const Product&) {
-  return Tiling{1, 256};
+  return Tiling{2, 256};
 }
 
 // Columns of C that one `end` call covers (how an epilogue with per-tile
@@ -505,7 +507,7 @@ int launch_tiles(const Product& q, const E& epi, cudaStream_t stream, unsigned f
 // kAKMajor / kBKMajor: how the operands lie, Operand::k_major at compile time.
 template <typename T, bool kAKMajor, bool kBKMajor, typename E>
 int launch_product(const Product& q, const E& epi, cudaStream_t stream, unsigned flags, const char* what) {
-  return launch_tiles<T, E, 1, 256, kAKMajor, kBKMajor>(q, epi, stream, flags, what);
+  return launch_tiles<T, E, 2, 256, kAKMajor, kBKMajor>(q, epi, stream, flags, what);
 }
 
 }  // namespace hprn
