@@ -27,58 +27,36 @@ namespace hprn {
 template <typename T, int ACT>
 struct GatedEpilogue {
   static constexpr bool kPaired = true;
-  uint16_t* out = nullptr;
-  int64_t ld = 0;
-  int64_t d = 0;
-  float* gate_up = nullptr;  // or null
-  int64_t gate_up_ld = 0;
+  Out16 out;
+  Out32 gate, up;  // null to leave out
 
   struct Row {};
-  __device__ __forceinline__ Row begin(int64_t) const { return {}; }
-  __device__ __forceinline__ void chunk(Row&, int64_t i, int64_t j, const float (&g)[kChunk],
-                                        const float (&u)[kChunk]) const {
-    if (gate_up) {
-      store_chunk_f32(gate_up + i * gate_up_ld, j, d, g);
-      store_chunk_f32(gate_up + i * gate_up_ld + d, j, d, u);
+  __device__ __forceinline__ Row begin(const Lane&, int64_t) const { return {}; }
+  __device__ __forceinline__ void chunk(Row&, const Lane& l, int64_t i, int64_t j, float (&g)[kChunk],
+                                        float (&u)[kChunk]) const {
+    if (gate.p) {
+      gate.store(l, i, j, g);
+      up.store(l, i, j, u);
     }
-    float h[kChunk];
 #pragma unroll
-    for (int k = 0; k < kChunk; ++k) h[k] = activate_with_slope<ACT>(g[k]).value * u[k];
-    store_chunk<T>(out + i * ld, j, d, h);
+    for (int k = 0; k < kChunk; ++k) u[k] *= activate_with_slope<ACT>(g[k]).value;
+    out.template store<T>(l, i, j, u);
   }
-  __device__ __forceinline__ void end(Row&, int64_t, int64_t) const {}
+  __device__ __forceinline__ void end(Row&, const Lane&, int64_t, int64_t) const {}
+  __device__ __forceinline__ void point(int64_t i, int64_t j, float g, float u) const {
+    if (gate.p) gate.p[i * gate.ld + j] = g, up.p[i * up.ld + j] = u;
+    out.p[i * out.ld + j] = pack1<T>(activate_with_slope<ACT>(g).value * u);
+  }
 };
 
-// S's chunk from the same chunk of G, U and D.
-template <typename T, int ACT>
-__device__ __forceinline__ void gated_gradients(float (&g)[kChunk], float (&u)[kChunk],
-                                                const float (&dout)[kChunk]) {
+// [dG | dU] in place of G and U, for the gradient D of act(G) U.
+template <int ACT, int N>
+__device__ __forceinline__ void gated_gradients(float (&g)[N], float (&u)[N], const float (&dout)[N]) {
 #pragma unroll
-  for (int k = 0; k < kChunk; ++k) {
+  for (int k = 0; k < N; ++k) {
     const ActValue a = activate_with_slope<ACT>(g[k]);
     g[k] = dout[k] * u[k] * a.slope;
     u[k] = dout[k] * a.value;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void load_chunk(const uint16_t* row, int64_t j, int64_t n,
-                                           float (&v)[kChunk]) {
-  const uint16_t* p = row + j;
-  if (j + kChunk <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-#pragma unroll
-    for (int h = 0; h < kChunk / 8; ++h) {
-      const uint4 q = reinterpret_cast<const uint4*>(p)[h];
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = unpack2<T>(w[k]);
-        v[8 * h + 2 * k] = f.x, v[8 * h + 2 * k + 1] = f.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kChunk; ++k) v[k] = j + k < n ? unpack1<T>(p[k]) : 0.f;
   }
 }
 
@@ -88,26 +66,49 @@ struct GatedGradEpilogue {
   static constexpr bool kPaired = true;
   const uint16_t* dout = nullptr;
   int64_t dout_ld = 0;
-  uint16_t* s = nullptr;
-  int64_t s_ld = 0;
-  int64_t d = 0;
+  bool dout_aligned = false;  // every row to 16 bytes
+  Out16 gate, up;
 
   struct Row {};
-  __device__ __forceinline__ Row begin(int64_t) const { return {}; }
-  __device__ __forceinline__ void chunk(Row&, int64_t i, int64_t j, const float (&g)[kChunk],
-                                        const float (&u)[kChunk]) const {
-    float dg[kChunk], du[kChunk], o[kChunk];
-    load_chunk<T>(dout + i * dout_ld, j, d, o);
+  __device__ __forceinline__ Row begin(const Lane&, int64_t) const { return {}; }
+  __device__ __forceinline__ void chunk(Row&, const Lane& l, int64_t i, int64_t j, float (&g)[kChunk],
+                                        float (&u)[kChunk]) const {
+    float o[kChunk] = {};
+    if (l.inside) {
+      const uint16_t* p = dout + i * dout_ld + j;
+      if (dout_aligned && j + kChunk <= gate.n) {
 #pragma unroll
-    for (int k = 0; k < kChunk; ++k) dg[k] = g[k], du[k] = u[k];
-    gated_gradients<T, ACT>(dg, du, o);
-    store_chunk<T>(s + i * s_ld, j, d, dg);
-    store_chunk<T>(s + i * s_ld + d, j, d, du);
+        for (int h = 0; h < kChunk / 8; ++h) {
+          const uint4 q = reinterpret_cast<const uint4*>(p)[h];
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack2<T>(w[k]);
+            o[8 * h + 2 * k] = f.x, o[8 * h + 2 * k + 1] = f.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k)
+          if (j + k < gate.n) o[k] = unpack1<T>(p[k]);
+      }
+    }
+    gated_gradients<ACT>(g, u, o);
+    gate.template store<T>(l, i, j, g);
+    up.template store<T>(l, i, j, u);
   }
-  __device__ __forceinline__ void end(Row&, int64_t, int64_t) const {}
+  __device__ __forceinline__ void end(Row&, const Lane&, int64_t, int64_t) const {}
+  __device__ __forceinline__ void point(int64_t i, int64_t j, float gi, float ui) const {
+    float g[1] = {gi}, u[1] = {ui}, o[1] = {unpack1<T>(dout[i * dout_ld + j])};
+    gated_gradients<ACT>(g, u, o);
+    gate.p[i * gate.ld + j] = pack1<T>(g[0]);
+    up.p[i * up.ld + j] = pack1<T>(u[0]);
+  }
 };
 
-// S from a kept gate_up.  Memory-bound: 14 bytes per output element.
+// S from a kept gate_up.  Memory-bound: 14 bytes per output element; a thread
+// takes V elements of a row, V = 8 where every row of every tensor starts on
+// a 16-byte boundary and d is a multiple of 8.
 struct GatedGradArgs {
   const uint16_t* dout;
   int64_t dout_ld;
@@ -118,18 +119,44 @@ struct GatedGradArgs {
   int64_t rows, d;
 };
 
-template <typename T, int ACT>
+template <typename T, int ACT, int V>
 __global__ void __launch_bounds__(256) gated_grad_rows(GatedGradArgs a) {
   pdl_wait();
-  const int64_t n = a.rows * a.d;
+  const int64_t per_row = a.d / V, n = a.rows * per_row;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n; e += step) {
-    const int64_t i = e / a.d, j = e - i * a.d;
-    const float g = a.gate_up[i * a.gate_up_ld + j], u = a.gate_up[i * a.gate_up_ld + a.d + j];
-    const float o = unpack1<T>(a.dout[i * a.dout_ld + j]);
-    const ActValue v = activate_with_slope<ACT>(g);
-    a.s[i * a.s_ld + j] = pack1<T>(o * u * v.slope);
-    a.s[i * a.s_ld + a.d + j] = pack1<T>(o * v.value);
+    const int64_t i = e / per_row, j = (e - i * per_row) * V;
+    const float* gp = a.gate_up + i * a.gate_up_ld + j;
+    const uint16_t* dp = a.dout + i * a.dout_ld + j;
+    uint16_t* sp = a.s + i * a.s_ld + j;
+    float g[V], u[V], o[V];
+    if constexpr (V == 8) {
+      const uint64_t pol = policy_evict_first();
+      const Vec<16> g0 = ld_stream<16>(gp, pol), g1 = ld_stream<16>(gp + 4, pol);
+      const Vec<16> u0 = ld_stream<16>(gp + a.d, pol), u1 = ld_stream<16>(gp + a.d + 4, pol);
+      const Vec<16> d0 = ld_stream<16>(dp, pol);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        g[k] = __uint_as_float(g0.w[k]), g[k + 4] = __uint_as_float(g1.w[k]);
+        u[k] = __uint_as_float(u0.w[k]), u[k + 4] = __uint_as_float(u1.w[k]);
+        const float2 f = unpack2<T>(d0.w[k]);
+        o[2 * k] = f.x, o[2 * k + 1] = f.y;
+      }
+      gated_gradients<ACT>(g, u, o);
+      Vec<16> sg, su;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        sg.w[k] = pack2<T>(g[2 * k], g[2 * k + 1]);
+        su.w[k] = pack2<T>(u[2 * k], u[2 * k + 1]);
+      }
+      st_global<16>(sp, sg);
+      st_global<16>(sp + a.d, su);
+    } else {
+      g[0] = gp[0], u[0] = gp[a.d], o[0] = unpack1<T>(dp[0]);
+      gated_gradients<ACT>(g, u, o);
+      sp[0] = pack1<T>(g[0]);
+      sp[a.d] = pack1<T>(u[0]);
+    }
   }
 }
 
@@ -183,6 +210,7 @@ int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* 
   Workspace ws(workspace, *workspace_bytes);
   const AlignedRows x(ws, input, rows, hidden, input_row_stride);
   const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride);
+  const PlannedProduct<true, true, true> product(ws, rows, d, hidden);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
@@ -209,9 +237,12 @@ int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* 
   return with_type_and_act(dtype, act, [&](auto t, auto a) {
     using T = decltype(t);
     GatedEpilogue<T, decltype(a)::value> e;
-    e.out = static_cast<uint16_t*>(out), e.ld = out_row_stride, e.d = d;
-    e.gate_up = gate_up, e.gate_up_ld = gate_up_row_stride;
-    return launch_product<T, true, true>(q, e, cs, flags, "gated_linear");
+    e.out = Out16(out, out_row_stride, d);
+    if (gate_up) {
+      e.gate = Out32(gate_up, gate_up_row_stride, d);
+      e.up = Out32(gate_up + d, gate_up_row_stride, d);
+    }
+    return product.launch<T>(q, e, cs, flags, "gated_linear");
   });
 }
 
@@ -235,6 +266,10 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
   const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride);
   const int64_t s_ld = round_up(2 * d, 16);
   uint16_t* s = ws.take<uint16_t>(rows * s_ld);
+  // Without the kept products the first sums are needed again.
+  const PlannedProduct<true, true, true> again(ws, gate_up ? 0 : rows, d, hidden);
+  const PlannedProduct<false, true, false> to_input(ws, rows, hidden, 2 * d);
+  const PlannedProduct<false, false, false> to_weight(ws, 2 * d, hidden, rows);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
@@ -258,17 +293,20 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  const char* what = "gated_linear_backward";
   if (rows > 0 && d > 0) {
     st = with_type_and_act(dtype, act, [&](auto t, auto a) {
       using T = decltype(t);
       constexpr int kAct = decltype(a)::value;
       if (gate_up) {
-        GatedGradArgs g{static_cast<const uint16_t*>(grad_out), grad_out_row_stride, gate_up,
-                        gate_up_row_stride, s, s_ld, rows, d};
-        const int64_t ctas = (rows * d + 1023) / 1024;
-        const int64_t most = 16 * dev->sm_count;
-        return launch_rows(gated_grad_rows<T, kAct>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
-                           dim3(256), cs, flags, "gated_linear_backward", g);
+        const GatedGradArgs g{static_cast<const uint16_t*>(grad_out), grad_out_row_stride, gate_up,
+                              gate_up_row_stride, s, s_ld, rows, d};
+        const bool wide = d % 8 == 0 && tma_rows(grad_out, rows, grad_out_row_stride) &&
+                          aligned(gate_up, 16) && (rows <= 1 || gate_up_row_stride % 4 == 0);
+        const int64_t ctas = (rows * d / (wide ? 8 : 1) + 255) / 256, most = 16 * dev->sm_count;
+        const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most));
+        return wide ? launch_rows(gated_grad_rows<T, kAct, 8>, grid, dim3(256), cs, flags, what, g)
+                    : launch_rows(gated_grad_rows<T, kAct, 1>, grid, dim3(256), cs, flags, what, g);
       }
       Product q;
       q.a = {x.data(), x.ld()};
@@ -276,35 +314,28 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
       q.m = rows, q.n = d, q.depth = hidden, q.pair_offset = d;
       GatedGradEpilogue<T, kAct> e;
       e.dout = static_cast<const uint16_t*>(grad_out), e.dout_ld = grad_out_row_stride;
-      e.s = s, e.s_ld = s_ld, e.d = d;
-      return launch_product<T, true, true>(q, e, cs, flags, "gated_linear_backward");
+      e.dout_aligned = tma_rows(grad_out, rows, grad_out_row_stride);
+      e.gate = Out16(s, s_ld, d), e.up = Out16(s + d, s_ld, d);
+      return again.launch<T>(q, e, cs, flags, what);
     });
     if (st != HPRN_OK) return st;
   }
   // Without rows the weight's gradient is zero, without columns the input's:
-  // sums of depth 0.
+  // sums of no terms.
   auto gradients = [&](auto t) {
     using T = decltype(t);
-    int r = HPRN_OK;
-    if (rows > 0) {
-      Product q;
-      q.a = {s, s_ld};
-      q.b = {w.data(), w.ld()};
-      q.m = rows, q.n = hidden, q.depth = 2 * d;
-      StoreEpilogue<T> e;
-      e.out = static_cast<uint16_t*>(grad_input), e.ld = grad_input_row_stride, e.n = hidden;
-      r = launch_product<T, true, false>(q, e, cs, flags, "gated_linear_backward");
-    }
-    if (r == HPRN_OK && d > 0) {
-      Product q;
-      q.a = {s, s_ld};
-      q.b = {x.data(), x.ld()};
-      q.m = 2 * d, q.n = hidden, q.depth = rows;
-      StoreEpilogue<T> e;
-      e.out = static_cast<uint16_t*>(grad_weight), e.ld = grad_weight_row_stride, e.n = hidden;
-      r = launch_product<T, false, false>(q, e, cs, flags, "gated_linear_backward");
-    }
-    return r;
+    Product q;
+    q.a = {s, s_ld};
+    q.b = {w.data(), w.ld()};
+    q.m = rows, q.n = hidden, q.depth = 2 * d;
+    StoreEpilogue<T> e;
+    e.out = Out16(grad_input, grad_input_row_stride, hidden);
+    const int r = to_input.launch<T>(q, e, cs, flags, what);
+    if (r != HPRN_OK) return r;
+    q.b = {x.data(), x.ld()};
+    q.m = 2 * d, q.depth = rows;
+    e.out = Out16(grad_weight, grad_weight_row_stride, hidden);
+    return to_weight.launch<T>(q, e, cs, flags, what);
   };
   return dtype == HPRN_DTYPE_BF16 ? gradients(__nv_bfloat16{}) : gradients(__half{});
 }

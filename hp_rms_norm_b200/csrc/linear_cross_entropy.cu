@@ -37,77 +37,86 @@ __device__ __forceinline__ int64_t target_of(const int64_t* target, int64_t i, i
   return t == ignore ? kIgnored : (t < 0 || t >= vocab) ? kInvalid : t;
 }
 
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// 2^x (the hardware's approximation, 2 ulp): exponentials are taken to base 2 of
+// logits times log2 e, one fma and this each.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct LossEpilogue {
   static constexpr bool kPaired = false;
-  float2* partial = nullptr;  // [tiles, rows]: {max, sum of exp(l - max)}
+  float2* partial = nullptr;  // [rows, parts]: {max of l log2 e, sum of 2^(l log2 e - max)}
   float* target_logit = nullptr;
   const int64_t* target = nullptr;
   int64_t ignore = 0;
-  int64_t rows = 0;
+  int64_t parts = 0;
   int64_t vocab = 0;
 
   struct Row {
     float m, s;
     int64_t t;
   };
-  __device__ __forceinline__ Row begin(int64_t i) const {
-    return Row{-INFINITY, 0.f, target_of(target, i, ignore, vocab)};
+  __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const {
+    return Row{-INFINITY, 0.f, l.inside ? target_of(target, i, ignore, vocab) : kIgnored};
   }
-  __device__ __forceinline__ void chunk(Row& r, int64_t i, int64_t j, const float (&v)[kChunk]) const {
-    const int64_t left = vocab - j;
-    float m = r.m;
+  __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
+    if (j + kChunk > vocab) {
+      const int left = static_cast<int>(vocab - j);
 #pragma unroll
-    for (int k = 0; k < kChunk; ++k)
-      if (k < left) m = fmaxf(m, v[k]);
-    // All so far -inf (or NaN, which fmaxf skips and the sum keeps): exp(-inf - 0) = 0.
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = r.s * expf(r.m - ref);
-#pragma unroll
-    for (int k = 0; k < kChunk; ++k)
-      if (k < left) s += expf(v[k] - ref);
-    r.m = m, r.s = s;
-    if (r.t >= j && r.t < j + kChunk) {
+      for (int k = 0; k < kChunk; ++k)
+        if (k >= left) v[k] = -INFINITY;
+    }
+    const int64_t at = r.t - j;
+    if (at >= 0 && at < kChunk) {
       float x = 0.f;
 #pragma unroll
-      for (int k = 0; k < kChunk; ++k) x = r.t == j + k ? v[k] : x;
+      for (int k = 0; k < kChunk; ++k) x = at == k ? v[k] : x;
       target_logit[i] = x;
     }
+    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int k = 4; k < kChunk; ++k) top[k % 4] = fmaxf(top[k % 4], v[k]);
+    const float m = fmaxf(r.m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * kLog2e);
+    // All so far -inf (or NaN, which fmaxf skips and the sum keeps): 2^(-inf - 0) = 0.
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s[4] = {r.s * exp2_fast(r.m - ref), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) s[k % 4] += exp2_fast(fmaf(v[k], kLog2e, -ref));
+    r.m = m, r.s = (s[0] + s[1]) + (s[2] + s[3]);
   }
-  __device__ __forceinline__ void end(Row& r, int64_t i, int64_t tile) const {
-    partial[tile * rows + i] = make_float2(r.m, r.s);
+  __device__ __forceinline__ void end(Row& r, const Lane& l, int64_t i, int64_t part) const {
+    if (l.inside) partial[i * parts + part] = make_float2(r.m, r.s);
   }
 };
 
-// Joins a row's tiles: one warp-sized group of threads per row would read the
-// partials of a row `rows` apart, so threads of a CTA take neighbouring rows
-// and the CTA's y groups take tiles in turn.
-constexpr int kJoinRows = 32;
-constexpr int kJoinGroups = 8;
-
-__global__ void __launch_bounds__(kJoinRows* kJoinGroups)
-    loss_join(const float2* partial, const float* target_logit, const int64_t* target,
-              int64_t ignore, int64_t rows, int64_t vocab, int64_t tiles, float* loss, float* lse) {
-  __shared__ float2 part[kJoinGroups][kJoinRows];
+// Joins a row's parts, one warp a row.
+__global__ void __launch_bounds__(256)
+    loss_join(const float2* partial, const float* target_logit, const int64_t* target, int64_t ignore,
+              int64_t rows, int64_t vocab, int64_t parts, float* loss, float* lse) {
   pdl_wait();
-  const int tx = threadIdx.x, ty = threadIdx.y;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kJoinRows + tx;
+  const int lane = threadIdx.x % 32;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  if (i >= rows) return;
   float m = -INFINITY, s = 0.f;
-  auto join = [](float& m, float& s, float2 p) {
+  auto join = [&](float2 p) {
     const float top = fmaxf(m, p.x);
     const float ref = top == -INFINITY ? 0.f : top;
-    s = s * expf(m - ref) + p.y * expf(p.x - ref);
+    s = s * exp2_fast(m - ref) + p.y * exp2_fast(p.x - ref);
     m = top;
   };
-  if (i < rows)
-    for (int64_t t = ty; t < tiles; t += kJoinGroups) join(m, s, partial[t * rows + i]);
-  part[ty][tx] = make_float2(m, s);
-  __syncthreads();
-  if (ty != 0 || i >= rows) return;
-  for (int g = 1; g < kJoinGroups; ++g) join(m, s, part[g][tx]);
-  const float l = (m == -INFINITY ? 0.f : m) + logf(s);
+  for (int64_t k = lane; k < parts; k += 32) join(partial[i * parts + k]);
+  for (int o = 16; o > 0; o >>= 1)
+    join(make_float2(__shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o)));
+  if (lane != 0) return;
+  if (parts == 0 && vocab > 0) m = 0.f, s = static_cast<float>(vocab);  // sums of no terms: logits 0
+  const float l = (m == -INFINITY ? 0.f : m * kLn2) + logf(s);
   lse[i] = l;
   const int64_t t = target_of(target, i, ignore, vocab);
-  loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - target_logit[i];
+  loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - (parts > 0 ? target_logit[i] : 0.f);
 }
 
 // {factor, 1 / factor}: the power of two S is held times.
@@ -137,8 +146,7 @@ __global__ void __launch_bounds__(1024) loss_grad_scale(const float* grad_loss, 
 template <typename T>
 struct LossGradEpilogue {
   static constexpr bool kPaired = false;
-  uint16_t* s = nullptr;
-  int64_t ld = 0;
+  Out16 s;  // the piece's columns
   const float* lse = nullptr;
   const float* grad_loss = nullptr;
   const float* factor = nullptr;  // or null for 1
@@ -146,32 +154,36 @@ struct LossGradEpilogue {
   int64_t ignore = 0;
   int64_t vocab = 0;
   int64_t first = 0;  // the piece's first column
-  int64_t cols = 0;   // the piece's columns
 
   struct Row {
-    float c, lse;
-    int64_t t;  // within the piece (or past its end); kInvalid before it
+    float c, lse2;
+    int64_t t;  // within the piece (or outside it)
   };
-  __device__ __forceinline__ Row begin(int64_t i) const {
-    const int64_t t = target_of(target, i, ignore, vocab);
-    float c = grad_loss[i] * (factor ? *factor : 1.f);
+  __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const {
+    const int64_t t = l.inside ? target_of(target, i, ignore, vocab) : kIgnored;
+    if (t == kIgnored) return Row{0.f, INFINITY, kIgnored};
     // A target outside the vocabulary has no loss: NaN, like the loss itself.
-    c = t == kInvalid ? __int_as_float(0x7fc00000) : c;
-    return Row{c, lse[i], t == kIgnored ? kIgnored : t >= first ? t - first : kInvalid};
+    const float c = t == kInvalid ? __int_as_float(0x7fc00000) : grad_loss[i] * (factor ? *factor : 1.f);
+    return Row{c, lse[i] * kLog2e, t >= first ? t - first : kInvalid};
   }
-  __device__ __forceinline__ void chunk(Row& r, int64_t i, int64_t j, const float (&v)[kChunk]) const {
-    float g[kChunk];
+  __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
+    const int64_t at = r.t - j;
+    const bool here = at >= 0 && at < kChunk;
     if (r.t == kIgnored) {
 #pragma unroll
-      for (int k = 0; k < kChunk; ++k) g[k] = 0.f;
+      for (int k = 0; k < kChunk; ++k) v[k] = 0.f;
     } else {
 #pragma unroll
-      for (int k = 0; k < kChunk; ++k)
-        g[k] = r.c * (expf(v[k] - r.lse) - (r.t == j + k ? 1.f : 0.f));
+      for (int k = 0; k < kChunk; ++k) v[k] = r.c * exp2_fast(fmaf(v[k], kLog2e, -r.lse2));
+      if (here) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k)
+          if (at == k) v[k] -= r.c;
+      }
     }
-    store_chunk<T>(s + i * ld, j, cols, g);
+    s.template store<T>(l, i, j, v);
   }
-  __device__ __forceinline__ void end(Row&, int64_t, int64_t) const {}
+  __device__ __forceinline__ void end(Row&, const Lane&, int64_t, int64_t) const {}
 };
 
 namespace {
@@ -222,12 +234,9 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   Workspace ws(workspace, *workspace_bytes);
   const AlignedRows x(ws, input, rows, hidden, input_row_stride);
   const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride);
-  Product q;
-  q.a = {x.data(), x.ld()};
-  q.b = {w.data(), w.ld()};
-  q.m = rows, q.n = vocab, q.depth = hidden;
-  const int64_t tiles = product_tiles<LossEpilogue>(q);
-  float2* partial = ws.take<float2>(tiles * rows);
+  const PlannedProduct<false, true, true> product(ws, rows, vocab, hidden, false);
+  const int64_t parts = product.parts(vocab);
+  float2* partial = ws.take<float2>(parts * rows);
   float* target_logit = ws.take<float>(rows);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
@@ -250,17 +259,20 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_cross_entropy";
   if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
-  if (vocab > 0) {
-    LossEpilogue e;
-    e.partial = partial, e.target_logit = target_logit, e.target = target;
-    e.ignore = ignore_index, e.rows = rows, e.vocab = vocab;
-    st = dtype == HPRN_DTYPE_BF16 ? launch_product<__nv_bfloat16, true, true>(q, e, cs, flags, what)
-                                  : launch_product<__half, true, true>(q, e, cs, flags, what);
+  Product q;
+  q.a = {x.data(), x.ld()};
+  q.b = {w.data(), w.ld()};
+  q.m = rows, q.n = vocab, q.depth = hidden;
+  LossEpilogue e;
+  e.partial = partial, e.target_logit = target_logit, e.target = target;
+  e.ignore = ignore_index, e.parts = parts, e.vocab = vocab;
+  if (hidden > 0) {
+    st = dtype == HPRN_DTYPE_BF16 ? product.launch_whole<__nv_bfloat16>(q, e, cs, flags, what)
+                                  : product.launch_whole<__half>(q, e, cs, flags, what);
     if (st != HPRN_OK) return st;
   }
-  return launch_rows(loss_join, dim3(static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows)),
-                     dim3(kJoinRows, kJoinGroups), cs, flags, what, partial, target_logit, target,
-                     ignore_index, rows, vocab, vocab > 0 ? tiles : 0, loss, lse);
+  return launch_rows(loss_join, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), cs, flags, what,
+                     partial, target_logit, target, ignore_index, rows, vocab, hidden > 0 ? parts : 0, loss, lse);
 }
 
 int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, const float* grad_loss,
@@ -281,8 +293,12 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride);
   const Pieces pieces = pieces_of(rows, vocab);
   uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
-  float* sum = pieces.count > 1 ? ws.take<float>(rows * hidden) : nullptr;
+  const int64_t sum_ld = round_up(hidden, kChunk);
+  float* sum = pieces.count > 1 ? ws.take<float>(rows * sum_ld) : nullptr;
   float* factor = dtype == HPRN_DTYPE_FP16 ? ws.take<float>(2) : nullptr;
+  const PlannedProduct<false, true, true> logits(ws, rows, pieces.cols, hidden, false);
+  const PlannedProduct<false, true, false> to_input(ws, rows, hidden, pieces.cols);
+  const PlannedProduct<false, false, false> to_weight(ws, pieces.cols, hidden, rows);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
@@ -320,38 +336,30 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
     for (int64_t p = 0; p < count && r == HPRN_OK; ++p) {
       const int64_t first = p * pieces.cols;
       const int64_t cols = vocab - first < pieces.cols ? vocab - first : pieces.cols;
-      if (rows > 0 && cols > 0) {
-        Product q;
-        q.a = {x.data(), x.ld()};
-        q.b = {w.data() + first * w.ld(), w.ld()};
-        q.m = rows, q.n = cols, q.depth = hidden;
-        LossGradEpilogue<T> e;
-        e.s = s, e.ld = pieces.cols, e.lse = lse, e.grad_loss = grad_loss, e.factor = factor;
-        e.target = target, e.ignore = ignore_index, e.vocab = vocab, e.first = first, e.cols = cols;
-        if ((r = launch_product<T, true, true>(q, e, cs, flags, what)) != HPRN_OK) break;
-      }
-      if (rows > 0) {
-        Product q;
-        q.a = {s, pieces.cols};
-        q.b = {w.data() + first * w.ld(), w.ld()};
-        q.m = rows, q.n = hidden, q.depth = cols;
-        StoreEpilogue<T> e;
-        e.out = static_cast<uint16_t*>(grad_input), e.ld = grad_input_row_stride, e.n = hidden;
-        e.sum = sum, e.first = p == 0, e.last = p == count - 1;
-        e.scale = factor ? factor + 1 : nullptr;
-        if ((r = launch_product<T, true, false>(q, e, cs, flags, what)) != HPRN_OK) break;
-      }
-      if (cols > 0) {
-        Product q;
-        q.a = {s, pieces.cols};
-        q.b = {x.data(), x.ld()};
-        q.m = cols, q.n = hidden, q.depth = rows;
-        StoreEpilogue<T> e;
-        e.out = static_cast<uint16_t*>(grad_weight) + first * grad_weight_row_stride;
-        e.ld = grad_weight_row_stride, e.n = hidden;
-        e.scale = factor && rows > 0 ? factor + 1 : nullptr;
-        r = launch_product<T, false, false>(q, e, cs, flags, what);
-      }
+      const uint16_t* wp = w.data() + first * w.ld();
+      Product q;
+      q.a = {x.data(), x.ld()};
+      q.b = {wp, w.ld()};
+      q.m = rows, q.n = cols, q.depth = hidden;
+      LossGradEpilogue<T> g;
+      g.s = Out16(s, pieces.cols, cols), g.lse = lse, g.grad_loss = grad_loss, g.factor = factor;
+      g.target = target, g.ignore = ignore_index, g.vocab = vocab, g.first = first;
+      if ((r = logits.launch_whole<T>(q, g, cs, flags, what)) != HPRN_OK) break;
+
+      q.a = {s, pieces.cols};
+      q.n = hidden, q.depth = cols;
+      StoreEpilogue<T> e;
+      e.out = Out16(grad_input, grad_input_row_stride, hidden);
+      e.sum = sum, e.sum_ld = sum_ld, e.first = p == 0, e.last = p == count - 1;
+      e.scale = factor && rows > 0 ? factor + 1 : nullptr;
+      if ((r = to_input.launch<T>(q, e, cs, flags, what)) != HPRN_OK) break;
+
+      q.b = {x.data(), x.ld()};
+      q.m = cols, q.depth = rows;
+      e.out = Out16(static_cast<uint16_t*>(grad_weight) + first * grad_weight_row_stride,
+                    grad_weight_row_stride, hidden);
+      e.sum = nullptr, e.first = e.last = true;
+      r = to_weight.launch<T>(q, e, cs, flags, what);
     }
     return r;
   };

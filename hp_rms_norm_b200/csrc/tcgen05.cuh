@@ -41,6 +41,21 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// A whole warp waits; the answer is the same in every lane, which lets the
+// compiler keep what depends on it in uniform registers.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, uint64_t limit_ns = kWaitLimitNs) {
+  return __all_sync(~0u, mbar_wait_bounded(bar, parity, limit_ns));
+}
+
 // ---------------------------------------------------------------------------
 // Tiled TMA load of one box: coordinates in elements, x along the contiguous
 // dimension; elements outside the tensor arrive as zeros and count as bytes.
