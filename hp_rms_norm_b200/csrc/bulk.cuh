@@ -45,6 +45,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
                : "memory");
 }
 
+// One arrival on a barrier of this CTA.
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // `bytes` from global `src` into this CTA's shared memory at `dst`; completes
 // as transaction bytes on `bar`.  L2 policy `pol` (evict_first for streamed rows).
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,

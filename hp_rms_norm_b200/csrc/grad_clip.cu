@@ -4,16 +4,17 @@
 //
 // The tensors' addresses, sizes and types travel as a kernel parameter (no
 // copy to the device, so the calls can be captured in a CUDA graph), up to
-// kMaxTensors a launch.  Every tensor is cut into chunks of kChunkElems
-// elements; a chunk's CTA finds its tensor by bisection over the first-chunk
-// numbers.  A chunk's squares are summed in fp32 (at most kChunkElems / threads
-// in a row per thread), the chunks' sums in fp64, in an order that depends on
-// the sizes alone, so the norm repeats bit for bit.
+// kMaxTensors a launch.  Every tensor is cut into chunks; a chunk's CTA finds
+// its tensor by bisection over the first-chunk numbers.  A chunk's squares are
+// summed in fp32 (eight sums a thread, at most 32 terms each), the chunks' sums
+// in fp64, in an order that depends on the sizes and alignments alone, so the
+// norm repeats bit for bit.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "runtime.cuh"
 #include "vec.cuh"
@@ -21,8 +22,16 @@
 namespace hprn {
 
 constexpr int kMaxTensors = 400;
-constexpr int64_t kChunkElems = 16384;
 constexpr int kClipThreads = 256;
+// Elements of a chunk: as many as give every SM some 8 chunks, within bounds
+// that keep a chunk's work above its start (looking up its tensor; 4096
+// elements took 5.8 us where 16384 take 4.1 on 3.5 million) and a large model's
+// chunks short enough to end together.
+constexpr int64_t kLeastChunk = 16384, kMostChunk = 65536;
+inline int64_t chunk_elems(int64_t total) {
+  const int64_t c = round_up(total / (148 * 8) + 1, 2048);
+  return c < kLeastChunk ? kLeastChunk : c > kMostChunk ? kMostChunk : c;
+}
 
 struct GradEntry {
   const void* in;
@@ -36,6 +45,7 @@ struct GradEntry {
 
 struct GradTable {
   GradEntry t[kMaxTensors];
+  int64_t chunk;  // elements
   int32_t n;
 };
 
@@ -49,30 +59,125 @@ __device__ __forceinline__ const GradEntry& find_entry(const GradTable& g, int64
   return g.t[lo];
 }
 
-__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
-  if (type == HPRN_DTYPE_FP32) return static_cast<const float*>(p)[i];
-  const uint16_t h = static_cast<const uint16_t*>(p)[i];
-  return type == HPRN_DTYPE_BF16 ? unpack1<__nv_bfloat16>(h) : unpack1<__half>(h);
+// Element types by hprn_dtype.
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<HPRN_DTYPE_BF16> {
+  using Raw = uint16_t;
+  static constexpr int kVec = 8;  // elements of a 16-byte vector
+  static __device__ __forceinline__ float get(Raw r) { return unpack1<__nv_bfloat16>(r); }
+  static __device__ __forceinline__ Raw put(float f) { return pack1<__nv_bfloat16>(f); }
+};
+template <>
+struct Elem<HPRN_DTYPE_FP16> {
+  using Raw = uint16_t;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float get(Raw r) { return unpack1<__half>(r); }
+  static __device__ __forceinline__ Raw put(float f) { return pack1<__half>(f); }
+};
+template <>
+struct Elem<HPRN_DTYPE_FP32> {
+  using Raw = float;
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ float get(Raw r) { return r; }
+  static __device__ __forceinline__ Raw put(float f) { return f; }
+};
+
+// Calls f(integral_constant<type>) for the type code.
+template <typename F>
+__device__ __forceinline__ void with_type(int type, F&& f) {
+  if (type == HPRN_DTYPE_BF16) f(std::integral_constant<int, HPRN_DTYPE_BF16>{});
+  else if (type == HPRN_DTYPE_FP16) f(std::integral_constant<int, HPRN_DTYPE_FP16>{});
+  else f(std::integral_constant<int, HPRN_DTYPE_FP32>{});
 }
 
-__device__ __forceinline__ void store_from_f32(void* p, int64_t i, int type, float v) {
-  if (type == HPRN_DTYPE_FP32) static_cast<float*>(p)[i] = v;
-  else static_cast<uint16_t*>(p)[i] = type == HPRN_DTYPE_BF16 ? pack1<__nv_bfloat16>(v) : pack1<__half>(v);
+// Eight elements as two or one 16-byte vectors.
+template <int TYPE>
+__device__ __forceinline__ void load8(const typename Elem<TYPE>::Raw* p, float (&v)[8]) {
+  if constexpr (TYPE == HPRN_DTYPE_FP32) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    using T = typename std::conditional<TYPE == HPRN_DTYPE_BF16, __nv_bfloat16, __half>::type;
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = unpack2<T>(w[k]);
+      v[2 * k] = f.x, v[2 * k + 1] = f.y;
+    }
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store8(typename Elem<TYPE>::Raw* p, const float (&v)[8]) {
+  if constexpr (TYPE == HPRN_DTYPE_FP32) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+  } else {
+    using T = typename std::conditional<TYPE == HPRN_DTYPE_BF16, __nv_bfloat16, __half>::type;
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                                   pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])));
+  }
+}
+
+// Elements before p's next 16-byte boundary.
+template <int TYPE>
+__device__ __forceinline__ int64_t ahead(const typename Elem<TYPE>::Raw* p) {
+  return static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(*p);
+}
+
+// Where element k of a tensor lies.
+__device__ __forceinline__ int64_t place(int64_t k, int64_t cols, int64_t stride) {
+  return stride == cols ? k : k / cols * stride + k % cols;
+}
+
+// A contiguous chunk is read in groups of eight elements from the first
+// 16-byte boundary on, four groups in flight a thread; its ends one by one.
+constexpr int kInFlight = 4;
+
+template <int TYPE>
+__device__ __forceinline__ float chunk_squares(const GradEntry& e, int64_t lo, int64_t hi) {
+  using Raw = typename Elem<TYPE>::Raw;
+  const Raw* p = static_cast<const Raw*>(e.in);
+  float s[8] = {};
+  auto one = [&](int64_t k) {
+    const float v = Elem<TYPE>::get(p[place(k, e.cols, e.in_stride)]);
+    s[0] = fmaf(v, v, s[0]);
+  };
+  if (e.in_stride != e.cols) {
+    for (int64_t k = lo + threadIdx.x; k < hi; k += kClipThreads) one(k);
+    return s[0];
+  }
+  const int64_t first = min(lo + ahead<TYPE>(p + lo), hi), groups = (hi - first) / 8;
+  for (int64_t g = threadIdx.x; g < groups; g += kClipThreads * kInFlight) {
+    float v[kInFlight][8];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (g + u * kClipThreads < groups) load8<TYPE>(p + first + (g + u * kClipThreads) * 8, v[u]);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (g + u * kClipThreads < groups) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = fmaf(v[u][k], v[u][k], s[k]);
+      }
+  }
+  for (int64_t k = lo + threadIdx.x; k < first; k += kClipThreads) one(k);
+  for (int64_t k = first + groups * 8 + threadIdx.x; k < hi; k += kClipThreads) one(k);
+  return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
 __global__ void __launch_bounds__(kClipThreads) grad_square_sums(const __grid_constant__ GradTable g,
                                                                  float* partial) {
   __shared__ float part[kClipThreads / 32];
-  pdl_wait();
   const GradEntry& e = find_entry(g, blockIdx.x);
-  const int64_t lo = (blockIdx.x - e.first_chunk) * kChunkElems;
-  const int64_t hi = min(lo + kChunkElems, e.count);
+  const int64_t lo = (blockIdx.x - e.first_chunk) * g.chunk;
+  const int64_t hi = min(lo + g.chunk, e.count);
+  pdl_wait();
   float s = 0.f;
-  for (int64_t k = lo + threadIdx.x; k < hi; k += kClipThreads) {
-    const int64_t at = e.in_stride == e.cols ? k : k / e.cols * e.in_stride + k % e.cols;
-    const float v = load_as_f32(e.in, at, e.in_type);
-    s = fmaf(v, v, s);
-  }
+  with_type(e.in_type, [&](auto t) { s = chunk_squares<decltype(t)::value>(e, lo, hi); });
+  pdl_trigger();
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
   __syncthreads();
@@ -85,7 +190,9 @@ __global__ void __launch_bounds__(kClipThreads) grad_square_sums(const __grid_co
 __global__ void __launch_bounds__(1024) grad_norm_join(const float* partial, int64_t n, float* norm) {
   __shared__ double part[32];
   pdl_wait();
+  pdl_trigger();
   double s = 0.0;
+#pragma unroll 8
   for (int64_t k = threadIdx.x; k < n; k += 1024) s += static_cast<double>(partial[k]);
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
@@ -96,21 +203,54 @@ __global__ void __launch_bounds__(1024) grad_norm_join(const float* partial, int
   if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
 }
 
+template <int IN, int OUT>
+__device__ __forceinline__ void chunk_scale(const GradEntry& e, int64_t lo, int64_t hi, float f) {
+  using RawIn = typename Elem<IN>::Raw;
+  using RawOut = typename Elem<OUT>::Raw;
+  const RawIn* p = static_cast<const RawIn*>(e.in);
+  RawOut* q = static_cast<RawOut*>(e.out);
+  auto one = [&](int64_t k) {
+    q[place(k, e.cols, e.out_stride)] = Elem<OUT>::put(Elem<IN>::get(p[place(k, e.cols, e.in_stride)]) * f);
+  };
+  const int64_t first = min(lo + ahead<IN>(p + lo), hi);
+  if (e.in_stride != e.cols || e.out_stride != e.cols || (reinterpret_cast<uintptr_t>(q + first) & 15) != 0) {
+    for (int64_t k = lo + threadIdx.x; k < hi; k += kClipThreads) one(k);
+    return;
+  }
+  const int64_t groups = (hi - first) / 8;
+  for (int64_t g = threadIdx.x; g < groups; g += kClipThreads * kInFlight) {
+    float v[kInFlight][8];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (g + u * kClipThreads < groups) load8<IN>(p + first + (g + u * kClipThreads) * 8, v[u]);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (g + u * kClipThreads < groups) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[u][k] *= f;
+        store8<OUT>(q + first + (g + u * kClipThreads) * 8, v[u]);
+      }
+  }
+  for (int64_t k = lo + threadIdx.x; k < first; k += kClipThreads) one(k);
+  for (int64_t k = first + groups * 8 + threadIdx.x; k < hi; k += kClipThreads) one(k);
+}
+
+// The chunks are taken last to first: the norm's pass read the last ones last,
+// so they are the ones L2 still holds.
 __global__ void __launch_bounds__(kClipThreads) grad_scale(const __grid_constant__ GradTable g,
                                                            const float* norm, float max_norm) {
+  const int64_t chunk = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
+  const GradEntry& e = find_entry(g, chunk);
+  const int64_t lo = (chunk - e.first_chunk) * g.chunk;
+  const int64_t hi = min(lo + g.chunk, e.count);
   pdl_wait();
   // min(1, .) written so that a NaN norm gives a NaN factor.
-  const float q = max_norm / (*norm + 1e-6f);
-  const float f = q >= 1.f ? 1.f : q;
-  const GradEntry& e = find_entry(g, blockIdx.x);
+  const float r = max_norm / (*norm + 1e-6f);
+  const float f = r >= 1.f ? 1.f : r;
   if (f == 1.f && e.in == e.out) return;  // in place, and nothing to change
-  const int64_t lo = (blockIdx.x - e.first_chunk) * kChunkElems;
-  const int64_t hi = min(lo + kChunkElems, e.count);
-  for (int64_t k = lo + threadIdx.x; k < hi; k += kClipThreads) {
-    const int64_t at = e.in_stride == e.cols ? k : k / e.cols * e.in_stride + k % e.cols;
-    const int64_t to = e.out_stride == e.cols ? k : k / e.cols * e.out_stride + k % e.cols;
-    store_from_f32(e.out, to, e.out_type, load_as_f32(e.in, at, e.in_type) * f);
-  }
+  with_type(e.in_type, [&](auto in) {
+    with_type(e.out_type, [&](auto out) { chunk_scale<decltype(in)::value, decltype(out)::value>(e, lo, hi, f); });
+  });
 }
 
 namespace {
@@ -147,18 +287,22 @@ int check_grads(const hprn_grad* g, int64_t count, bool with_out) {
   return HPRN_OK;
 }
 
-int64_t chunks_of(const hprn_grad& e) {
-  return e.rows == 0 || e.cols == 0 ? 0 : (e.rows * e.cols + kChunkElems - 1) / kChunkElems;
+int64_t total_of(const hprn_grad* g, int64_t count) {
+  int64_t n = 0;
+  for (int64_t k = 0; k < count; ++k) n += g[k].rows * g[k].cols;
+  return n;
 }
+int64_t chunks_of(const hprn_grad& e, int64_t chunk) { return (e.rows * e.cols + chunk - 1) / chunk; }
 
 // Calls f(table, chunks) for every launch's worth of tensors.
 template <typename F>
 int for_tables(const hprn_grad* g, int64_t count, F&& f) {
   GradTable table;
   table.n = 0;
+  table.chunk = chunk_elems(total_of(g, count));
   int64_t chunks = 0;
   for (int64_t k = 0; k < count; ++k) {
-    const int64_t c = chunks_of(g[k]);
+    const int64_t c = chunks_of(g[k], table.chunk);
     if (c == 0) continue;
     if (c > 2147483647) return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor too large");
     if (table.n == kMaxTensors || chunks + c > 2147483647) {
@@ -191,8 +335,9 @@ int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* wor
   if (!workspace_bytes) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace_bytes pointer required");
   int st = check_grads(grads, count, false);
   if (st != HPRN_OK) return st;
+  const int64_t chunk = chunk_elems(total_of(grads, count));
   int64_t total = 0;
-  for (int64_t k = 0; k < count; ++k) total += chunks_of(grads[k]);
+  for (int64_t k = 0; k < count; ++k) total += chunks_of(grads[k], chunk);
   Workspace ws(workspace, *workspace_bytes);
   float* partial = ws.take<float>(total);
   if (flags & HPRN_WORKSPACE_QUERY) {

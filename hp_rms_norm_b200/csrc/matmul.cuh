@@ -566,11 +566,6 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // Host side.
 
-// TMA reads rows that start on 16-byte boundaries.
-inline bool tma_rows(const void* p, int64_t rows, int64_t ld) {
-  return aligned(p, 16) && (rows <= 1 || ld % 8 == 0);
-}
-
 // A [rows, cols] operand TMA can read: the tensor itself, or a copy of it with
 // aligned rows taken from the workspace.
 class AlignedRows {
@@ -614,10 +609,6 @@ Tiling choose_tiling(const TilingQuery& q);
 // The tensor map of `rows` x `cols` 16-bit elements, boxes of box_rows x 64.
 int encode_rows(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows,
                 const char* what);
-// The counter of waits that ran out, on the current device.
-int timeout_counter(unsigned** out);
-// Raises a kernel's dynamic shared memory limit, once per device.
-int allow_smem(const DeviceInfo* dev, const void* fn, int bytes, const char* what);
 
 // A product with its tiling and, where its sums are split, the workspace for
 // the shares.  kAKMajor / kBKMajor: how the operands lie.

@@ -8,11 +8,18 @@
 // dx is the gradient of both the input and the residual.
 //
 // All sums are fp32; dx and dw are rounded to 16 bits once.
+//
+// Memory-bound: x, D (and E) in, dx out, 6 (8) bytes per element.  norm_grad_rows
+// reads them once: rows wait in shared memory, several deep, between memory
+// and the two passes over them; dw's sums over a CTA's rows stay in registers,
+// and the CTAs' sums are joined by a second kernel.  Rows too long for that
+// (see norm_grad_plan) are read twice, by norm_grad_stats and norm_grad_columns.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <string>
 
+#include "bulk.cuh"
 #include "runtime.cuh"
 #include "vec.cuh"
 
@@ -29,28 +36,336 @@ struct NormGradArgs {
   int64_t dx_stride, dy_stride, x_stride, extra_stride;
   float eps;
   float2* stats;   // per row: {inv, mean_k(w_k D_k n_k)}
-  float* partial;  // [groups, hidden]: dw's sums over a group's rows
+  float* partial;  // [groups, partial_ld]: dw's sums over a group's rows
+  int64_t partial_ld;
   int64_t groups;
+  int row_threads, row_groups, slots;  // of norm_grad_rows
+  bool weight_staged;                  // in shared memory
+  bool dense;                          // every tensor's rows follow each other
+  unsigned* timeouts;
 };
 
-__device__ __forceinline__ float2 block_sum(float2 v) {
-  __shared__ float2 part[32];
-  const int warps = blockDim.x / 32;
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(~0u, v.x, o);
-    v.y += __shfl_xor_sync(~0u, v.y, o);
+// Both of a pair's sums over a warp: the lower half warp adds up .x, the upper
+// .y, one shuffle a step instead of two.  The lower lanes return the sum of .x,
+// the upper ones that of .y.
+__device__ __forceinline__ float half_sum(float v) {
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_halves(float2 v) {
+  const bool lower = threadIdx.x % 32 < 16;
+  const float mine = lower ? v.x : v.y, other = lower ? v.y : v.x;
+  return half_sum(mine + __shfl_xor_sync(~0u, other, 16));
+}
+
+__device__ __forceinline__ void group_barrier(int barrier, int warps) {
+  if (warps == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+}
+
+// Both sums over the `warps` (at most 32) warps from `first_warp` that hold a
+// row, which meet at hardware barrier `barrier`.  `part` is one of two buffers that calls
+// alternate between, so one barrier a call is enough.
+__device__ __forceinline__ float2 row_sum2(float2 v, float (*part)[32], int warp, int warps, int barrier,
+                                           int first_warp) {
+  const int lane = threadIdx.x % 32;
+  float s = warp_halves(v);
+  if (warps > 1) {
+    if (lane % 16 == 0) part[lane / 16][warp] = s;
+    group_barrier(barrier, warps);
+    const int k = lane % 16;
+    s = k < warps ? part[lane / 16][first_warp + k] : 0.f;
+    if (k + 16 < warps) s += part[lane / 16][first_warp + k + 16];
+    s = half_sum(s);
+  } else {
+    __syncwarp();
   }
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+  return make_float2(__shfl_sync(~0u, s, 0), __shfl_sync(~0u, s, 16));
+}
+
+constexpr int kMostRowGroups = 16;
+constexpr int kMostSlots = 4;
+
+__device__ __forceinline__ void lds4(uint32_t (&w)[4], uint32_t addr) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void sts4(uint32_t addr, const uint32_t (&w)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+
+// A CTA is `groups` groups of `row_threads` threads, and one warp more; a group
+// works on one row at a time, each thread on the same W / 4 vectors of eight
+// elements of every row.  A group's rows arrive in a ring of `slots` row
+// buffers in shared memory.  Where every row of every tensor starts on a
+// 16-byte boundary and hidden is a multiple of 8 (kBulk) the extra warp keeps
+// the ring filled by bulk copies, a round's neighbouring rows in one where they
+// follow each other; else the group copies its next rows itself, element by
+// element.
+//
+// Registers hold dw's sums (2 W floats) and, up to 16 words, w D between the
+// two passes.  4096 x 8192 with E: 48.0 us (0.87 of a copy of the same bytes),
+// against 55.8 with the rows themselves in registers, which spilled or kept
+// one row a CTA in flight.
+//
+// A wait that runs out (mbar_wait_bounded) ends its group after the copies
+// still in flight, counted in `timeouts`; the rows it had not finished keep
+// their dx.
+constexpr int kNormThreads = 512;
+
+template <typename T, int W, bool EXTRA, bool kBulk>
+__global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradArgs a) {
+  constexpr int kVecs = W / 4;
+  constexpr int kTensors = EXTRA ? 3 : 2;
+  constexpr bool kHold = W <= 16;
+  extern __shared__ __align__(128) unsigned char row_mem[];
+  __shared__ __align__(8) uint64_t full[kMostSlots], empty[kMostSlots];
+  __shared__ float part[2][2][32];  // a group's warps follow those of the groups before it
+  __shared__ int gave_up[kMostRowGroups];
+  const int tid = threadIdx.x, row_threads = a.row_threads, groups = a.row_groups;
+  const int workers = groups * row_threads;
+  const bool copier = tid >= workers;
+  const int group = copier ? tid - workers : tid / row_threads, in = copier ? 0 : tid - group * row_threads;
+  const int warps = row_threads / 32, barrier = 1 + group;
+  const int hidden = static_cast<int>(a.hidden), nvec = (hidden + 7) / 8;
+  // A slot: `groups` rows of x, then of D, then of E.
+  const uint32_t row_bytes = static_cast<uint32_t>(nvec) * 16, tensor_bytes = row_bytes * groups;
+  const uint32_t slot_bytes = tensor_bytes * kTensors;
+  const uint32_t w_row = smem_u32(row_mem);
+  unsigned char* slots_p = row_mem + (a.weight_staged ? row_bytes : 0);
+  unsigned char* ring_p = slots_p + group * row_bytes;
+  const uint32_t ring = smem_u32(ring_p);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * groups + group;
+  const uint64_t pol = policy_evict_first();
+  // The tensors' rows `i`, in a slot's order.
+  auto row_of = [&](int t, int64_t i) {
+    return t == 0 ? a.x + i * a.x_stride : t == 1 ? a.dy + i * a.dy_stride : a.extra + i * a.extra_stride;
+  };
+  // A row element by element: pairs, eight a thread in flight.
+  auto copy_row = [&](unsigned char* to, const uint16_t* p) {
+    uint32_t* q = reinterpret_cast<uint32_t*>(to);
+    const int pairs = nvec * 4;
+    for (int j0 = in; j0 < pairs; j0 += 8 * row_threads) {
+      uint32_t w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int j = 2 * (j0 + u * row_threads);
+        const uint32_t lo = j < hidden ? ld_stream<2>(p + j, pol).h : 0;
+        const uint32_t hi = j + 1 < hidden ? ld_stream<2>(p + j + 1, pol).h : 0;
+        w[u] = lo | hi << 16;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (j0 + u * row_threads < pairs) q[j0 + u * row_threads] = w[u];
+    }
+  };
+  auto fill = [&](int64_t i, int slot) {  // !kBulk
+    for (int t = 0; t < kTensors; ++t) copy_row(ring_p + slot * slot_bytes + t * tensor_bytes, row_of(t, i));
+  };
+
+  const int lane = tid % 32;
+  // Bytes of the rows that a round of the CTA has of one tensor.
+  auto round_bytes = [&](int64_t base) {
+    return static_cast<uint32_t>(min(static_cast<int64_t>(groups), a.rows - base)) * row_bytes;
+  };
+  if (copier) {
+    if (lane < groups) gave_up[lane] = 0;
+    if (lane == 0) {
+      for (int s = 0; s < a.slots; ++s) {
+        mbar_init(smem_u32(&full[s]), 1);
+        mbar_init(smem_u32(&empty[s]), groups * warps);
+      }
+      mbar_init_fence();
+    }
+    if (kBulk) {
+      // The first rows, into L2, while the preceding grid drains.
+      for (int s = 0; s < a.slots; ++s) {
+        const int64_t i = first - group + s * step + lane;
+        if (lane < groups && i < a.rows)
+          for (int t = 0; t < kTensors; ++t) prefetch_l2(row_of(t, i), row_bytes);
+      }
+    }
+  }
   __syncthreads();
-  float2 s = make_float2(0.f, 0.f);
-  for (int k = 0; k < warps; ++k) s.x += part[k].x, s.y += part[k].y;
-  return s;
+  pdl_wait();
+
+  if (copier) {
+    if constexpr (kBulk) {
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < a.rows; base += step) {
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1));
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&full[slot]), bytes = round_bytes(base);
+        const uint32_t to = smem_u32(slots_p) + slot * slot_bytes;
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes * kTensors);
+        __syncwarp();
+        const int64_t next = base + a.slots * step;  // few buffers: asked into L2
+        if (a.dense) {  // a tensor's rows follow each other: one copy
+          if (lane < kTensors) {
+            bulk_load(to + lane * tensor_bytes, row_of(lane, base), bytes, bar, pol);
+            if (a.slots < 3 && next < a.rows) prefetch_l2(row_of(lane, next), round_bytes(next));
+          }
+        } else if (lane < groups && base + lane < a.rows) {
+          for (int t = 0; t < kTensors; ++t) {
+            bulk_load(to + t * tensor_bytes + lane * row_bytes, row_of(t, base + lane), row_bytes, bar, pol);
+            if (a.slots < 3 && next + lane < a.rows) prefetch_l2(row_of(t, next + lane), row_bytes);
+          }
+        }
+        if (++slot == a.slots) slot = 0, phase ^= 1;
+      }
+      if (!ok) {
+        if (lane == 0) atomicAdd(a.timeouts, 1u);
+        for (int k = 0; k < a.slots; ++k) {  // copies still in flight
+          if (--slot < 0) slot = a.slots - 1, phase ^= 1;
+          mbar_wait_bounded(smem_u32(&full[slot]), phase, kWaitLimitNs / 16);
+        }
+      }
+    }
+    __syncwarp();
+    if (groups > 1) {
+      __syncthreads();
+      __syncthreads();
+    }
+    return;
+  }
+
+  float2 acc[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) acc[k] = make_float2(0.f, 0.f);
+  if (!kBulk)
+    for (int s = 0; s < a.slots && first + s * step < a.rows; ++s) fill(first + s * step, s);
+  // Every group writes the same weight row, and reads it after its own barrier.
+  if (a.weight_staged) copy_row(row_mem, a.w);
+  group_barrier(barrier, warps);
+  pdl_trigger();
+  const uint64_t keep = policy_evict_last();
+  auto load_weight = [&](uint32_t (&w)[4], int v) {
+    if (a.weight_staged) {
+      lds4(w, w_row + v * 16);
+    } else {
+      const Vec<16> q = ld_weight<16>(a.w + v * 8, keep);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = q.w[e];
+    }
+  };
+
+  const float scale = 1.0f / static_cast<float>(hidden);
+  int slot = 0, turn = 0;
+  uint32_t phase = 0;
+  for (int64_t i = first; i < a.rows; i += step) {
+    const uint32_t xs = ring + slot * slot_bytes, ds = xs + tensor_bytes, es = ds + tensor_bytes;
+    if constexpr (kBulk) {
+      if (!mbar_wait_bounded(smem_u32(&full[slot]), phase)) gave_up[group] = 1;
+    }
+    float2 ss = make_float2(0.f, 0.f), sd = ss;
+    float2 wd[kHold ? W : 1];  // w D, for both passes
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int v = in + k * row_threads;
+      if (v >= nvec) break;
+      uint32_t x[4], d[4], w[4];
+      lds4(x, xs + v * 16);
+      lds4(d, ds + v * 16);
+      load_weight(w, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 xf = unpack2<T>(x[e]), p = mul_pair<T>(w[e], d[e]);
+        ss = __ffma2_rn(xf, xf, ss);
+        sd = __ffma2_rn(p, xf, sd);
+        if constexpr (kHold) wd[4 * k + e] = p;
+      }
+    }
+    const float2 s =
+        row_sum2(make_float2(ss.x + ss.y, sd.x + sd.y), part[turn], tid / 32, warps, barrier, group * warps);
+    if (kBulk && *static_cast<volatile int*>(&gave_up[group])) break;
+    if constexpr (!kBulk) {
+      // The group is past the previous row: its buffer takes the row `slots` on.
+      const int64_t next = i + (a.slots - 1) * step;
+      if (a.slots > 1 && i > first && next < a.rows) fill(next, slot == 0 ? a.slots - 1 : slot - 1);
+    }
+    const float inv = rsqrtf(s.x * scale + a.eps), mean = s.y * inv * scale;
+    const float2 inv2 = make_float2(inv, inv), minus = make_float2(-mean * inv, -mean * inv);
+    uint16_t* dx = a.dx + i * a.dx_stride;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int v = in + k * row_threads;
+      if (v >= nvec) break;
+      uint32_t x[4], d[4], w[4], e4[4];
+      lds4(x, xs + v * 16);
+      lds4(d, ds + v * 16);
+      if constexpr (!kHold) load_weight(w, v);
+      if constexpr (EXTRA) lds4(e4, es + v * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 n = __fmul2_rn(unpack2<T>(x[e]), inv2);
+        acc[4 * k + e] = __ffma2_rn(unpack2<T>(d[e]), n, acc[4 * k + e]);
+        float2 p;
+        if constexpr (kHold) p = wd[4 * k + e];
+        else p = mul_pair<T>(w[e], d[e]);
+        float2 g = __ffma2_rn(p, inv2, __fmul2_rn(n, minus));
+        if constexpr (EXTRA) g = __fadd2_rn(g, unpack2<T>(e4[e]));
+        x[e] = pack2<T>(g.x, g.y);
+      }
+      if constexpr (kBulk) *reinterpret_cast<uint4*>(dx + v * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+      else sts4(xs + v * 16, x);
+    }
+    if constexpr (kBulk) {
+      __syncwarp();
+      if (tid % 32 == 0) mbar_arrive(smem_u32(&empty[slot]));
+    } else {
+      group_barrier(barrier, warps);
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(ring_p + slot * slot_bytes);
+#pragma unroll 4
+      for (int j = in; j < hidden; j += row_threads) dx[j] = q[j];
+      if (a.slots == 1 && i + step < a.rows) {
+        group_barrier(barrier, warps);
+        fill(i + step, 0);
+        group_barrier(barrier, warps);
+      }
+    }
+    turn ^= 1;
+    if (++slot == a.slots) slot = 0, phase ^= 1;
+  }
+  // The groups' sums meet in shared memory (every copy has landed); the first
+  // group writes the CTA's.
+  if (groups > 1) {
+    __syncthreads();
+    float2* sums = reinterpret_cast<float2*>(row_mem);
+#pragma unroll
+    for (int k = 0; k < W; ++k) sums[k * workers + tid] = acc[k];
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g < groups; ++g) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc[k] = __fadd2_rn(acc[k], sums[k * workers + g * row_threads + tid]);
+    }
+  }
+  // (partial's rows are padded to whole vectors.)
+  float* out = a.partial + blockIdx.x * static_cast<int64_t>(nvec) * 8;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int v = in + k * row_threads;
+    if (v >= nvec) break;
+    Vec<32> q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      q.w[2 * e] = __float_as_uint(acc[4 * k + e].x);
+      q.w[2 * e + 1] = __float_as_uint(acc[4 * k + e].y);
+    }
+    st_global<32>(out + v * 8, q);
+  }
 }
 
 // One CTA per row: the row's two sums.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_grad_stats(NormGradArgs a) {
   pdl_wait();
+  __shared__ float part[2][32];
   const int64_t i = blockIdx.x;
   const uint16_t* x = a.x + i * a.x_stride;
   const uint16_t* dy = a.dy + i * a.dy_stride;
@@ -60,7 +375,7 @@ __global__ void __launch_bounds__(256) norm_grad_stats(NormGradArgs a) {
     s.x = fmaf(v, v, s.x);
     s.y = fmaf(unpack1<T>(a.w[j]) * unpack1<T>(dy[j]), v, s.y);
   }
-  s = block_sum(s);
+  s = row_sum2(s, part, threadIdx.x / 32, 8, 1, 0);
   if (threadIdx.x == 0) {
     const float inv = rsqrtf(s.x / static_cast<float>(a.hidden) + a.eps);
     a.stats[i] = make_float2(inv, s.y * inv / static_cast<float>(a.hidden));
@@ -84,32 +399,109 @@ __global__ void __launch_bounds__(256) norm_grad_columns(NormGradArgs a) {
     if (a.extra) g += unpack1<T>(a.extra[i * a.extra_stride + j]);
     a.dx[i * a.dx_stride + j] = pack1<T>(g);
   }
-  a.partial[blockIdx.y * a.hidden + j] = sum;
+  a.partial[blockIdx.y * a.partial_ld + j] = sum;
 }
 
+// dw from the groups' sums: 32 columns a CTA, its 8 warps taking groups in turn.
+// (256 threads, so that the CTAs fit beside norm_grad_rows' and wait there for
+// its end.)
 template <typename T>
 __global__ void __launch_bounds__(256) norm_grad_weight(NormGradArgs a) {
+  __shared__ float part[8][32];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + tx;
+  pdl_trigger();
   pdl_wait();
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (j >= a.hidden) return;
   float sum = 0.f;
-  for (int64_t g = 0; g < a.groups; ++g) sum += a.partial[g * a.hidden + j];
+  if (j < a.hidden) {
+#pragma unroll 10
+    for (int64_t g = ty; g < a.groups; g += 8) sum += a.partial[g * a.partial_ld + j];
+  }
+  part[ty][tx] = sum;
+  __syncthreads();
+  if (ty > 0 || j >= a.hidden) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sum += part[k][tx];
   a.dw[j] = pack1<T>(sum);
 }
 
+// How norm_grad_rows takes the rows: words (of two elements) a thread, threads a
+// row, rows a CTA works on at once, row buffers each, and CTAs (also dw's
+// partial sums).  words 0: rows that are read twice.
+constexpr int kNormSmem = 220 * 1024;
+struct NormGradPlan {
+  int words, row_threads, row_groups, slots, smem;
+  bool bulk, weight_staged;
+  int64_t ctas;
+};
+
+// One CTA per SM.  The fewest elements a thread that keep a row within the CTA's
+// 512 threads, from 8 for short rows (up to 1024) or few of them, from 16 else:
+// 4096 x 4096 with E takes 25.5 us with 16 elements and two rows at once, 30.7
+// with 8 and one; 4096 x 1024 13.7 with 8, 14.8 with 16; 512 x 4096 9.6 with 8,
+// 10.5 with 16.  As many rows at once as have threads and two buffers each.
+// The weight is kept in shared memory beside the rows unless that leaves them
+// fewer than two buffers.
+NormGradPlan norm_grad_plan(const NormGradArgs& a) {
+  auto fits = [&](const void* p, int64_t stride) { return !p || tma_rows(p, a.rows, stride); };
+  NormGradPlan p{};
+  p.bulk = a.hidden % 8 == 0 && fits(a.x, a.x_stride) && fits(a.dy, a.dy_stride) && fits(a.dx, a.dx_stride) &&
+           fits(a.extra, a.extra_stride);
+  const int64_t nvec = (a.hidden + 7) / 8, row = nvec * 16, slot = row * (a.extra ? 3 : 2);
+  for (int words : {4, 8, 16, 32}) {
+    const int64_t threads = round_up((nvec + words / 4 - 1) / (words / 4), 32);
+    if (threads > kNormThreads) continue;
+    if (words == 4 && threads > 128 && a.rows > 4 * 148) continue;
+    int64_t groups = kNormThreads / threads;
+    while (groups > 1 && row + 2 * groups * slot > kNormSmem) --groups;
+    int64_t slots = (kNormSmem - row) / (groups * slot);
+    p.weight_staged = slots >= 2 || !p.bulk || !aligned(a.w, 16);
+    if (!p.weight_staged) slots = kNormSmem / (groups * slot);
+    if (slots < 1) break;
+    p.words = words, p.row_threads = static_cast<int>(threads), p.row_groups = static_cast<int>(groups);
+    p.slots = static_cast<int>(slots < kMostSlots ? slots : kMostSlots);
+    const int64_t ring = (p.weight_staged ? row : 0) + groups * p.slots * slot;
+    const int64_t sums = groups > 1 ? words * threads * groups * 8 : 0;
+    p.smem = static_cast<int>(ring > sums ? ring : sums);
+    const int64_t need = (a.rows + groups - 1) / groups;
+    p.ctas = need < 148 ? need : 148;
+    return p;
+  }
+  p.ctas = a.rows < 64 ? a.rows : 64;
+  return p;
+}
+
+template <typename T, bool EXTRA, bool kBulk>
+void (*norm_grad_kernel(int words))(NormGradArgs) {
+  switch (words) {
+    case 4: return norm_grad_rows<T, 4, EXTRA, kBulk>;
+    case 8: return norm_grad_rows<T, 8, EXTRA, kBulk>;
+    case 16: return norm_grad_rows<T, 16, EXTRA, kBulk>;
+    default: return norm_grad_rows<T, 32, EXTRA, kBulk>;
+  }
+}
+
 template <typename T>
-int launch_norm_grad(const NormGradArgs& a, cudaStream_t stream, unsigned flags) {
+int launch_norm_grad(const NormGradArgs& a, const NormGradPlan& p, const DeviceInfo* dev, cudaStream_t stream,
+                     unsigned flags) {
   const char* what = "rms_norm_backward";
-  const unsigned cols = static_cast<unsigned>((a.hidden + 255) / 256);
-  if (a.rows > 0) {
-    int st = launch_rows(norm_grad_stats<T>, dim3(static_cast<unsigned>(a.rows)), dim3(256), stream, flags,
-                         what, a);
+  int st = HPRN_OK;
+  if (a.rows > 0 && p.words > 0) {
+    auto fn = p.bulk ? (a.extra ? norm_grad_kernel<T, true, true>(p.words) : norm_grad_kernel<T, false, true>(p.words))
+                     : (a.extra ? norm_grad_kernel<T, true, false>(p.words) : norm_grad_kernel<T, false, false>(p.words));
+    if ((st = allow_smem(dev, reinterpret_cast<const void*>(fn), kNormSmem, what)) != HPRN_OK) return st;
+    st = launch_rows_smem(fn, dim3(static_cast<unsigned>(p.ctas)),
+                          dim3(static_cast<unsigned>(p.row_threads * p.row_groups + 32)), p.smem, stream, flags, what, a);
+  } else if (a.rows > 0) {
+    const unsigned cols = static_cast<unsigned>((a.hidden + 255) / 256);
+    st = launch_rows(norm_grad_stats<T>, dim3(static_cast<unsigned>(a.rows)), dim3(256), stream, flags, what, a);
     if (st != HPRN_OK) return st;
     st = launch_rows(norm_grad_columns<T>, dim3(cols, static_cast<unsigned>(a.groups)), dim3(256), stream,
                      flags, what, a);
-    if (st != HPRN_OK) return st;
   }
-  return launch_rows(norm_grad_weight<T>, dim3(cols), dim3(256), stream, flags, what, a);
+  if (st != HPRN_OK) return st;
+  return launch_rows(norm_grad_weight<T>, dim3(static_cast<unsigned>((a.hidden + 31) / 32)), dim3(256), stream,
+                     flags, what, a);
 }
 
 }  // namespace hprn
@@ -134,10 +526,22 @@ extern "C" int hprn_rms_norm_backward(void* grad_input, void* grad_weight, const
                    input_row_stride < hidden || (grad_residual && grad_residual_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   NormGradArgs a{};
-  a.groups = rows < 64 ? rows : 64;
+  a.dx = static_cast<uint16_t*>(grad_input), a.dw = static_cast<uint16_t*>(grad_weight);
+  a.dy = static_cast<const uint16_t*>(grad_out), a.x = static_cast<const uint16_t*>(input);
+  a.w = static_cast<const uint16_t*>(weight), a.extra = static_cast<const uint16_t*>(grad_residual);
+  a.rows = rows, a.hidden = hidden;
+  a.dx_stride = grad_input_row_stride, a.dy_stride = grad_out_row_stride;
+  a.x_stride = input_row_stride, a.extra_stride = grad_residual_row_stride;
+  a.eps = static_cast<float>(eps);
+  const NormGradPlan plan = norm_grad_plan(a);
+  a.groups = plan.ctas, a.row_threads = plan.row_threads;
+  a.dense = rows <= 1 || (input_row_stride == hidden && grad_out_row_stride == hidden &&
+                          (!grad_residual || grad_residual_row_stride == hidden));
+  a.row_groups = plan.row_groups, a.slots = plan.slots, a.weight_staged = plan.weight_staged;
   Workspace ws(workspace, *workspace_bytes);
-  a.stats = ws.take<float2>(rows);
-  a.partial = ws.take<float>(a.groups * hidden);
+  a.stats = ws.take<float2>(plan.words > 0 ? 0 : rows);
+  a.partial_ld = round_up(hidden, 8);
+  a.partial = ws.take<float>(a.groups * a.partial_ld);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
@@ -158,14 +562,8 @@ extern "C" int hprn_rms_norm_backward(void* grad_input, void* grad_weight, const
   const DeviceInfo* dev = nullptr;
   int st = current_device(&dev);
   if (st != HPRN_OK) return st;
-  a.dx = static_cast<uint16_t*>(grad_input), a.dw = static_cast<uint16_t*>(grad_weight);
-  a.dy = static_cast<const uint16_t*>(grad_out), a.x = static_cast<const uint16_t*>(input);
-  a.w = static_cast<const uint16_t*>(weight), a.extra = static_cast<const uint16_t*>(grad_residual);
-  a.rows = rows, a.hidden = hidden;
-  a.dx_stride = grad_input_row_stride, a.dy_stride = grad_out_row_stride;
-  a.x_stride = input_row_stride, a.extra_stride = grad_residual_row_stride;
-  a.eps = static_cast<float>(eps);
+  if ((st = timeout_counter(&a.timeouts)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  return dtype == HPRN_DTYPE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, cs, flags)
-                                  : launch_norm_grad<__half>(a, cs, flags);
+  return dtype == HPRN_DTYPE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, plan, dev, cs, flags)
+                                  : launch_norm_grad<__half>(a, plan, dev, cs, flags);
 }

@@ -113,6 +113,22 @@ int resident_ctas_per_sm(const DeviceInfo* dev, const void* fn, int threads, siz
   return ctas;
 }
 
+int allow_smem(const DeviceInfo* dev, const void* fn, int bytes, const char* what) {
+  constexpr int kMost = 512;
+  static std::mutex mu;
+  static const void* done_fn[kMost];
+  static int done_device[kMost];
+  static int done = 0;
+  std::lock_guard<std::mutex> lock(mu);
+  for (int k = 0; k < done; ++k)
+    if (done_fn[k] == fn && done_device[k] == dev->device) return HPRN_OK;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess)
+    return fail(HPRN_ERR_CUDA, std::string(what) + ": shared memory limit: " + cudaGetErrorString(e));
+  if (done < kMost) done_fn[done] = fn, done_device[done] = dev->device, ++done;
+  return HPRN_OK;
+}
+
 int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

@@ -118,12 +118,13 @@ bool disjoint(const Extent (&outs)[NO], const Extent (&ins)[NI]) {
 // Launches a kernel that begins with pdl_wait(), with programmatic stream
 // serialization where `flags` ask for it.
 template <typename... P, typename... A>
-int launch_rows(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, unsigned flags,
-                const char* what, A&&... args) {
+int launch_rows_smem(void (*fn)(P...), dim3 grid, dim3 block, int smem, cudaStream_t stream,
+                     unsigned flags, const char* what, A&&... args) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
   cfg.attrs = attr;
   if (flags & HPRN_LAUNCH_PDL) {
@@ -135,6 +136,22 @@ int launch_rows(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, un
   if (e != cudaSuccess)
     return fail(HPRN_ERR_CUDA, std::string(what) + " launch failed: " + cudaGetErrorString(e));
   return ok();
+}
+
+template <typename... P, typename... A>
+int launch_rows(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, unsigned flags,
+                const char* what, A&&... args) {
+  return launch_rows_smem(fn, grid, block, 0, stream, flags, what, static_cast<A&&>(args)...);
+}
+
+// The counter of waits that ran out, on the current device.
+int timeout_counter(unsigned** out);
+// Raises a kernel's dynamic shared memory limit, once per device.
+int allow_smem(const DeviceInfo* dev, const void* fn, int bytes, const char* what);
+
+// TMA reads rows that start on 16-byte boundaries.
+inline bool tma_rows(const void* p, int64_t rows, int64_t ld) {
+  return aligned(p, 16) && (rows <= 1 || ld % 8 == 0);
 }
 
 // Reports a failed launch (cudaGetLastError after the launch) as HPRN_ERR_CUDA.

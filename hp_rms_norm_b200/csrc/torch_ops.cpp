@@ -600,17 +600,22 @@ std::vector<hprn_grad> grad_table(at::TensorList grads, const at::TensorList* ou
   return table;
 }
 
-void grad_norm(at::Tensor& norm, at::TensorList grads) {
-  const std::vector<hprn_grad> table = grad_table(grads, nullptr, norm);
+void run_grad_norm(at::Tensor& norm, const std::vector<hprn_grad>& table) {
   with_workspace(norm, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
     return hprn_grad_norm(norm.data_ptr<float>(), table.data(), static_cast<int64_t>(table.size()),
                           ws, bytes, s, flags);
   });
 }
 
-void grad_clip(at::TensorList out, at::TensorList grads, const at::Tensor& norm, double max_norm) {
+void grad_norm(at::Tensor& norm, at::TensorList grads) {
+  run_grad_norm(norm, grad_table(grads, nullptr, norm));
+}
+
+void clip_grad_norm(at::TensorList out, at::Tensor& norm, at::TensorList grads, double max_norm) {
   TORCH_CHECK(out.size() == grads.size(), "out must have one tensor per gradient");
+  TORCH_CHECK(max_norm >= 0, "max_norm must be >= 0");
   const std::vector<hprn_grad> table = grad_table(grads, &out, norm);
+  run_grad_norm(norm, table);
   const c10::cuda::CUDAGuard guard(norm.device());
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(norm.device().index()).stream();
   check_status(hprn_grad_clip(table.data(), static_cast<int64_t>(table.size()),
@@ -629,7 +634,7 @@ void linear_cross_entropy_backward_meta(at::Tensor&, at::Tensor&, const at::Tens
 void rms_norm_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
                             const at::Tensor&, c10::optional<at::Tensor>, double) {}
 void grad_norm_meta(at::Tensor&, at::TensorList) {}
-void grad_clip_meta(at::TensorList, at::TensorList, const at::Tensor&, double) {}
+void clip_grad_norm_meta(at::TensorList, at::Tensor&, at::TensorList, double) {}
 
 // Shape-only kernels for tracing (torch.compile / FakeTensor): the ops return
 // nothing and only mutate their annotated arguments.
@@ -678,7 +683,7 @@ TORCH_LIBRARY(hp_rms_norm, m) {
   m.def("rms_norm_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, Tensor grad_out, "
         "Tensor input, Tensor weight, Tensor? grad_residual, float eps) -> ()");
   m.def("grad_norm(Tensor(a!) norm, Tensor[] grads) -> ()");
-  m.def("grad_clip(Tensor(a!)[] out, Tensor[] grads, Tensor norm, float max_norm) -> ()");
+  m.def("clip_grad_norm(Tensor(a!)[] out, Tensor(b!) norm, Tensor[] grads, float max_norm) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
@@ -697,7 +702,7 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward);
   m.impl("rms_norm_backward", &rms_norm_backward);
   m.impl("grad_norm", &grad_norm);
-  m.impl("grad_clip", &grad_clip);
+  m.impl("clip_grad_norm", &clip_grad_norm);
 }
 
 TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
@@ -716,5 +721,5 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_meta);
   m.impl("rms_norm_backward", &rms_norm_backward_meta);
   m.impl("grad_norm", &grad_norm_meta);
-  m.impl("grad_clip", &grad_clip_meta);
+  m.impl("clip_grad_norm", &clip_grad_norm_meta);
 }

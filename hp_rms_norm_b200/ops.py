@@ -204,10 +204,11 @@ def clip_grad_norm(grads, max_norm, out=None):
     them, in place or into the tensors of ``out`` (of any of the three types: 16-bit gradients
     into an optimiser's float32 buffers, say).  Returns the norm before clipping, a float32
     scalar tensor; nothing waits for the GPU."""
-    norm = grad_norm(grads)
-    if len(grads):
-        torch.ops.hp_rms_norm.grad_clip.default(grads if out is None else out, grads, norm,
-                                                max_norm)
+    if not len(grads):
+        return torch.zeros((), dtype=torch.float32)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    torch.ops.hp_rms_norm.clip_grad_norm.default(grads if out is None else out, norm, grads,
+                                                 max_norm)
     return norm
 
 
