@@ -106,9 +106,9 @@ struct GatedGradEpilogue {
   }
 };
 
-// S from a kept gate_up.  Memory-bound: 14 bytes per output element; a thread
-// takes V elements of a row, V = 8 where every row of every tensor starts on
-// a 16-byte boundary and d is a multiple of 8.
+// S from a kept gate_up.  Memory-bound: 14 bytes per output element.  Eight
+// elements a thread where every row of every tensor starts on a 16-byte
+// boundary and d is a multiple of 8.
 struct GatedGradArgs {
   const uint16_t* dout;
   int64_t dout_ld;
@@ -119,43 +119,62 @@ struct GatedGradArgs {
   int64_t rows, d;
 };
 
-template <typename T, int ACT, int V>
-__global__ void __launch_bounds__(256) gated_grad_rows(GatedGradArgs a) {
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) gated_grad_vectors(GatedGradArgs a) {
   pdl_wait();
-  const int64_t per_row = a.d / V, n = a.rows * per_row;
+  const int64_t per_row = a.d / 8, n = a.rows * per_row;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const uint64_t pol = policy_evict_first();
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n; e += step) {
-    const int64_t i = e / per_row, j = (e - i * per_row) * V;
+    const int64_t i = e / per_row, j = (e - i * per_row) * 8;
     const float* gp = a.gate_up + i * a.gate_up_ld + j;
-    const uint16_t* dp = a.dout + i * a.dout_ld + j;
     uint16_t* sp = a.s + i * a.s_ld + j;
-    float g[V], u[V], o[V];
-    if constexpr (V == 8) {
-      const uint64_t pol = policy_evict_first();
-      const Vec<16> g0 = ld_stream<16>(gp, pol), g1 = ld_stream<16>(gp + 4, pol);
-      const Vec<16> u0 = ld_stream<16>(gp + a.d, pol), u1 = ld_stream<16>(gp + a.d + 4, pol);
-      const Vec<16> d0 = ld_stream<16>(dp, pol);
+    const Vec<16> g0 = ld_stream<16>(gp, pol), g1 = ld_stream<16>(gp + 4, pol);
+    const Vec<16> u0 = ld_stream<16>(gp + a.d, pol), u1 = ld_stream<16>(gp + a.d + 4, pol);
+    const Vec<16> d0 = ld_stream<16>(a.dout + i * a.dout_ld + j, pol);
+    float g[8], u[8], o[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        g[k] = __uint_as_float(g0.w[k]), g[k + 4] = __uint_as_float(g1.w[k]);
-        u[k] = __uint_as_float(u0.w[k]), u[k + 4] = __uint_as_float(u1.w[k]);
-        const float2 f = unpack2<T>(d0.w[k]);
-        o[2 * k] = f.x, o[2 * k + 1] = f.y;
-      }
-      gated_gradients<ACT>(g, u, o);
-      Vec<16> sg, su;
+    for (int k = 0; k < 4; ++k) {
+      g[k] = __uint_as_float(g0.w[k]), g[k + 4] = __uint_as_float(g1.w[k]);
+      u[k] = __uint_as_float(u0.w[k]), u[k + 4] = __uint_as_float(u1.w[k]);
+      const float2 f = unpack2<T>(d0.w[k]);
+      o[2 * k] = f.x, o[2 * k + 1] = f.y;
+    }
+    gated_gradients<ACT>(g, u, o);
+    Vec<16> sg, su;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        sg.w[k] = pack2<T>(g[2 * k], g[2 * k + 1]);
-        su.w[k] = pack2<T>(u[2 * k], u[2 * k + 1]);
-      }
-      st_global<16>(sp, sg);
-      st_global<16>(sp + a.d, su);
-    } else {
-      g[0] = gp[0], u[0] = gp[a.d], o[0] = unpack1<T>(dp[0]);
-      gated_gradients<ACT>(g, u, o);
-      sp[0] = pack1<T>(g[0]);
-      sp[a.d] = pack1<T>(u[0]);
+    for (int k = 0; k < 4; ++k) {
+      sg.w[k] = pack2<T>(g[2 * k], g[2 * k + 1]);
+      su.w[k] = pack2<T>(u[2 * k], u[2 * k + 1]);
+    }
+    st_global<16>(sp, sg);
+    st_global<16>(sp + a.d, su);
+  }
+}
+
+// The same for any alignment: a CTA takes 1024 columns of a row, four a thread.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) gated_grad_elements(GatedGradArgs a) {
+  constexpr int N = 4;
+  pdl_wait();
+  const int64_t per_row = (a.d + 1023) / 1024, n = a.rows * per_row;
+  for (int64_t c = blockIdx.x; c < n; c += gridDim.x) {
+    const int64_t i = c / per_row, j0 = (c - i * per_row) * 1024 + threadIdx.x;
+    const float* gp = a.gate_up + i * a.gate_up_ld;
+    const uint16_t* dp = a.dout + i * a.dout_ld;
+    uint16_t* sp = a.s + i * a.s_ld;
+    float g[N], u[N], o[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t j = j0 + k * 256;
+      g[k] = u[k] = o[k] = 0.f;
+      if (j < a.d) g[k] = gp[j], u[k] = gp[a.d + j], o[k] = unpack1<T>(dp[j]);
+    }
+    gated_gradients<ACT>(g, u, o);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t j = j0 + k * 256;
+      if (j < a.d) sp[j] = pack1<T>(g[k]), sp[a.d + j] = pack1<T>(u[k]);
     }
   }
 }
@@ -208,8 +227,8 @@ int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* 
       (d > 0 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
-  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
-  const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride, 2 * d);
+  const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride, rows);
   const PlannedProduct<true, true, true> product(ws, rows, d, hidden);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
@@ -229,7 +248,7 @@ int hprn_gated_linear(void* out, float* gate_up, const void* input, const void* 
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
   Product q;
   q.a = {x.data(), x.ld()};
   q.b = {w.data(), w.ld()};
@@ -262,8 +281,8 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
       (d > 0 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
-  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
-  const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride, (gate_up ? 0 : 2) * d);
+  const AlignedRows w(ws, weight, 2 * d, hidden, weight_row_stride, gate_up ? 0 : rows);
   const int64_t s_ld = round_up(2 * d, 16);
   uint16_t* s = ws.take<uint16_t>(rows * s_ld);
   // Without the kept products the first sums are needed again.
@@ -292,7 +311,7 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
   const char* what = "gated_linear_backward";
   if (rows > 0 && d > 0) {
     st = with_type_and_act(dtype, act, [&](auto t, auto a) {
@@ -303,10 +322,11 @@ int hprn_gated_linear_backward(void* grad_input, void* grad_weight, const void* 
                               gate_up_row_stride, s, s_ld, rows, d};
         const bool wide = d % 8 == 0 && tma_rows(grad_out, rows, grad_out_row_stride) &&
                           aligned(gate_up, 16) && (rows <= 1 || gate_up_row_stride % 4 == 0);
-        const int64_t ctas = (rows * d / (wide ? 8 : 1) + 255) / 256, most = 16 * dev->sm_count;
+        const int64_t ctas = wide ? (rows * (d / 8) + 255) / 256 : rows * ((d + 1023) / 1024);
+        const int64_t most = 16 * dev->sm_count;
         const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most));
-        return wide ? launch_rows(gated_grad_rows<T, kAct, 8>, grid, dim3(256), cs, flags, what, g)
-                    : launch_rows(gated_grad_rows<T, kAct, 1>, grid, dim3(256), cs, flags, what, g);
+        return launch_rows(wide ? gated_grad_vectors<T, kAct> : gated_grad_elements<T, kAct>, grid, dim3(256),
+                           cs, flags, what, g);
       }
       Product q;
       q.a = {x.data(), x.ld()};

@@ -21,7 +21,9 @@
 
 namespace hprn {
 
-constexpr int kMaxTensors = 400;
+// Tables of two sizes: a launch copies its parameters, which for the large one
+// costs the host some 3 us.
+constexpr int kMaxTensors = 400, kFewTensors = 50;
 constexpr int kClipThreads = 256;
 // Elements of a chunk: as many as give every SM some 8 chunks, within bounds
 // that keep a chunk's work above its start (looking up its tensor; 4096
@@ -43,13 +45,16 @@ struct GradEntry {
   int32_t in_type, out_type;
 };
 
+template <int N>
 struct GradTable {
-  GradEntry t[kMaxTensors];
+  static constexpr int kSize = N;
   int64_t chunk;  // elements
   int32_t n;
+  GradEntry t[N];
 };
 
-__device__ __forceinline__ const GradEntry& find_entry(const GradTable& g, int64_t chunk) {
+template <int N>
+__device__ __forceinline__ const GradEntry& find_entry(const GradTable<N>& g, int64_t chunk) {
   int lo = 0, hi = g.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -168,7 +173,8 @@ __device__ __forceinline__ float chunk_squares(const GradEntry& e, int64_t lo, i
   return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
-__global__ void __launch_bounds__(kClipThreads) grad_square_sums(const __grid_constant__ GradTable g,
+template <int N>
+__global__ void __launch_bounds__(kClipThreads) grad_square_sums(const __grid_constant__ GradTable<N> g,
                                                                  float* partial) {
   __shared__ float part[kClipThreads / 32];
   const GradEntry& e = find_entry(g, blockIdx.x);
@@ -237,7 +243,8 @@ __device__ __forceinline__ void chunk_scale(const GradEntry& e, int64_t lo, int6
 
 // The chunks are taken last to first: the norm's pass read the last ones last,
 // so they are the ones L2 still holds.
-__global__ void __launch_bounds__(kClipThreads) grad_scale(const __grid_constant__ GradTable g,
+template <int N>
+__global__ void __launch_bounds__(kClipThreads) grad_scale(const __grid_constant__ GradTable<N> g,
                                                            const float* norm, float max_norm) {
   const int64_t chunk = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
   const GradEntry& e = find_entry(g, chunk);
@@ -295,9 +302,9 @@ int64_t total_of(const hprn_grad* g, int64_t count) {
 int64_t chunks_of(const hprn_grad& e, int64_t chunk) { return (e.rows * e.cols + chunk - 1) / chunk; }
 
 // Calls f(table, chunks) for every launch's worth of tensors.
-template <typename F>
-int for_tables(const hprn_grad* g, int64_t count, F&& f) {
-  GradTable table;
+template <int N, typename F>
+int for_tables_of(const hprn_grad* g, int64_t count, F&& f) {
+  GradTable<N> table;
   table.n = 0;
   table.chunk = chunk_elems(total_of(g, count));
   int64_t chunks = 0;
@@ -305,7 +312,7 @@ int for_tables(const hprn_grad* g, int64_t count, F&& f) {
     const int64_t c = chunks_of(g[k], table.chunk);
     if (c == 0) continue;
     if (c > 2147483647) return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor too large");
-    if (table.n == kMaxTensors || chunks + c > 2147483647) {
+    if (table.n == N || chunks + c > 2147483647) {
       const int st = f(table, chunks);
       if (st != HPRN_OK) return st;
       table.n = 0, chunks = 0;
@@ -320,6 +327,10 @@ int for_tables(const hprn_grad* g, int64_t count, F&& f) {
     chunks += c;
   }
   return table.n > 0 ? f(table, chunks) : HPRN_OK;
+}
+template <typename F>
+int for_tables(const hprn_grad* g, int64_t count, F&& f) {
+  return count <= kFewTensors ? for_tables_of<kFewTensors>(g, count, f) : for_tables_of<kMaxTensors>(g, count, f);
 }
 
 }  // namespace
@@ -351,10 +362,11 @@ int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* wor
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   int64_t at = 0;
-  st = for_tables(grads, count, [&](const GradTable& t, int64_t chunks) {
+  st = for_tables(grads, count, [&](const auto& t, int64_t chunks) {
     float* part = partial + at;
     at += chunks;
-    return launch_rows(grad_square_sums, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
+    constexpr int kTensors = std::decay_t<decltype(t)>::kSize;
+    return launch_rows(grad_square_sums<kTensors>, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
                        "grad_norm", t, part);
   });
   if (st != HPRN_OK) return st;
@@ -375,8 +387,9 @@ int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm, dou
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  st = for_tables(grads, count, [&](const GradTable& t, int64_t chunks) {
-    return launch_rows(grad_scale, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
+  st = for_tables(grads, count, [&](const auto& t, int64_t chunks) {
+    constexpr int kTensors = std::decay_t<decltype(t)>::kSize;
+    return launch_rows(grad_scale<kTensors>, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
                        "grad_clip", t, norm, static_cast<float>(max_norm));
   });
   return st == HPRN_OK ? ok() : st;

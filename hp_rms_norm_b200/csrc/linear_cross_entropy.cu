@@ -232,8 +232,8 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   if ((rows > 1 && input_row_stride < hidden) || (vocab > 1 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
-  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
-  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride, vocab);
+  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride, rows);
   const PlannedProduct<false, true, true> product(ws, rows, vocab, hidden, false);
   const int64_t parts = product.parts(vocab);
   float2* partial = ws.take<float2>(parts * rows);
@@ -258,7 +258,7 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_cross_entropy";
-  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
   Product q;
   q.a = {x.data(), x.ld()};
   q.b = {w.data(), w.ld()};
@@ -289,8 +289,8 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       (vocab > 1 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
-  const AlignedRows x(ws, input, rows, hidden, input_row_stride);
-  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride, 2 * vocab);
+  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride, rows);
   const Pieces pieces = pieces_of(rows, vocab);
   uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
   const int64_t sum_ld = round_up(hidden, kChunk);
@@ -322,7 +322,7 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_cross_entropy_backward";
-  if ((st = x.prepare(cs, flags)) != HPRN_OK || (st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
   if (factor && rows > 0) {
     st = launch_rows(loss_grad_scale, dim3(1), dim3(1024), cs, flags, what, grad_loss, target, ignore_index,
                      rows, factor);

@@ -566,22 +566,28 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // Host side.
 
-// A [rows, cols] operand TMA can read: the tensor itself, or a copy of it with
-// aligned rows taken from the workspace.
+// A [rows, cols] operand as TMA reads it best: the tensor itself, or a copy of
+// it with aligned rows taken from the workspace.  TMA needs rows on 16-byte
+// boundaries.  Where a k-major operand's rows start inside a 32-byte sector the
+// product takes up to half as long again (4096 x 2056 x 32768: 577 us; rows
+// 2064 long 382), a copy 4 bytes an element, so such rows are copied where each
+// element meets `reads` >= 2000 rows of the other operand in such products.
 class AlignedRows {
  public:
-  AlignedRows(Workspace& ws, const void* p, int64_t rows, int64_t cols, int64_t ld)
+  AlignedRows(Workspace& ws, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t reads)
       : src_(static_cast<const uint16_t*>(p)), rows_(rows), cols_(cols), src_ld_(ld), ld_(ld) {
     if (rows <= 1) ld_ = round_up(cols > 0 ? cols : 1, 8);
-    if (rows > 0 && cols > 0 && !tma_rows(p, rows, ld)) {
-      ld_ = round_up(cols, 8);
-      copies_ = true;
-      copy_ = ws.take<uint16_t>(rows * ld_);
-    }
+    if (rows <= 0 || cols <= 0) return;
+    const bool split = rows > 1 && (!aligned(p, 32) || ld % 16 != 0);
+    if (tma_rows(p, rows, ld) && !(split && reads >= 2000)) return;
+    ld_ = round_up(cols, 16);
+    copies_ = true;
+    copy_ = ws.take<uint16_t>(rows * ld_);
   }
-  int prepare(cudaStream_t stream, unsigned flags) const;
   const uint16_t* data() const { return copies_ ? copy_ : src_; }
   int64_t ld() const { return ld_; }
+  // Makes the copies of a call's two operands.
+  static int prepare(const AlignedRows& x, const AlignedRows& w, cudaStream_t stream, unsigned flags);
 
  private:
   const uint16_t* src_;
@@ -666,7 +672,7 @@ class PlannedProduct {
     args.stages = stages < kMaxStages ? stages : kMaxStages;
     args.band = 8;
     args.m = q.m, args.n = q.n, args.pair_offset = static_cast<int32_t>(q.pair_offset);
-    if ((st = timeout_counter(&args.timeouts)) != HPRN_OK) return st;
+    if ((st = timeout_counter(dev, &args.timeouts)) != HPRN_OK) return st;
     CUtensorMap map_a, map_b;
     st = kAKMajor ? encode_rows(&map_a, q.a.p, q.m, q.depth, q.a.ld, args.a_rows, what)
                   : encode_rows(&map_a, q.a.p, q.depth, q.m, q.a.ld, kDepthBlock, what);

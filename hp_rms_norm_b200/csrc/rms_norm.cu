@@ -965,12 +965,16 @@ int run(const Problem& q, void* stream, unsigned flags) {
 
 // The wait counter's address on the current device, for the kernels of other
 // files.
-int timeout_counter(unsigned** out) {
-  void* p = nullptr;
-  const cudaError_t e = cudaGetSymbolAddress(&p, g_wait_timeouts);
-  if (e != cudaSuccess)
-    return fail(HPRN_ERR_CUDA, std::string("the wait-timeout count: ") + cudaGetErrorString(e));
-  *out = static_cast<unsigned*>(p);
+int timeout_counter(const DeviceInfo* dev, unsigned** out) {
+  static std::atomic<unsigned*> known[64];
+  unsigned* p = known[dev->device].load(std::memory_order_relaxed);
+  if (!p) {
+    const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_wait_timeouts);
+    if (e != cudaSuccess)
+      return fail(HPRN_ERR_CUDA, std::string("the wait-timeout count: ") + cudaGetErrorString(e));
+    known[dev->device].store(p, std::memory_order_relaxed);
+  }
+  *out = p;
   return HPRN_OK;
 }
 

@@ -562,7 +562,7 @@ extern "C" int hprn_rms_norm_backward(void* grad_input, void* grad_weight, const
   const DeviceInfo* dev = nullptr;
   int st = current_device(&dev);
   if (st != HPRN_OK) return st;
-  if ((st = timeout_counter(&a.timeouts)) != HPRN_OK) return st;
+  if ((st = timeout_counter(dev, &a.timeouts)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   return dtype == HPRN_DTYPE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, plan, dev, cs, flags)
                                   : launch_norm_grad<__half>(a, plan, dev, cs, flags);

@@ -145,7 +145,7 @@ int launch_rows(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, un
 }
 
 // The counter of waits that ran out, on the current device.
-int timeout_counter(unsigned** out);
+int timeout_counter(const DeviceInfo* dev, unsigned** out);
 // Raises a kernel's dynamic shared memory limit, once per device.
 int allow_smem(const DeviceInfo* dev, const void* fn, int bytes, const char* what);
 

@@ -129,6 +129,10 @@ def gelu_tanh_and_mul(input, out=None):
     return _act_and_mul(torch.ops.hp_rms_norm.gelu_tanh_and_mul.default, input, out)
 
 
+def _new_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def gated_linear(input, weight, act="silu", out=None, gate_up=None):
     """out = act(input Wg^T) * (input Wu^T), the first half of a SwiGLU / GeGLU feed-forward
     block in one kernel.  ``input`` [..., hidden], ``weight`` [2 d, hidden] holding Wg's rows,
@@ -136,8 +140,7 @@ def gated_linear(input, weight, act="silu", out=None, gate_up=None):
     'gelu_tanh'.  ``gate_up``, a float32 [..., 2 d] tensor, receives the two products for
     ``gated_linear_backward``.  Returns ``out`` [..., d]."""
     if out is None:
-        out = torch.empty(input.shape[:-1] + (weight.shape[0] // 2,), dtype=input.dtype,
-                          device=input.device)
+        out = input.new_empty(input.shape[:-1] + (weight.shape[0] // 2,))
     torch.ops.hp_rms_norm.gated_linear.default(out, gate_up, input, weight, act)
     return out
 
@@ -146,8 +149,8 @@ def gated_linear_backward(grad_out, input, weight, act="silu", gate_up=None):
     """Gradients (grad_input, grad_weight) of ``gated_linear`` for a gradient of its output.
     With the ``gate_up`` that the forward call wrote the two products are read from it, without
     it they are computed again."""
-    grad_input = torch.empty(input.shape, dtype=input.dtype, device=input.device)
-    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    grad_input = _new_like(input)
+    grad_weight = _new_like(weight)
     torch.ops.hp_rms_norm.gated_linear_backward.default(grad_input, grad_weight, grad_out, input,
                                                         weight, gate_up, act)
     return grad_input, grad_weight
@@ -160,7 +163,7 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100):
     where it is otherwise outside the vocabulary) and the logits' log-sum-exp, which
     ``linear_cross_entropy_backward`` takes."""
     loss = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
-    lse = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
+    lse = torch.empty_like(loss)
     torch.ops.hp_rms_norm.linear_cross_entropy.default(loss, lse, input, weight, target,
                                                        ignore_index)
     return loss, lse
@@ -170,8 +173,8 @@ def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, ignore_
     """Gradients (grad_input, grad_weight) of ``linear_cross_entropy`` for the gradients of the
     rows' losses, ``grad_loss`` float32 [...]; the logits are computed again, one piece of the
     vocabulary at a time."""
-    grad_input = torch.empty(input.shape, dtype=input.dtype, device=input.device)
-    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    grad_input = _new_like(input)
+    grad_weight = _new_like(weight)
     torch.ops.hp_rms_norm.linear_cross_entropy_backward.default(
         grad_input, grad_weight, grad_loss, input, weight, target, lse, ignore_index)
     return grad_input, grad_weight
@@ -182,8 +185,8 @@ def rms_norm_backward(grad_out, input, weight, eps, grad_residual=None):
     fused forms ``input`` is the updated residual, and ``grad_residual`` the gradient that
     reaches it from its other uses, which is added: grad_input is then the gradient of both
     addends."""
-    grad_input = torch.empty(input.shape, dtype=input.dtype, device=input.device)
-    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    grad_input = _new_like(input)
+    grad_weight = _new_like(weight)
     torch.ops.hp_rms_norm.rms_norm_backward.default(grad_input, grad_weight, grad_out, input,
                                                     weight, grad_residual, eps)
     return grad_input, grad_weight
