@@ -373,10 +373,24 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
   if constexpr (kGroup == 2) cluster_sync_all();
   tmem_fence_after();
   const uint32_t tmem = tmem_base;
-  pdl_wait();
-
   const int32_t items = args.tiles_m * args.tiles_n * args.splits;
   const int32_t first = blockIdx.x / kGroup, step = gridDim.x / kGroup;
+  if (kBKMajor && warp == 0 && first < items) {
+    // The first stages of B (the weight, in the products that end in an
+    // operator's own output) into L2 while the preceding grid drains: 48 rows
+    // of A against 2 x 14336 x 4096, launches back to back, 40.5 us instead of
+    // 41.7.  (Asking for a tile's rows of B a kilobyte at a time, ahead of the
+    // loads all along, took 74.)
+    const Item it = item_at(args, first);
+    const DepthRange range = depth_range(args, it.split);
+    const int32_t half = kGroup == 2 ? static_cast<int32_t>(rank) : lane % 2;
+    const int32_t y = it.tn * c_cols + (E::kPaired ? half * args.pair_offset
+                                                   : kGroup == 2 ? half * static_cast<int32_t>(b_rows) : 0);
+    const int32_t k = range.first + (kGroup == 1 && E::kPaired ? lane / 2 : lane);
+    if (k < range.last && k < range.first + stages) tma_prefetch_2d(&map_b, k * kDepthBlock, y);
+    __syncwarp();
+  }
+  pdl_wait();
 
   if (warp == 0) {
     // Loads.  A pair's stage completes on the first CTA's barrier, which
