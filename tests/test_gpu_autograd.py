@@ -1,0 +1,135 @@
+"""The differentiable forms against torch's own autograd in 64 bits, and the training example."""
+import importlib.util
+import os
+
+import pytest
+import torch
+
+from hp_rms_norm_b200 import autograd as A
+from tests import training_reference as R
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def load_example():
+    spec = importlib.util.spec_from_file_location(
+        "train_language_model", os.path.join(ROOT, "examples", "train_language_model.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def leaf(*shape, device, seed, scale=1.0, dtype=torch.bfloat16):
+    g = torch.Generator(device=device).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=device) * scale).to(dtype).requires_grad_()
+
+
+def doubles(ts):
+    return [t.detach().double().requires_grad_() for t in ts]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("keep", [True, False])
+def test_gated_linear(cuda, act, keep):
+    x, w = leaf(3, 20, 64, device=cuda, seed=0), leaf(2 * 40, 64, device=cuda, seed=1, scale=0.125)
+    y = A.gated_linear(x, w, act, keep_products=keep)
+    # sum() hands the backward pass a gradient of one broadcast value.
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    xd, wd = doubles((x, w))
+    s = R.gated_linear_backward(torch.ones(60, 40, device=cuda), xd.view(60, 64), wd, act)
+    R.assert_near(gx.view(60, 64), s[0].detach(), R.rounding_noise(s[2], wd, x.dtype).detach(), "dx")
+    R.assert_near(gw, s[1].detach(), R.rounding_noise(s[2].T, xd.view(60, 64), x.dtype).detach(), "dw")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_linear_cross_entropy(cuda, reduction):
+    x, w = leaf(5, 14, 96, device=cuda, seed=2), leaf(333, 96, device=cuda, seed=3, scale=0.2)
+    t = torch.randint(0, 333, (5, 14), device=cuda)
+    t[0, :3] = -100
+    loss = A.linear_cross_entropy(x, w, t, reduction=reduction)
+    c = torch.linspace(0.5, 1.5, 70, device=cuda).view(5, 14)
+    total = loss if loss.dim() == 0 else (loss * c).sum()
+    gx, gw = torch.autograd.grad(total, (x, w))
+    xd, wd = doubles((x, w))
+    want = torch.nn.functional.cross_entropy((xd @ wd.T).view(70, 333), t.view(70), reduction=reduction)
+    # fp32 losses of about 6, from fp32 sums of 96 and 333 terms
+    assert (loss.double().view(-1) - want.view(-1)).abs().max() <= 6 * 500 * R.F32
+    want = want if want.dim() == 0 else (want * c.view(70).double()).sum()
+    wx, ww = torch.autograd.grad(want, (xd, wd))
+    counts = (t != -100).view(70)
+    rows = c.view(70) if reduction == "none" else torch.ones(70, device=cuda)
+    rows = rows / counts.sum() if reduction == "mean" else rows
+    s = R.linear_cross_entropy_backward(rows, xd.detach().view(70, 96), wd.detach(), t.view(70), -100)[2]
+    R.assert_near(gx, wx, R.rounding_noise(s, wd.detach(), x.dtype).view(5, 14, 96), "dx")
+    R.assert_near(gw, ww, R.rounding_noise(s.T, xd.detach().view(70, 96), x.dtype), "dw")
+
+
+def test_norms(cuda):
+    x, r = leaf(7, 9, 320, device=cuda, seed=4), leaf(7, 9, 320, device=cuda, seed=5)
+    w = leaf(320, device=cuda, seed=6)
+    y, total = A.fused_add_rms_norm(x, r, w, 1e-6)
+    y2 = A.rms_norm(total, w, 1e-6)
+    before = total.clone()
+    gx, gr, gw = torch.autograd.grad((y * y2).sum() + total.sum(), (x, r, w))
+    assert torch.equal(gx, gr) and torch.equal(total, before)
+    td, wd = doubles((total, w))
+    inv = torch.rsqrt(td.square().mean(-1, keepdim=True) + 1e-6)
+    n = td * inv * wd
+    want_t, want_w = torch.autograd.grad((n * n).sum() + td.sum(), (td, wd))
+    # y, y2, each norm's gradient and the sums of two gradients are rounded: four
+    # roundings of the terms that the two norms' gradients are made of.
+    with torch.no_grad():
+        unit, g = (td * inv).abs(), (wd * n).abs()
+        size_t = 2 * inv * (g + unit * (g * unit).mean(-1, keepdim=True)) + want_t.abs()
+        size_w = 2 * (n * unit).square().sum((0, 1)).sqrt() + want_w.abs()
+    R.assert_near(gx, want_t, 4 * R.U[x.dtype] * size_t, "dx")
+    R.assert_near(gw, want_w, 4 * R.U[x.dtype] * size_w, "dw")
+
+
+def test_example_learns(cuda):
+    losses = load_example().train(steps=30, layers=2, hidden=256, ffn=700, vocab=1000, batch=8, length=128)
+    losses = losses.cpu()
+    # It starts at guessing (the logarithm of the vocabulary) or above.
+    assert torch.isfinite(losses).all() and losses[0] > 6.5
+    assert losses[-5:].mean() < losses[:5].mean() - 0.5
+
+
+def test_example_gradients_match_plain_torch(cuda):
+    """One backward pass of the example's model against the same model in plain torch, float64."""
+    ex = load_example()
+    p = ex.parameters(2, 128, 200, 300, cuda, torch.bfloat16)
+    tokens = torch.randint(0, 300, (4, 32), device=cuda)
+    targets = torch.randint(0, 300, (4, 32), device=cuda)
+    loss = ex.loss_of(p, 2, tokens, targets)
+    names = list(p)
+    grads = torch.autograd.grad(loss, [p[n] for n in names])
+
+    class Plain:
+        @staticmethod
+        def fused_add_rms_norm(x, r, w, eps):
+            t = x + r
+            return t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * w, t
+
+        @staticmethod
+        def gated_linear(x, w, act="silu"):
+            g, u = (x @ w.T).chunk(2, -1)
+            return torch.nn.functional.silu(g) * u
+
+        @staticmethod
+        def linear_cross_entropy(x, w, t):
+            return torch.nn.functional.cross_entropy((x @ w.T).flatten(0, 1), t.flatten())
+
+    q = {n: p[n].detach().double().requires_grad_() for n in names}
+    kept, ex.A = ex.A, Plain
+    try:
+        want_loss = ex.loss_of(q, 2, tokens, targets)
+    finally:
+        ex.A = kept
+    want = torch.autograd.grad(want_loss, [q[n] for n in names])
+    # Some twenty roundings of u = 2^-8 between the embedding and the loss and
+    # as many on the way back, independent of each other: sqrt(40) u.
+    assert abs(loss.item() - want_loss.item()) <= 40 ** 0.5 * 2 ** -8 * want_loss.item()
+    for n, got, exact in zip(names, grads, want):
+        rel = float((got.double() - exact).norm() / exact.norm())
+        assert rel <= 40 ** 0.5 * 2 ** -8, (n, rel)
