@@ -37,19 +37,38 @@ __device__ __forceinline__ int64_t target_of(const int64_t* target, int64_t i, i
   return t == ignore ? kIgnored : (t < 0 || t >= vocab) ? kInvalid : t;
 }
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
-// 2^x (the hardware's approximation, 2 ulp): exponentials are taken to base 2 of
-// logits times log2 e, one fma and this each.
-__device__ __forceinline__ float exp2_fast(float x) {
+// exp(x) as 2^(x log2 e), by the hardware's approximation (2 ulp); 1 at 0.
+__device__ __forceinline__ float exp_fast(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
   return y;
+}
+__device__ __forceinline__ float2 exp_fast2(float2 x) {
+  const float2 t = __fmul2_rn(x, make_float2(kLog2e, kLog2e));
+  float2 y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(t.y));
+  return y;
+}
+
+// What a logit's sum is multiplied by.  The tensor cores' adder cuts off what
+// falls below the running sum's last place, 16 terms a step, so a sum of n
+// steps comes out short by about n * 2^-24 * 0.22 of itself (bf16) or 0.28
+// (fp16): the slope against 64-bit sums, the same at 256 and 1024 terms and
+// with terms of mean zero or not; sums of one sign lose more.  A loss is a
+// difference of logits near the largest ones and would be short throughout:
+// 2048 x 5120 x 100003 1.8e-6 of itself without the factor, 1024 x 5120 x 20000 with it 5.5e-7.
+float sum_correction(int64_t depth, int dtype) {
+  const double steps = static_cast<double>((depth + 15) / 16);
+  return static_cast<float>(1.0 + steps * (dtype == HPRN_DTYPE_BF16 ? 0.22 : 0.28) / 16777216.0);
 }
 
 struct LossEpilogue {
   static constexpr bool kPaired = false;
-  float2* partial = nullptr;  // [rows, parts]: {max of l log2 e, sum of 2^(l log2 e - max)}
+  float correction = 1.f;     // sum_correction
+  float2* partial = nullptr;  // [rows, parts]: {max of l, sum of exp(l - max)}
   float* target_logit = nullptr;
   const int64_t* target = nullptr;
   int64_t ignore = 0;
@@ -75,18 +94,22 @@ struct LossEpilogue {
       float x = 0.f;
 #pragma unroll
       for (int k = 0; k < kChunk; ++k) x = at == k ? v[k] : x;
-      target_logit[i] = x;
+      target_logit[i] = x * correction;
     }
     float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int k = 4; k < kChunk; ++k) top[k % 4] = fmaxf(top[k % 4], v[k]);
-    const float m = fmaxf(r.m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * kLog2e);
-    // All so far -inf (or NaN, which fmaxf skips and the sum keeps): 2^(-inf - 0) = 0.
+    const float m = fmaxf(r.m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * correction);
+    // All so far -inf (or NaN, which fmaxf skips and the sum keeps): exp(-inf - 0) = 0.
     const float ref = m == -INFINITY ? 0.f : m;
-    float s[4] = {r.s * exp2_fast(r.m - ref), 0.f, 0.f, 0.f};
+    const float2 c2 = make_float2(correction, correction), minus = make_float2(-ref, -ref);
+    float2 s[2] = {make_float2(r.s * exp_fast(r.m - ref), 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int k = 0; k < kChunk; ++k) s[k % 4] += exp2_fast(fmaf(v[k], kLog2e, -ref));
-    r.m = m, r.s = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int k = 0; k < kChunk / 2; ++k) {
+      const float2 l = __fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), c2);
+      s[k % 2] = __fadd2_rn(s[k % 2], exp_fast2(__fadd2_rn(l, minus)));
+    }
+    r.m = m, r.s = (s[0].x + s[0].y) + (s[1].x + s[1].y);
   }
   __device__ __forceinline__ void end(Row& r, const Lane& l, int64_t i, int64_t part) const {
     if (l.inside) partial[i * parts + part] = make_float2(r.m, r.s);
@@ -105,7 +128,7 @@ __global__ void __launch_bounds__(256)
   auto join = [&](float2 p) {
     const float top = fmaxf(m, p.x);
     const float ref = top == -INFINITY ? 0.f : top;
-    s = s * exp2_fast(m - ref) + p.y * exp2_fast(p.x - ref);
+    s = s * exp_fast(m - ref) + p.y * exp_fast(p.x - ref);
     m = top;
   };
   for (int64_t k = lane; k < parts; k += 32) join(partial[i * parts + k]);
@@ -113,7 +136,7 @@ __global__ void __launch_bounds__(256)
     join(make_float2(__shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o)));
   if (lane != 0) return;
   if (parts == 0 && vocab > 0) m = 0.f, s = static_cast<float>(vocab);  // sums of no terms: logits 0
-  const float l = (m == -INFINITY ? 0.f : m * kLn2) + logf(s);
+  const float l = (m == -INFINITY ? 0.f : m) + logf(s);
   lse[i] = l;
   const int64_t t = target_of(target, i, ignore, vocab);
   loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - (parts > 0 ? target_logit[i] : 0.f);
@@ -146,7 +169,8 @@ __global__ void __launch_bounds__(1024) loss_grad_scale(const float* grad_loss, 
 template <typename T>
 struct LossGradEpilogue {
   static constexpr bool kPaired = false;
-  Out16 s;  // the piece's columns
+  float correction = 1.f;  // as in LossEpilogue
+  Out16 s;                 // the piece's columns
   const float* lse = nullptr;
   const float* grad_loss = nullptr;
   const float* factor = nullptr;  // or null for 1
@@ -156,7 +180,7 @@ struct LossGradEpilogue {
   int64_t first = 0;  // the piece's first column
 
   struct Row {
-    float c, lse2;
+    float c, lse;
     int64_t t;  // within the piece (or outside it)
   };
   __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const {
@@ -164,7 +188,7 @@ struct LossGradEpilogue {
     if (t == kIgnored) return Row{0.f, INFINITY, kIgnored};
     // A target outside the vocabulary has no loss: NaN, like the loss itself.
     const float c = t == kInvalid ? __int_as_float(0x7fc00000) : grad_loss[i] * (factor ? *factor : 1.f);
-    return Row{c, lse[i] * kLog2e, t >= first ? t - first : kInvalid};
+    return Row{c, lse[i], t >= first ? t - first : kInvalid};
   }
   __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
     const int64_t at = r.t - j;
@@ -174,7 +198,12 @@ struct LossGradEpilogue {
       for (int k = 0; k < kChunk; ++k) v[k] = 0.f;
     } else {
 #pragma unroll
-      for (int k = 0; k < kChunk; ++k) v[k] = r.c * exp2_fast(fmaf(v[k], kLog2e, -r.lse2));
+      for (int k = 0; k < kChunk / 2; ++k) {
+        // Rounded as the forward pass rounded it, so that exp(0) is where lse is a logit.
+        const float2 l = __fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(correction, correction));
+        const float2 p = __fmul2_rn(exp_fast2(__fadd2_rn(l, make_float2(-r.lse, -r.lse))), make_float2(r.c, r.c));
+        v[2 * k] = p.x, v[2 * k + 1] = p.y;
+      }
       if (here) {
 #pragma unroll
         for (int k = 0; k < kChunk; ++k)
@@ -264,6 +293,7 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   q.b = {w.data(), w.ld()};
   q.m = rows, q.n = vocab, q.depth = hidden;
   LossEpilogue e;
+  e.correction = sum_correction(hidden, dtype);
   e.partial = partial, e.target_logit = target_logit, e.target = target;
   e.ignore = ignore_index, e.parts = parts, e.vocab = vocab;
   if (hidden > 0) {
@@ -342,6 +372,7 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       q.b = {wp, w.ld()};
       q.m = rows, q.n = cols, q.depth = hidden;
       LossGradEpilogue<T> g;
+      g.correction = sum_correction(hidden, dtype);
       g.s = Out16(s, pieces.cols, cols), g.lse = lse, g.grad_loss = grad_loss, g.factor = factor;
       g.target = target, g.ignore = ignore_index, g.vocab = vocab, g.first = first;
       if ((r = logits.launch_whole<T>(q, g, cs, flags, what)) != HPRN_OK) break;
