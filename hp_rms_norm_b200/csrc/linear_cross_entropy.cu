@@ -14,10 +14,14 @@
 // and leave as S (16-bit, the tensor cores' operand), dW's rows of that piece
 // are complete, and dX is summed over the pieces in fp32 and rounded once.
 //
-// S in fp16: softmax values of a large vocabulary times a mean's 1/rows fall
-// below fp16's smallest normal (6e-5), so S is held times a power of two that
-// puts the largest |c_i| between 2^14 and 2^15, and the sums are divided by it.
-// bf16 has fp32's range and needs none.
+// S is held as c_i / c_max (exp(L_ij - lse_i) - [j == t_i]), c_max the largest
+// |c_i|, and the sums are multiplied by c_max.  A mean gives every row the same
+// c, and then the entries that matter most, -c at the targets, would all be
+// rounded to 16 bits alike and the gradients come out up to 2^-9 short or long;
+// -1 is exact (8192 x 4096 x 131072, one draw of the targets: 3.5e-3 off without,
+// 1.7e-3, the rounding of the outputs themselves, with it).  In fp16 S is held
+// times 2^14 as well: softmax values of a large vocabulary fall below its
+// smallest normal, 6e-5.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -59,7 +63,7 @@ __device__ __forceinline__ float2 exp_fast2(float2 x) {
 // (fp16): the slope against 64-bit sums, the same at 256 and 1024 terms and
 // with terms of mean zero or not; sums of one sign lose more.  A loss is a
 // difference of logits near the largest ones and would be short throughout:
-// 2048 x 5120 x 100003 1.8e-6 of itself without the factor, 1024 x 5120 x 20000 with it 5.5e-7.
+// 2048 x 5120 x 100003 (fp16) 1.8e-6 of itself without the factor, 4.4e-7 with it.
 float sum_correction(int64_t depth, int dtype) {
   const double steps = static_cast<double>((depth + 15) / 16);
   return static_cast<float>(1.0 + steps * (dtype == HPRN_DTYPE_BF16 ? 0.22 : 0.28) / 16777216.0);
@@ -142,11 +146,12 @@ __global__ void __launch_bounds__(256)
   loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - (parts > 0 ? target_logit[i] : 0.f);
 }
 
-// {factor, 1 / factor}: the power of two S is held times.
+// c_max, and what the sums are multiplied by: c_max / held.
 __global__ void __launch_bounds__(1024) loss_grad_scale(const float* grad_loss, const int64_t* target,
-                                                        int64_t ignore, int64_t rows, float* out) {
+                                                        int64_t ignore, int64_t rows, float held, float* out) {
   __shared__ float part[32];
   pdl_wait();
+  pdl_trigger();
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
     if (target[i] != ignore) m = fmaxf(m, fabsf(grad_loss[i]));
@@ -156,14 +161,9 @@ __global__ void __launch_bounds__(1024) loss_grad_scale(const float* grad_loss, 
   if (threadIdx.x >= 32) return;
   m = part[threadIdx.x];
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  if (threadIdx.x == 0) {
-    // m in [2^e, 2^(e+1)): times 2^(14 - e).  Exponents are kept where both
-    // factors are normal; 0, infinities and NaN take 1.
-    int e = 14;
-    if (m > 0.f && m <= 3.402823466e38f) e = max(-100, min(100, ilogbf(m)));
-    out[0] = ldexpf(1.f, 14 - e);
-    out[1] = ldexpf(1.f, e - 14);
-  }
+  // An infinite gradient spoils its own row and the weight's, not the other rows.
+  if (!(m > 0.f && m < INFINITY)) m = 1.f;
+  if (threadIdx.x == 0) out[0] = m, out[1] = m / held;
 }
 
 template <typename T>
@@ -173,7 +173,8 @@ struct LossGradEpilogue {
   Out16 s;                 // the piece's columns
   const float* lse = nullptr;
   const float* grad_loss = nullptr;
-  const float* factor = nullptr;  // or null for 1
+  const float* most = nullptr;  // c_max
+  float held = 1.f;             // what S is held times
   const int64_t* target = nullptr;
   int64_t ignore = 0;
   int64_t vocab = 0;
@@ -187,7 +188,7 @@ struct LossGradEpilogue {
     const int64_t t = l.inside ? target_of(target, i, ignore, vocab) : kIgnored;
     if (t == kIgnored) return Row{0.f, INFINITY, kIgnored};
     // A target outside the vocabulary has no loss: NaN, like the loss itself.
-    const float c = t == kInvalid ? __int_as_float(0x7fc00000) : grad_loss[i] * (factor ? *factor : 1.f);
+    const float c = t == kInvalid ? __int_as_float(0x7fc00000) : grad_loss[i] / *most * held;
     return Row{c, lse[i], t >= first ? t - first : kInvalid};
   }
   __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
@@ -325,7 +326,8 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
   const int64_t sum_ld = round_up(hidden, kChunk);
   float* sum = pieces.count > 1 ? ws.take<float>(rows * sum_ld) : nullptr;
-  float* factor = dtype == HPRN_DTYPE_FP16 ? ws.take<float>(2) : nullptr;
+  float* scale = ws.take<float>(2);
+  const float held = dtype == HPRN_DTYPE_FP16 ? 16384.f : 1.f;
   const PlannedProduct<false, true, true> logits(ws, rows, pieces.cols, hidden, false);
   const PlannedProduct<false, true, false> to_input(ws, rows, hidden, pieces.cols);
   const PlannedProduct<false, false, false> to_weight(ws, pieces.cols, hidden, rows);
@@ -353,9 +355,9 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_cross_entropy_backward";
   if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
-  if (factor && rows > 0) {
+  if (rows > 0) {
     st = launch_rows(loss_grad_scale, dim3(1), dim3(1024), cs, flags, what, grad_loss, target, ignore_index,
-                     rows, factor);
+                     rows, held, scale);
     if (st != HPRN_OK) return st;
   }
   auto all = [&](auto t) {
@@ -373,7 +375,7 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       q.m = rows, q.n = cols, q.depth = hidden;
       LossGradEpilogue<T> g;
       g.correction = sum_correction(hidden, dtype);
-      g.s = Out16(s, pieces.cols, cols), g.lse = lse, g.grad_loss = grad_loss, g.factor = factor;
+      g.s = Out16(s, pieces.cols, cols), g.lse = lse, g.grad_loss = grad_loss, g.most = scale, g.held = held;
       g.target = target, g.ignore = ignore_index, g.vocab = vocab, g.first = first;
       if ((r = logits.launch_whole<T>(q, g, cs, flags, what)) != HPRN_OK) break;
 
@@ -382,7 +384,7 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       StoreEpilogue<T> e;
       e.out = Out16(grad_input, grad_input_row_stride, hidden);
       e.sum = sum, e.sum_ld = sum_ld, e.first = p == 0, e.last = p == count - 1;
-      e.scale = factor && rows > 0 ? factor + 1 : nullptr;
+      e.scale = rows > 0 ? scale + 1 : nullptr;
       if ((r = to_input.launch<T>(q, e, cs, flags, what)) != HPRN_OK) break;
 
       q.b = {x.data(), x.ld()};

@@ -271,12 +271,12 @@ HPRN_API int hprn_linear_cross_entropy(float* loss, float* lse, const void* inpu
 /*
  * Gradients of hprn_linear_cross_entropy for gradients c[i] = grad_loss[i] of
  * the rows' losses (fp32), lse from the forward call:
- *   S_ij = round_T(c_i (exp(L_ij - lse_i) - [j == target_i])); 0 in rows with
+ *   S_ij = c_i (exp(L_ij - lse_i) - [j == target_i]) to 16 bits; 0 in rows with
  *          target_i == ignore_index, NaN in rows with any other invalid target
  *   grad_input [rows, hidden]  = round_T(S weight)
  *   grad_weight [vocab, hidden] = round_T(S^T input)
- * In fp16, S is held times a power of two (the largest |c_i| brought to
- * [2^14, 2^15)), so small probabilities do not underflow.
+ * S is held divided by the largest |c_i| (and in fp16 times 2^14), so equal c_i
+ * are not all rounded alike and small probabilities do not underflow.
  */
 HPRN_API int hprn_linear_cross_entropy_backward(
     void* grad_input, void* grad_weight, const float* grad_loss, const void* input,

@@ -115,6 +115,33 @@ def test_ignored_and_invalid_rows(cuda):
     assert (loss == 0).sum() == 126
 
 
+def test_equal_row_gradients_are_not_rounded_alike(cuda):
+    """A mean's factor lies between two 16-bit numbers; the gradients must not inherit its
+    rounding: nearly all of them is -c at the targets."""
+    x, w, t, c = make(256, 128, 5000, torch.bfloat16, cuda, ignored=0.0, scale=1.0)
+    c[:] = 1.00390625 * (1 - 2.0 ** -16)  # almost half a bf16 step above 1
+    _, lse = hp.linear_cross_entropy(x, w, t)
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    want_x, want_w, s = R.linear_cross_entropy_backward(c, x, w, t, IGNORE)
+    # The outputs' own roundings leave no slope: each is within u, of either sign, and
+    # over n values their mean within 4 u / sqrt(n).  Rounded alike, S would be 2^-8 off.
+    for got, want in ((dx, want_x), (dw, want_w)):
+        slope = float((got.double() * want).sum() / want.square().sum()) - 1
+        assert abs(slope) <= 4 * R.U[torch.bfloat16] / want.numel() ** 0.5 + 2.0 ** -12
+
+
+def test_infinite_row_gradient_stays_in_its_row(cuda):
+    x, w, t, c = make(140, 64, 300, torch.bfloat16, cuda, ignored=0.0)
+    _, lse = hp.linear_cross_entropy(x, w, t)
+    clean, _ = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    c[7] = float("inf")
+    dx, _ = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    keep = torch.arange(140, device=cuda) != 7
+    assert torch.isfinite(dx[keep]).all() and not torch.isfinite(dx[7]).any()
+    # c_max differs between the two calls, and with it S's roundings.
+    assert (dx[keep].double() - clean[keep].double()).norm() <= 4 * R.U[w.dtype] * clean.double().norm()
+
+
 def test_pieces_of_the_vocabulary(cuda):
     """Enough rows for the vocabulary to be taken in several pieces (512 MiB of 16-bit logit
     gradients each): the input's gradient is summed over them."""
