@@ -91,31 +91,40 @@ __device__ __forceinline__ void lds4(uint32_t (&w)[4], uint32_t addr) {
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                : "r"(addr));
 }
-__device__ __forceinline__ void sts4(uint32_t addr, const uint32_t (&w)[4]) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-               : "memory");
+__device__ __forceinline__ uint32_t lds1(uint32_t addr) {
+  uint32_t w;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(addr));
+  return w;
+}
+__device__ __forceinline__ void sts_half(uint32_t addr, uint16_t h) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(h) : "memory");
 }
 
 // A CTA is `groups` groups of `row_threads` threads, and one warp more; a group
-// works on one row at a time, each thread on the same W / 4 vectors of eight
-// elements of every row.  A group's rows arrive in a ring of `slots` row
-// buffers in shared memory.  Where every row of every tensor starts on a
-// 16-byte boundary and hidden is a multiple of 8 (kBulk) the extra warp keeps
-// the ring filled by bulk copies, a round's neighbouring rows in one where they
-// follow each other; else the group copies its next rows itself, element by
-// element.
+// works on one row at a time, each thread on the same W words (pairs of
+// elements) of every row.  A group's rows arrive in a ring of `slots` row
+// buffers in shared memory, which the extra warp keeps filled by bulk copies.
+//   kVectors: every row of every tensor starts on a 16-byte boundary and hidden
+// is a multiple of 8.  Rows that follow each other come in one copy; threads
+// take vectors of eight elements.
+//   Else a row is copied with the 16-byte granules it lies in, so that it starts
+// as far into its buffer as it does into its first granule (the first and the
+// last row's elements in granules that reach out of the tensor come by
+// ordinary loads); threads take single words, neighbouring threads
+// neighbouring ones, put together from two where the row starts on an odd element.
 //
 // Registers hold dw's sums (2 W floats) and, up to 16 words, w D between the
 // two passes.  4096 x 8192 with E: 48.0 us (0.87 of a copy of the same bytes),
 // against 55.8 with the rows themselves in registers, which spilled or kept
-// one row a CTA in flight.
+// one row a CTA in flight.  4096 x 5001 with E: 90 us, bound by issue, against 155 with rows copied
+// element by element.
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies
 // still in flight, counted in `timeouts`; the rows it had not finished keep
 // their dx.
 constexpr int kNormThreads = 512;
 
-template <typename T, int W, bool EXTRA, bool kBulk>
+template <typename T, int W, bool EXTRA, bool kVectors>
 __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradArgs a) {
   constexpr int kVecs = W / 4;
   constexpr int kTensors = EXTRA ? 3 : 2;
@@ -130,13 +139,12 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
   const int group = copier ? tid - workers : tid / row_threads, in = copier ? 0 : tid - group * row_threads;
   const int warps = row_threads / 32, barrier = 1 + group;
   const int hidden = static_cast<int>(a.hidden), nvec = (hidden + 7) / 8;
-  // A slot: `groups` rows of x, then of D, then of E.
-  const uint32_t row_bytes = static_cast<uint32_t>(nvec) * 16, tensor_bytes = row_bytes * groups;
-  const uint32_t slot_bytes = tensor_bytes * kTensors;
-  const uint32_t w_row = smem_u32(row_mem);
-  unsigned char* slots_p = row_mem + (a.weight_staged ? row_bytes : 0);
-  unsigned char* ring_p = slots_p + group * row_bytes;
-  const uint32_t ring = smem_u32(ring_p);
+  const int words = (hidden + 1) / 2;
+  // A slot: `groups` rows of x, then of D, then of E; `pitch` bytes a row.
+  const uint32_t row_bytes = static_cast<uint32_t>(nvec) * 16, pitch = row_bytes + (kVectors ? 0 : 16);
+  const uint32_t tensor_bytes = pitch * groups, slot_bytes = tensor_bytes * kTensors;
+  const uint32_t w_row = smem_u32(row_mem), slots_at = w_row + (a.weight_staged ? row_bytes : 0);
+  const uint32_t ring = slots_at + group * pitch;
   const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * groups + group;
   const uint64_t pol = policy_evict_first();
@@ -144,28 +152,6 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
   auto row_of = [&](int t, int64_t i) {
     return t == 0 ? a.x + i * a.x_stride : t == 1 ? a.dy + i * a.dy_stride : a.extra + i * a.extra_stride;
   };
-  // A row element by element: pairs, eight a thread in flight.
-  auto copy_row = [&](unsigned char* to, const uint16_t* p) {
-    uint32_t* q = reinterpret_cast<uint32_t*>(to);
-    const int pairs = nvec * 4;
-    for (int j0 = in; j0 < pairs; j0 += 8 * row_threads) {
-      uint32_t w[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int j = 2 * (j0 + u * row_threads);
-        const uint32_t lo = j < hidden ? ld_stream<2>(p + j, pol).h : 0;
-        const uint32_t hi = j + 1 < hidden ? ld_stream<2>(p + j + 1, pol).h : 0;
-        w[u] = lo | hi << 16;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (j0 + u * row_threads < pairs) q[j0 + u * row_threads] = w[u];
-    }
-  };
-  auto fill = [&](int64_t i, int slot) {  // !kBulk
-    for (int t = 0; t < kTensors; ++t) copy_row(ring_p + slot * slot_bytes + t * tensor_bytes, row_of(t, i));
-  };
-
   const int lane = tid % 32;
   // Bytes of the rows that a round of the CTA has of one tensor.
   auto round_bytes = [&](int64_t base) {
@@ -180,12 +166,12 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
       }
       mbar_init_fence();
     }
-    if (kBulk) {
+    {
       // The first rows, into L2, while the preceding grid drains.
       for (int s = 0; s < a.slots; ++s) {
         const int64_t i = first - group + s * step + lane;
         if (lane < groups && i < a.rows)
-          for (int t = 0; t < kTensors; ++t) prefetch_l2(row_of(t, i), row_bytes);
+          for (int t = 0; t < kTensors; ++t) prefetch_l2(row_of(t, i), static_cast<uint64_t>(hidden) * 2);
       }
     }
   }
@@ -193,37 +179,69 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
   pdl_wait();
 
   if (copier) {
-    if constexpr (kBulk) {
-      int slot = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < a.rows; base += step) {
-        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1));
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&full[slot]), bytes = round_bytes(base);
-        const uint32_t to = smem_u32(slots_p) + slot * slot_bytes;
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < a.rows; base += step) {
+      ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1));
+      if (!ok) break;
+      const uint32_t bar = smem_u32(&full[slot]), to = slots_at + slot * slot_bytes;
+      const int64_t next = base + a.slots * step;  // few buffers: asked into L2
+      if (kVectors && a.dense) {
+        const uint32_t bytes = round_bytes(base);
         if (lane == 0) mbar_arrive_expect_tx(bar, bytes * kTensors);
         __syncwarp();
-        const int64_t next = base + a.slots * step;  // few buffers: asked into L2
-        if (a.dense) {  // a tensor's rows follow each other: one copy
-          if (lane < kTensors) {
-            bulk_load(to + lane * tensor_bytes, row_of(lane, base), bytes, bar, pol);
-            if (a.slots < 3 && next < a.rows) prefetch_l2(row_of(lane, next), round_bytes(next));
-          }
-        } else if (lane < groups && base + lane < a.rows) {
-          for (int t = 0; t < kTensors; ++t) {
-            bulk_load(to + t * tensor_bytes + lane * row_bytes, row_of(t, base + lane), row_bytes, bar, pol);
-            if (a.slots < 3 && next + lane < a.rows) prefetch_l2(row_of(t, next + lane), row_bytes);
-          }
+        if (lane < kTensors) {
+          bulk_load(to + lane * tensor_bytes, row_of(lane, base), bytes, bar, pol);
+          if (a.slots < 3 && next < a.rows) prefetch_l2(row_of(lane, next), round_bytes(next));
         }
-        if (++slot == a.slots) slot = 0, phase ^= 1;
+      } else {
+        const bool mine = lane < groups && base + lane < a.rows;
+        const int64_t i = base + lane;
+        const unsigned char* from[kTensors];
+        uint32_t bytes[kTensors], at[kTensors], total = 0;
+#pragma unroll
+        for (int t = 0; t < kTensors; ++t) {
+          bytes[t] = 0;
+          if (!mine) continue;
+          const unsigned char* p = reinterpret_cast<const unsigned char*>(row_of(t, i));
+          const uint32_t off = kVectors ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
+          at[t] = to + t * tensor_bytes + lane * pitch;
+          // Granules [lo, hi) of the row's span, from its first one.
+          const uint32_t end = off + static_cast<uint32_t>(hidden) * 2;
+          uint32_t lo = 0, hi = (end + 15) & ~15u;
+          // Granules that reach out of the tensor are left out, their elements
+          // of this row stored one by one.
+          const int64_t stride = t == 0 ? a.x_stride : t == 1 ? a.dy_stride : a.extra_stride;
+          if (off > i * stride * 2) lo = 16;
+          if (hi - end > (a.rows - 1 - i) * stride * 2) hi -= 16;
+          hi = max(hi, lo);
+          const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+          if (lo > 0)
+            for (int j = 0; j < hidden && off + 2 * j < lo; ++j) sts_half(at[t] + off + 2 * j, q[j]);
+          if (hi < end)
+            for (int j = hi > off ? static_cast<int>(hi - off) / 2 : 0; j < hidden; ++j)
+              sts_half(at[t] + off + 2 * j, q[j]);
+          from[t] = p - off + lo, at[t] += lo, bytes[t] = hi - lo, total += bytes[t];
+        }
+        total = __reduce_add_sync(~0u, total);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bar, total);
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < kTensors; ++t) {
+          if (bytes[t] > 0) bulk_load(at[t], from[t], bytes[t], bar, pol);
+          if (a.slots < 3 && lane < groups && next + lane < a.rows)
+            prefetch_l2(row_of(t, next + lane), static_cast<uint64_t>(hidden) * 2);
+        }
       }
-      if (!ok) {
-        if (lane == 0) atomicAdd(a.timeouts, 1u);
-        for (int k = 0; k < a.slots; ++k) {  // copies still in flight
-          if (--slot < 0) slot = a.slots - 1, phase ^= 1;
-          mbar_wait_bounded(smem_u32(&full[slot]), phase, kWaitLimitNs / 16);
-        }
+      if (++slot == a.slots) slot = 0, phase ^= 1;
+    }
+    if (!ok) {
+      if (lane == 0) atomicAdd(a.timeouts, 1u);
+      for (int k = 0; k < a.slots; ++k) {  // copies still in flight
+        if (--slot < 0) slot = a.slots - 1, phase ^= 1;
+        mbar_wait_bounded(smem_u32(&full[slot]), phase, kWaitLimitNs / 16);
       }
     }
     __syncwarp();
@@ -237,41 +255,79 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
   float2 acc[W];
 #pragma unroll
   for (int k = 0; k < W; ++k) acc[k] = make_float2(0.f, 0.f);
-  if (!kBulk)
-    for (int s = 0; s < a.slots && first + s * step < a.rows; ++s) fill(first + s * step, s);
-  // Every group writes the same weight row, and reads it after its own barrier.
-  if (a.weight_staged) copy_row(row_mem, a.w);
+  // Every group writes the same weight row, pairs with eight a thread in flight,
+  // and reads it after its own barrier.
+  if (a.weight_staged) {
+    uint32_t* q = reinterpret_cast<uint32_t*>(row_mem);
+    for (int j0 = in; j0 < nvec * 4; j0 += 8 * row_threads) {
+      uint32_t w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int j = 2 * (j0 + u * row_threads);
+        const uint32_t lo = j < hidden ? ld_stream<2>(a.w + j, pol).h : 0;
+        const uint32_t hi = j + 1 < hidden ? ld_stream<2>(a.w + j + 1, pol).h : 0;
+        w[u] = lo | hi << 16;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (j0 + u * row_threads < nvec * 4) q[j0 + u * row_threads] = w[u];
+    }
+  }
   group_barrier(barrier, warps);
   pdl_trigger();
   const uint64_t keep = policy_evict_last();
-  auto load_weight = [&](uint32_t (&w)[4], int v) {
-    if (a.weight_staged) {
-      lds4(w, w_row + v * 16);
+  // Words 4 k to 4 k + 3 of this thread's: one vector, or one word every row_threads.
+  auto inside = [&](int k) { return kVectors ? in + k * row_threads < nvec : in + 4 * k * row_threads < words; };
+  auto word_at = [&](int k, int e) { return in + (4 * k + e) * row_threads; };
+  auto load_weight = [&](uint32_t (&w)[4], int k) {
+    if constexpr (!kVectors) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = word_at(k, e) < words ? lds1(w_row + word_at(k, e) * 4) : 0;
+    } else if (a.weight_staged) {
+      lds4(w, w_row + (in + k * row_threads) * 16);
     } else {
-      const Vec<16> q = ld_weight<16>(a.w + v * 8, keep);
+      const Vec<16> q = ld_weight<16>(a.w + (in + k * row_threads) * 8, keep);
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = q.w[e];
     }
+  };
+  // The same of a row that starts at shared address `at`.
+  auto load_row = [&](uint32_t (&w)[4], uint32_t at, int k) {
+    if constexpr (kVectors) {
+      lds4(w, at + (in + k * row_threads) * 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = word_at(k, e);
+        w[e] = 0;
+        if (j >= words) continue;
+        if (at & 2) w[e] = __funnelshift_r(lds1(at - 2 + 4 * j), lds1(at + 2 + 4 * j), 16);
+        else w[e] = lds1(at + 4 * j);
+        if (2 * j + 1 == hidden) w[e] &= 0xffffu;
+      }
+    }
+  };
+  auto offset_of = [&](const uint16_t* p) {
+    return kVectors ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
   };
 
   const float scale = 1.0f / static_cast<float>(hidden);
   int slot = 0, turn = 0;
   uint32_t phase = 0;
   for (int64_t i = first; i < a.rows; i += step) {
-    const uint32_t xs = ring + slot * slot_bytes, ds = xs + tensor_bytes, es = ds + tensor_bytes;
-    if constexpr (kBulk) {
-      if (!mbar_wait_bounded(smem_u32(&full[slot]), phase)) gave_up[group] = 1;
-    }
+    const uint32_t at = ring + slot * slot_bytes;
+    const uint32_t xs = at + offset_of(row_of(0, i)), ds = at + tensor_bytes + offset_of(row_of(1, i));
+    const uint32_t es = EXTRA ? at + 2 * tensor_bytes + offset_of(row_of(2, i)) : 0;
+    if (!mbar_wait_bounded(smem_u32(&full[slot]), phase)) gave_up[group] = 1;
     float2 ss = make_float2(0.f, 0.f), sd = ss;
     float2 wd[kHold ? W : 1];  // w D, for both passes
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-      const int v = in + k * row_threads;
-      if (v >= nvec) break;
+      if (!inside(k)) break;
       uint32_t x[4], d[4], w[4];
-      lds4(x, xs + v * 16);
-      lds4(d, ds + v * 16);
-      load_weight(w, v);
+      load_row(x, xs, k);
+      load_row(d, ds, k);
+      load_weight(w, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 xf = unpack2<T>(x[e]), p = mul_pair<T>(w[e], d[e]);
@@ -282,24 +338,18 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
     }
     const float2 s =
         row_sum2(make_float2(ss.x + ss.y, sd.x + sd.y), part[turn], tid / 32, warps, barrier, group * warps);
-    if (kBulk && *static_cast<volatile int*>(&gave_up[group])) break;
-    if constexpr (!kBulk) {
-      // The group is past the previous row: its buffer takes the row `slots` on.
-      const int64_t next = i + (a.slots - 1) * step;
-      if (a.slots > 1 && i > first && next < a.rows) fill(next, slot == 0 ? a.slots - 1 : slot - 1);
-    }
+    if (*static_cast<volatile int*>(&gave_up[group])) break;
     const float inv = rsqrtf(s.x * scale + a.eps), mean = s.y * inv * scale;
     const float2 inv2 = make_float2(inv, inv), minus = make_float2(-mean * inv, -mean * inv);
     uint16_t* dx = a.dx + i * a.dx_stride;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-      const int v = in + k * row_threads;
-      if (v >= nvec) break;
+      if (!inside(k)) break;
       uint32_t x[4], d[4], w[4], e4[4];
-      lds4(x, xs + v * 16);
-      lds4(d, ds + v * 16);
-      if constexpr (!kHold) load_weight(w, v);
-      if constexpr (EXTRA) lds4(e4, es + v * 16);
+      load_row(x, xs, k);
+      load_row(d, ds, k);
+      if constexpr (!kHold) load_weight(w, k);
+      if constexpr (EXTRA) load_row(e4, es, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 n = __fmul2_rn(unpack2<T>(x[e]), inv2);
@@ -311,23 +361,25 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
         if constexpr (EXTRA) g = __fadd2_rn(g, unpack2<T>(e4[e]));
         x[e] = pack2<T>(g.x, g.y);
       }
-      if constexpr (kBulk) *reinterpret_cast<uint4*>(dx + v * 8) = make_uint4(x[0], x[1], x[2], x[3]);
-      else sts4(xs + v * 16, x);
-    }
-    if constexpr (kBulk) {
-      __syncwarp();
-      if (tid % 32 == 0) mbar_arrive(smem_u32(&empty[slot]));
-    } else {
-      group_barrier(barrier, warps);
-      const uint16_t* q = reinterpret_cast<const uint16_t*>(ring_p + slot * slot_bytes);
-#pragma unroll 4
-      for (int j = in; j < hidden; j += row_threads) dx[j] = q[j];
-      if (a.slots == 1 && i + step < a.rows) {
-        group_barrier(barrier, warps);
-        fill(i + step, 0);
-        group_barrier(barrier, warps);
+      if constexpr (kVectors) {
+        *reinterpret_cast<uint4*>(dx + (in + k * row_threads) * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = word_at(k, e);
+          uint16_t* q = dx + 2 * j;
+          if (j >= words) continue;
+          if (2 * j + 1 < hidden && (reinterpret_cast<uintptr_t>(q) & 2) == 0) {
+            *reinterpret_cast<uint32_t*>(q) = x[e];
+          } else {
+            q[0] = static_cast<uint16_t>(x[e]);
+            if (2 * j + 1 < hidden) q[1] = static_cast<uint16_t>(x[e] >> 16);
+          }
+        }
       }
     }
+    __syncwarp();
+    if (tid % 32 == 0) mbar_arrive(smem_u32(&empty[slot]));
     turn ^= 1;
     if (++slot == a.slots) slot = 0, phase ^= 1;
   }
@@ -349,15 +401,20 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
   float* out = a.partial + blockIdx.x * static_cast<int64_t>(nvec) * 8;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
-    const int v = in + k * row_threads;
-    if (v >= nvec) break;
-    Vec<32> q;
+    if (!inside(k)) break;
+    if constexpr (kVectors) {
+      Vec<32> q;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      q.w[2 * e] = __float_as_uint(acc[4 * k + e].x);
-      q.w[2 * e + 1] = __float_as_uint(acc[4 * k + e].y);
+      for (int e = 0; e < 4; ++e) {
+        q.w[2 * e] = __float_as_uint(acc[4 * k + e].x);
+        q.w[2 * e + 1] = __float_as_uint(acc[4 * k + e].y);
+      }
+      st_global<32>(out + (in + k * row_threads) * 8, q);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (word_at(k, e) < words) reinterpret_cast<float2*>(out)[word_at(k, e)] = acc[4 * k + e];
     }
-    st_global<32>(out + v * 8, q);
   }
 }
 
@@ -431,7 +488,7 @@ __global__ void __launch_bounds__(256) norm_grad_weight(NormGradArgs a) {
 constexpr int kNormSmem = 220 * 1024;
 struct NormGradPlan {
   int words, row_threads, row_groups, slots, smem;
-  bool bulk, weight_staged;
+  bool vectors, weight_staged;
   int64_t ctas;
 };
 
@@ -445,17 +502,19 @@ struct NormGradPlan {
 NormGradPlan norm_grad_plan(const NormGradArgs& a) {
   auto fits = [&](const void* p, int64_t stride) { return !p || tma_rows(p, a.rows, stride); };
   NormGradPlan p{};
-  p.bulk = a.hidden % 8 == 0 && fits(a.x, a.x_stride) && fits(a.dy, a.dy_stride) && fits(a.dx, a.dx_stride) &&
+  p.vectors = a.hidden % 8 == 0 && fits(a.x, a.x_stride) && fits(a.dy, a.dy_stride) && fits(a.dx, a.dx_stride) &&
            fits(a.extra, a.extra_stride);
-  const int64_t nvec = (a.hidden + 7) / 8, row = nvec * 16, slot = row * (a.extra ? 3 : 2);
+  const int64_t nvec = (a.hidden + 7) / 8, row = nvec * 16, pairs = (a.hidden + 1) / 2;
+  const int64_t slot = (row + (p.vectors ? 0 : 16)) * (a.extra ? 3 : 2);
   for (int words : {4, 8, 16, 32}) {
-    const int64_t threads = round_up((nvec + words / 4 - 1) / (words / 4), 32);
+    const int64_t threads =
+        round_up(p.vectors ? (nvec + words / 4 - 1) / (words / 4) : (pairs + words - 1) / words, 32);
     if (threads > kNormThreads) continue;
     if (words == 4 && threads > 128 && a.rows > 4 * 148) continue;
     int64_t groups = kNormThreads / threads;
     while (groups > 1 && row + 2 * groups * slot > kNormSmem) --groups;
     int64_t slots = (kNormSmem - row) / (groups * slot);
-    p.weight_staged = slots >= 2 || !p.bulk || !aligned(a.w, 16);
+    p.weight_staged = slots >= 2 || !p.vectors || !aligned(a.w, 16);
     if (!p.weight_staged) slots = kNormSmem / (groups * slot);
     if (slots < 1) break;
     p.words = words, p.row_threads = static_cast<int>(threads), p.row_groups = static_cast<int>(groups);
@@ -471,13 +530,13 @@ NormGradPlan norm_grad_plan(const NormGradArgs& a) {
   return p;
 }
 
-template <typename T, bool EXTRA, bool kBulk>
+template <typename T, bool EXTRA, bool kVectors>
 void (*norm_grad_kernel(int words))(NormGradArgs) {
   switch (words) {
-    case 4: return norm_grad_rows<T, 4, EXTRA, kBulk>;
-    case 8: return norm_grad_rows<T, 8, EXTRA, kBulk>;
-    case 16: return norm_grad_rows<T, 16, EXTRA, kBulk>;
-    default: return norm_grad_rows<T, 32, EXTRA, kBulk>;
+    case 4: return norm_grad_rows<T, 4, EXTRA, kVectors>;
+    case 8: return norm_grad_rows<T, 8, EXTRA, kVectors>;
+    case 16: return norm_grad_rows<T, 16, EXTRA, kVectors>;
+    default: return norm_grad_rows<T, 32, EXTRA, kVectors>;
   }
 }
 
@@ -487,7 +546,7 @@ int launch_norm_grad(const NormGradArgs& a, const NormGradPlan& p, const DeviceI
   const char* what = "rms_norm_backward";
   int st = HPRN_OK;
   if (a.rows > 0 && p.words > 0) {
-    auto fn = p.bulk ? (a.extra ? norm_grad_kernel<T, true, true>(p.words) : norm_grad_kernel<T, false, true>(p.words))
+    auto fn = p.vectors ? (a.extra ? norm_grad_kernel<T, true, true>(p.words) : norm_grad_kernel<T, false, true>(p.words))
                      : (a.extra ? norm_grad_kernel<T, true, false>(p.words) : norm_grad_kernel<T, false, false>(p.words));
     if ((st = allow_smem(dev, reinterpret_cast<const void*>(fn), kNormSmem, what)) != HPRN_OK) return st;
     st = launch_rows_smem(fn, dim3(static_cast<unsigned>(p.ctas)),
