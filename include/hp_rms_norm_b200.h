@@ -374,12 +374,16 @@ HPRN_API int hprn_rms_norm_plan(int64_t rows, int64_t hidden, int dtype, const v
 HPRN_API int hprn_set_plan_override(const char* plan);
 
 /*
- * No reference counterpart.  Kernels that stage rows through TMA bulk copies
- * (plan kind tma, reached only through a plan override) wait on mbarriers with
- * a bound (one second); a CTA that gives up a wait leaves the row it gave up
- * on and its remaining rows untouched (input and residual as they were) and
- * counts itself here, on its device.  The call that launched it still returns
- * HPRN_OK: a caller that forces a tma plan must read this count.
+ * No reference counterpart.  Kernels that wait on mbarriers for asynchronous
+ * copies and matrix instructions do so with a bound (one second): those that
+ * stage rows of hprn_rms_norm* through TMA bulk copies (plan kind tma, reached
+ * only through a plan override), the matrix products of hprn_gated_linear* and
+ * hprn_linear_cross_entropy*, and hprn_rms_norm_backward.  A CTA that gives up
+ * a wait stops, once its copies in flight have landed, and counts itself here,
+ * on its device: in the tma plans it leaves the row it gave up on and its
+ * remaining rows untouched (input and residual as they were), in the others
+ * the outputs it had not written.  The call that launched it still returns
+ * HPRN_OK.  No wait gives up on a GPU that works.
  * Writes the current device's count into *count and, if `reset` is non-zero,
  * clears it.  Synchronous; synchronise the streams that launched the kernels
  * first.  A non-zero count means the launches since the last reset produced

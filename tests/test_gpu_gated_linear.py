@@ -141,6 +141,34 @@ def test_streams_and_graphs(cuda):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_no_wait_gave_up(cuda):
+    """The products' and the norm's backward kernels wait with a limit; none may run out."""
+    import ctypes
+
+    from hp_rms_norm_b200 import capi
+
+    x, w, dout = make(700, 192, 130, torch.bfloat16, cuda)
+    hp.gated_linear(x, w)
+    hp.gated_linear_backward(dout, x, w)
+    hp.rms_norm_backward(x, x, x[0].contiguous(), 1e-6)
+    t = torch.zeros(700, dtype=torch.int64, device=cuda)
+    hp.linear_cross_entropy(x, w, t)
+    torch.cuda.synchronize()
+    count = ctypes.c_uint(7)
+    assert capi.load().hprn_wait_timeouts(ctypes.byref(count), 0) == 0 and count.value == 0
+
+
+@pytest.mark.parametrize("rows", [600, 2100])
+def test_unaligned_rows_in_large_products(cuda, rows):
+    """Operands that are copied to aligned rows, and outputs on odd addresses."""
+    x, w, dout = make(rows, 129, 140, torch.float16, cuda)
+    check_forward(hp.gated_linear(x, w), x, w, "silu", f"{rows}")
+    check_backward(*hp.gated_linear_backward(dout, x, w), dout, x, w, "silu", f"{rows}")
+    x, w, dout = make(rows, 136, 140, torch.bfloat16, cuda)  # 16-byte rows inside 32-byte sectors
+    check_forward(hp.gated_linear(x, w), x, w, "silu", f"{rows}")
+    check_backward(*hp.gated_linear_backward(dout, x, w), dout, x, w, "silu", f"{rows}")
+
+
 def test_refusals(cuda):
     x, w, dout = make(4, 32, 16, torch.bfloat16, cuda)
     for bad in (lambda: hp.gated_linear(x.cpu(), w), lambda: hp.gated_linear(x, w.half()),
