@@ -113,11 +113,12 @@ __device__ __forceinline__ void sts_half(uint32_t addr, uint16_t h) {
 // ordinary loads); threads take single words, neighbouring threads
 // neighbouring ones, put together from two where the row starts on an odd element.
 //
-// Registers hold dw's sums (2 W floats) and, up to 16 words, w D between the
-// two passes.  4096 x 8192 with E: 48.0 us (0.87 of a copy of the same bytes),
+// Registers hold dw's sums (2 W floats) and, up to 8 words, w D between the
+// two passes (held at 16 words it spilled: 4096 x 16384 106 us instead of 93).
+// 4096 x 8192 with E: 48.0 us (0.87 of a copy of the same bytes),
 // against 55.8 with the rows themselves in registers, which spilled or kept
-// one row a CTA in flight.  4096 x 5001 with E: 90 us, bound by issue, against 155 with rows copied
-// element by element.
+// one row a CTA in flight.  4096 x 5001 with E: 72 us, bound by issue, against
+// 155 with rows copied element by element.
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies
 // still in flight, counted in `timeouts`; the rows it had not finished keep
@@ -128,7 +129,7 @@ template <typename T, int W, bool EXTRA, bool kVectors>
 __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradArgs a) {
   constexpr int kVecs = W / 4;
   constexpr int kTensors = EXTRA ? 3 : 2;
-  constexpr bool kHold = W <= 16;
+  constexpr bool kHold = W <= 8;
   extern __shared__ __align__(128) unsigned char row_mem[];
   __shared__ __align__(8) uint64_t full[kMostSlots], empty[kMostSlots];
   __shared__ float part[2][2][32];  // a group's warps follow those of the groups before it
@@ -492,42 +493,47 @@ struct NormGradPlan {
   int64_t ctas;
 };
 
-// One CTA per SM.  The fewest elements a thread that keep a row within the CTA's
-// 512 threads, from 8 for short rows (up to 1024) or few of them, from 16 else:
-// 4096 x 4096 with E takes 25.5 us with 16 elements and two rows at once, 30.7
-// with 8 and one; 4096 x 1024 13.7 with 8, 14.8 with 16; 512 x 4096 9.6 with 8,
-// 10.5 with 16.  As many rows at once as have threads and two buffers each.
-// The weight is kept in shared memory beside the rows unless that leaves them
-// fewer than two buffers.
+// One CTA per SM.  The words a thread decide how many of the CTA's 512 threads
+// have work: a row takes as many as it has, and as many rows go at once as have
+// threads and two buffers each.  The fewest words that employ 416 threads or
+// more win, else the most threads; 4 words (the shortest way through a row)
+// only for rows up to 1024 elements or few rows: 4096 x 4096 with E takes
+// 25.5 us with 8 words and two rows at once, 30.7 with 4 and one; 4096 x 1024
+// 13.7 with 4, 14.8 with 8; 512 x 4096 9.6 with 4, 10.5 with 8; 4096 x 16448
+// 95 with 20 words and 416 threads, about 160 with 32 and 288.  The weight is kept in shared memory beside the rows unless that
+// leaves them fewer than two buffers.
 NormGradPlan norm_grad_plan(const NormGradArgs& a) {
   auto fits = [&](const void* p, int64_t stride) { return !p || tma_rows(p, a.rows, stride); };
-  NormGradPlan p{};
-  p.vectors = a.hidden % 8 == 0 && fits(a.x, a.x_stride) && fits(a.dy, a.dy_stride) && fits(a.dx, a.dx_stride) &&
-           fits(a.extra, a.extra_stride);
+  const bool vectors = a.hidden % 8 == 0 && fits(a.x, a.x_stride) && fits(a.dy, a.dy_stride) &&
+                       fits(a.dx, a.dx_stride) && fits(a.extra, a.extra_stride);
   const int64_t nvec = (a.hidden + 7) / 8, row = nvec * 16, pairs = (a.hidden + 1) / 2;
-  const int64_t slot = (row + (p.vectors ? 0 : 16)) * (a.extra ? 3 : 2);
-  for (int words : {4, 8, 16, 32}) {
-    const int64_t threads =
-        round_up(p.vectors ? (nvec + words / 4 - 1) / (words / 4) : (pairs + words - 1) / words, 32);
-    if (threads > kNormThreads) continue;
-    if (words == 4 && threads > 128 && a.rows > 4 * 148) continue;
+  const int64_t slot = (row + (vectors ? 0 : 16)) * (a.extra ? 3 : 2);
+  NormGradPlan best{};
+  best.ctas = a.rows < 64 ? a.rows : 64;
+  for (int words : {4, 8, 12, 16, 20, 24, 32}) {
+    const int64_t threads = round_up(vectors ? (nvec + words / 4 - 1) / (words / 4) : (pairs + words - 1) / words, 32);
+    const bool few = a.rows <= 4 * 148;
+    if (threads > kNormThreads || (words == 4 && threads > 128 && !few)) continue;
     int64_t groups = kNormThreads / threads;
     while (groups > 1 && row + 2 * groups * slot > kNormSmem) --groups;
     int64_t slots = (kNormSmem - row) / (groups * slot);
-    p.weight_staged = slots >= 2 || !p.vectors || !aligned(a.w, 16);
-    if (!p.weight_staged) slots = kNormSmem / (groups * slot);
+    const bool staged = slots >= 2 || !vectors || !aligned(a.w, 16);
+    if (!staged) slots = kNormSmem / (groups * slot);
     if (slots < 1) break;
+    if (threads * groups <= best.row_threads * best.row_groups) continue;
+    NormGradPlan p{};
+    p.vectors = vectors, p.weight_staged = staged;
     p.words = words, p.row_threads = static_cast<int>(threads), p.row_groups = static_cast<int>(groups);
     p.slots = static_cast<int>(slots < kMostSlots ? slots : kMostSlots);
-    const int64_t ring = (p.weight_staged ? row : 0) + groups * p.slots * slot;
+    const int64_t ring = (staged ? row : 0) + groups * p.slots * slot;
     const int64_t sums = groups > 1 ? words * threads * groups * 8 : 0;
     p.smem = static_cast<int>(ring > sums ? ring : sums);
     const int64_t need = (a.rows + groups - 1) / groups;
     p.ctas = need < 148 ? need : 148;
-    return p;
+    best = p;
+    if (few || threads * groups >= 416) break;
   }
-  p.ctas = a.rows < 64 ? a.rows : 64;
-  return p;
+  return best;
 }
 
 template <typename T, bool EXTRA, bool kVectors>
@@ -535,7 +541,10 @@ void (*norm_grad_kernel(int words))(NormGradArgs) {
   switch (words) {
     case 4: return norm_grad_rows<T, 4, EXTRA, kVectors>;
     case 8: return norm_grad_rows<T, 8, EXTRA, kVectors>;
+    case 12: return norm_grad_rows<T, 12, EXTRA, kVectors>;
     case 16: return norm_grad_rows<T, 16, EXTRA, kVectors>;
+    case 20: return norm_grad_rows<T, 20, EXTRA, kVectors>;
+    case 24: return norm_grad_rows<T, 24, EXTRA, kVectors>;
     default: return norm_grad_rows<T, 32, EXTRA, kVectors>;
   }
 }

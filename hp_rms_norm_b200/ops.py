@@ -18,6 +18,8 @@ by this package's compiled ``_C`` extension.
 """
 import torch
 
+_ops = torch.ops.hp_rms_norm
+
 
 def hp_rms_norm(
     input,
@@ -141,7 +143,7 @@ def gated_linear(input, weight, act="silu", out=None, gate_up=None):
     ``gated_linear_backward``.  Returns ``out`` [..., d]."""
     if out is None:
         out = input.new_empty(input.shape[:-1] + (weight.shape[0] // 2,))
-    torch.ops.hp_rms_norm.gated_linear.default(out, gate_up, input, weight, act)
+    _ops.gated_linear.default(out, gate_up, input, weight, act)
     return out
 
 
@@ -151,7 +153,7 @@ def gated_linear_backward(grad_out, input, weight, act="silu", gate_up=None):
     it they are computed again."""
     grad_input = _new_like(input)
     grad_weight = _new_like(weight)
-    torch.ops.hp_rms_norm.gated_linear_backward.default(grad_input, grad_weight, grad_out, input,
+    _ops.gated_linear_backward.default(grad_input, grad_weight, grad_out, input,
                                                         weight, gate_up, act)
     return grad_input, grad_weight
 
@@ -164,7 +166,7 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100):
     ``linear_cross_entropy_backward`` takes."""
     loss = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
     lse = torch.empty_like(loss)
-    torch.ops.hp_rms_norm.linear_cross_entropy.default(loss, lse, input, weight, target,
+    _ops.linear_cross_entropy.default(loss, lse, input, weight, target,
                                                        ignore_index)
     return loss, lse
 
@@ -175,7 +177,7 @@ def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, ignore_
     vocabulary at a time."""
     grad_input = _new_like(input)
     grad_weight = _new_like(weight)
-    torch.ops.hp_rms_norm.linear_cross_entropy_backward.default(
+    _ops.linear_cross_entropy_backward.default(
         grad_input, grad_weight, grad_loss, input, weight, target, lse, ignore_index)
     return grad_input, grad_weight
 
@@ -187,7 +189,7 @@ def rms_norm_backward(grad_out, input, weight, eps, grad_residual=None):
     addends."""
     grad_input = _new_like(input)
     grad_weight = _new_like(weight)
-    torch.ops.hp_rms_norm.rms_norm_backward.default(grad_input, grad_weight, grad_out, input,
+    _ops.rms_norm_backward.default(grad_input, grad_weight, grad_out, input,
                                                     weight, grad_residual, eps)
     return grad_input, grad_weight
 
@@ -198,7 +200,7 @@ def grad_norm(grads):
     if not len(grads):
         return torch.zeros((), dtype=torch.float32)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    torch.ops.hp_rms_norm.grad_norm.default(norm, grads)
+    _ops.grad_norm.default(norm, grads)
     return norm
 
 
@@ -210,7 +212,7 @@ def clip_grad_norm(grads, max_norm, out=None):
     if not len(grads):
         return torch.zeros((), dtype=torch.float32)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    torch.ops.hp_rms_norm.clip_grad_norm.default(grads if out is None else out, norm, grads,
+    _ops.clip_grad_norm.default(grads if out is None else out, norm, grads,
                                                  max_norm)
     return norm
 
