@@ -1,6 +1,8 @@
 """The differentiable forms against torch's own autograd in 64 bits, and the training example."""
 import importlib.util
 import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -133,3 +135,41 @@ def test_example_gradients_match_plain_torch(cuda):
     for n, got, exact in zip(names, grads, want):
         rel = float((got.double() - exact).norm() / exact.norm())
         assert rel <= 40 ** 0.5 * 2 ** -8, (n, rel)
+
+
+def test_first_calls_inside_graph_capture(cuda):
+    worker = os.path.join(ROOT, "tests", "graph_first_training_call_worker.py")
+    r = subprocess.run([sys.executable, worker], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "OK" in r.stdout, r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(cuda):
+    """A weight of more than 2^31 elements: the last vocabulary rows, and their gradients."""
+    import hp_rms_norm_b200 as hp
+
+    rows, hidden, vocab = 5, 2048, 1_050_000
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.randn(rows, hidden, generator=g, device=cuda).bfloat16()
+    w = torch.empty(vocab, hidden, dtype=torch.bfloat16, device=cuda)
+    w.normal_(0, hidden ** -0.5, generator=g)
+    t = torch.tensor([0, 1, vocab - 1, vocab - 2, 777_777], device=cuda)
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    logits = torch.cat([x.double() @ p.double().T for p in w.split(70_000)], 1)
+    want = torch.logsumexp(logits, 1)
+    # fp32 sums of `hidden` terms, and of `vocab` exponentials in float32 tiles
+    assert (lse.double() - want).abs().max() <= hidden * R.F32 * 40 + 64 * R.F32 * 20
+    assert (loss.double() - (want - logits.gather(1, t[:, None])[:, 0])).abs().max() <= hidden * R.F32 * 80
+    c = torch.ones(rows, device=cuda)
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    s = torch.exp(logits - want[:, None])
+    s[torch.arange(rows, device=cuda), t] -= 1
+    want_x = sum(a @ p.double() for a, p in zip(s.split(70_000, 1), w.split(70_000)))
+    R.assert_near(dx, want_x, R.U[x.dtype] * torch.sqrt(s.square().sum(1, keepdim=True)) * hidden ** -0.5 * 4
+                  * torch.ones_like(want_x), "dx")
+    for rows_of in (slice(0, 64), slice(777_700, 777_800), slice(vocab - 64, vocab)):
+        part = s[:, rows_of].T
+        R.assert_near(dw[rows_of], part @ x.double(), R.rounding_noise(part, x.double(), x.dtype), "dw")
+    half = vocab // 2
+    out = hp.gated_linear(x, w, "silu")
+    gate, up = x.double() @ w[half - 50:half].double().T, x.double() @ w[-50:].double().T
+    R.assert_near(out[:, -50:], torch.nn.functional.silu(gate) * up, hidden * R.F32 * up.abs(), "gated")
