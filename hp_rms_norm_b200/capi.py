@@ -61,6 +61,7 @@ EXPORTED = (
     "hprn_rms_norm_backward",
     "hprn_grad_norm",
     "hprn_grad_clip",
+    "hprn_clip_grad_norm",
 )
 
 
@@ -135,10 +136,11 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.hprn_rms_norm_backward.argtypes = [vp] * 6 + [i64] * 6 + [ctypes.c_double, c_int, vp, wsp,
                                                                 vp, u32]
     lib.hprn_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, vp, wsp, vp, u32]
+    lib.hprn_clip_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, ctypes.c_double, vp, wsp, vp, u32]
     lib.hprn_grad_clip.argtypes = [ctypes.POINTER(Grad), i64, vp, ctypes.c_double, vp, u32]
     for fn in (lib.hprn_gated_linear, lib.hprn_gated_linear_backward, lib.hprn_linear_cross_entropy,
                lib.hprn_linear_cross_entropy_backward, lib.hprn_rms_norm_backward,
-               lib.hprn_grad_norm, lib.hprn_grad_clip):
+               lib.hprn_grad_norm, lib.hprn_grad_clip, lib.hprn_clip_grad_norm):
         fn.restype = c_int
     _lib = lib
     return lib

@@ -193,20 +193,33 @@ __global__ void __launch_bounds__(kClipThreads) grad_square_sums(const __grid_co
   }
 }
 
-__global__ void __launch_bounds__(1024) grad_norm_join(const float* partial, int64_t n, float* norm) {
+// The root of the sum of n partial sums, by THREADS threads, in the order of
+// 1024 of them: the same bits whichever kernel joins them.  Thread 0 has it.
+template <int THREADS>
+__device__ __forceinline__ float join_norm(const float* partial, int64_t n) {
+  constexpr int kShares = 1024 / THREADS;
   __shared__ double part[32];
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int v = 0; v < kShares; ++v) {
+    const int share = threadIdx.x + v * THREADS;
+    double s = 0.0;
+#pragma unroll 8
+    for (int64_t k = share; k < n; k += 1024) s += static_cast<double>(partial[k]);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    if (lane == 0) part[share / 32] = s;
+  }
+  __syncthreads();
+  double s = part[lane];
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return static_cast<float>(sqrt(s));
+}
+
+__global__ void __launch_bounds__(1024) grad_norm_join(const float* partial, int64_t n, float* norm) {
   pdl_wait();
   pdl_trigger();
-  double s = 0.0;
-#pragma unroll 8
-  for (int64_t k = threadIdx.x; k < n; k += 1024) s += static_cast<double>(partial[k]);
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  s = part[threadIdx.x];
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
+  const float r = join_norm<1024>(partial, n);
+  if (threadIdx.x == 0) *norm = r;
 }
 
 template <int IN, int OUT>
@@ -243,16 +256,25 @@ __device__ __forceinline__ void chunk_scale(const GradEntry& e, int64_t lo, int6
 
 // The chunks are taken last to first: the norm's pass read the last ones last,
 // so they are the ones L2 still holds.
+//
+// With `partial`, every CTA joins the norm's `parts` partial sums for itself and
+// one writes it down: a launch less where there are few (33 tensors of 3.5
+// million gradients 18.9 us a call instead of 20.5).
+constexpr int64_t kFewParts = 2048;
+
 template <int N>
-__global__ void __launch_bounds__(kClipThreads) grad_scale(const __grid_constant__ GradTable<N> g,
-                                                           const float* norm, float max_norm) {
+__global__ void __launch_bounds__(kClipThreads)
+    grad_scale(const __grid_constant__ GradTable<N> g, const float* partial, int64_t parts, float* norm,
+               float max_norm) {
   const int64_t chunk = static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x;
   const GradEntry& e = find_entry(g, chunk);
   const int64_t lo = (chunk - e.first_chunk) * g.chunk;
   const int64_t hi = min(lo + g.chunk, e.count);
   pdl_wait();
   // min(1, .) written so that a NaN norm gives a NaN factor.
-  const float r = max_norm / (*norm + 1e-6f);
+  const float length = partial ? join_norm<kClipThreads>(partial, parts) : *norm;
+  if (partial && blockIdx.x == 0 && threadIdx.x == 0) *norm = length;
+  const float r = max_norm / (length + 1e-6f);
   const float f = r >= 1.f ? 1.f : r;
   if (f == 1.f && e.in == e.out) return;  // in place, and nothing to change
   with_type(e.in_type, [&](auto in) {
@@ -336,21 +358,50 @@ int for_tables(const hprn_grad* g, int64_t count, F&& f) {
 }  // namespace
 }  // namespace hprn
 
-extern "C" {
+namespace hprn {
+namespace {
 
-int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* workspace,
-                   int64_t* workspace_bytes, void* stream, unsigned flags) {
-  using namespace hprn;
-  if (flags & ~static_cast<unsigned>(HPRN_LAUNCH_PDL | HPRN_WORKSPACE_QUERY))
-    return fail(HPRN_ERR_INVALID_ARGUMENT, "unknown launch flags");
-  if (!workspace_bytes) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace_bytes pointer required");
-  int st = check_grads(grads, count, false);
-  if (st != HPRN_OK) return st;
+// The squares' pass; leaves one partial sum a chunk.
+int launch_squares(const hprn_grad* grads, int64_t count, float* partial, cudaStream_t cs, unsigned flags,
+                   const char* what) {
+  int64_t at = 0;
+  return for_tables(grads, count, [&](const auto& t, int64_t chunks) {
+    float* part = partial + at;
+    at += chunks;
+    constexpr int kTensors = std::decay_t<decltype(t)>::kSize;
+    return launch_rows(grad_square_sums<kTensors>, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs,
+                       flags, what, t, part);
+  });
+}
+
+int launch_scale(const hprn_grad* grads, int64_t count, const float* partial, int64_t parts, float* norm,
+                 double max_norm, cudaStream_t cs, unsigned flags, const char* what) {
+  return for_tables(grads, count, [&](const auto& t, int64_t chunks) {
+    constexpr int kTensors = std::decay_t<decltype(t)>::kSize;
+    return launch_rows(grad_scale<kTensors>, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
+                       what, t, partial, parts, norm, static_cast<float>(max_norm));
+  });
+}
+
+int64_t parts_of(const hprn_grad* grads, int64_t count) {
   const int64_t chunk = chunk_elems(total_of(grads, count));
   int64_t total = 0;
   for (int64_t k = 0; k < count; ++k) total += chunks_of(grads[k], chunk);
+  return total;
+}
+
+// hprn_grad_norm, and with `clip` the scaling after it.
+int norm_and_clip(float* norm, const hprn_grad* grads, int64_t count, bool clip, double max_norm,
+                  void* workspace, int64_t* workspace_bytes, void* stream, unsigned flags, const char* what) {
+  if (flags & ~static_cast<unsigned>(HPRN_LAUNCH_PDL | HPRN_WORKSPACE_QUERY))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "unknown launch flags");
+  if (!workspace_bytes) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace_bytes pointer required");
+  if (clip && !(max_norm >= 0)) return fail(HPRN_ERR_INVALID_ARGUMENT, "max_norm must be >= 0");
+  int st = check_grads(grads, count, clip);
+  if (st != HPRN_OK) return st;
+  const int64_t parts = parts_of(grads, count);
   Workspace ws(workspace, *workspace_bytes);
-  float* partial = ws.take<float>(total);
+  float* partial = ws.take<float>(parts);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
@@ -361,16 +412,32 @@ int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* wor
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  int64_t at = 0;
-  st = for_tables(grads, count, [&](const auto& t, int64_t chunks) {
-    float* part = partial + at;
-    at += chunks;
-    constexpr int kTensors = std::decay_t<decltype(t)>::kSize;
-    return launch_rows(grad_square_sums<kTensors>, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
-                       "grad_norm", t, part);
-  });
-  if (st != HPRN_OK) return st;
-  return launch_rows(grad_norm_join, dim3(1), dim3(1024), cs, flags, "grad_norm", partial, total, norm);
+  if ((st = launch_squares(grads, count, partial, cs, flags, what)) != HPRN_OK) return st;
+  // In place, a joining CTA must not find a gradient already scaled: the
+  // partial sums are complete before the first of them starts.
+  if (clip && parts > 0 && parts <= kFewParts)
+    return launch_scale(grads, count, partial, parts, norm, max_norm, cs, flags, what);
+  st = launch_rows(grad_norm_join, dim3(1), dim3(1024), cs, flags, what, partial, parts, norm);
+  if (st != HPRN_OK || !clip) return st;
+  st = launch_scale(grads, count, nullptr, 0, norm, max_norm, cs, flags, what);
+  return st == HPRN_OK ? ok() : st;
+}
+
+}  // namespace
+}  // namespace hprn
+
+extern "C" {
+
+int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, void* workspace,
+                   int64_t* workspace_bytes, void* stream, unsigned flags) {
+  return hprn::norm_and_clip(norm, grads, count, false, 0.0, workspace, workspace_bytes, stream, flags,
+                             "grad_norm");
+}
+
+int hprn_clip_grad_norm(float* norm, const hprn_grad* grads, int64_t count, double max_norm, void* workspace,
+                        int64_t* workspace_bytes, void* stream, unsigned flags) {
+  return hprn::norm_and_clip(norm, grads, count, true, max_norm, workspace, workspace_bytes, stream, flags,
+                             "clip_grad_norm");
 }
 
 int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm, double max_norm,
@@ -386,12 +453,8 @@ int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm, dou
   if (!aligned(norm, 4)) return fail(HPRN_ERR_INVALID_ARGUMENT, "norm must be 4-byte aligned");
   const DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != HPRN_OK) return st;
-  cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  st = for_tables(grads, count, [&](const auto& t, int64_t chunks) {
-    constexpr int kTensors = std::decay_t<decltype(t)>::kSize;
-    return launch_rows(grad_scale<kTensors>, dim3(static_cast<unsigned>(chunks)), dim3(kClipThreads), cs, flags,
-                       "grad_clip", t, norm, static_cast<float>(max_norm));
-  });
+  st = launch_scale(grads, count, nullptr, 0, const_cast<float*>(norm), max_norm,
+                    static_cast<cudaStream_t>(stream), flags, "grad_clip");
   return st == HPRN_OK ? ok() : st;
 }
 

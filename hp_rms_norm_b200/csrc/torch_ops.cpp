@@ -618,26 +618,21 @@ std::vector<hprn_grad> grad_table(at::TensorList grads, const at::TensorList* ou
   return table;
 }
 
-void run_grad_norm(at::Tensor& norm, const std::vector<hprn_grad>& table) {
-  with_workspace(norm, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
-    return hprn_grad_norm(norm.data_ptr<float>(), table.data(), static_cast<int64_t>(table.size()),
-                          ws, bytes, s, flags);
-  });
-}
-
 void grad_norm(at::Tensor& norm, at::TensorList grads) {
-  run_grad_norm(norm, grad_table(grads, nullptr, norm));
+  const std::vector<hprn_grad> table = grad_table(grads, nullptr, norm);
+  with_workspace(norm, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_grad_norm(norm.data_ptr<float>(), table.data(), static_cast<int64_t>(table.size()), ws,
+                          bytes, s, flags);
+  });
 }
 
 void clip_grad_norm(at::TensorList out, at::Tensor& norm, at::TensorList grads, double max_norm) {
   TORCH_CHECK(out.size() == grads.size(), "out must have one tensor per gradient");
-  TORCH_CHECK(max_norm >= 0, "max_norm must be >= 0");
   const std::vector<hprn_grad> table = grad_table(grads, &out, norm);
-  run_grad_norm(norm, table);
-  const c10::cuda::CUDAGuard guard(norm.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(norm.device().index()).stream();
-  check_status(hprn_grad_clip(table.data(), static_cast<int64_t>(table.size()),
-                              norm.data_ptr<float>(), max_norm, stream, HPRN_LAUNCH_DEFAULT));
+  with_workspace(norm, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_clip_grad_norm(norm.data_ptr<float>(), table.data(), static_cast<int64_t>(table.size()),
+                               max_norm, ws, bytes, s, flags);
+  });
 }
 
 void gated_linear_meta(at::Tensor&, c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,

@@ -328,6 +328,13 @@ HPRN_API int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, 
 HPRN_API int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm,
                             double max_norm, void* stream, unsigned flags);
 
+/*
+ * hprn_grad_norm and hprn_grad_clip in one call, the same results.
+ */
+HPRN_API int hprn_clip_grad_norm(float* norm, const hprn_grad* grads, int64_t count,
+                                 double max_norm, void* workspace, int64_t* workspace_bytes,
+                                 void* stream, unsigned flags);
+
 /* Message for the last non-OK status returned on this thread ("" if none). */
 HPRN_API const char* hprn_last_error(void);
 
