@@ -146,24 +146,81 @@ __global__ void __launch_bounds__(256)
   loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - (parts > 0 ? target_logit[i] : 0.f);
 }
 
-// c_max, and what the sums are multiplied by: c_max / held.
-__global__ void __launch_bounds__(1024) loss_grad_scale(const float* grad_loss, const int64_t* target,
-                                                        int64_t ignore, int64_t rows, float held, float* out) {
-  __shared__ float part[32];
+// What the backward products need first.  X with the ignored rows zeroed (on
+// aligned rows): a row that is left out leaves dW alone whatever it holds, where
+// 0 times its infinities or NaN would not.  And, by the first CTA, c_max and
+// what the sums are multiplied by, c_max / held.  A warp takes kPrepareSpan
+// elements of a row, all its loads in flight: 16 bytes a lane where X's rows
+// start on 16-byte boundaries, else two 2-byte loads a word.
+constexpr int kPrepareSpan = 512;
+
+struct LossPrepareArgs {
+  const uint16_t* x;
+  uint16_t* out;
+  int64_t x_ld, out_ld, rows, hidden, spans;  // spans of a row
+  bool vectors;
+  const float* grad_loss;
+  const int64_t* target;
+  int64_t ignore;
+  float held;
+  float* scale;
+};
+
+__global__ void __launch_bounds__(256) loss_grad_prepare(LossPrepareArgs a) {
+  __shared__ float part[8];
   pdl_wait();
   pdl_trigger();
-  float m = 0.f;
-  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
-    if (target[i] != ignore) m = fmaxf(m, fabsf(grad_loss[i]));
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  m = part[threadIdx.x];
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  // An infinite gradient spoils its own row and the weight's, not the other rows.
-  if (!(m > 0.f && m < INFINITY)) m = 1.f;
-  if (threadIdx.x == 0) out[0] = m, out[1] = m / held;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  if (blockIdx.x == 0) {
+    float m = 0.f;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < a.rows; i += 256)
+      if (a.target[i] != a.ignore) m = fmaxf(m, fabsf(a.grad_loss[i]));
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    if (lane == 0) part[warp] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int k = 1; k < 8; ++k) m = fmaxf(m, part[k]);
+      // An infinite gradient spoils its own row and the weight's, not the other rows.
+      if (!(m > 0.f && m < INFINITY)) m = 1.f;
+      a.scale[0] = m, a.scale[1] = m / a.held;
+    }
+  }
+  const int64_t all = a.rows * a.spans;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 8 + warp; e < all; e += static_cast<int64_t>(gridDim.x) * 8) {
+    const int64_t i = e / a.spans, j0 = (e - i * a.spans) * kPrepareSpan;
+    const uint16_t* p = a.x + i * a.x_ld + j0;
+    uint16_t* q = a.out + i * a.out_ld + j0;
+    const int width = static_cast<int>(min(static_cast<int64_t>(kPrepareSpan), a.out_ld - j0));  // a multiple of 16
+    int inside = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kPrepareSpan), a.hidden - j0)));
+    if (a.target[i] == a.ignore) inside = 0;
+    if (a.vectors && inside % 8 == 0) {
+      uint4 v[kPrepareSpan / 256];
+#pragma unroll
+      for (int k = 0; k < kPrepareSpan / 256; ++k) {
+        const int j = k * 256 + lane * 8;
+        v[k] = j < inside ? *reinterpret_cast<const uint4*>(p + j) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kPrepareSpan / 256; ++k) {
+        const int j = k * 256 + lane * 8;
+        if (j < width) *reinterpret_cast<uint4*>(q + j) = v[k];
+      }
+      continue;
+    }
+    uint32_t w[kPrepareSpan / 64];
+#pragma unroll
+    for (int k = 0; k < kPrepareSpan / 64; ++k) {
+      const int j = k * 64 + lane * 2;
+      const uint32_t lo = j < inside ? p[j] : 0, hi = j + 1 < inside ? p[j + 1] : 0;
+      w[k] = lo | hi << 16;
+    }
+#pragma unroll
+    for (int k = 0; k < kPrepareSpan / 64; ++k) {
+      const int j = k * 64 + lane * 2;
+      if (j < width) *reinterpret_cast<uint32_t*>(q + j) = w[k];
+    }
+  }
 }
 
 template <typename T>
@@ -320,7 +377,8 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       (vocab > 1 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
   Workspace ws(workspace, *workspace_bytes);
-  const AlignedRows x(ws, input, rows, hidden, input_row_stride, 2 * vocab);
+  const int64_t x_ld = round_up(hidden, 16);
+  uint16_t* x = ws.take<uint16_t>(rows * x_ld);  // X without the ignored rows
   const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride, rows);
   const Pieces pieces = pieces_of(rows, vocab);
   uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
@@ -354,10 +412,17 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_cross_entropy_backward";
-  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
+  if ((st = w.prepare(cs, flags)) != HPRN_OK) return st;
   if (rows > 0) {
-    st = launch_rows(loss_grad_scale, dim3(1), dim3(1024), cs, flags, what, grad_loss, target, ignore_index,
-                     rows, held, scale);
+    LossPrepareArgs a{};
+    a.x = static_cast<const uint16_t*>(input), a.x_ld = input_row_stride;
+    a.out = x, a.out_ld = x_ld, a.rows = rows, a.hidden = hidden;
+    a.spans = (x_ld + kPrepareSpan - 1) / kPrepareSpan;
+    a.vectors = tma_rows(input, rows, input_row_stride);
+    a.grad_loss = grad_loss, a.target = target, a.ignore = ignore_index, a.held = held, a.scale = scale;
+    const int64_t ctas = (rows * a.spans + 7) / 8, most = 16 * dev->sm_count;
+    st = launch_rows(loss_grad_prepare, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), cs,
+                     flags, what, a);
     if (st != HPRN_OK) return st;
   }
   auto all = [&](auto t) {
@@ -370,7 +435,7 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       const int64_t cols = vocab - first < pieces.cols ? vocab - first : pieces.cols;
       const uint16_t* wp = w.data() + first * w.ld();
       Product q;
-      q.a = {x.data(), x.ld()};
+      q.a = {x, x_ld};
       q.b = {wp, w.ld()};
       q.m = rows, q.n = cols, q.depth = hidden;
       LossGradEpilogue<T> g;
@@ -387,7 +452,7 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       e.scale = rows > 0 ? scale + 1 : nullptr;
       if ((r = to_input.launch<T>(q, e, cs, flags, what)) != HPRN_OK) break;
 
-      q.b = {x.data(), x.ld()};
+      q.b = {x, x_ld};
       q.m = cols, q.depth = rows;
       e.out = Out16(static_cast<uint16_t*>(grad_weight) + first * grad_weight_row_stride,
                     grad_weight_row_stride, hidden);

@@ -102,9 +102,10 @@ __global__ void __launch_bounds__(256) copy_rows(RowCopies both) {
 int AlignedRows::prepare(const AlignedRows& x, const AlignedRows& w, cudaStream_t stream, unsigned flags) {
   RowCopies both = {};
   int64_t spans = 0;
-  for (const AlignedRows* a : {&x, &w}) {
-    RowCopy& c = both.c[a == &w];
-    c.dst_ld = 1;
+  both.c[0].dst_ld = both.c[1].dst_ld = 1;
+  for (int k = 0; k < (&x == &w ? 1 : 2); ++k) {
+    const AlignedRows* a = k == 0 ? &x : &w;
+    RowCopy& c = both.c[k];
     if (!a->copies_) continue;
     c = RowCopy{a->copy_, a->ld_, a->src_, a->src_ld_, a->rows_, a->cols_,
                 tma_rows(a->src_, a->rows_, a->src_ld_), a->rows_ * ((a->ld_ + kSpan - 1) / kSpan)};

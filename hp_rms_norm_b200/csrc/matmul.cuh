@@ -600,8 +600,9 @@ class AlignedRows {
   }
   const uint16_t* data() const { return copies_ ? copy_ : src_; }
   int64_t ld() const { return ld_; }
-  // Makes the copies of a call's two operands.
+  // Makes the copies of a call's two operands, or of one.
   static int prepare(const AlignedRows& x, const AlignedRows& w, cudaStream_t stream, unsigned flags);
+  int prepare(cudaStream_t stream, unsigned flags) const { return prepare(*this, *this, stream, flags); }
 
  private:
   const uint16_t* src_;

@@ -115,6 +115,22 @@ def test_ignored_and_invalid_rows(cuda):
     assert (loss == 0).sum() == 126
 
 
+@pytest.mark.parametrize("hidden", [64, 129])
+def test_ignored_rows_may_hold_anything(cuda, hidden):
+    """What an ignored row holds, infinities and NaN among it, reaches no gradient."""
+    x, w, t, c = make(200, hidden, 300, torch.bfloat16, cuda, ignored=0.3)
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    want = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    out = t == IGNORE
+    x[out] = float("nan")
+    x[out.nonzero()[0]] = float("inf")
+    c[out] = float("nan")
+    got_loss, lse = hp.linear_cross_entropy(x, w, t)
+    got = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    assert torch.equal(loss, got_loss)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
 def test_equal_row_gradients_are_not_rounded_alike(cuda):
     """A mean's factor lies between two 16-bit numbers; the gradients must not inherit its
     rounding: nearly all of them is -c at the targets."""
