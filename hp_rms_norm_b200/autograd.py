@@ -5,8 +5,10 @@
 their forward and backward passes are the kernels behind the functions of
 ``hp_rms_norm_b200.ops`` with the same names.  Nothing is changed in place: the
 values a backward pass needs (a block's residual among them) stay as they were.
+The gradients have no gradients of their own: a second derivative is refused.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -19,6 +21,7 @@ class _RMSNorm(torch.autograd.Function):
         return ops.rms_norm(input, weight, eps)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         input, weight = ctx.saved_tensors
         grad_input, grad_weight = ops.rms_norm_backward(grad_out.contiguous(), input, weight, ctx.eps)
@@ -32,13 +35,19 @@ class _FusedAddRMSNorm(torch.autograd.Function):
         out = ops.fused_add_rms_norm(input, total, weight, eps)
         ctx.save_for_backward(total, weight)
         ctx.eps = eps
+        ctx.set_materialize_grads(False)  # a last block's sum has no user, so no gradient to read
         return out, total
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out, grad_total):
+        if grad_out is None:
+            return grad_total, grad_total, None, None
         total, weight = ctx.saved_tensors
+        if grad_total is not None:
+            grad_total = grad_total.contiguous()
         grad, grad_weight = ops.rms_norm_backward(grad_out.contiguous(), total, weight, ctx.eps,
-                                                  grad_residual=grad_total.contiguous())
+                                                  grad_residual=grad_total)
         return grad, grad, grad_weight, None
 
 
@@ -55,6 +64,7 @@ class _GatedLinear(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         input, weight, gate_up = ctx.saved_tensors
         grad_input, grad_weight = ops.gated_linear_backward(grad_out.contiguous(), input, weight,
@@ -71,6 +81,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_loss):
         input, weight, target, lse = ctx.saved_tensors
         grad_input, grad_weight = ops.linear_cross_entropy_backward(

@@ -89,6 +89,33 @@ def test_norms(cuda):
     R.assert_near(gw, want_w, 4 * R.U[x.dtype] * size_w, "dw")
 
 
+def test_norm_with_one_of_its_results_used(cuda):
+    x, r = leaf(6, 256, device=cuda, seed=7), leaf(6, 256, device=cuda, seed=8)
+    w = leaf(256, device=cuda, seed=9)
+    c = leaf(6, 256, device=cuda, seed=10).detach()
+    y, total = A.fused_add_rms_norm(x, r, w, 1e-6)
+    # Only the norm: what a zero gradient for the sum gives.
+    got = torch.autograd.grad(y, (x, r, w), c, retain_graph=True)
+    want = torch.autograd.grad((y, total), (x, r, w), (c, torch.zeros_like(c)), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # Only the sum: its gradient as it is, and none for the weight.
+    gx, gr, gw = torch.autograd.grad(total, (x, r, w), c, allow_unused=True)
+    assert torch.equal(gx, c) and torch.equal(gr, c) and gw is None
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "fused_add_rms_norm", "gated_linear", "linear_cross_entropy"])
+def test_second_derivatives_are_refused(cuda, name):
+    x, w = leaf(4, 64, device=cuda, seed=11), leaf(32, 64, device=cuda, seed=12)
+    n = leaf(64, device=cuda, seed=13)
+    y = {"rms_norm": lambda: A.rms_norm(x, n, 1e-6),
+         "fused_add_rms_norm": lambda: A.fused_add_rms_norm(x, x, n, 1e-6)[0],
+         "gated_linear": lambda: A.gated_linear(x, w),
+         "linear_cross_entropy": lambda: A.linear_cross_entropy(x, w, torch.tensor([0, 1, 2, 3], device=cuda))}[name]()
+    (gx,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gx.float().sum().backward()
+
+
 def test_example_learns(cuda):
     losses = load_example().train(steps=30, layers=2, hidden=256, ffn=700, vocab=1000, batch=8, length=128)
     losses = losses.cpu()
