@@ -207,13 +207,13 @@ def grad_norm(grads):
 def clip_grad_norm(grads, max_norm, out=None):
     """Scales every gradient by min(1, max_norm / (norm + 1e-6)), norm the 2-norm over all of
     them, in place or into the tensors of ``out`` (of any of the three types: 16-bit gradients
-    into an optimiser's float32 buffers, say).  Returns the norm before clipping, a float32
-    scalar tensor; nothing waits for the GPU."""
+    into an optimiser's float32 buffers, say).  What is written may share elements with no
+    other tensor of the call, so a tensor is listed once.  Returns the norm before clipping, a
+    float32 scalar tensor; nothing waits for the GPU."""
     if not len(grads):
         return torch.zeros((), dtype=torch.float32)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _ops.clip_grad_norm.default(grads if out is None else out, norm, grads,
-                                                 max_norm)
+    _ops.clip_grad_norm.default(grads if out is None else out, norm, grads, max_norm)
     return norm
 
 

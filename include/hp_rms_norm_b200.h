@@ -324,6 +324,8 @@ HPRN_API int hprn_grad_norm(float* norm, const hprn_grad* grads, int64_t count, 
  * out = round(grad * min(1, max_norm / (*norm + 1e-6))) for every tensor; a NaN
  * norm makes every output NaN.  `out` may be the gradient itself (same type and
  * stride), which is then left unwritten where the factor is 1; otherwise it must not overlap it.
+ * No `out` may share elements with another tensor of the list or with `norm` (not checked:
+ * rows of several tensors may lie interleaved); a tensor listed twice is one such.
  */
 HPRN_API int hprn_grad_clip(const hprn_grad* grads, int64_t count, const float* norm,
                             double max_norm, void* stream, unsigned flags);

@@ -136,6 +136,22 @@ def test_gradient_lists():
     assert n.value == 0
 
 
+def test_norm_and_clip_in_one_call():
+    lib = capi.load()
+    ok = dict(grad=A[0], out=A[1], rows=1, cols=10, row_stride=10, out_row_stride=10, dtype=2, out_dtype=0)
+
+    def both(norm=A[6], most=1.0, ws=A[7], given=1 << 20, flags=0, **k):
+        n = ctypes.c_int64(given)
+        size = None if given is None else ctypes.byref(n)
+        return lib.hprn_clip_grad_norm(norm, (capi.Grad * 1)(capi.Grad(**{**ok, **k})), 1, most, ws, size, None, flags)
+
+    for bad in (dict(norm=0), dict(norm=A[6] + 2), dict(most=-1.0), dict(most=float("nan")), dict(out=0),
+                dict(out=A[0]), dict(out=A[1] + 1), dict(rows=2, out_row_stride=9), dict(ws=0), dict(given=0),
+                dict(flags=64)):
+        assert both(**bad) == capi.ERR_INVALID_ARGUMENT, bad
+    assert both(out_dtype=9) == capi.ERR_UNSUPPORTED_DTYPE
+
+
 def test_torch_operators_are_cuda_only_and_trace():
     names = ("gated_linear", "gated_linear_backward", "linear_cross_entropy",
              "linear_cross_entropy_backward", "rms_norm_backward", "grad_norm", "clip_grad_norm")
