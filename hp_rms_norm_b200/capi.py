@@ -62,6 +62,7 @@ EXPORTED = (
     "hprn_grad_norm",
     "hprn_grad_clip",
     "hprn_clip_grad_norm",
+    "hprn_test_loss_backward_piece",
 )
 
 
@@ -138,6 +139,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.hprn_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, vp, wsp, vp, u32]
     lib.hprn_clip_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, ctypes.c_double, vp, wsp, vp, u32]
     lib.hprn_grad_clip.argtypes = [ctypes.POINTER(Grad), i64, vp, ctypes.c_double, vp, u32]
+    lib.hprn_test_loss_backward_piece.argtypes = [i64] * 4 + [wsp]
+    lib.hprn_test_loss_backward_piece.restype = c_int
     for fn in (lib.hprn_gated_linear, lib.hprn_gated_linear_backward, lib.hprn_linear_cross_entropy,
                lib.hprn_linear_cross_entropy_backward, lib.hprn_rms_norm_backward,
                lib.hprn_grad_norm, lib.hprn_grad_clip, lib.hprn_clip_grad_norm):

@@ -464,4 +464,20 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
   return dtype == HPRN_DTYPE_BF16 ? all(__nv_bfloat16{}) : all(__half{});
 }
 
+int hprn_test_loss_backward_piece(int64_t rows, int64_t hidden, int64_t vocab, int64_t piece, int64_t* out) {
+  using namespace hprn;
+  int64_t none = 0;
+  const int st = check_common(rows, hidden, vocab, HPRN_DTYPE_BF16, 0, &none);
+  if (st != HPRN_OK) return st;
+  const Pieces pieces = pieces_of(rows, vocab);
+  if (!out || piece < 0 || piece >= pieces.count)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "no such piece of the vocabulary");
+  Workspace ws(nullptr, 0);
+  const PlannedProduct<false, true, false> to_input(ws, rows, hidden, pieces.cols);
+  const int64_t left = vocab - piece * pieces.cols, cols = left < pieces.cols ? left : pieces.cols;
+  out[0] = pieces.count, out[1] = cols;
+  out[2] = (cols + kDepthBlock - 1) / kDepthBlock, out[3] = to_input.shares(cols);
+  return ok();
+}
+
 }  // extern "C"

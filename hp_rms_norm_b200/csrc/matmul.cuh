@@ -646,39 +646,57 @@ class PlannedProduct {
   int c_cols() const { return tiling_.cols / (kPaired ? 2 : 1); }
   // How many `part` numbers the epilogue's `end` sees.
   int64_t parts(int64_t n) const { return (n + c_cols() - 1) / c_cols() * kColumnGroups; }
+  // Shares that a sum of `depth` terms is dealt out to: as planned, but each
+  // has a stage.  A product may have less depth than its plan (the vocabulary's
+  // last piece); a share without a stage would have no MMA to finish it.
+  int shares(int64_t depth) const {
+    const int64_t stages = (depth + kDepthBlock - 1) / kDepthBlock;
+    return static_cast<int>(tiling_.splits < stages ? tiling_.splits : stages);
+  }
 
   template <typename T, typename E>
   int launch(const Product& q, const E& epi, cudaStream_t stream, unsigned flags, const char* what) const {
     if (q.m <= 0 || q.n <= 0) return HPRN_OK;
     if (q.depth <= 0) return join(q, epi, 0, stream, flags, what);
-    if (tiling_.splits == 1) return launch_whole<T>(q, epi, stream, flags, what);
-    const int st = launch_whole<T>(q, shares_, stream, flags, what);
-    return st != HPRN_OK ? st : join(q, epi, tiling_.splits, stream, flags, what);
+    const int n = shares(q.depth);
+    if (n == 1) return launch_shares<T>(q, epi, 1, stream, flags, what);
+    const int st = launch_shares<T>(q, shares_, n, stream, flags, what);
+    return st != HPRN_OK ? st : join(q, epi, n, stream, flags, what);
   }
 
-  // The same without splits and with depth > 0, for epilogues that have no point().
+  // The same for products planned without shares and with depth > 0, for
+  // epilogues that have no point().
   template <typename T, typename E>
   int launch_whole(const Product& q, const E& epi, cudaStream_t stream, unsigned flags,
                    const char* what) const {
     if (q.m <= 0 || q.n <= 0) return HPRN_OK;
-    return tiling_.group == 2 ? tiles<T, 2>(q, epi, stream, flags, what)
-                              : tiles<T, 1>(q, epi, stream, flags, what);
+    return launch_shares<T>(q, epi, 1, stream, flags, what);
   }
 
  private:
+  template <typename T, typename E>
+  int launch_shares(const Product& q, const E& epi, int shares, cudaStream_t stream, unsigned flags,
+                    const char* what) const {
+    return tiling_.group == 2 ? tiles<T, 2>(q, epi, shares, stream, flags, what)
+                              : tiles<T, 1>(q, epi, shares, stream, flags, what);
+  }
+
   template <typename T, int kGroup, typename E>
-  int tiles(const Product& q, const E& epi, cudaStream_t stream, unsigned flags, const char* what) const {
+  int tiles(const Product& q, const E& epi, int shares, cudaStream_t stream, unsigned flags,
+            const char* what) const {
     const DeviceInfo* dev = nullptr;
     int st = current_device(&dev);
     if (st != HPRN_OK) return st;
     MatmulArgs args;
     const int64_t rows = 128 * kGroup;
     const int64_t tm = (q.m + rows - 1) / rows, tn = (q.n + c_cols() - 1) / c_cols();
-    const int64_t items = tm * tn * tiling_.splits;
+    const int64_t items = tm * tn * shares;
     if (items > (int64_t{1} << 30)) return fail(HPRN_ERR_INVALID_ARGUMENT, "product too large for one launch");
     args.tiles_m = static_cast<int32_t>(tm), args.tiles_n = static_cast<int32_t>(tn);
-    args.splits = tiling_.splits;
+    args.splits = shares;
     args.depth_blocks = static_cast<int32_t>((q.depth + kDepthBlock - 1) / kDepthBlock);
+    if (shares < 1 || shares > args.depth_blocks)
+      return fail(HPRN_ERR_INVALID_ARGUMENT, std::string(what) + ": a share of a sum without terms");
     args.cols = tiling_.cols;
     args.a_rows = kAKMajor && q.m < 128 ? static_cast<int32_t>(round_up(q.m, 8)) : 128;
     const int stage = args.a_rows * 128 + tiling_.cols / kGroup * 128;

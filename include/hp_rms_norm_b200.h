@@ -416,6 +416,16 @@ HPRN_API int hprn_wait_timeouts(unsigned int* count, int reset);
  */
 HPRN_API int hprn_test_stall_bulk_copy(int64_t row, uint64_t wait_limit_ns);
 
+/*
+ * No reference counterpart.  Test hook, launches nothing: how
+ * hprn_linear_cross_entropy_backward takes the input gradient's sums over piece
+ * `piece` of the vocabulary.  Writes to out[0..3] the number of pieces, the
+ * piece's columns, the stages of 64 terms that these make, and the shares that
+ * the stages are dealt out to.
+ */
+HPRN_API int hprn_test_loss_backward_piece(int64_t rows, int64_t hidden, int64_t vocab,
+                                           int64_t piece, int64_t* out);
+
 #ifdef __cplusplus
 }
 #endif

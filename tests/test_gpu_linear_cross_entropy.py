@@ -247,3 +247,29 @@ def test_refusals(cuda):
                 lambda: hp.linear_cross_entropy_backward(c[:2], x, w, t, lse)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("case", [(63130, 10, 61441), (44032, 64, 159000)], ids=str)
+def test_short_last_piece_of_the_vocabulary(cuda, case):
+    """Many pieces, the last one of a few columns: fewer terms than a full piece's sums have
+    shares.  Rows that are left out keep the 64-bit formula to the others."""
+    import ctypes
+
+    from hp_rms_norm_b200 import capi
+
+    rows, hidden, vocab = case
+    x, w, t, c = make(rows, hidden, vocab, torch.bfloat16, cuda)
+    keep = torch.arange(0, rows, rows // 96, device=cuda)
+    t[keep[0]], t[keep[1]] = vocab - 1, 0
+    counted = torch.full_like(t, IGNORE)
+    counted[keep] = t[keep]
+    loss, lse = hp.linear_cross_entropy(x, w, counted)
+    dx, dw = hp.linear_cross_entropy_backward(c, x, w, counted, lse)
+    check_loss(loss[keep], lse[keep], x[keep], w, counted[keep], f"{case}")
+    check_backward(dx[keep], dw, c[keep], x[keep], w, counted[keep], f"{case}")
+    rest = torch.ones(rows, dtype=torch.bool, device=cuda)
+    rest[keep] = False
+    assert not dx[rest].any()
+    torch.cuda.synchronize()
+    count = ctypes.c_uint(7)
+    assert capi.load().hprn_wait_timeouts(ctypes.byref(count), 0) == 0 and count.value == 0
