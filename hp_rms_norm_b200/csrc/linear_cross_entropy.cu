@@ -15,7 +15,7 @@
 // are complete, and dX is summed over the pieces in fp32 and rounded once.
 //
 // S is held as c_i / c_max (exp(L_ij - lse_i) - [j == t_i]), c_max the largest
-// |c_i|, and the sums are multiplied by c_max.  A mean gives every row the same
+// finite |c_i|, and the sums are multiplied by c_max.  A mean gives every row the same
 // c, and then the entries that matter most, -c at the targets, would all be
 // rounded to 16 bits alike and the gradients come out up to 2^-9 short or long;
 // -1 is exact (8192 x 4096 x 131072, one draw of the targets: 3.5e-3 off without,
@@ -174,15 +174,18 @@ __global__ void __launch_bounds__(256) loss_grad_prepare(LossPrepareArgs a) {
   if (blockIdx.x == 0) {
     float m = 0.f;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < a.rows; i += 256)
-      if (a.target[i] != a.ignore) m = fmaxf(m, fabsf(a.grad_loss[i]));
+    for (int64_t i = threadIdx.x; i < a.rows; i += 256) {
+      // The largest finite one: an infinite or NaN gradient spoils its own row
+      // and the weight's, not the scale of the other rows.
+      const float c = fabsf(a.grad_loss[i]);
+      if (a.target[i] != a.ignore && c < INFINITY) m = fmaxf(m, c);
+    }
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     if (lane == 0) part[warp] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int k = 1; k < 8; ++k) m = fmaxf(m, part[k]);
-      // An infinite gradient spoils its own row and the weight's, not the other rows.
-      if (!(m > 0.f && m < INFINITY)) m = 1.f;
+      if (m == 0.f) m = 1.f;
       a.scale[0] = m, a.scale[1] = m / a.held;
     }
   }

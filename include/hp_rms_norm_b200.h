@@ -275,8 +275,9 @@ HPRN_API int hprn_linear_cross_entropy(float* loss, float* lse, const void* inpu
  *          target_i == ignore_index, NaN in rows with any other invalid target
  *   grad_input [rows, hidden]  = round_T(S weight)
  *   grad_weight [vocab, hidden] = round_T(S^T input)
- * S is held divided by the largest |c_i| (and in fp16 times 2^14), so equal c_i
- * are not all rounded alike and small probabilities do not underflow.
+ * S is held divided by the largest finite |c_i| (and in fp16 times 2^14), so equal
+ * c_i are not all rounded alike and small probabilities do not underflow.  Where
+ * c_i is infinite or NaN, so are row i of grad_input and grad_weight.
  */
 HPRN_API int hprn_linear_cross_entropy_backward(
     void* grad_input, void* grad_weight, const float* grad_loss, const void* input,

@@ -273,3 +273,19 @@ def test_short_last_piece_of_the_vocabulary(cuda, case):
     torch.cuda.synchronize()
     count = ctypes.c_uint(7)
     assert capi.load().hprn_wait_timeouts(ctypes.byref(count), 0) == 0 and count.value == 0
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_infinite_row_gradient_beside_large_ones(cuda, dt):
+    """Factors of several hundred, as under loss scaling, beside one infinite and one NaN: the
+    other rows' gradients are what they are without those two."""
+    x, w, t, c = make(140, 64, 300, DTYPES[dt], cuda, ignored=0.0)
+    c = c * 400
+    _, lse = hp.linear_cross_entropy(x, w, t)
+    c[7], c[9] = float("inf"), float("nan")
+    dx, _ = hp.linear_cross_entropy_backward(c, x, w, t, lse)
+    keep = torch.ones(140, dtype=torch.bool, device=cuda)
+    keep[7] = keep[9] = False
+    clean, _ = hp.linear_cross_entropy_backward(torch.where(keep, c, 0.0), x, w, t, lse)
+    assert torch.equal(dx[keep], clean[keep]) and torch.isfinite(clean).all()
+    assert not torch.isfinite(dx[7]).any() and dx[9].isnan().all()
