@@ -27,6 +27,7 @@ namespace hprn {
 template <typename T, int ACT>
 struct GatedEpilogue {
   static constexpr bool kPaired = true;
+  static constexpr int kSegment = 0;
   Out16 out;
   Out32 gate, up;  // null to leave out
 
@@ -64,6 +65,7 @@ __device__ __forceinline__ void gated_gradients(float (&g)[N], float (&u)[N], co
 template <typename T, int ACT>
 struct GatedGradEpilogue {
   static constexpr bool kPaired = true;
+  static constexpr int kSegment = 0;
   const uint16_t* dout = nullptr;
   int64_t dout_ld = 0;
   bool dout_aligned = false;  // every row to 16 bytes

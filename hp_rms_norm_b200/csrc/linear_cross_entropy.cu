@@ -57,21 +57,17 @@ __device__ __forceinline__ float2 exp_fast2(float2 x) {
   return y;
 }
 
-// What a logit's sum is multiplied by.  The tensor cores' adder cuts off what
-// falls below the running sum's last place, 16 terms a step, so a sum of n
-// steps comes out short by about n * 2^-24 * 0.22 of itself (bf16) or 0.28
-// (fp16): the slope against 64-bit sums, the same at 256 and 1024 terms and
-// with terms of mean zero or not; sums of one sign lose more.  A loss is a
-// difference of logits near the largest ones and would be short throughout:
-// 2048 x 5120 x 100003 (fp16) 1.8e-6 of itself without the factor, 4.4e-7 with it.
-float sum_correction(int64_t depth, int dtype) {
-  const double steps = static_cast<double>((depth + 15) / 16);
-  return static_cast<float>(1.0 + steps * (dtype == HPRN_DTYPE_BF16 ? 0.22 : 0.28) / 16777216.0);
-}
+// Stages that the tensor cores sum at once, 512 terms: a loss is a difference
+// of logits near the largest ones and would be short throughout.  2048 x 5120 x
+// 100003 (fp16): 1.8e-6 of itself with whole sums, 2.0e-7 with these (1.9e-7 in
+// fp32 operations), 1685 us instead of 1650; 1670 with 1024 terms.  The backward
+// pass takes the same, since its logits have to be the forward pass's.
+constexpr int kLogitSegment = 8;
 
 struct LossEpilogue {
   static constexpr bool kPaired = false;
-  float correction = 1.f;     // sum_correction
+  static constexpr int kSegment = kLogitSegment;
+  static constexpr bool kUnrolled = true;
   float2* partial = nullptr;  // [rows, parts]: {max of l, sum of exp(l - max)}
   float* target_logit = nullptr;
   const int64_t* target = nullptr;
@@ -98,21 +94,19 @@ struct LossEpilogue {
       float x = 0.f;
 #pragma unroll
       for (int k = 0; k < kChunk; ++k) x = at == k ? v[k] : x;
-      target_logit[i] = x * correction;
+      target_logit[i] = x;
     }
     float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int k = 4; k < kChunk; ++k) top[k % 4] = fmaxf(top[k % 4], v[k]);
-    const float m = fmaxf(r.m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * correction);
+    const float m = fmaxf(r.m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
     // All so far -inf (or NaN, which fmaxf skips and the sum keeps): exp(-inf - 0) = 0.
     const float ref = m == -INFINITY ? 0.f : m;
-    const float2 c2 = make_float2(correction, correction), minus = make_float2(-ref, -ref);
+    const float2 minus = make_float2(-ref, -ref);
     float2 s[2] = {make_float2(r.s * exp_fast(r.m - ref), 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int k = 0; k < kChunk / 2; ++k) {
-      const float2 l = __fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), c2);
-      s[k % 2] = __fadd2_rn(s[k % 2], exp_fast2(__fadd2_rn(l, minus)));
-    }
+    for (int k = 0; k < kChunk / 2; ++k)
+      s[k % 2] = __fadd2_rn(s[k % 2], exp_fast2(__fadd2_rn(make_float2(v[2 * k], v[2 * k + 1]), minus)));
     r.m = m, r.s = (s[0].x + s[0].y) + (s[1].x + s[1].y);
   }
   __device__ __forceinline__ void end(Row& r, const Lane& l, int64_t i, int64_t part) const {
@@ -229,7 +223,8 @@ __global__ void __launch_bounds__(256) loss_grad_prepare(LossPrepareArgs a) {
 template <typename T>
 struct LossGradEpilogue {
   static constexpr bool kPaired = false;
-  float correction = 1.f;  // as in LossEpilogue
+  static constexpr int kSegment = kLogitSegment;
+  static constexpr bool kUnrolled = false;
   Out16 s;                 // the piece's columns
   const float* lse = nullptr;
   const float* grad_loss = nullptr;
@@ -260,8 +255,7 @@ struct LossGradEpilogue {
     } else {
 #pragma unroll
       for (int k = 0; k < kChunk / 2; ++k) {
-        // Rounded as the forward pass rounded it, so that exp(0) is where lse is a logit.
-        const float2 l = __fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(correction, correction));
+        const float2 l = make_float2(v[2 * k], v[2 * k + 1]);
         const float2 p = __fmul2_rn(exp_fast2(__fadd2_rn(l, make_float2(-r.lse, -r.lse))), make_float2(r.c, r.c));
         v[2 * k] = p.x, v[2 * k + 1] = p.y;
       }
@@ -354,7 +348,6 @@ int hprn_linear_cross_entropy(float* loss, float* lse, const void* input, const 
   q.b = {w.data(), w.ld()};
   q.m = rows, q.n = vocab, q.depth = hidden;
   LossEpilogue e;
-  e.correction = sum_correction(hidden, dtype);
   e.partial = partial, e.target_logit = target_logit, e.target = target;
   e.ignore = ignore_index, e.parts = parts, e.vocab = vocab;
   if (hidden > 0) {
@@ -442,7 +435,6 @@ int hprn_linear_cross_entropy_backward(void* grad_input, void* grad_weight, cons
       q.b = {wp, w.ld()};
       q.m = rows, q.n = cols, q.depth = hidden;
       LossGradEpilogue<T> g;
-      g.correction = sum_correction(hidden, dtype);
       g.s = Out16(s, pieces.cols, cols), g.lse = lse, g.grad_loss = grad_loss, g.most = scale, g.held = held;
       g.target = target, g.ignore = ignore_index, g.vocab = vocab, g.first = first;
       if ((r = logits.launch_whole<T>(q, g, cs, flags, what)) != HPRN_OK) break;

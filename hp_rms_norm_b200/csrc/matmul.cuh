@@ -20,6 +20,12 @@
 // of B's rows j and pair_offset + j (gate and up).  The chunks of a tile's row
 // are shared out to kColumnGroups lanes; `part` numbers these shares along C's
 // columns.
+// kSegment, stages: 0 leaves a tile's whole sum to the tensor cores.  Their
+// adder cuts off what falls below the running sum's last place, 16 terms a step,
+// so a sum of n steps comes out short by about n * 2^-24 * 0.22 (bf16) to 0.28
+// (fp16) of itself, by up to 1.6 where all terms have one sign, and by nothing
+// where no term is cut.  With kSegment the tensor cores sum that many stages at
+// a time and the segments' sums join in registers by rounded additions.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -167,6 +173,7 @@ struct Out32 {
 template <typename T>
 struct StoreEpilogue {
   static constexpr bool kPaired = false;
+  static constexpr int kSegment = 0;
   Out16 out;             // written by the last piece
   float* sum = nullptr;  // rows of sum_ld (a multiple of 32), or null when there is one piece
   int64_t sum_ld = 0;
@@ -214,6 +221,7 @@ struct StoreEpilogue {
 template <bool kPair>
 struct SplitEpilogue {
   static constexpr bool kPaired = kPair;
+  static constexpr int kSegment = 0;
   float* partial = nullptr;  // [splits][rows][ld]; a pair's second values follow its first
   int64_t ld = 0;            // columns of one value, a multiple of 32
   int64_t rows = 0;
@@ -337,6 +345,68 @@ __device__ __forceinline__ void run_epilogue(const E& epi, const Lane& l, int64_
   }
   epi.end(row, l, i, part);
 }
+
+// The same for a sum in segments: a lane's share of the tile's row, held in
+// 128 registers.  kUnrolled: the epilogue's code once a chunk, each on its own
+// registers, else one copy of it that the chunks move up to.  The softmax sums
+// fit unrolled (7 x 1024 x 32768: 19.7 us, moving 20.5; 2048 x 5120 x 100003:
+// 1685, 1725); the logit gradients then spill 800 bytes (1023 x 2056 x 50001
+// with both gradients: 843 us, moving 783).  Loads of 32 columns instead of 16
+// spill 24 to 300 bytes more and are no faster.
+constexpr int kLaneChunks = 256 / kChunk / kColumnGroups;
+
+struct LaneSums {
+  float v[kLaneChunks][kChunk];
+  __device__ __forceinline__ static int column(int k, int group) { return (k * kColumnGroups + group) * kChunk; }
+  // Adds the accumulators of one more segment (sets them, of the first).
+  __device__ __forceinline__ void add(uint32_t acc, bool first, int cols, int group) {
+#pragma unroll
+    for (int k = 0; k < kLaneChunks; ++k) {
+      const int c = column(k, group);
+      if (c >= cols) break;
+      if (first) {
+        tmem_load_32(acc + c, v[k]);
+        tmem_wait_load(v[k]);
+        continue;
+      }
+#pragma unroll
+      for (int h = 0; h < kChunk; h += 16) {
+        float w[16];
+        tmem_load_16(acc + c + h, w);
+        tmem_wait_load(w);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[k][h + e] += w[e];
+      }
+    }
+  }
+  template <typename E>
+  __device__ __forceinline__ void run(const E& epi, const Lane& l, int64_t i, int64_t j0, int64_t n, int cols,
+                                      int group, int64_t part) {
+    auto row = epi.begin(l, i);
+    if constexpr (E::kUnrolled) {
+#pragma unroll
+      for (int k = 0; k < kLaneChunks; ++k) {
+        const int c = column(k, group);
+        if (c >= cols || j0 + c >= n) break;
+        epi.chunk(row, l, i, j0 + c, v[k]);
+        __syncwarp();
+      }
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < kLaneChunks; ++k) {
+        const int c = column(k, group);
+        if (c >= cols || j0 + c >= n) break;
+        epi.chunk(row, l, i, j0 + c, v[0]);
+#pragma unroll
+        for (int q = 1; q < kLaneChunks; ++q)
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e) v[q - 1][e] = v[q][e];
+        __syncwarp();
+      }
+    }
+    epi.end(row, l, i, part);
+  }
+};
 
 template <typename T, typename E, int kGroup, bool kAKMajor, bool kBKMajor>
 __global__ void __launch_bounds__(kMatmulThreads, 1)
@@ -467,30 +537,34 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
     bool ok = true;
     for (int32_t t = first; t < items && ok; t += step) {
       const DepthRange range = depth_range(args, t % args.splits);
-      if (!mbar_wait_warp(acc_empty(buf), buf_phase ^ 1)) {
-        ok = false;
-        break;
-      }
-      tmem_fence_after();
-      const uint32_t d = tmem + buf * (kTmemColumns / 2);
-      for (int32_t k = range.first; k < range.last; ++k) {
-        if (!mbar_wait_warp(full(s), phase)) {
+      for (int32_t begin = range.first; begin < range.last && ok;) {
+        const int32_t end = E::kSegment > 0 ? min(begin + E::kSegment, range.last) : range.last;
+        if (!mbar_wait_warp(acc_empty(buf), buf_phase ^ 1)) {
           ok = false;
           break;
         }
         tmem_fence_after();
-        if (elect_one()) {
-          const uint64_t a = a_desc + s * (stage_bytes / 16), b = b_desc + s * (stage_bytes / 16);
+        const uint32_t d = tmem + buf * (kTmemColumns / 2);
+        for (int32_t k = begin; k < end; ++k) {
+          if (!mbar_wait_warp(full(s), phase)) {
+            ok = false;
+            break;
+          }
+          tmem_fence_after();
+          if (elect_one()) {
+            const uint64_t a = a_desc + s * (stage_bytes / 16), b = b_desc + s * (stage_bytes / 16);
 #pragma unroll
-          for (int j = 0; j < kDepthBlock / 16; ++j)
-            mma_f16<kGroup>(d, a + j * kAStep, b + j * kBStep, idesc, k > range.first || j > 0);
-          mma_commit<kGroup>(empty(s));
-          if (k + 1 == range.last) mma_commit<kGroup>(acc_full(buf));
+            for (int j = 0; j < kDepthBlock / 16; ++j)
+              mma_f16<kGroup>(d, a + j * kAStep, b + j * kBStep, idesc, k > begin || j > 0);
+            mma_commit<kGroup>(empty(s));
+            if (k + 1 == end) mma_commit<kGroup>(acc_full(buf));
+          }
+          __syncwarp();
+          if (++s == stages) s = 0, phase ^= 1;
         }
-        __syncwarp();
-        if (++s == stages) s = 0, phase ^= 1;
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
+        begin = end;
       }
-      if (++buf == 2) buf = 0, buf_phase ^= 1;
     }
     if (!ok) {
       if (elect_one()) {
@@ -510,33 +584,57 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
       const int64_t i = static_cast<int64_t>(it.tm) * (128 * kGroup) + rank * 128 + quarter * 32 + lane;
       const int64_t j0 = static_cast<int64_t>(it.tn) * c_cols;
       l.inside = i < args.m, l.split = it.split;
-      if (!mbar_wait_warp(acc_full(buf), phase)) {
-        if (lane == 0) atomicAdd(args.timeouts, 1u);
-        break;
-      }
-      tmem_fence_after();
-      const uint32_t acc = tmem + buf * (kTmemColumns / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
-      if (__any_sync(~0u, l.inside)) {
-        if constexpr (E::kPaired) {
-          run_epilogue(epi, l, i, j0, args.n, c_cols, group, it.tn * kColumnGroups + group,
-                       [&](int c, float (&v)[kChunk], int c2, float (&u)[kChunk]) {
-                         tmem_load_32(acc + c, v);
-                         tmem_load_32(acc + c2, u);
-                         tmem_wait_load(v);
-                         tmem_wait_load(u);
-                       });
-        } else {
-          run_epilogue(epi, l, i, j0, args.n, c_cols, group, it.tn * kColumnGroups + group,
-                       [&](int c, float (&v)[kChunk]) {
-                         tmem_load_32(acc + c, v);
-                         tmem_wait_load(v);
-                       });
+      const bool any = __any_sync(~0u, l.inside);
+      // Waits for the accumulators that are due next; their address.
+      auto take = [&](uint32_t& acc) {
+        if (!mbar_wait_warp(acc_full(buf), phase)) {
+          if (lane == 0) atomicAdd(args.timeouts, 1u);
+          return false;
         }
+        tmem_fence_after();
+        acc = tmem + buf * (kTmemColumns / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
+        return true;
+      };
+      // Hands them back to the MMA warp.
+      auto give = [&] {
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_shared(acc_empty(buf), 0));
+        if (++buf == 2) buf = 0, phase ^= 1;
+      };
+      uint32_t acc = 0;
+      const int64_t part = it.tn * kColumnGroups + group;
+      if constexpr (E::kSegment > 0) {
+        const DepthRange range = depth_range(args, it.split);
+        LaneSums sums;
+        bool ok = true;
+        for (int32_t begin = range.first; begin < range.last; begin += E::kSegment) {
+          if (!(ok = take(acc))) break;
+          if (any) sums.add(acc, begin == range.first, c_cols, group);
+          give();
+        }
+        if (!ok) break;
+        if (any) sums.run(epi, l, i, j0, args.n, c_cols, group, part);
+      } else {
+        if (!take(acc)) break;
+        if (any) {
+          if constexpr (E::kPaired) {
+            run_epilogue(epi, l, i, j0, args.n, c_cols, group, part,
+                         [&](int c, float (&v)[kChunk], int c2, float (&u)[kChunk]) {
+                           tmem_load_32(acc + c, v);
+                           tmem_load_32(acc + c2, u);
+                           tmem_wait_load(v);
+                           tmem_wait_load(u);
+                         });
+          } else {
+            run_epilogue(epi, l, i, j0, args.n, c_cols, group, part, [&](int c, float (&v)[kChunk]) {
+              tmem_load_32(acc + c, v);
+              tmem_wait_load(v);
+            });
+          }
+        }
+        give();
       }
-      tmem_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_shared(acc_empty(buf), 0));
-      if (++buf == 2) buf = 0, phase ^= 1;
     }
   }
   __syncwarp();

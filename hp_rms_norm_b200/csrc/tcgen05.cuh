@@ -137,11 +137,24 @@ __device__ __forceinline__ void tmem_load_32(uint32_t addr, float (&v)[32]) {
       : "r"(addr)
       : "memory");
 }
+// The same for 16 columns.
+__device__ __forceinline__ void tmem_load_16(uint32_t addr, float (&v)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+        "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
+        "=r"(u[14]), "=r"(u[15])
+      : "r"(addr)
+      : "memory");
+}
 // The load's registers pass through the wait, so nothing reads them before it.
-__device__ __forceinline__ void tmem_wait_load(float (&v)[32]) {
+template <int N>
+__device__ __forceinline__ void tmem_wait_load(float (&v)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(v[k]));
+  for (int k = 0; k < N; ++k) asm volatile("" : "+f"(v[k]));
 }
 
 // ---------------------------------------------------------------------------

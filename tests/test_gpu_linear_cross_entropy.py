@@ -289,3 +289,41 @@ def test_infinite_row_gradient_beside_large_ones(cuda, dt):
     clean, _ = hp.linear_cross_entropy_backward(torch.where(keep, c, 0.0), x, w, t, lse)
     assert torch.equal(dx[keep], clean[keep]) and torch.isfinite(clean).all()
     assert not torch.isfinite(dx[7]).any() and dx[9].isnan().all()
+
+
+def check_sums(x, w, logit_bound, label):
+    t = torch.arange(x.shape[0], device=x.device) % w.shape[0]
+    loss, lse = hp.linear_cross_entropy(x, w, t)
+    want, want_lse, logits = R.linear_cross_entropy(x, w, t, IGNORE)
+    # As in check_loss, with this bound on the logits.
+    spread = (logits.max(-1).values - logits.min(-1).values).clamp(min=1)
+    e = logit_bound * logits.abs().max(-1).values
+    el = e + w.shape[0] * R.F32 + 4 * R.F32 * (2 + spread) + 2 * R.F32 * want_lse.abs()
+    R.assert_within(lse, want_lse, el, label + " lse")
+    R.assert_within(loss, want, el + e + 2 * R.F32 * (want.abs() + want_lse.abs()), label)
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("hidden", [4096, 16384])
+def test_exact_logits_stay_exact(cuda, hidden, dt):
+    """Long sums without a rounding: one term, and many whole numbers."""
+    g = torch.Generator(device=cuda).manual_seed(hidden)
+    x = torch.zeros(32, hidden, device=cuda)
+    x[torch.arange(32, device=cuda), torch.randint(0, hidden, (32,), generator=g, device=cuda)] = 1
+    w = (torch.randint(-240, 241, (8, hidden), generator=g, device=cuda) / 8).to(DTYPES[dt])
+    check_sums(x.to(w.dtype), w, 0.0, "one hot")
+    x = torch.randint(-1, 2, (32, hidden), generator=g, device=cuda) / 4
+    w = torch.randint(-1, 2, (8, hidden), generator=g, device=cuda)
+    check_sums(x.to(DTYPES[dt]), w.to(DTYPES[dt]), 0.0, "whole numbers")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("hidden", [4096, 16384])
+def test_sums_of_one_sign(cuda, hidden, dt):
+    """The sums that lose most to an adder that cuts off.  It takes 16 terms a step and aligns
+    them, so a step may lose 4 last places (17 addends of 4 guard bits); 512 terms, 32 steps, are
+    summed that way, and such sums join by rounded additions."""
+    g = torch.Generator(device=cuda).manual_seed(hidden)
+    x = torch.rand(32, hidden, generator=g, device=cuda) + 0.5
+    w = (torch.rand(8, hidden, generator=g, device=cuda) + 0.5) * (32 / hidden)
+    check_sums(x.to(DTYPES[dt]), w.to(DTYPES[dt]), (32 * 4 + hidden / 512) * R.F32, "one sign")
