@@ -134,10 +134,14 @@ __global__ void __launch_bounds__(256)
     join(make_float2(__shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o)));
   if (lane != 0) return;
   if (parts == 0 && vocab > 0) m = 0.f, s = static_cast<float>(vocab);  // sums of no terms: logits 0
-  const float l = (m == -INFINITY ? 0.f : m) + logf(s);
-  lse[i] = l;
+  const float top = m == -INFINITY ? 0.f : m, log_s = logf(s);
+  lse[i] = top + log_s;
   const int64_t t = target_of(target, i, ignore, vocab);
-  loss[i] = t == kIgnored ? 0.f : t == kInvalid ? __int_as_float(0x7fc00000) : l - (parts > 0 ? target_logit[i] : 0.f);
+  // The two logits first: where the target is the largest one the loss is log s,
+  // which a sum with a logit of 30 would round to multiples of 2^-19.
+  loss[i] = t == kIgnored    ? 0.f
+            : t == kInvalid ? __int_as_float(0x7fc00000)
+                            : (top - (parts > 0 ? target_logit[i] : 0.f)) + log_s;
 }
 
 // What the backward products need first.  X with the ignored rows zeroed (on

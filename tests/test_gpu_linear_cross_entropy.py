@@ -327,3 +327,20 @@ def test_sums_of_one_sign(cuda, hidden, dt):
     x = torch.rand(32, hidden, generator=g, device=cuda) + 0.5
     w = (torch.rand(8, hidden, generator=g, device=cuda) + 0.5) * (32 / hidden)
     check_sums(x.to(DTYPES[dt]), w.to(DTYPES[dt]), (32 * 4 + hidden / 512) * R.F32, "one sign")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_small_losses_of_confident_rows(cuda, dt):
+    """A target that is the largest logit by far: the loss is log(1 + e^-gap), not a difference of
+    two numbers near 30.  One hot rows, so the logits are exact."""
+    x = torch.eye(64, device=cuda).to(DTYPES[dt])
+    w = torch.full((8, 64), -100.0, device=cuda)
+    w[0] = 30
+    w[1] = 17 - 0.125 * torch.arange(64, device=cuda)
+    w = w.to(DTYPES[dt])
+    loss, _ = hp.linear_cross_entropy(x, w, torch.zeros(64, dtype=torch.int64, device=cuda))
+    want = torch.log1p(torch.exp(w[1].double() - w[0].double()))
+    assert want.max() > 2e-6 and want.min() < 1e-9
+    # One rounding of 1 + e^-gap, one where a row's parts are joined, e^-gap within
+    # 2^-20 of itself, and the logarithm of a number next to 1.
+    assert ((loss.double() - want).abs() <= 2.0 ** -22 + 2.0 ** -20 * want).all()
