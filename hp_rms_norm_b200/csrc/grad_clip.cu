@@ -138,6 +138,28 @@ __device__ __forceinline__ int64_t place(int64_t k, int64_t cols, int64_t stride
   return stride == cols ? k : k / cols * stride + k % cols;
 }
 
+// A chunk of a tensor whose rows have gaps: eight sums as below, row and column
+// stepping along instead of a division an element.  A function of its own:
+// inlined, it cost the dense loop a fifth (77 million bf16: 39.7 us, 31.7).
+template <int TYPE>
+__device__ __noinline__ float strided_squares(const GradEntry& e, int64_t lo, int64_t hi) {
+  const typename Elem<TYPE>::Raw* p = static_cast<const typename Elem<TYPE>::Raw*>(e.in);
+  float s[8] = {};
+  const int64_t row_step = kClipThreads / e.cols, col_step = kClipThreads % e.cols;
+  int64_t k = lo + threadIdx.x, row = k / e.cols, col = k % e.cols;
+  while (k < hi) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (k >= hi) break;
+      const float v = Elem<TYPE>::get(p[row * e.in_stride + col]);
+      s[u] = fmaf(v, v, s[u]);
+      k += kClipThreads, row += row_step, col += col_step;
+      if (col >= e.cols) col -= e.cols, ++row;
+    }
+  }
+  return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+}
+
 // A contiguous chunk is read in groups of eight elements from the first
 // 16-byte boundary on, four groups in flight a thread; its ends one by one.
 constexpr int kInFlight = 4;
@@ -151,10 +173,7 @@ __device__ __forceinline__ float chunk_squares(const GradEntry& e, int64_t lo, i
     const float v = Elem<TYPE>::get(p[place(k, e.cols, e.in_stride)]);
     s[0] = fmaf(v, v, s[0]);
   };
-  if (e.in_stride != e.cols) {
-    for (int64_t k = lo + threadIdx.x; k < hi; k += kClipThreads) one(k);
-    return s[0];
-  }
+  if (e.in_stride != e.cols) return strided_squares<TYPE>(e, lo, hi);
   const int64_t first = min(lo + ahead<TYPE>(p + lo), hi), groups = (hi - first) / 8;
   for (int64_t g = threadIdx.x; g < groups; g += kClipThreads * kInFlight) {
     float v[kInFlight][8];

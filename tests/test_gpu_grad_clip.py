@@ -136,3 +136,20 @@ def test_refusals(cuda):
                 lambda: hp.clip_grad_norm([b[0:4].view(-1)], 1.0, out=[b.view(-1)[1:33]])):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_strided_sums_are_short(cuda):
+    """A chunk of a strided tensor is summed like one of a dense tensor: a thread's 256 terms in
+    eight sums of 32.  The first term of each thread's is 1, the others half its last place, which
+    vanish one by one beside it and count where they are summed among themselves."""
+    n = 77_000_000  # enough for the longest chunks, 65536 elements
+    flat = torch.full((n,), (0.98 * 2.0 ** -24) ** 0.5, device=cuda)
+    flat[:n // 65536 * 65536].view(-1, 65536)[:, :256] = 1
+    g = torch.zeros(n // 1000, 1024, device=cuda)[:, :1000]
+    g.copy_(flat.view(-1, 1000))
+    want = flat.double().square().sum().sqrt()
+    # 32 terms, 3 joins of the eight sums, 5 in a warp and 7 of the warps, 2^-24 each;
+    # half of that in the root, and its own rounding.
+    bound = (47 / 2 + 1) * 2.0 ** -24 * want.item()
+    assert abs(hp.grad_norm([flat]).item() - want.item()) <= bound
+    assert abs(hp.grad_norm([g]).item() - want.item()) <= bound
