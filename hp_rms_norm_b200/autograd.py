@@ -102,8 +102,9 @@ def fused_add_rms_norm(input, residual, weight, eps):
 def gated_linear(input, weight, act="silu", keep_products=True):
     """act(input Wg^T) * (input Wu^T), ``weight`` = [Wg; Wu].  ``keep_products`` keeps the two
     products (float32, 8 bytes for each output element) for the backward pass; without it they
-    are computed again there."""
-    return _GatedLinear.apply(input, weight, act, keep_products)
+    are computed again there.  Where no graph is recorded nothing is kept."""
+    # needs_input_grad tells a leaf's wish, not whether a graph is being recorded.
+    return _GatedLinear.apply(input, weight, act, keep_products and torch.is_grad_enabled())
 
 
 def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction="mean"):
