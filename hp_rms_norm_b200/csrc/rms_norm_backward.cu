@@ -225,6 +225,9 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
               sts_half(at[t] + off + 2 * j, q[j]);
           from[t] = p - off + lo, at[t] += lo, bytes[t] = hi - lo, total += bytes[t];
         }
+        // The stores above, in this round and in earlier ones of this buffer, before
+        // the bulk copies that write there by another proxy.
+        if constexpr (!kVectors) fence_proxy_async_smem();
         total = __reduce_add_sync(~0u, total);
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(bar, total);

@@ -108,3 +108,20 @@ def test_refusals(cuda):
                 lambda: hp.rms_norm_backward(dy.cpu(), x, w, 1e-6)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("hidden", [501, 5001])
+@pytest.mark.parametrize("start", [1, 6])
+def test_ends_off_boundaries_and_buffers_used_again(cuda, hidden, start):
+    """Tensors whose first and last elements lie inside a 16-byte granule, with enough rows that
+    the buffers which took these elements one by one are filled by copies later."""
+    rows = 6000
+    g = torch.Generator(device=cuda).manual_seed(hidden + start)
+    odd = lambda: torch.randn(start + rows * hidden, generator=g, device=cuda).bfloat16()[start:].view(rows, hidden)
+    x, dy, extra = odd(), odd(), odd()
+    w = (1 + 0.1 * torch.randn(hidden, generator=g, device=cuda)).bfloat16()
+    for e in (None, extra):
+        dx, dw = hp.rms_norm_backward(dy, x, w, 1e-6, grad_residual=e)
+        check(dx, dw, dy, x, w, 1e-6, e, f"{hidden} {start} {e is not None}")
+        again = hp.rms_norm_backward(dy, x, w, 1e-6, grad_residual=e)
+        assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
