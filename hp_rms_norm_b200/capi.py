@@ -63,6 +63,7 @@ EXPORTED = (
     "hprn_grad_clip",
     "hprn_clip_grad_norm",
     "hprn_test_loss_backward_piece",
+    "hprn_test_stall_loads",
 )
 
 
@@ -141,6 +142,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.hprn_grad_clip.argtypes = [ctypes.POINTER(Grad), i64, vp, ctypes.c_double, vp, u32]
     lib.hprn_test_loss_backward_piece.argtypes = [i64] * 4 + [wsp]
     lib.hprn_test_loss_backward_piece.restype = c_int
+    lib.hprn_test_stall_loads.argtypes = [c_int, ctypes.c_uint64]
+    lib.hprn_test_stall_loads.restype = c_int
     for fn in (lib.hprn_gated_linear, lib.hprn_gated_linear_backward, lib.hprn_linear_cross_entropy,
                lib.hprn_linear_cross_entropy_backward, lib.hprn_rms_norm_backward,
                lib.hprn_grad_norm, lib.hprn_grad_clip, lib.hprn_clip_grad_norm):
@@ -247,6 +250,12 @@ def test_stall_bulk_copy(row: int | None, wait_limit_ns: int = 0) -> None:
     """Test hook (hprn_test_stall_bulk_copy): later TMA-staged launches make the
     staged copy of `row` stall so its bounded wait runs out; None turns it off."""
     _check(load().hprn_test_stall_bulk_copy(-1 if row is None else row, wait_limit_ns))
+
+
+def test_stall_loads(on: bool, wait_limit_ns: int = 0) -> None:
+    """Test hook (hprn_test_stall_loads): later launches of the training operators' products and
+    of rms_norm_backward load nothing, so their bounded waits run out."""
+    _check(load().hprn_test_stall_loads(1 if on else 0, wait_limit_ns))
 
 
 def version() -> int:

@@ -268,7 +268,7 @@ struct SplitEpilogue {
 // those rows of the accumulator are not looked at.
 //
 // Every wait has a limit (mbar_wait_bounded).  A role whose wait runs out
-// counts itself in `timeouts` and stops; the others' waits then run out too,
+// says so (report_give_up) and stops; the others' waits then run out too,
 // and the CTA ends after its copies and MMAs in flight.
 constexpr int kDepthBlock = 64;  // 16-bit elements in a 128-byte row of a stage
 constexpr int kMatmulThreads = 384;
@@ -289,7 +289,7 @@ struct MatmulArgs {
   int32_t band;      // tile rows taken together
   int32_t pair_offset;
   int64_t m, n;
-  unsigned* timeouts;
+  Waits waits;
 };
 
 struct Item {
@@ -469,13 +469,13 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
     uint32_t phase = 0;
     bool ok = true;
     int64_t issued = 0;
-    for (int32_t t = first; t < items && ok; t += step) {
+    for (int32_t t = args.waits.stall ? items : first; t < items && ok; t += step) {
       const Item it = item_at(args, t);
       const int32_t row = it.tm * (128 * kGroup) + static_cast<int32_t>(rank) * 128;
       const int32_t col = it.tn * c_cols;
       const DepthRange range = depth_range(args, it.split);
       for (int32_t k = range.first; k < range.last; ++k) {
-        if (!mbar_wait_warp(empty(s), phase ^ 1)) {
+        if (!mbar_wait_warp(empty(s), phase ^ 1, args.waits.limit_ns)) {
           ok = false;
           break;
         }
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
     }
     pdl_trigger();
     if (!ok) {
-      if (lane == 0) atomicAdd(args.timeouts, 1u);
+      if (lane == 0) report_give_up(args.waits);
       // The stages issued last and not known to have landed.
       if (rank == 0) {
         for (int j = 0; j < stages && j < issued; ++j) {
@@ -539,14 +539,14 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
       const DepthRange range = depth_range(args, t % args.splits);
       for (int32_t begin = range.first; begin < range.last && ok;) {
         const int32_t end = E::kSegment > 0 ? min(begin + E::kSegment, range.last) : range.last;
-        if (!mbar_wait_warp(acc_empty(buf), buf_phase ^ 1)) {
+        if (!mbar_wait_warp(acc_empty(buf), buf_phase ^ 1, args.waits.limit_ns)) {
           ok = false;
           break;
         }
         tmem_fence_after();
         const uint32_t d = tmem + buf * (kTmemColumns / 2);
         for (int32_t k = begin; k < end; ++k) {
-          if (!mbar_wait_warp(full(s), phase)) {
+          if (!mbar_wait_warp(full(s), phase, args.waits.limit_ns)) {
             ok = false;
             break;
           }
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
     }
     if (!ok) {
       if (elect_one()) {
-        atomicAdd(args.timeouts, 1u);
+        report_give_up(args.waits);
         mma_commit<kGroup>(drained);
       }
       __syncwarp();
@@ -587,8 +587,8 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
       const bool any = __any_sync(~0u, l.inside);
       // Waits for the accumulators that are due next; their address.
       auto take = [&](uint32_t& acc) {
-        if (!mbar_wait_warp(acc_full(buf), phase)) {
-          if (lane == 0) atomicAdd(args.timeouts, 1u);
+        if (!mbar_wait_warp(acc_full(buf), phase, args.waits.limit_ns)) {
+          if (lane == 0) report_give_up(args.waits);
           return false;
         }
         tmem_fence_after();
@@ -806,7 +806,7 @@ class PlannedProduct {
     // 696, 3290); the gradients' products differ by less than 1% from 4 to 16.
     args.band = kAKMajor && kBKMajor ? 16 : 8;
     args.m = q.m, args.n = q.n, args.pair_offset = static_cast<int32_t>(q.pair_offset);
-    if ((st = timeout_counter(dev, &args.timeouts)) != HPRN_OK) return st;
+    if ((st = waits_of(dev, &args.waits, what)) != HPRN_OK) return st;
     CUtensorMap map_a, map_b;
     st = kAKMajor ? encode_rows(&map_a, q.a.p, q.m, q.depth, q.a.ld, args.a_rows, what)
                   : encode_rows(&map_a, q.a.p, q.depth, q.m, q.a.ld, kDepthBlock, what);

@@ -963,10 +963,49 @@ int run(const Problem& q, void* stream, unsigned flags) {
   return ok();
 }
 
-// The wait counter's address on the current device, for the kernels of other
-// files.
-int timeout_counter(const DeviceInfo* dev, unsigned** out) {
-  static std::atomic<unsigned*> known[64];
+namespace {
+
+// Test hook of the kernels that waits_of serves (hprn_test_stall_loads).
+std::atomic<bool> g_stall_loads{false};
+std::atomic<uint64_t> g_stall_loads_wait_ns{kWaitLimitNs};
+
+constexpr int kMostDevices = 64;
+
+// One word a device, in host memory that every device can write.
+volatile unsigned* seen_words() {
+  static std::mutex mu;
+  static std::atomic<unsigned*> words{nullptr};
+  unsigned* p = words.load(std::memory_order_acquire);
+  if (p) return p;
+  std::lock_guard<std::mutex> lock(mu);
+  if ((p = words.load(std::memory_order_relaxed))) return p;
+  // Allowed while a stream of this thread is being captured.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  void* q = nullptr;
+  const cudaError_t e = cudaHostAlloc(&q, kMostDevices * sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  p = static_cast<unsigned*>(q);
+  for (int k = 0; k < kMostDevices; ++k) p[k] = 0;
+  words.store(p, std::memory_order_release);
+  return p;
+}
+
+}  // namespace
+
+int waits_of(const DeviceInfo* dev, Waits* out, const char* what) {
+  static std::atomic<unsigned*> known[kMostDevices];
+  volatile unsigned* seen = seen_words();
+  if (!seen) return fail(HPRN_ERR_CUDA, std::string(what) + ": no host memory for the wait reports");
+  seen += dev->device;
+  if (*seen)
+    return fail(HPRN_ERR_CUDA, std::string(what) +
+                                   ": a wait of an earlier launch on this device ran out, its outputs are "
+                                   "incomplete (hprn_wait_timeouts with reset clears this)");
   unsigned* p = known[dev->device].load(std::memory_order_relaxed);
   if (!p) {
     const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_wait_timeouts);
@@ -974,8 +1013,15 @@ int timeout_counter(const DeviceInfo* dev, unsigned** out) {
       return fail(HPRN_ERR_CUDA, std::string("the wait-timeout count: ") + cudaGetErrorString(e));
     known[dev->device].store(p, std::memory_order_relaxed);
   }
-  *out = p;
+  out->count = p, out->seen = seen;
+  out->limit_ns = g_stall_loads_wait_ns.load(std::memory_order_relaxed);
+  out->stall = g_stall_loads.load(std::memory_order_relaxed);
   return HPRN_OK;
+}
+
+void forget_give_ups(const DeviceInfo* dev) {
+  volatile unsigned* seen = seen_words();
+  if (seen) seen[dev->device] = 0;
 }
 
 }  // namespace hprn
@@ -1075,7 +1121,17 @@ int hprn_wait_timeouts(unsigned int* count, int reset) {
   }
   if (e != cudaSuccess)
     return fail(HPRN_ERR_CUDA, std::string("reading the wait-timeout count: ") + cudaGetErrorString(e));
+  if (reset) forget_give_ups(dev);
   *count = v;
+  return ok();
+}
+
+int hprn_test_stall_loads(int on, uint64_t wait_limit_ns) {
+  using namespace hprn;
+  if (wait_limit_ns > kWaitLimitNs)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "wait_limit_ns must be at most one second");
+  g_stall_loads_wait_ns.store(on && wait_limit_ns ? wait_limit_ns : kWaitLimitNs, std::memory_order_relaxed);
+  g_stall_loads.store(on != 0, std::memory_order_relaxed);
   return ok();
 }
 

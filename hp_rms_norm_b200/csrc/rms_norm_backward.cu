@@ -42,7 +42,7 @@ struct NormGradArgs {
   int row_threads, row_groups, slots;  // of norm_grad_rows
   bool weight_staged;                  // in shared memory
   bool dense;                          // every tensor's rows follow each other
-  unsigned* timeouts;
+  Waits waits;
 };
 
 // Both of a pair's sums over a warp: the lower half warp adds up .x, the upper
@@ -121,8 +121,8 @@ __device__ __forceinline__ void sts_half(uint32_t addr, uint16_t h) {
 // 155 with rows copied element by element.
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies
-// still in flight, counted in `timeouts`; the rows it had not finished keep
-// their dx.
+// still in flight, and says so (report_give_up); the rows it had not finished
+// keep their dx.
 constexpr int kNormThreads = 512;
 
 template <typename T, int W, bool EXTRA, bool kVectors>
@@ -183,8 +183,9 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < a.rows; base += step) {
-      ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1));
+    for (int64_t base = a.waits.stall ? a.rows : static_cast<int64_t>(blockIdx.x) * groups; base < a.rows;
+         base += step) {
+      ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1, a.waits.limit_ns));
       if (!ok) break;
       const uint32_t bar = smem_u32(&full[slot]), to = slots_at + slot * slot_bytes;
       const int64_t next = base + a.slots * step;  // few buffers: asked into L2
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
       if (++slot == a.slots) slot = 0, phase ^= 1;
     }
     if (!ok) {
-      if (lane == 0) atomicAdd(a.timeouts, 1u);
+      if (lane == 0) report_give_up(a.waits);
       for (int k = 0; k < a.slots; ++k) {  // copies still in flight
         if (--slot < 0) slot = a.slots - 1, phase ^= 1;
         mbar_wait_bounded(smem_u32(&full[slot]), phase, kWaitLimitNs / 16);
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
     const uint32_t at = ring + slot * slot_bytes;
     const uint32_t xs = at + offset_of(row_of(0, i)), ds = at + tensor_bytes + offset_of(row_of(1, i));
     const uint32_t es = EXTRA ? at + 2 * tensor_bytes + offset_of(row_of(2, i)) : 0;
-    if (!mbar_wait_bounded(smem_u32(&full[slot]), phase)) gave_up[group] = 1;
+    if (!mbar_wait_bounded(smem_u32(&full[slot]), phase, a.waits.limit_ns)) gave_up[group] = 1;
     float2 ss = make_float2(0.f, 0.f), sd = ss;
     float2 wd[kHold ? W : 1];  // w D, for both passes
 #pragma unroll
@@ -342,7 +343,11 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
     }
     const float2 s =
         row_sum2(make_float2(ss.x + ss.y, sd.x + sd.y), part[turn], tid / 32, warps, barrier, group * warps);
-    if (*static_cast<volatile int*>(&gave_up[group])) break;
+    if (*static_cast<volatile int*>(&gave_up[group])) {
+      // The copier may have issued its last row and left without a wait.
+      if (in == 0) report_give_up(a.waits);
+      break;
+    }
     const float inv = rsqrtf(s.x * scale + a.eps), mean = s.y * inv * scale;
     const float2 inv2 = make_float2(inv, inv), minus = make_float2(-mean * inv, -mean * inv);
     uint16_t* dx = a.dx + i * a.dx_stride;
@@ -633,7 +638,7 @@ extern "C" int hprn_rms_norm_backward(void* grad_input, void* grad_weight, const
   const DeviceInfo* dev = nullptr;
   int st = current_device(&dev);
   if (st != HPRN_OK) return st;
-  if ((st = timeout_counter(dev, &a.timeouts)) != HPRN_OK) return st;
+  if ((st = waits_of(dev, &a.waits, "rms_norm_backward")) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   return dtype == HPRN_DTYPE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, plan, dev, cs, flags)
                                   : launch_norm_grad<__half>(a, plan, dev, cs, flags);

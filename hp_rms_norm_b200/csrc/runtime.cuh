@@ -144,8 +144,29 @@ int launch_rows(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, un
   return launch_rows_smem(fn, grid, block, 0, stream, flags, what, static_cast<A&&>(args)...);
 }
 
-// The counter of waits that ran out, on the current device.
-int timeout_counter(const DeviceInfo* dev, unsigned** out);
+// The bounded waits of a launch.  A role whose wait runs out says so in two
+// places: a count on the device (hprn_wait_timeouts), and a word of host memory
+// that later calls look at without waiting for the GPU.
+struct Waits {
+  unsigned* count;
+  volatile unsigned* seen;
+  uint64_t limit_ns;
+  bool stall;  // test hook: nothing is loaded, so that every wait for loads runs out
+};
+// The current device's; an error where an earlier launch's wait ran out and
+// nobody has reset the count since.
+int waits_of(const DeviceInfo* dev, Waits* out, const char* what);
+// Clears the word in host memory.
+void forget_give_ups(const DeviceInfo* dev);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void report_give_up(const Waits& w) {
+  atomicAdd(w.count, 1u);
+  *w.seen = 1u;
+  __threadfence_system();
+}
+#endif
+
 // Raises a kernel's dynamic shared memory limit, once per device.
 int allow_smem(const DeviceInfo* dev, const void* fn, int bytes, const char* what);
 

@@ -393,7 +393,10 @@ HPRN_API int hprn_set_plan_override(const char* plan);
  * on its device: in the tma plans it leaves the row it gave up on and its
  * remaining rows untouched (input and residual as they were), in the others
  * the outputs it had not written.  The call that launched it still returns
- * HPRN_OK.  No wait gives up on a GPU that works.
+ * HPRN_OK; later calls of hprn_gated_linear*, hprn_linear_cross_entropy* and
+ * hprn_rms_norm_backward on that device return HPRN_ERR_CUDA once a launch of
+ * these has given up a wait, until the count is reset.  No wait gives up on a
+ * GPU that works.
  * Writes the current device's count into *count and, if `reset` is non-zero,
  * clears it.  Synchronous; synchronise the streams that launched the kernels
  * first.  A non-zero count means the launches since the last reset produced
@@ -416,6 +419,16 @@ HPRN_API int hprn_wait_timeouts(unsigned int* count, int reset);
  * for tests only.
  */
 HPRN_API int hprn_test_stall_bulk_copy(int64_t row, uint64_t wait_limit_ns);
+
+/*
+ * No reference counterpart.  Test hook for the same waits of the training
+ * operators: while `on` is non-zero, every launch of their matrix products and
+ * of hprn_rms_norm_backward loads nothing, so that its waits run out, after
+ * `wait_limit_ns` nanoseconds each (at most one second; 0 keeps that), and its
+ * CTAs take their give-up path.  No fault and no hang: every wait stays
+ * bounded.  Process-global; for tests only.
+ */
+HPRN_API int hprn_test_stall_loads(int on, uint64_t wait_limit_ns);
 
 /*
  * No reference counterpart.  Test hook, launches nothing: how

@@ -167,3 +167,8 @@ def test_torch_operators_are_cuda_only_and_trace():
     t = torch.zeros(4, dtype=torch.int64, device="meta")
     assert hp.linear_cross_entropy(m(x), m(w), t)[0].shape == (4,)
     assert hp.rms_norm_backward(m(x), m(x), m(x[0]), 1e-6)[1].shape == (8,)
+
+
+def test_stall_hook_refuses_long_waits():
+    assert capi.load().hprn_test_stall_loads(1, 1_000_000_001) == capi.ERR_INVALID_ARGUMENT
+    capi.test_stall_loads(False)
