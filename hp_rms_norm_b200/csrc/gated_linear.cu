@@ -12,7 +12,8 @@
 // S is what the tensor cores read, so its rounding to 16 bits is the one
 // rounding between the inputs and the fp32 sums of dX and dW.  G and U come
 // from `gate_up`, or are computed again (4 rows hidden d more operations, no
-// 8 rows d bytes kept).
+// 8 rows d bytes kept): 4096 x 4096 x 2 * 14336 bf16, backward 1536 us with the
+// products kept, 2195 without, forward 648 us writing them, 590 without.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

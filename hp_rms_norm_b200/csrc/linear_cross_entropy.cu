@@ -21,7 +21,7 @@
 // -1 is exact (8192 x 4096 x 131072, one draw of the targets: 3.5e-3 off without,
 // 1.7e-3, the rounding of the outputs themselves, with it).  In fp16 S is held
 // times 2^14 as well: softmax values of a large vocabulary fall below its
-// smallest normal, 6e-5.
+// smallest normal, 6e-5 (now those below 3.7e-9 c_max / |c_i| do).
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -117,7 +117,7 @@ __device__ __forceinline__ void sts_half(uint32_t addr, uint16_t h) {
 // two passes (held at 16 words it spilled: 4096 x 16384 106 us instead of 93).
 // 4096 x 8192 with E: 48.0 us (0.87 of a copy of the same bytes),
 // against 55.8 with the rows themselves in registers, which spilled or kept
-// one row a CTA in flight.  4096 x 5001 with E: 72 us, bound by issue, against
+// one row a CTA in flight.  4096 x 5001 with E: 73 us, bound by issue, against
 // 155 with rows copied element by element.
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies
@@ -427,6 +427,11 @@ __global__ void __launch_bounds__(kNormThreads + 32, 1) norm_grad_rows(NormGradA
   }
 }
 
+// Rows too long for norm_grad_rows (more than 32768 elements, or about 28,150 off
+// 16-byte boundaries with E) in two readings of single elements, bound by the
+// loads in flight: 4096 x 32769 with E 476 us, 0.35 of a copy's rate, where
+// 32768 takes 277.
+//
 // One CTA per row: the row's two sums.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_grad_stats(NormGradArgs a) {

@@ -276,7 +276,8 @@ HPRN_API int hprn_linear_cross_entropy(float* loss, float* lse, const void* inpu
  *   grad_input [rows, hidden]  = round_T(S weight)
  *   grad_weight [vocab, hidden] = round_T(S^T input)
  * S is held divided by the largest finite |c_i| (and in fp16 times 2^14), so equal
- * c_i are not all rounded alike and small probabilities do not underflow.  Where
+ * c_i are not all rounded alike, and in fp16 only entries below 3.7e-9 of that
+ * largest one fall under the smallest normal number.  Where
  * c_i is infinite or NaN, so are row i of grad_input and grad_weight.
  */
 HPRN_API int hprn_linear_cross_entropy_backward(
