@@ -1,7 +1,7 @@
 """The operators that have a backward pass, as torch.autograd functions.
 
-``rms_norm``, ``fused_add_rms_norm``, ``gated_linear`` and
-``linear_cross_entropy`` take and return tensors like torch's own functions do;
+``rms_norm``, ``fused_add_rms_norm``, ``gated_add_rms_norm``, ``gated_linear``,
+``linear_cross_entropy`` and ``linear_log_probs`` take and return tensors like torch's own functions do;
 their forward and backward passes are the kernels behind the functions of
 ``hp_rms_norm_b200.ops`` with the same names.  Nothing is changed in place: the
 values a backward pass needs (a block's residual among them) stay as they were.
@@ -89,6 +89,60 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return grad_input, grad_weight, None, None
 
 
+class _GatedAddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, residual, post_weight, weight, gate, eps, residual_scale):
+        total = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        out = ops.gated_add_rms_norm(input, residual, post_weight, weight, eps, gate=gate,
+                                     residual_scale=residual_scale, residual_out=total)
+        ctx.save_for_backward(input, total, post_weight, weight, gate)
+        ctx.eps, ctx.residual_scale = eps, residual_scale
+        ctx.set_materialize_grads(False)
+        return out, total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_total):
+        input, total, post_weight, weight, gate = ctx.saved_tensors
+        if grad_out is None:
+            if grad_total is None:
+                return (None,) * 7
+            grad_out = torch.zeros_like(total)
+        if grad_total is not None:
+            grad_total = grad_total.contiguous()
+        grads = ops.gated_add_rms_norm_backward(grad_out.contiguous(), input, total, post_weight,
+                                                weight, ctx.eps, gate=gate,
+                                                residual_scale=ctx.residual_scale,
+                                                grad_residual=grad_total)
+        return grads + (None, None)
+
+
+class _LinearLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, weight, target, temperature, ignore_index):
+        found = ops.linear_log_probs(input, weight, target, temperature=temperature,
+                                     ignore_index=ignore_index)
+        ctx.save_for_backward(input, weight, target, found.lse, found.entropy)
+        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.set_materialize_grads(False)
+        return found.log_prob, found.entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_log_prob, grad_entropy):
+        if grad_log_prob is None and grad_entropy is None:
+            return (None,) * 5
+        input, weight, target, lse, entropy = ctx.saved_tensors
+        if grad_log_prob is None:
+            grad_log_prob = torch.zeros_like(grad_entropy)
+        if grad_entropy is not None:
+            grad_entropy = grad_entropy.contiguous()
+        grad_input, grad_weight = ops.linear_log_probs_backward(
+            grad_log_prob.contiguous(), input, weight, target, lse, entropy=entropy,
+            grad_entropy=grad_entropy, temperature=ctx.temperature, ignore_index=ctx.ignore_index)
+        return grad_input, grad_weight, None, None, None
+
+
 def rms_norm(input, weight, eps):
     """RMSNorm(input) * weight."""
     return _RMSNorm.apply(input, weight, eps)
@@ -97,6 +151,12 @@ def rms_norm(input, weight, eps):
 def fused_add_rms_norm(input, residual, weight, eps):
     """(RMSNorm(total) * weight, total) for total = input + residual."""
     return _FusedAddRMSNorm.apply(input, residual, weight, eps)
+
+
+def gated_add_rms_norm(input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0):
+    """(RMSNorm(total) * weight, total) for total = residual_scale * residual + gate *
+    (RMSNorm(input) * post_weight); ``post_weight`` and ``gate`` as in ``ops.gated_add_rms_norm``."""
+    return _GatedAddRMSNorm.apply(input, residual, post_weight, weight, gate, eps, residual_scale)
 
 
 def gated_linear(input, weight, act="silu", keep_products=True):
@@ -118,4 +178,11 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction="me
     return loss.sum() / (target != ignore_index).sum() if reduction == "mean" else loss.sum()
 
 
-__all__ = ["rms_norm", "fused_add_rms_norm", "gated_linear", "linear_cross_entropy"]
+def linear_log_probs(input, weight, target, temperature=1.0, ignore_index=-100):
+    """(log_prob, entropy) of each row under softmax(input weight^T / temperature), both with
+    gradients; 0 where the target is ``ignore_index``."""
+    return _LinearLogProbs.apply(input, weight, target, temperature, ignore_index)
+
+
+__all__ = ["rms_norm", "fused_add_rms_norm", "gated_add_rms_norm", "gated_linear",
+           "linear_cross_entropy", "linear_log_probs"]

@@ -62,6 +62,12 @@ EXPORTED = (
     "hprn_grad_norm",
     "hprn_grad_clip",
     "hprn_clip_grad_norm",
+    "hprn_gated_add_rms_norm",
+    "hprn_gated_add_rms_norm_backward",
+    "hprn_linear_log_probs",
+    "hprn_linear_log_probs_backward",
+    "hprn_rms_norm_int8",
+    "hprn_linear_int8",
     "hprn_test_loss_backward_piece",
     "hprn_test_stall_loads",
 )
@@ -140,13 +146,25 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.hprn_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, vp, wsp, vp, u32]
     lib.hprn_clip_grad_norm.argtypes = [vp, ctypes.POINTER(Grad), i64, ctypes.c_double, vp, wsp, vp, u32]
     lib.hprn_grad_clip.argtypes = [ctypes.POINTER(Grad), i64, vp, ctypes.c_double, vp, u32]
+    dbl = ctypes.c_double
+    lib.hprn_gated_add_rms_norm.argtypes = [vp] * 7 + [i64] * 9 + [dbl, dbl, c_int, vp, u32]
+    lib.hprn_gated_add_rms_norm_backward.argtypes = ([vp] * 12 + [i64] * 12 + [dbl, dbl, c_int]
+                                                     + [vp, wsp, vp, u32])
+    lib.hprn_linear_log_probs.argtypes = [vp] * 8 + [i64, dbl] + [i64] * 6 + [c_int, vp, wsp, vp, u32]
+    lib.hprn_linear_log_probs_backward.argtypes = ([vp] * 9 + [i64, dbl] + [i64] * 7
+                                                   + [c_int, vp, wsp, vp, u32])
+    lib.hprn_rms_norm_int8.argtypes = [vp] * 6 + [i64] * 6 + [dbl, c_int, vp, u32]
+    lib.hprn_linear_int8.argtypes = [vp] * 6 + [i64] * 6 + [c_int, vp, wsp, vp, u32]
     lib.hprn_test_loss_backward_piece.argtypes = [i64] * 4 + [wsp]
     lib.hprn_test_loss_backward_piece.restype = c_int
     lib.hprn_test_stall_loads.argtypes = [c_int, ctypes.c_uint64]
     lib.hprn_test_stall_loads.restype = c_int
     for fn in (lib.hprn_gated_linear, lib.hprn_gated_linear_backward, lib.hprn_linear_cross_entropy,
                lib.hprn_linear_cross_entropy_backward, lib.hprn_rms_norm_backward,
-               lib.hprn_grad_norm, lib.hprn_grad_clip, lib.hprn_clip_grad_norm):
+               lib.hprn_grad_norm, lib.hprn_grad_clip, lib.hprn_clip_grad_norm,
+               lib.hprn_gated_add_rms_norm, lib.hprn_gated_add_rms_norm_backward,
+               lib.hprn_linear_log_probs, lib.hprn_linear_log_probs_backward,
+               lib.hprn_rms_norm_int8, lib.hprn_linear_int8):
         fn.restype = c_int
     _lib = lib
     return lib

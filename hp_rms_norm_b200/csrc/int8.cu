@@ -1,0 +1,445 @@
+// Linear layers in 8-bit integers: tokens quantised with one scale each (by
+// themselves, or as the output of an RMSNorm), the weight with one scale for
+// each output channel.
+//   scale_i = max(max_j |y_ij|, 1e-12) / 127,  q_ij = round(y_ij (1 / scale_i))
+//   out_ij = (sum_k q_ik v_jk) scale_i channel_j + bias_j
+// The sum is an exact 32-bit integer from the tensor cores; it is rounded to
+// fp32 once, and the result to 16 bits once.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "matmul.cuh"
+#include "rows.cuh"
+#include "runtime.cuh"
+
+namespace hprn {
+
+// ---------------------------------------------------------------------------
+// Quantised rows: y = RMSNorm(t) w with t = x [+ r], or y = x without a weight.
+
+struct QuantArgs {
+  int8_t* q;
+  float* scales;
+  uint16_t* t;        // the sum x + r, where there is an r
+  const uint16_t* x;
+  const uint16_t* r;  // or null
+  const uint16_t* w;  // or null: no norm
+  int64_t q_stride, t_stride, x_stride, r_stride;
+  int32_t rows, hidden;
+  int32_t row_threads, nvec;
+  float eps, inv_hidden;
+};
+
+// max(m, |a|, |b|), NaN where one is: a row with a NaN gets a NaN scale.
+__device__ __forceinline__ float amax_nan(float m, float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return d;
+}
+
+// The largest over the threads that hold a row, as row_sum.
+__device__ __forceinline__ float row_amax(float v, float* part, int warps, int first_warp) {
+  auto over = [](float m) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = amax_nan(m, __shfl_xor_sync(~0u, m, o), 0.f);
+    return m;
+  };
+  v = over(v);
+  if (warps == 1) return v;
+  const int lane = threadIdx.x % 32;
+  if (lane == 0) part[threadIdx.x / 32] = v;
+  __syncthreads();
+  return over(lane < warps ? part[first_warp + lane] : 0.f);
+}
+
+// A pair's codes, the first in the low byte.  (cvt.rni of a NaN is 0.)
+__device__ __forceinline__ uint32_t codes_of(float2 y, float inv) {
+  uint32_t d;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(d) : "r"(__float2int_rn(y.y * inv)), "r"(__float2int_rn(y.x * inv)));
+  return d & 0xffffu;
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t* q, const float2 (&y)[Pairs<VEC>::kCount], float inv) {
+  if constexpr (VEC == 2) {
+    *q = static_cast<int8_t>(codes_of(y[0], inv));
+  } else if constexpr (VEC == 4) {
+    *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(codes_of(y[0], inv));
+  } else {
+    Vec<VEC / 2> o;
+#pragma unroll
+    for (int k = 0; k < VEC / 8; ++k) o.w[k] = codes_of(y[2 * k], inv) | codes_of(y[2 * k + 1], inv) << 16;
+    st_global<VEC / 2>(q, o);
+  }
+}
+
+// Rows held in registers, laid out over threads as in gated_norm.cu.
+template <typename T, int VEC, int VPT>
+__global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) quant_rows(QuantArgs a) {
+  constexpr int P = Pairs<VEC>::kCount;
+  __shared__ float part[2][32];
+  const int in = threadIdx.x % a.row_threads, group = threadIdx.x / a.row_threads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.row_threads) + group;
+  const int warps = a.row_threads / 32, first_warp = group * warps;
+  const bool valid = row < a.rows;
+  auto inside = [&](int k) { return valid && in + k * a.row_threads < a.nvec; };
+  auto at = [&](int k) { return static_cast<int64_t>(in + k * a.row_threads) * Vec<VEC>::kElems; };
+  const uint64_t once = policy_evict_first(), keep = policy_evict_last();
+  pdl_wait();
+
+  Vec<VEC> x[VPT], r[VPT];
+#pragma unroll
+  for (int k = 0; k < VPT; ++k)
+    if (inside(k)) x[k] = ld_stream<VEC>(a.x + row * a.x_stride + at(k), once);
+  if (a.r) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+      if (inside(k)) r[k] = ld_stream<VEC>(a.r + row * a.r_stride + at(k), once);
+  }
+  float2 y[VPT][P], s = make_float2(0.f, 0.f);
+  float most = 0.f;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    if (!inside(k)) break;
+    Vec<VEC> o, w;
+    if (a.w) w = ld_weight<VEC>(a.w + at(k), keep);
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      float2 v = pair_of<T, VEC>(x[k], e);
+      if (a.r) {
+        v = __fadd2_rn(v, pair_of<T, VEC>(r[k], e));
+        set_pair<T, VEC>(o, e, v);
+      }
+      s = __ffma2_rn(v, v, s);
+      if (a.w) v = __fmul2_rn(v, pair_of<T, VEC>(w, e));
+      y[k][e] = v;
+      most = amax_nan(most, v.x, v.y);
+    }
+    if (a.r) st_global<VEC>(a.t + row * a.t_stride + at(k), o);
+  }
+  float inv = 1.f;
+  if (a.w) inv = rsqrtf(row_sum(s.x + s.y, part[0], warps, first_warp) * a.inv_hidden + a.eps);
+  // max |y inv| = max |y| inv, rounded once: rounding keeps the order.
+  most = row_amax(most, part[1], warps, first_warp) * inv;
+  pdl_trigger();
+  const float scale = amax_nan(1e-12f, most, 0.f) / 127.f, by = 1.f / scale;
+  if (valid && in == 0) a.scales[row] = scale;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    if (!inside(k)) break;
+#pragma unroll
+    for (int e = 0; e < P; ++e) y[k][e] = __fmul2_rn(y[k][e], make_float2(inv, inv));
+    store_codes<VEC>(a.q + row * a.q_stride + at(k), y[k], by);
+  }
+}
+
+// Rows too long for registers, one CTA a row, read twice.  The second reading
+// finds the same x and r: where the residual is updated in place, its new value
+// is written then.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(1024) quant_long_rows(QuantArgs a) {
+  constexpr int P = Pairs<VEC>::kCount;
+  __shared__ float part[2][32];
+  const int64_t row = blockIdx.x;
+  pdl_wait();
+  Vec<VEC> rounded;
+  float2 y[P], sum[P];
+  auto load = [&](int64_t at) {
+    const Vec<VEC> x = ld_l2<VEC>(a.x + row * a.x_stride + at);
+    Vec<VEC> r;
+    if (a.r) r = ld_l2<VEC>(a.r + row * a.r_stride + at);
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      sum[e] = pair_of<T, VEC>(x, e);
+      if (a.r) {
+        sum[e] = __fadd2_rn(sum[e], pair_of<T, VEC>(r, e));
+        set_pair<T, VEC>(rounded, e, sum[e]);
+      }
+      y[e] = a.w ? __fmul2_rn(sum[e], load_pair<T, VEC>(a.w + at, e)) : sum[e];
+    }
+  };
+  float2 s = make_float2(0.f, 0.f);
+  float most = 0.f;
+  for (int v = threadIdx.x; v < a.nvec; v += 1024) {
+    load(static_cast<int64_t>(v) * Vec<VEC>::kElems);
+#pragma unroll
+    for (int e = 0; e < P; ++e) s = __ffma2_rn(sum[e], sum[e], s), most = amax_nan(most, y[e].x, y[e].y);
+  }
+  float inv = 1.f;
+  if (a.w) inv = rsqrtf(row_sum(s.x + s.y, part[0], 32, 0) * a.inv_hidden + a.eps);
+  most = row_amax(most, part[1], 32, 0) * inv;
+  pdl_trigger();
+  const float scale = amax_nan(1e-12f, most, 0.f) / 127.f, by = 1.f / scale;
+  if (threadIdx.x == 0) a.scales[row] = scale;
+  for (int v = threadIdx.x; v < a.nvec; v += 1024) {
+    const int64_t at = static_cast<int64_t>(v) * Vec<VEC>::kElems;
+    load(at);
+    if (a.r) st_global<VEC>(a.t + row * a.t_stride + at, rounded);
+#pragma unroll
+    for (int e = 0; e < P; ++e) y[e] = __fmul2_rn(y[e], make_float2(inv, inv));
+    store_codes<VEC>(a.q + row * a.q_stride + at, y, by);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The product.
+
+// Rows of bytes copied to rows on 32-byte boundaries, zeros behind them.
+struct ByteCopy {
+  uint8_t* dst;
+  const uint8_t* src;
+  int64_t dst_ld, src_ld, rows, cols;
+};
+struct ByteCopies {
+  ByteCopy c[2];
+};
+
+__global__ void __launch_bounds__(256) copy_byte_rows(ByteCopies both) {
+  pdl_wait();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const ByteCopy& c = both.c[k];
+    const int64_t per_row = c.dst_ld / 4, all = c.rows * per_row;
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < all;
+         e += static_cast<int64_t>(gridDim.x) * 256) {
+      const int64_t i = e / per_row, j = (e - i * per_row) * 4;
+      const uint8_t* p = c.src + i * c.src_ld + j;
+      uint32_t w = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (j + b < c.cols) w |= static_cast<uint32_t>(p[b]) << (8 * b);
+      *reinterpret_cast<uint32_t*>(c.dst + i * c.dst_ld + j) = w;
+    }
+  }
+}
+
+// An operand as TMA reads it: rows on 16-byte boundaries and of an even length
+// (the tensor map counts pairs), or a copy of it.
+class ByteRows {
+ public:
+  ByteRows(Workspace& ws, const void* p, int64_t rows, int64_t cols, int64_t ld)
+      : src_(static_cast<const uint8_t*>(p)), rows_(rows), cols_(cols), src_ld_(ld), ld_(ld) {
+    if (rows <= 1) ld_ = round_up(cols > 0 ? cols : 1, 16);
+    if (rows <= 0 || cols <= 0 || (aligned(p, 16) && (rows <= 1 || ld % 16 == 0) && cols % 2 == 0)) return;
+    ld_ = round_up(cols, 32);
+    copies_ = true;
+    copy_ = ws.take<uint8_t>(rows * ld_);
+  }
+  // Pairs of bytes, as the products count.
+  const uint16_t* data() const { return reinterpret_cast<const uint16_t*>(copies_ ? copy_ : src_); }
+  int64_t ld() const { return ld_ / 2; }
+  ByteCopy copy() const { return copies_ ? ByteCopy{copy_, src_, ld_, src_ld_, rows_, cols_} : ByteCopy{}; }
+
+ private:
+  const uint8_t* src_;
+  int64_t rows_, cols_, src_ld_, ld_;
+  bool copies_ = false;
+  uint8_t* copy_ = nullptr;
+};
+
+template <typename T>
+struct ScaledEpilogue {
+  static constexpr bool kPaired = false;
+  static constexpr int kSegment = 0;
+  static constexpr bool kInteger = true;
+  Out16 out;
+  const float* row_scale = nullptr;
+  const float* channel_scale = nullptr;
+  const uint16_t* bias = nullptr;  // or null
+
+  struct Row {
+    float scale;
+  };
+  __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const { return Row{l.inside ? row_scale[i] : 0.f}; }
+  __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+      const int64_t c = j + k < out.n ? j + k : out.n - 1;
+      v[k] = value(v[k], r.scale, c);
+    }
+    out.template store<T>(l, i, j, v);
+  }
+  __device__ __forceinline__ float value(float bits, float scale, int64_t j) const {
+    const float y = static_cast<float>(__float_as_int(bits)) * scale * channel_scale[j];
+    return bias ? y + unpack1<T>(bias[j]) : y;
+  }
+  __device__ __forceinline__ void end(Row&, const Lane&, int64_t, int64_t) const {}
+  __device__ __forceinline__ void point(int64_t i, int64_t j, float v) const {
+    out.p[i * out.ld + j] = pack1<T>(value(v, row_scale[i], j));
+  }
+};
+
+namespace {
+
+template <typename T>
+void (*quant_kernel(int vec, int vpt))(QuantArgs) {
+  switch (vec * 100 + vpt) {
+    case 3201: return quant_rows<T, 32, 1>;
+    case 3202: return quant_rows<T, 32, 2>;
+    case 1601: return quant_rows<T, 16, 1>;
+    case 1602: return quant_rows<T, 16, 2>;
+    case 401: return quant_rows<T, 4, 1>;
+    case 402: return quant_rows<T, 4, 2>;
+    case 404: return quant_rows<T, 4, 4>;
+    case 408: return quant_rows<T, 4, 8>;
+    case 201: return quant_rows<T, 2, 1>;
+    case 202: return quant_rows<T, 2, 2>;
+    case 204: return quant_rows<T, 2, 4>;
+    case 208: return quant_rows<T, 2, 8>;
+    case 216: return quant_rows<T, 2, 16>;
+    default: return nullptr;
+  }
+}
+
+template <typename T>
+int launch_quant(QuantArgs& a, int vec, cudaStream_t stream, unsigned flags) {
+  const char* what = "rms_norm_int8";
+  a.nvec = static_cast<int32_t>(static_cast<int64_t>(a.hidden) * 2 / vec);
+  for (int vpt = 1; vpt <= 16; vpt *= 2) {
+    const auto fn = quant_kernel<T>(vec, vpt);
+    const int64_t threads = round_up((a.nvec + vpt - 1) / vpt, 32);
+    if (!fn || threads > (vpt * vec > 32 ? 512 : 1024)) continue;
+    a.row_threads = static_cast<int32_t>(threads);
+    const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
+    return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),
+                       dim3(static_cast<unsigned>(threads * groups)), stream, flags, what, a);
+  }
+  if (vec >= 16) {
+    a.nvec = a.hidden / 8;
+    return launch_rows(quant_long_rows<T, 16>, dim3(a.rows), dim3(1024), stream, flags, what, a);
+  }
+  a.nvec = a.hidden;
+  return launch_rows(quant_long_rows<T, 2>, dim3(a.rows), dim3(1024), stream, flags, what, a);
+}
+
+}  // namespace
+}  // namespace hprn
+
+extern "C" {
+
+int hprn_rms_norm_int8(int8_t* out, float* scales, void* residual_out, const void* input, const void* weight,
+                       const void* residual, int64_t rows, int64_t hidden, int64_t out_row_stride,
+                       int64_t residual_out_row_stride, int64_t input_row_stride, int64_t residual_row_stride,
+                       double eps, int dtype, void* stream, unsigned flags) {
+  using namespace hprn;
+  if (flags & ~static_cast<unsigned>(HPRN_LAUNCH_PDL)) return fail(HPRN_ERR_INVALID_ARGUMENT, "unknown launch flags");
+  if (dtype != HPRN_DTYPE_BF16 && dtype != HPRN_DTYPE_FP16)
+    return fail(HPRN_ERR_UNSUPPORTED_DTYPE, "dtype must be kFloat16 or kBFloat16");
+  if (rows < 0 || hidden < 0) return fail(HPRN_ERR_INVALID_ARGUMENT, "sizes must be >= 0");
+  if (rows > kMaxExtent || hidden > kMaxExtent)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "rows and hidden must be at most 2^30");
+  if ((residual != nullptr) != (residual_out != nullptr))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "residual and residual_out go together");
+  if (rows > 1 && (out_row_stride < hidden || input_row_stride < hidden ||
+                   (residual && (residual_row_stride < hidden || residual_out_row_stride < hidden))))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  if (rows == 0 || hidden == 0) return ok();
+  if (!out || !scales || !input) return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  for (const void* p : {static_cast<const void*>(residual_out), input, weight, residual})
+    if (!aligned(p, 2)) return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  if (!aligned(scales, 4)) return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  if (rows == 1) out_row_stride = residual_out_row_stride = input_row_stride = residual_row_stride = hidden;
+  const Extent r = extent16(residual, rows, hidden, residual_row_stride),
+               t = extent16(residual_out, rows, hidden, residual_out_row_stride);
+  const Extent outs[] = {extent_of(out, rows, hidden, out_row_stride, 1), extent32(scales, 1, rows, rows), t};
+  const Extent ins[] = {extent16(input, rows, hidden, input_row_stride), extent16(weight, 1, hidden, hidden)};
+  const bool same_r = residual_out == residual && residual_out_row_stride == residual_row_stride;
+  if (!disjoint(outs, ins) || extents_overlap(outs[0], r) || extents_overlap(outs[1], r) ||
+      (!same_r && extents_overlap(t, r)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors, but for residual_out == residual");
+  const DeviceInfo* dev = nullptr;
+  const int st = current_device(&dev);
+  if (st != HPRN_OK) return st;
+  QuantArgs a{};
+  a.q = out, a.scales = scales, a.t = static_cast<uint16_t*>(residual_out);
+  a.x = static_cast<const uint16_t*>(input), a.r = static_cast<const uint16_t*>(residual);
+  a.w = static_cast<const uint16_t*>(weight);
+  a.q_stride = out_row_stride, a.t_stride = residual_out_row_stride, a.x_stride = input_row_stride;
+  a.r_stride = residual_row_stride;
+  a.rows = static_cast<int32_t>(rows), a.hidden = static_cast<int32_t>(hidden);
+  a.eps = static_cast<float>(eps), a.inv_hidden = 1.f / static_cast<float>(hidden);
+  int vec = 2;
+  for (int v : {32, 16, 4}) {
+    auto fits = [&](const void* p, int64_t stride, int bytes) {
+      return aligned(p, v * bytes / 2) && (rows <= 1 || !p || stride * bytes % (v * bytes / 2) == 0);
+    };
+    if (hidden * 2 % v == 0 && fits(out, out_row_stride, 1) && fits(residual_out, residual_out_row_stride, 2) &&
+        fits(input, input_row_stride, 2) && fits(residual, residual_row_stride, 2) && aligned(weight, v)) {
+      vec = v;
+      break;
+    }
+  }
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  return dtype == HPRN_DTYPE_BF16 ? launch_quant<__nv_bfloat16>(a, vec, cs, flags)
+                                  : launch_quant<__half>(a, vec, cs, flags);
+}
+
+int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, const int8_t* weight,
+                     const float* weight_scale, const void* bias, int64_t rows, int64_t hidden, int64_t channels,
+                     int64_t out_row_stride, int64_t input_row_stride, int64_t weight_row_stride, int dtype,
+                     void* workspace, int64_t* workspace_bytes, void* stream, unsigned flags) {
+  using namespace hprn;
+  if (flags & ~static_cast<unsigned>(HPRN_LAUNCH_PDL | HPRN_WORKSPACE_QUERY))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "unknown launch flags");
+  if (dtype != HPRN_DTYPE_BF16 && dtype != HPRN_DTYPE_FP16)
+    return fail(HPRN_ERR_UNSUPPORTED_DTYPE, "dtype must be kFloat16 or kBFloat16");
+  if (rows < 0 || hidden < 0 || channels < 0) return fail(HPRN_ERR_INVALID_ARGUMENT, "sizes must be >= 0");
+  if (rows > kMaxExtent || channels > kMaxExtent)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "rows and channels must be at most 2^30");
+  if (hidden > 131071)  // (-128)^2 * 131072 = 2^31
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "hidden must be at most 131071: the sums are 32-bit integers");
+  if (!workspace_bytes) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace_bytes pointer required");
+  if ((rows > 1 && (input_row_stride < hidden || out_row_stride < channels)) ||
+      (channels > 1 && weight_row_stride < hidden))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  Workspace ws(workspace, *workspace_bytes);
+  const ByteRows x(ws, input, rows, hidden, input_row_stride);
+  const ByteRows w(ws, weight, channels, hidden, weight_row_stride);
+  const int64_t pairs = (hidden + 1) / 2;
+  const PlannedProduct<false, true, true> product(ws, rows, channels, pairs);
+  if (flags & HPRN_WORKSPACE_QUERY) {
+    *workspace_bytes = ws.needed();
+    return ok();
+  }
+  if (rows == 0 || channels == 0) return ok();
+  if (!out || !input_scale || !weight_scale || (hidden > 0 && (!input || !weight)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(out, 2) || !aligned(input_scale, 4) || !aligned(weight_scale, 4) || !aligned(bias, 2))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  const Extent outs[] = {extent16(out, rows, channels, out_row_stride)};
+  const Extent ins[] = {extent_of(input, rows, hidden, input_row_stride, 1),
+                        extent_of(weight, channels, hidden, weight_row_stride, 1),
+                        extent32(input_scale, 1, rows, rows), extent32(weight_scale, 1, channels, channels),
+                        extent16(bias, 1, channels, channels)};
+  if (!disjoint(outs, ins)) return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors");
+  if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
+  const DeviceInfo* dev = nullptr;
+  int st = current_device(&dev);
+  if (st != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const char* what = "linear_int8";
+  const ByteCopies copies{{x.copy(), w.copy()}};
+  const int64_t words = (copies.c[0].rows * copies.c[0].dst_ld + copies.c[1].rows * copies.c[1].dst_ld) / 4;
+  if (words > 0) {
+    const int64_t ctas = (words + 255) / 256, most = 32 * dev->sm_count;
+    st = launch_rows(copy_byte_rows, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), cs, flags, what,
+                     copies);
+    if (st != HPRN_OK) return st;
+  }
+  Product q;
+  q.a = {x.data(), x.ld()};
+  q.b = {w.data(), w.ld()};
+  q.m = rows, q.n = channels, q.depth = pairs;
+  auto launch = [&](auto t) {
+    using T = decltype(t);
+    ScaledEpilogue<T> e;
+    e.out = Out16(out, out_row_stride, channels);
+    e.row_scale = input_scale, e.channel_scale = weight_scale, e.bias = static_cast<const uint16_t*>(bias);
+    return product.template launch<int8_t>(q, e, cs, flags, what);
+  };
+  return dtype == HPRN_DTYPE_BF16 ? launch(__nv_bfloat16{}) : launch(__half{});
+}
+
+}  // extern "C"

@@ -1,0 +1,608 @@
+// Log probabilities under the softmax of a linear layer over a vocabulary,
+// without keeping the logits: with L = X W^T / T (T the temperature),
+//   lse_i = log sum_j exp(L_ij),  log_prob_i = L_{i, t_i} - lse_i,
+//   entropy_i = -sum_j p_ij log p_ij,  p_ij = exp(L_ij - lse_i),
+// both 0 where the target t_i is `ignore_index`, and the `top` largest log
+// probabilities of a row with their indices.
+//
+// Forward: each tile of X W^T leaves, per row, its largest value m, and relative
+// to it s = sum_j e_j and a = sum_j e_j x_j, e_j = 2^x_j, x_j = (l_j - m) log2(e) / T.
+// Joined over the tiles (s, a and m the row's), lse = m / T + log s and
+// entropy = log s - ln(2) a / s.
+//
+// The largest ones are found in two steps.  Where they are asked for, the tiles
+// also leave the logits of a block of rows and the largest of every 32
+// neighbouring ones (LogProbEpilogue<true>); the `top` largest logits lie among the `top`
+// groups of 32 with the largest maxima, so that a row's search reads a 32nd of
+// its logits' number and a few groups.  A few more than `top` are taken, their
+// logits summed again in 64 bits, and ordered by those; equal ones go to the
+// lowest index.  So the order does not hang on how the tensor cores' sums fall
+// out in their last bits.
+//
+// Backward, g_i and h_i the gradients of log_prob_i and entropy_i:
+//   S_ij = (g_i ([j == t_i] - p_ij) - h_i p_ij (log p_ij + entropy_i)) / T
+//   dX = S W,  dW = S^T X
+// in pieces of the vocabulary as in linear_cross_entropy.cu, S held relative to
+// the largest finite |g_i| or |h_i| and, in fp16, times 2^14 without and 2^13
+// with an entropy gradient: |p (log p + entropy)| is at most 0.7 + ln(vocab) / 4,
+// 5.9 for the largest vocabulary, which with 1 for the other term and 2^13 stays
+// below 65504.
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "matmul.cuh"
+#include "runtime.cuh"
+#include "vocabulary.cuh"
+
+namespace hprn {
+
+// max(a, b), NaN where one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Exponents below this have powers of 0; -inf itself would make 0 * -inf of them.
+constexpr float kLeastExponent = -200.f;
+
+template <bool kTop>
+struct LogProbEpilogue {
+  static constexpr bool kPaired = false;
+  static constexpr int kSegment = kLogitSegment;
+  static constexpr bool kUnrolled = true;
+  float4* partial = nullptr;  // [rows, parts]: {m, s, a, 0}
+  float* target_logit = nullptr;
+  const int64_t* target = nullptr;
+  int64_t ignore = 0;
+  int64_t parts = 0;
+  int64_t vocab = 0;
+  float to_log2 = kLog2e;  // log2(e) / T
+  float* logits = nullptr;     // [rows, 32 groups]
+  float* group_max = nullptr;  // [rows, groups]
+  int64_t groups = 0;
+
+  struct Row {
+    float m, s, a;
+    int64_t t;
+  };
+  __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const {
+    return Row{-INFINITY, 0.f, 0.f, l.inside ? target_of(target, i, ignore, vocab) : kIgnored};
+  }
+  __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
+    if (j + kChunk > vocab) {
+      const int left = static_cast<int>(vocab - j);
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+        if (k >= left) v[k] = -INFINITY;
+    }
+    const int64_t at = r.t - j;
+    if (at >= 0 && at < kChunk) {
+      float x = 0.f;
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) x = at == k ? v[k] : x;
+      target_logit[i] = x;
+    }
+    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int k = 4; k < kChunk; ++k) top[k % 4] = fmaxf(top[k % 4], v[k]);
+    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if constexpr (kTop) {
+      if (l.inside) {
+        float* q = logits + i * (groups * kChunk) + j;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          Vec<32> o;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o.w[k] = __float_as_uint(v[8 * h + k]);
+          st_global<32>(q + 8 * h, o);
+        }
+        group_max[i * groups + j / kChunk] = most;
+      }
+    }
+    const float m = fmaxf(r.m, most);
+    // All so far -inf (or NaN, which fmaxf skips and the sums keep): 2^(-inf) = 0.
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float x0 = max_nan((r.m - ref) * to_log2, kLeastExponent), f = exp2_fast(x0);
+    const float2 minus = make_float2(-ref, -ref), c = make_float2(to_log2, to_log2);
+    float2 s[2] = {make_float2(r.s * f, 0.f), make_float2(0.f, 0.f)};
+    float2 a[2] = {make_float2(f * fmaf(r.s, x0, r.a), 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int k = 0; k < kChunk / 2; ++k) {
+      float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[2 * k], v[2 * k + 1]), minus), c);
+      x.x = max_nan(x.x, kLeastExponent), x.y = max_nan(x.y, kLeastExponent);
+      const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+      s[k % 2] = __fadd2_rn(s[k % 2], e);
+      a[k % 2] = __ffma2_rn(e, x, a[k % 2]);
+    }
+    r.m = m, r.s = (s[0].x + s[0].y) + (s[1].x + s[1].y), r.a = (a[0].x + a[0].y) + (a[1].x + a[1].y);
+  }
+  __device__ __forceinline__ void end(Row& r, const Lane& l, int64_t i, int64_t part) const {
+    if (l.inside) partial[i * parts + part] = make_float4(r.m, r.s, r.a, 0.f);
+  }
+};
+
+struct LogProbJoin {
+  const float4* partial;
+  const float* target_logit;
+  const int64_t* target;
+  int64_t ignore, rows, vocab, parts;  // parts 0: logits that are sums of no terms
+  float inv_t, to_log2;
+  float *log_prob, *entropy, *lse;
+};
+
+// Joins a row's parts, one warp a row.
+__global__ void __launch_bounds__(256) log_prob_join(LogProbJoin q) {
+  pdl_wait();
+  const int lane = threadIdx.x % 32;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  if (i >= q.rows) return;
+  float m = -INFINITY, s = 0.f, a = 0.f;
+  auto join = [&](float pm, float ps, float pa) {
+    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
+    const float x0 = max_nan((m - ref) * q.to_log2, kLeastExponent), f0 = exp2_fast(x0);
+    const float x1 = max_nan((pm - ref) * q.to_log2, kLeastExponent), f1 = exp2_fast(x1);
+    a = f0 * fmaf(s, x0, a) + f1 * fmaf(ps, x1, pa);
+    s = s * f0 + ps * f1;
+    m = top;
+  };
+  for (int64_t k = lane; k < q.parts; k += 32) {
+    const float4 p = q.partial[i * q.parts + k];
+    join(p.x, p.y, p.z);
+  }
+  for (int o = 16; o > 0; o >>= 1)
+    join(__shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), __shfl_xor_sync(~0u, a, o));
+  if (lane != 0) return;
+  if (q.parts == 0 && q.vocab > 0) m = 0.f, s = static_cast<float>(q.vocab), a = 0.f;
+  const float top = m == -INFINITY ? 0.f : m, log_s = logf(s);
+  q.lse[i] = fmaf(top, q.inv_t, log_s);
+  const int64_t t = target_of(q.target, i, q.ignore, q.vocab);
+  // The two logits first: where the target is the largest one the log probability
+  // is -log s, which a sum with a logit of 30 would round to multiples of 2^-19.
+  q.log_prob[i] = t == kIgnored   ? 0.f
+                  : t == kInvalid ? __int_as_float(0x7fc00000)
+                                  : ((q.parts > 0 ? q.target_logit[i] : 0.f) - top) * q.inv_t - log_s;
+  q.entropy[i] = t == kIgnored ? 0.f : log_s - 0.693147180559945f * (a / s);
+}
+
+// ---------------------------------------------------------------------------
+// The largest logits of a row.
+
+constexpr int kMostTop = 64;
+// Candidates past the ones asked for: so many logits may differ from the last
+// one's by no more than the rounding of an fp32 sum before one is missed.
+constexpr int kSpareTop = 4;
+constexpr int kMostCandidates = kMostTop + kSpareTop;
+constexpr int kTopThreads = 256;
+constexpr int kHeld = (kMostCandidates * kChunk + kTopThreads - 1) / kTopThreads;
+
+struct TopArgs {
+  const float* logits;
+  const float* group_max;
+  int64_t groups, vocab, hidden;
+  const uint16_t* x;
+  const uint16_t* w;
+  int64_t x_ld, w_ld;
+  const float* lse;
+  double inv_t;
+  int32_t top, candidates;
+  float* values;
+  int64_t* indices;
+};
+
+// Numbers in the order of floats (NaN above all, -0 beside 0), the lower index
+// above the higher among equals.  Never 0.
+__device__ __forceinline__ uint64_t order_key(float v, uint32_t index) {
+  uint32_t u = __float_as_uint(v + 0.f);
+  u = v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  return static_cast<uint64_t>(u) << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - static_cast<uint32_t>(key); }
+__device__ __forceinline__ uint64_t order_bits(double v) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return v != v ? ~uint64_t{0} : (u >> 63) ? ~u : u | uint64_t{1} << 63;
+}
+
+// The largest key of the CTA, in every thread.  `part`: one of two buffers that
+// calls alternate between.
+__device__ __forceinline__ uint64_t block_most(uint64_t key, uint64_t* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t other = __shfl_xor_sync(~0u, key, o);
+    key = other > key ? other : key;
+  }
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = key;
+  __syncthreads();
+  key = part[0];
+#pragma unroll
+  for (int k = 1; k < kTopThreads / 32; ++k) key = part[k] > key ? part[k] : key;
+  return key;
+}
+
+// sum_k x_k w_k in 64 bits, by a warp: the product of two 16-bit numbers is exact
+// in 32.  Both rows start on 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ double exact_dot(const uint16_t* x, const uint16_t* w, int64_t n) {
+  const int lane = threadIdx.x % 32;
+  double s = 0.0;
+  for (int64_t k = lane * 8; k < n; k += 256) {
+    if (k + 8 <= n) {
+      const uint4 a = *reinterpret_cast<const uint4*>(x + k), b = *reinterpret_cast<const uint4*>(w + k);
+      const float2 p[4] = {mul_pair<T>(a.x, b.x), mul_pair<T>(a.y, b.y), mul_pair<T>(a.z, b.z), mul_pair<T>(a.w, b.w)};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += static_cast<double>(p[e].x), s += static_cast<double>(p[e].y);
+    } else {
+      for (int64_t e = k; e < n; ++e) s += static_cast<double>(unpack1<T>(x[e]) * unpack1<T>(w[e]));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return s;
+}
+
+// One CTA per row.
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
+  __shared__ uint64_t part[2][kTopThreads / 32];
+  __shared__ uint32_t group_at[kMostCandidates], column[kMostCandidates];
+  __shared__ double exact[kMostCandidates];
+  pdl_wait();
+  const int64_t i = blockIdx.x;
+  const int tid = threadIdx.x;
+  float* values = a.values + i * a.top;
+  int64_t* indices = a.indices + i * a.top;
+  if (a.hidden == 0) {  // logits that are sums of no terms
+    if (tid < a.top) values[tid] = -a.lse[i], indices[tid] = tid;
+    return;
+  }
+  const int groups = static_cast<int>(a.groups);
+  const float* maxima = a.group_max + i * a.groups;
+  int turn = 0;
+  // The groups with the largest maxima.
+  auto best_below = [&](uint64_t limit) {
+    uint64_t best = 0;
+    for (int k = tid; k < groups; k += kTopThreads) {
+      const uint64_t key = order_key(maxima[k], static_cast<uint32_t>(k));
+      if (key < limit && key > best) best = key;
+    }
+    return best;
+  };
+  const int wanted = min(a.candidates, groups);
+  uint64_t mine = best_below(~uint64_t{0});
+  for (int c = 0; c < wanted; ++c) {
+    const uint64_t best = block_most(mine, part[turn]);
+    turn ^= 1;
+    if (mine == best) group_at[c] = key_index(best), mine = best_below(best);
+  }
+  __syncthreads();
+  // The largest of their logits.
+  const float* row = a.logits + i * a.groups * kChunk;
+  uint64_t keys[kHeld];
+  mine = 0;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int slot = tid + k * kTopThreads;
+    keys[k] = 0;
+    if (slot < wanted * kChunk) {
+      const uint32_t j = group_at[slot / kChunk] * kChunk + slot % kChunk;
+      if (j < a.vocab) keys[k] = order_key(row[j], j);
+    }
+    mine = keys[k] > mine ? keys[k] : mine;
+  }
+  for (int c = 0; c < a.candidates; ++c) {
+    const uint64_t best = block_most(mine, part[turn]);
+    turn ^= 1;
+    if (mine == best) {
+      column[c] = key_index(best);
+      mine = 0;
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        if (keys[k] < best) mine = keys[k] > mine ? keys[k] : mine;
+      }
+    }
+  }
+  __syncthreads();
+  for (int c = tid / 32; c < a.candidates; c += kTopThreads / 32) {
+    const double s = exact_dot<T>(a.x + i * a.x_ld, a.w + static_cast<int64_t>(column[c]) * a.w_ld, a.hidden);
+    if (tid % 32 == 0) exact[c] = s;
+  }
+  __syncthreads();
+  if (tid >= a.candidates) return;
+  const uint64_t bits = order_bits(exact[tid]);
+  int rank = 0;
+  for (int c = 0; c < a.candidates; ++c) {
+    const uint64_t other = order_bits(exact[c]);
+    rank += other > bits || (other == bits && column[c] < column[tid]);
+  }
+  if (rank >= a.top) return;
+  values[rank] = static_cast<float>(exact[tid] * a.inv_t - static_cast<double>(a.lse[i]));
+  indices[rank] = column[tid];
+}
+
+// ---------------------------------------------------------------------------
+
+template <typename T, bool kEntropy>
+struct LogProbGradEpilogue {
+  static constexpr bool kPaired = false;
+  static constexpr int kSegment = kLogitSegment;
+  static constexpr bool kUnrolled = false;
+  Out16 s;  // the piece's columns
+  const float* lse = nullptr;
+  const float* entropy = nullptr;
+  const float* grad_log_prob = nullptr;
+  const float* grad_entropy = nullptr;
+  const float* most = nullptr;  // the largest gradient
+  float held = 1.f;             // what S is held times
+  float inv_t = 1.f;
+  const int64_t* target = nullptr;
+  int64_t ignore = 0;
+  int64_t vocab = 0;
+  int64_t first = 0;  // the piece's first column
+
+  // S_ij = p (c + d (log p + entropy)) - c [j == t], c = -g and d = -h.
+  struct Row {
+    float c, lse, d, entropy;
+    int64_t t;  // within the piece (or outside it)
+  };
+  __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const {
+    const int64_t t = l.inside ? target_of(target, i, ignore, vocab) : kIgnored;
+    if (t == kIgnored) return Row{0.f, INFINITY, 0.f, 0.f, kIgnored};
+    // A target outside the vocabulary has no log probability: NaN, like itself.
+    const float c = t == kInvalid ? __int_as_float(0x7fc00000) : -grad_log_prob[i] / *most * held;
+    float d = 0.f, e = 0.f;
+    if constexpr (kEntropy) d = -grad_entropy[i] / *most * held, e = entropy[i];
+    return Row{c, lse[i], d, e, t >= first ? t - first : kInvalid};
+  }
+  __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
+    const int64_t at = r.t - j;
+    const bool here = at >= 0 && at < kChunk;
+    if (r.t == kIgnored) {
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) v[k] = 0.f;
+    } else {
+      const float2 c = make_float2(r.c, r.c), d = make_float2(r.d, r.d), scale = make_float2(inv_t, inv_t);
+      const float2 minus = make_float2(-r.lse, -r.lse), base = make_float2(r.entropy, r.entropy);
+#pragma unroll
+      for (int k = 0; k < kChunk / 2; ++k) {
+        const float2 log_p = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), scale, minus);
+        float2 by = c;
+        if constexpr (kEntropy) by = __ffma2_rn(__fadd2_rn(log_p, base), d, c);
+        const float2 p = __fmul2_rn(exp_fast2(log_p), by);
+        v[2 * k] = p.x, v[2 * k + 1] = p.y;
+      }
+      if (here) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k)
+          if (at == k) v[k] -= r.c;
+      }
+    }
+    s.template store<T>(l, i, j, v);
+  }
+  __device__ __forceinline__ void end(Row&, const Lane&, int64_t, int64_t) const {}
+};
+
+namespace {
+
+// What a block of rows may take for its logits.
+constexpr int64_t kLogitBytes = int64_t{1} << 30;
+
+int64_t rows_of_block(int64_t rows, int64_t groups) {
+  int64_t most = kLogitBytes / (groups > 0 ? groups * kChunk * 4 : 1) / 256 * 256;
+  if (most < 256) most = 256;
+  return rows < most ? rows : most;
+}
+
+}  // namespace
+}  // namespace hprn
+
+extern "C" {
+
+int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* top_log_probs, int64_t* top_indices,
+                          const void* input, const void* weight, const int64_t* target, int64_t ignore_index,
+                          double temperature, int64_t top, int64_t rows, int64_t hidden, int64_t vocab,
+                          int64_t input_row_stride, int64_t weight_row_stride, int dtype, void* workspace,
+                          int64_t* workspace_bytes, void* stream, unsigned flags) {
+  using namespace hprn;
+  int st = check_vocabulary(rows, hidden, vocab, dtype, flags, workspace_bytes);
+  if (st != HPRN_OK) return st;
+  if ((rows > 1 && input_row_stride < hidden) || (vocab > 1 && weight_row_stride < hidden))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  if (!(temperature > 0.0) || !(temperature < INFINITY))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (top < 0 || top > kMostTop || top > vocab)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "top must be between 0 and 64 and at most vocab");
+  Workspace ws(workspace, *workspace_bytes);
+  const AlignedRows x(ws, input, rows, hidden, input_row_stride, vocab);
+  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride, rows);
+  const int64_t groups = top > 0 ? (vocab + kChunk - 1) / kChunk : 0;
+  const int64_t block = top > 0 ? rows_of_block(rows, groups) : rows;
+  const PlannedProduct<false, true, true> product(ws, block, vocab, hidden, false);
+  const int64_t parts = product.parts(vocab);
+  float4* partial = ws.take<float4>(parts * block);
+  float* target_logit = ws.take<float>(block);
+  float* group_max = ws.take<float>(groups * block);
+  float* logits = ws.take<float>(groups * kChunk * block);
+  if (flags & HPRN_WORKSPACE_QUERY) {
+    *workspace_bytes = ws.needed();
+    return ok();
+  }
+  if (rows == 0) return ok();
+  if (!log_prob || !entropy || !lse || !target || (hidden > 0 && (!input || (vocab > 0 && !weight))) ||
+      (top > 0 && (!top_log_probs || !top_indices)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(log_prob, 4) || !aligned(entropy, 4) || !aligned(lse, 4) || !aligned(top_log_probs, 4) ||
+      !aligned(top_indices, 8) || !aligned(target, 8) || !aligned(input, 2) || !aligned(weight, 2))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  const Extent outs[] = {extent32(log_prob, 1, rows, rows), extent32(entropy, 1, rows, rows),
+                         extent32(lse, 1, rows, rows),
+                         extent32(top > 0 ? top_log_probs : nullptr, 1, rows * top, rows * top),
+                         extent_of(top > 0 ? top_indices : nullptr, 1, rows * top, rows * top, 8)};
+  const Extent ins[] = {extent16(input, rows, hidden, input_row_stride),
+                        extent16(weight, vocab, hidden, weight_row_stride), extent_of(target, 1, rows, rows, 8)};
+  if (!disjoint(outs, ins)) return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors");
+  if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
+  const DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const char* what = "linear_log_probs";
+  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
+  auto all = [&](auto t) {
+    using T = decltype(t);
+    auto launch = [&](auto epilogue, int64_t first, int64_t count) {
+      Product q;
+      q.a = {x.data() + first * x.ld(), x.ld()};
+      q.b = {w.data(), w.ld()};
+      q.m = count, q.n = vocab, q.depth = hidden;
+      epilogue.partial = partial, epilogue.target_logit = target_logit, epilogue.target = target + first;
+      epilogue.ignore = ignore_index, epilogue.parts = parts, epilogue.vocab = vocab;
+      epilogue.to_log2 = static_cast<float>(1.4426950408889634 / temperature);
+      epilogue.logits = logits, epilogue.group_max = group_max, epilogue.groups = groups;
+      return product.launch_whole<T>(q, epilogue, cs, flags, what);
+    };
+    int r = HPRN_OK;
+    for (int64_t first = 0; first < rows; first += block) {
+      const int64_t count = rows - first < block ? rows - first : block;
+      if (hidden > 0) {
+        r = top > 0 ? launch(LogProbEpilogue<true>{}, first, count) : launch(LogProbEpilogue<false>{}, first, count);
+        if (r != HPRN_OK) return r;
+      }
+      LogProbJoin q{};
+      q.partial = partial, q.target_logit = target_logit, q.target = target + first, q.ignore = ignore_index;
+      q.rows = count, q.vocab = vocab, q.parts = hidden > 0 ? parts : 0;
+      q.inv_t = static_cast<float>(1.0 / temperature);
+      q.to_log2 = static_cast<float>(1.4426950408889634 / temperature);
+      q.log_prob = log_prob + first, q.entropy = entropy + first, q.lse = lse + first;
+      r = launch_rows(log_prob_join, dim3(static_cast<unsigned>((count + 7) / 8)), dim3(256), cs, flags, what, q);
+      if (r != HPRN_OK) return r;
+      if (top == 0) continue;
+      TopArgs a{};
+      a.logits = logits, a.group_max = group_max, a.groups = groups, a.vocab = vocab, a.hidden = hidden;
+      a.x = x.data() + first * x.ld(), a.x_ld = x.ld(), a.w = w.data(), a.w_ld = w.ld();
+      a.lse = lse + first, a.inv_t = 1.0 / temperature;
+      a.top = static_cast<int32_t>(top);
+      a.candidates = static_cast<int32_t>(top + kSpareTop < vocab ? top + kSpareTop : vocab);
+      a.values = top_log_probs + first * top, a.indices = top_indices + first * top;
+      r = launch_rows(log_prob_top<T>, dim3(static_cast<unsigned>(count)), dim3(kTopThreads), cs, flags, what, a);
+      if (r != HPRN_OK) return r;
+    }
+    return r;
+  };
+  return dtype == HPRN_DTYPE_BF16 ? all(__nv_bfloat16{}) : all(__half{});
+}
+
+int hprn_linear_log_probs_backward(void* grad_input, void* grad_weight, const float* grad_log_prob,
+                                   const float* grad_entropy, const void* input, const void* weight,
+                                   const int64_t* target, const float* lse, const float* entropy,
+                                   int64_t ignore_index, double temperature, int64_t rows, int64_t hidden,
+                                   int64_t vocab, int64_t grad_input_row_stride, int64_t grad_weight_row_stride,
+                                   int64_t input_row_stride, int64_t weight_row_stride, int dtype, void* workspace,
+                                   int64_t* workspace_bytes, void* stream, unsigned flags) {
+  using namespace hprn;
+  int st = check_vocabulary(rows, hidden, vocab, dtype, flags, workspace_bytes);
+  if (st != HPRN_OK) return st;
+  if ((rows > 1 && (input_row_stride < hidden || grad_input_row_stride < hidden)) ||
+      (vocab > 1 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  if (!(temperature > 0.0) || !(temperature < INFINITY))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  Workspace ws(workspace, *workspace_bytes);
+  const int64_t x_ld = round_up(hidden, 16);
+  uint16_t* x = ws.take<uint16_t>(rows * x_ld);  // X without the ignored rows
+  const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride, rows);
+  const Pieces pieces = pieces_of(rows, vocab);
+  uint16_t* s = ws.take<uint16_t>(rows * pieces.cols);
+  const int64_t sum_ld = round_up(hidden, kChunk);
+  float* sum = pieces.count > 1 ? ws.take<float>(rows * sum_ld) : nullptr;
+  float* scale = ws.take<float>(2);
+  const float held = dtype != HPRN_DTYPE_FP16 ? 1.f : grad_entropy ? 8192.f : 16384.f;
+  const PlannedProduct<false, true, true> logits(ws, rows, pieces.cols, hidden, false);
+  const PlannedProduct<false, true, false> to_input(ws, rows, hidden, pieces.cols);
+  const PlannedProduct<false, false, false> to_weight(ws, pieces.cols, hidden, rows);
+  if (flags & HPRN_WORKSPACE_QUERY) {
+    *workspace_bytes = ws.needed();
+    return ok();
+  }
+  if (hidden == 0) return ok();
+  if ((rows > 0 && (!grad_input || !grad_log_prob || !input || !target || !lse || (grad_entropy && !entropy))) ||
+      (vocab > 0 && (!grad_weight || !weight)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned(grad_input, 2) || !aligned(grad_weight, 2) || !aligned(grad_log_prob, 4) ||
+      !aligned(grad_entropy, 4) || !aligned(input, 2) || !aligned(weight, 2) || !aligned(target, 8) ||
+      !aligned(lse, 4) || !aligned(entropy, 4))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  const Extent outs[] = {extent16(grad_input, rows, hidden, grad_input_row_stride),
+                         extent16(grad_weight, vocab, hidden, grad_weight_row_stride)};
+  const Extent ins[] = {extent32(grad_log_prob, 1, rows, rows), extent32(grad_entropy, 1, rows, rows),
+                        extent16(input, rows, hidden, input_row_stride),
+                        extent16(weight, vocab, hidden, weight_row_stride), extent_of(target, 1, rows, rows, 8),
+                        extent32(lse, 1, rows, rows), extent32(entropy, 1, rows, rows)};
+  if (!disjoint(outs, ins)) return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors");
+  if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
+  const DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const char* what = "linear_log_probs_backward";
+  if ((st = w.prepare(cs, flags)) != HPRN_OK) return st;
+  if (rows > 0) {
+    LossPrepareArgs a{};
+    a.x = static_cast<const uint16_t*>(input), a.x_ld = input_row_stride;
+    a.out = x, a.out_ld = x_ld, a.rows = rows, a.hidden = hidden;
+    a.spans = (x_ld + kPrepareSpan - 1) / kPrepareSpan;
+    a.vectors = tma_rows(input, rows, input_row_stride);
+    a.grad_loss = grad_log_prob, a.grad_entropy = grad_entropy, a.target = target, a.ignore = ignore_index;
+    // S is held without the 1 / T of its logits; the sums are multiplied by it.
+    a.held = static_cast<float>(held * temperature), a.scale = scale;
+    const int64_t ctas = (rows * a.spans + 7) / 8, most = 16 * dev->sm_count;
+    st = launch_rows(grad_entropy ? loss_grad_prepare<true> : loss_grad_prepare<false>,
+                     dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), cs, flags, what, a);
+    if (st != HPRN_OK) return st;
+  }
+  auto all = [&](auto t, auto entropy_too) {
+    using T = decltype(t);
+    int r = HPRN_OK;
+    // Without a vocabulary the input's gradient is an empty sum: zero.
+    const int64_t count = pieces.count > 0 ? pieces.count : 1;
+    for (int64_t p = 0; p < count && r == HPRN_OK; ++p) {
+      const int64_t first = p * pieces.cols;
+      const int64_t cols = vocab - first < pieces.cols ? vocab - first : pieces.cols;
+      const uint16_t* wp = w.data() + first * w.ld();
+      Product q;
+      q.a = {x, x_ld};
+      q.b = {wp, w.ld()};
+      q.m = rows, q.n = cols, q.depth = hidden;
+      LogProbGradEpilogue<T, decltype(entropy_too)::value> g;
+      g.s = Out16(s, pieces.cols, cols), g.lse = lse, g.entropy = entropy, g.grad_log_prob = grad_log_prob;
+      g.grad_entropy = grad_entropy, g.most = scale, g.held = held;
+      g.inv_t = static_cast<float>(1.0 / temperature);
+      g.target = target, g.ignore = ignore_index, g.vocab = vocab, g.first = first;
+      if ((r = logits.launch_whole<T>(q, g, cs, flags, what)) != HPRN_OK) break;
+
+      q.a = {s, pieces.cols};
+      q.n = hidden, q.depth = cols;
+      StoreEpilogue<T> e;
+      e.out = Out16(grad_input, grad_input_row_stride, hidden);
+      e.sum = sum, e.sum_ld = sum_ld, e.first = p == 0, e.last = p == count - 1;
+      e.scale = rows > 0 ? scale + 1 : nullptr;
+      if ((r = to_input.launch<T>(q, e, cs, flags, what)) != HPRN_OK) break;
+
+      q.b = {x, x_ld};
+      q.m = cols, q.depth = rows;
+      e.out = Out16(static_cast<uint16_t*>(grad_weight) + first * grad_weight_row_stride,
+                    grad_weight_row_stride, hidden);
+      e.sum = nullptr, e.first = e.last = true;
+      r = to_weight.launch<T>(q, e, cs, flags, what);
+    }
+    return r;
+  };
+  auto typed = [&](auto t) { return grad_entropy ? all(t, std::true_type{}) : all(t, std::false_type{}); };
+  return dtype == HPRN_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
+}
+
+}  // extern "C"

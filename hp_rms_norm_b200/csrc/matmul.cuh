@@ -8,6 +8,11 @@
 // linear layer (forward, gradient of the input, gradient of the weight) read
 // the tensors as they are.
 //
+// With T = int8_t both operands are signed 8-bit and k-major; what is said of
+// 16-bit elements then goes for pairs of terms (depths, strides and boxes count
+// pairs), and the accumulators are exact 32-bit integers, handed to the epilogue
+// as their bits in floats.  Such an epilogue has `kInteger`.
+//
 // What happens to the accumulators is an epilogue: a struct whose methods a
 // warp calls together, each lane for the row i it holds (`Lane::inside` where
 // i < m):
@@ -56,6 +61,11 @@ struct Product {
 constexpr int kChunk = 32;         // accumulators a thread hands to an epilogue at once
 constexpr int kColumnGroups = 2;   // lanes that share a tile's row
 constexpr int kScratchWords = 32 * 17;  // a warp's transposition buffer
+
+template <typename E, typename = void>
+struct IsInteger : std::false_type {};
+template <typename E>
+struct IsInteger<E, std::enable_if_t<E::kInteger>> : std::true_type {};
 
 struct Lane {
   uint32_t* scratch;  // kScratchWords words of the warp's own
@@ -523,10 +533,14 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
       }
     }
   } else if (warp == 1 && rank == 0) {
-    const uint32_t idesc = mma_descriptor(std::is_same<T, __nv_bfloat16>::value, !kAKMajor, !kBKMajor,
-                                          128 * kGroup, args.cols);
-    // 16 of the stage's 64 terms per MMA: 32 bytes along a k-major tile's
-    // rows, two atoms of a row-major tile.  In descriptors, 16 bytes a unit.
+    constexpr bool kInt8 = std::is_same<T, int8_t>::value;
+    static_assert(!kInt8 || (kAKMajor && kBKMajor), "8-bit operands are k-major");
+    const uint32_t idesc = kInt8 ? mma_descriptor_i8(128 * kGroup, args.cols)
+                                 : mma_descriptor(std::is_same<T, __nv_bfloat16>::value, !kAKMajor, !kBKMajor,
+                                                  128 * kGroup, args.cols);
+    // 16 of the stage's 64 terms (32 of 128 8-bit ones) per MMA: 32 bytes along a
+    // k-major tile's rows, two atoms of a row-major tile.  In descriptors, 16
+    // bytes a unit.
     constexpr uint32_t kAStep = (kAKMajor ? 32 : 2048) / 16, kBStep = (kBKMajor ? 32 : 2048) / 16;
     const uint64_t a_desc = smem_descriptor(ring, kAKMajor ? 16 : 8192);
     const uint64_t b_desc = smem_descriptor(ring + a_bytes, kBKMajor ? 16 : 8192);
@@ -554,8 +568,10 @@ __global__ void __launch_bounds__(kMatmulThreads, 1)
           if (elect_one()) {
             const uint64_t a = a_desc + s * (stage_bytes / 16), b = b_desc + s * (stage_bytes / 16);
 #pragma unroll
-            for (int j = 0; j < kDepthBlock / 16; ++j)
-              mma_f16<kGroup>(d, a + j * kAStep, b + j * kBStep, idesc, k > begin || j > 0);
+            for (int j = 0; j < kDepthBlock / 16; ++j) {
+              if constexpr (kInt8) mma_i8<kGroup>(d, a + j * kAStep, b + j * kBStep, idesc, k > begin || j > 0);
+              else mma_f16<kGroup>(d, a + j * kAStep, b + j * kBStep, idesc, k > begin || j > 0);
+            }
             mma_commit<kGroup>(empty(s));
             if (k + 1 == end) mma_commit<kGroup>(acc_full(buf));
           }
@@ -663,7 +679,11 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int h = 0; h < (E::kPaired ? 2 : 1); ++h) {
         const float4 q = *reinterpret_cast<const float4*>(p + h * shares.ld);
-        v[h][0] += q.x, v[h][1] += q.y, v[h][2] += q.z, v[h][3] += q.w;
+        auto add = [](float& sum, float share) {
+          if constexpr (IsInteger<E>::value) sum = __int_as_float(__float_as_int(sum) + __float_as_int(share));
+          else sum += share;
+        };
+        add(v[h][0], q.x), add(v[h][1], q.y), add(v[h][2], q.z), add(v[h][3], q.w);
       }
     }
 #pragma unroll

@@ -635,6 +635,265 @@ void clip_grad_norm(at::TensorList out, at::Tensor& norm, at::TensorList grads, 
   });
 }
 
+// A gate over `input`: rows of `width` (1 or hidden) values, each for the rows of
+// input that the gate's trailing dimensions of 1 span.
+struct Gate {
+  Rows rows;
+  int64_t width = 1, rows_per_gate = 1;
+};
+
+Gate gate_arg(const at::Tensor& gate, const char* name, const at::Tensor& input) {
+  TORCH_CHECK(gate.dim() >= 1 && gate.dim() <= input.dim(), name, " must have 1 to input.dim() dimensions");
+  Gate g;
+  g.width = gate.size(-1);
+  TORCH_CHECK(g.width == input.size(-1) || g.width == 1, name, ".size(-1) must be 1 or hidden_dim");
+  // From the last leading dimension outwards: dimensions of 1, then input's own.
+  bool own = false;
+  for (int64_t k = 2; k <= input.dim(); ++k) {
+    const int64_t n = k <= gate.dim() ? gate.size(-k) : 1, of = input.size(-k);
+    TORCH_CHECK(n == of || (n == 1 && !own), name,
+                " must broadcast over input's trailing leading dimensions only");
+    if (n != of) g.rows_per_gate *= of;
+    own = own || (n == of && n != 1);
+  }
+  g.rows = rows_arg(gate, name, g.width, input, input.scalar_type());
+  return g;
+}
+
+struct BlockNorm {
+  int dtype;
+  int64_t hidden, rows, rows_per_gate = 1, gate_width = 1;
+  Rows x, p, w, g;
+};
+
+BlockNorm check_block_norm(const at::Tensor& input, const c10::optional<at::Tensor>& post_weight,
+                           const at::Tensor& weight, const c10::optional<at::Tensor>& gate) {
+  BlockNorm c;
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(weight.dim() == 1, "weight.dim() == 1");
+  c.hidden = weight.size(0);
+  TORCH_CHECK(input.size(-1) == c.hidden, "input.size(-1) == hidden_dim");
+  c.dtype = dtype_code(input);
+  c.rows = leading(input);
+  c.x = rows_arg(input, "input", c.hidden, input, input.scalar_type());
+  c.w = rows_arg(weight, "weight", c.hidden, input, input.scalar_type());
+  if (post_weight.has_value()) {
+    TORCH_CHECK(post_weight->dim() == 1, "post_weight.dim() == 1");
+    c.p = rows_arg(*post_weight, "post_weight", c.hidden, input, input.scalar_type());
+  }
+  if (gate.has_value()) {
+    const Gate g = gate_arg(*gate, "gate", input);
+    c.g = g.rows, c.gate_width = g.width, c.rows_per_gate = g.rows_per_gate > 0 ? g.rows_per_gate : 1;
+  }
+  return c;
+}
+
+void gated_add_rms_norm(at::Tensor& out, at::Tensor& residual, c10::optional<at::Tensor> residual_out,
+                        const at::Tensor& input, c10::optional<at::Tensor> post_weight,
+                        const at::Tensor& weight, c10::optional<at::Tensor> gate,
+                        double residual_scale, double eps) {
+  const BlockNorm c = check_block_norm(input, post_weight, weight, gate);
+  const at::ScalarType type = input.scalar_type();
+  const at::Tensor& total = residual_out.has_value() ? *residual_out : residual;
+  TORCH_CHECK(out.sizes() == input.sizes(), "out must have the input's shape");
+  TORCH_CHECK(residual.sizes() == input.sizes(), "residual must have the input's shape");
+  TORCH_CHECK(total.sizes() == input.sizes(), "residual_out must have the input's shape");
+  const Rows o = rows_arg(out, "out", c.hidden, input, type);
+  const Rows r = rows_arg(residual, "residual", c.hidden, input, type);
+  const Rows t = rows_arg(total, "residual_out", c.hidden, input, type);
+  if (c.rows == 0 || c.hidden == 0) return;
+  const c10::cuda::CUDAGuard guard(input.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(input.device().index()).stream();
+  check_status(hprn_gated_add_rms_norm(o.p, t.p, c.x.p, r.p, c.p.p, c.w.p, c.g.p, c.rows, c.hidden,
+                                       c.rows_per_gate, c.gate_width, o.stride, t.stride, c.x.stride,
+                                       r.stride, c.g.stride, residual_scale, eps, c.dtype, stream,
+                                       HPRN_LAUNCH_DEFAULT));
+}
+
+void gated_add_rms_norm_backward(at::Tensor& grad_input, at::Tensor& grad_residual,
+                                 c10::optional<at::Tensor> grad_post_weight, at::Tensor& grad_weight,
+                                 c10::optional<at::Tensor> grad_gate, const at::Tensor& grad_out,
+                                 c10::optional<at::Tensor> grad_residual_out,
+                                 const at::Tensor& input, const at::Tensor& residual_out,
+                                 c10::optional<at::Tensor> post_weight, const at::Tensor& weight,
+                                 c10::optional<at::Tensor> gate, double residual_scale, double eps) {
+  const BlockNorm c = check_block_norm(input, post_weight, weight, gate);
+  const at::ScalarType type = input.scalar_type();
+  TORCH_CHECK(grad_out.sizes() == input.sizes(), "grad_out must have the input's shape");
+  TORCH_CHECK(residual_out.sizes() == input.sizes(), "residual must have the input's shape");
+  TORCH_CHECK(grad_input.sizes() == input.sizes(), "grad_input must have the input's shape");
+  TORCH_CHECK(grad_residual.sizes() == input.sizes(), "grad_residual must have the input's shape");
+  TORCH_CHECK(grad_weight.sizes() == weight.sizes(), "grad_weight must have the weight's shape");
+  TORCH_CHECK(grad_post_weight.has_value() == post_weight.has_value(),
+              "grad_post_weight and post_weight go together");
+  TORCH_CHECK(grad_gate.has_value() == gate.has_value(), "grad_gate and gate go together");
+  const Rows d = rows_arg(grad_out, "grad_out", c.hidden, input, type);
+  const Rows t = rows_arg(residual_out, "residual", c.hidden, input, type);
+  const Rows gi = rows_arg(grad_input, "grad_input", c.hidden, input, type);
+  const Rows gr = rows_arg(grad_residual, "grad_residual", c.hidden, input, type);
+  const Rows gw = rows_arg(grad_weight, "grad_weight", c.hidden, input, type);
+  Rows e, gp, gg;
+  if (grad_residual_out.has_value()) {
+    TORCH_CHECK(grad_residual_out->sizes() == input.sizes(), "grad_residual must have the input's shape");
+    e = rows_arg(*grad_residual_out, "grad_residual", c.hidden, input, type);
+  }
+  if (post_weight.has_value()) {
+    TORCH_CHECK(grad_post_weight->dim() == 1, "grad_post_weight.dim() == 1");
+    gp = rows_arg(*grad_post_weight, "grad_post_weight", c.hidden, input, type);
+  }
+  if (gate.has_value()) {
+    TORCH_CHECK(grad_gate->sizes() == gate->sizes(), "grad_gate must have the gate's shape");
+    gg = rows_arg(*grad_gate, "grad_gate", c.gate_width, input, type);
+  }
+  if (c.hidden == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_gated_add_rms_norm_backward(
+        gi.p, gr.p, gp.p, gw.p, gg.p, d.p, e.p, c.x.p, t.p, c.p.p, c.w.p, c.g.p, c.rows, c.hidden,
+        c.rows_per_gate, c.gate_width, gi.stride, gr.stride, gg.stride, d.stride, e.stride, c.x.stride,
+        t.stride, c.g.stride, residual_scale, eps, c.dtype, ws, bytes, s, flags);
+  });
+}
+
+float* float_out(const at::Tensor& t, const char* name, int64_t count, const at::Tensor& like) {
+  return const_cast<float*>(float_rows(t, name, count, like));
+}
+
+void linear_log_probs(at::Tensor& log_prob, at::Tensor& entropy, at::Tensor& lse,
+                      c10::optional<at::Tensor> top_log_probs, c10::optional<at::Tensor> top_indices,
+                      const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
+                      double temperature, int64_t ignore_index) {
+  const LossCall c = check_loss(input, weight, target);
+  float* lp = float_out(log_prob, "log_prob", c.rows, input);
+  float* hp = float_out(entropy, "entropy", c.rows, input);
+  float* ep = float_out(lse, "lse", c.rows, input);
+  TORCH_CHECK(top_log_probs.has_value() == top_indices.has_value(),
+              "top_log_probs and top_indices go together");
+  int64_t top = 0;
+  float* vp = nullptr;
+  int64_t* ip = nullptr;
+  if (top_log_probs.has_value()) {
+    TORCH_CHECK(top_log_probs->dim() >= 1 && top_indices->sizes() == top_log_probs->sizes(),
+                "top_log_probs and top_indices must have one shape");
+    top = top_log_probs->size(-1);
+    TORCH_CHECK(top >= 1 && top <= 64 && top <= c.vocab, "top must be between 0 and 64 and at most vocab");
+    TORCH_CHECK(top_indices->scalar_type() == at::kLong && top_indices->is_contiguous() &&
+                    top_indices->is_cuda() && top_indices->device() == input.device(),
+                "top_indices must be a contiguous int64 tensor");
+    vp = float_out(*top_log_probs, "top_log_probs", c.rows * top, input);
+    ip = top_indices->data_ptr<int64_t>();
+  }
+  if (c.rows == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_linear_log_probs(lp, hp, ep, vp, ip, c.x.p, c.w.p, c.target, ignore_index, temperature, top,
+                                 c.rows, c.hidden, c.vocab, c.x.stride, c.w.stride, c.dtype, ws, bytes, s,
+                                 flags);
+  });
+}
+
+void linear_log_probs_backward(at::Tensor& grad_input, at::Tensor& grad_weight,
+                               const at::Tensor& grad_log_prob, c10::optional<at::Tensor> grad_entropy,
+                               const at::Tensor& input, const at::Tensor& weight,
+                               const at::Tensor& target, const at::Tensor& lse,
+                               c10::optional<at::Tensor> entropy, double temperature,
+                               int64_t ignore_index) {
+  const LossCall c = check_loss(input, weight, target);
+  TORCH_CHECK(grad_input.sizes() == input.sizes(), "grad_input must have the input's shape");
+  TORCH_CHECK(grad_weight.sizes() == weight.sizes(), "grad_weight must have the weight's shape");
+  const Rows gi = rows_arg(grad_input, "grad_input", c.hidden, input, input.scalar_type());
+  const Rows gw = rows_arg(grad_weight, "grad_weight", c.hidden, input, input.scalar_type());
+  const float* gl = float_rows(grad_log_prob, "grad_log_prob", c.rows, input);
+  const float* ep = float_rows(lse, "lse", c.rows, input);
+  const float *ge = nullptr, *hp = nullptr;
+  if (grad_entropy.has_value()) {
+    TORCH_CHECK(entropy.has_value(), "grad_entropy needs the forward call's entropy");
+    ge = float_rows(*grad_entropy, "grad_entropy", c.rows, input);
+    hp = float_rows(*entropy, "entropy", c.rows, input);
+  }
+  if (c.hidden == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_linear_log_probs_backward(gi.p, gw.p, gl, ge, c.x.p, c.w.p, c.target, ep, hp, ignore_index,
+                                          temperature, c.rows, c.hidden, c.vocab, gi.stride, gw.stride,
+                                          c.x.stride, c.w.stride, c.dtype, ws, bytes, s, flags);
+  });
+}
+
+void rms_norm_int8(at::Tensor& out, at::Tensor& scales, const at::Tensor& input,
+                   c10::optional<at::Tensor> weight, c10::optional<at::Tensor> residual,
+                   c10::optional<at::Tensor> residual_out, double eps) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  const int dtype = dtype_code(input);
+  const int64_t hidden = input.size(-1), rows = leading(input);
+  const at::ScalarType type = input.scalar_type();
+  TORCH_CHECK(out.sizes() == input.sizes(), "out must have the input's shape");
+  TORCH_CHECK(residual.has_value() || !residual_out.has_value(), "residual_out needs a residual");
+  const Rows x = rows_arg(input, "input", hidden, input, type);
+  const Rows q = rows_arg(out, "out", hidden, input, at::kChar);
+  float* sp = float_out(scales, "scales", rows, input);
+  Rows w, r, t;
+  if (weight.has_value()) {
+    TORCH_CHECK(weight->dim() == 1, "weight.dim() == 1");
+    w = rows_arg(*weight, "weight", hidden, input, type);
+  }
+  if (residual.has_value()) {
+    const at::Tensor& total = residual_out.has_value() ? *residual_out : *residual;
+    TORCH_CHECK(residual->sizes() == input.sizes(), "residual must have the input's shape");
+    TORCH_CHECK(total.sizes() == input.sizes(), "residual_out must have the input's shape");
+    r = rows_arg(*residual, "residual", hidden, input, type);
+    t = rows_arg(total, "residual_out", hidden, input, type);
+  }
+  if (rows == 0 || hidden == 0) return;
+  const c10::cuda::CUDAGuard guard(input.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(input.device().index()).stream();
+  check_status(hprn_rms_norm_int8(static_cast<int8_t*>(q.p), sp, t.p, x.p, w.p, r.p, rows, hidden, q.stride,
+                                  t.stride, x.stride, r.stride, eps, dtype, stream, HPRN_LAUNCH_DEFAULT));
+}
+
+void linear_int8(at::Tensor& out, const at::Tensor& input, const at::Tensor& input_scale,
+                 const at::Tensor& weight, const at::Tensor& weight_scale, c10::optional<at::Tensor> bias) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(weight.dim() == 2, "weight must be [channels, hidden]");
+  const int dtype = dtype_code(out);
+  const int64_t hidden = input.size(-1), rows = leading(input), channels = weight.size(0);
+  check_leading(out, "out", input);
+  const Rows x = rows_arg(input, "input", hidden, input, at::kChar);
+  const Rows w = rows_arg(weight, "weight", hidden, input, at::kChar);
+  const Rows o = rows_arg(out, "out", channels, input, out.scalar_type());
+  const float* xs = float_rows(input_scale, "input_scale", rows, input);
+  const float* wsc = float_rows(weight_scale, "weight_scale", channels, input);
+  Rows b;
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->dim() == 1, "bias.dim() == 1");
+    b = rows_arg(*bias, "bias", channels, input, out.scalar_type());
+  }
+  if (rows == 0 || channels == 0) return;
+  with_workspace(input, [&](void* ws, int64_t* bytes, cudaStream_t s, unsigned flags) {
+    return hprn_linear_int8(o.p, static_cast<const int8_t*>(x.p), xs, static_cast<const int8_t*>(w.p), wsc, b.p,
+                            rows, hidden, channels, o.stride, x.stride, w.stride, dtype, ws, bytes, s, flags);
+  });
+}
+
+void gated_add_rms_norm_meta(at::Tensor&, at::Tensor&, c10::optional<at::Tensor>, const at::Tensor&,
+                             c10::optional<at::Tensor>, const at::Tensor&, c10::optional<at::Tensor>,
+                             double, double) {}
+void gated_add_rms_norm_backward_meta(at::Tensor&, at::Tensor&, c10::optional<at::Tensor>, at::Tensor&,
+                                      c10::optional<at::Tensor>, const at::Tensor&,
+                                      c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
+                                      c10::optional<at::Tensor>, const at::Tensor&,
+                                      c10::optional<at::Tensor>, double, double) {}
+void linear_log_probs_meta(at::Tensor&, at::Tensor&, at::Tensor&, c10::optional<at::Tensor>,
+                           c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
+                           const at::Tensor&, double, int64_t) {}
+void linear_log_probs_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&,
+                                    c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
+                                    const at::Tensor&, const at::Tensor&, c10::optional<at::Tensor>,
+                                    double, int64_t) {}
+void rms_norm_int8_meta(at::Tensor&, at::Tensor&, const at::Tensor&, c10::optional<at::Tensor>,
+                        c10::optional<at::Tensor>, c10::optional<at::Tensor>, double) {}
+void linear_int8_meta(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                      const at::Tensor&, c10::optional<at::Tensor>) {}
 void gated_linear_meta(at::Tensor&, c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
                        c10::string_view) {}
 void gated_linear_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
@@ -695,6 +954,23 @@ TORCH_LIBRARY(hp_rms_norm, m) {
         "int ignore_index) -> ()");
   m.def("rms_norm_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, Tensor grad_out, "
         "Tensor input, Tensor weight, Tensor? grad_residual, float eps) -> ()");
+  m.def("gated_add_rms_norm(Tensor(a!) out, Tensor(b!) residual, Tensor(c!)? residual_out, Tensor input, "
+        "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
+  m.def("gated_add_rms_norm_backward(Tensor(a!) grad_input, Tensor(b!) grad_residual, "
+        "Tensor(c!)? grad_post_weight, Tensor(d!) grad_weight, Tensor(e!)? grad_gate, Tensor grad_out, "
+        "Tensor? grad_residual_out, Tensor input, Tensor residual_out, Tensor? post_weight, "
+        "Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
+  m.def("linear_log_probs(Tensor(a!) log_prob, Tensor(b!) entropy, Tensor(c!) lse, "
+        "Tensor(d!)? top_log_probs, Tensor(e!)? top_indices, Tensor input, Tensor weight, Tensor target, "
+        "float temperature, int ignore_index) -> ()");
+  m.def("linear_log_probs_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, Tensor grad_log_prob, "
+        "Tensor? grad_entropy, Tensor input, Tensor weight, Tensor target, Tensor lse, Tensor? entropy, "
+        "float temperature, int ignore_index) -> ()");
+  // Extensions: 8-bit integers.
+  m.def("rms_norm_int8(Tensor(a!) out, Tensor(b!) scales, Tensor input, Tensor? weight, "
+        "Tensor(c!)? residual, Tensor(d!)? residual_out, float eps) -> ()");
+  m.def("linear_int8(Tensor(a!) out, Tensor input, Tensor input_scale, Tensor weight, "
+        "Tensor weight_scale, Tensor? bias) -> ()");
   m.def("grad_norm(Tensor(a!) norm, Tensor[] grads) -> ()");
   m.def("clip_grad_norm(Tensor(a!)[] out, Tensor(b!) norm, Tensor[] grads, float max_norm) -> ()");
 }
@@ -716,6 +992,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("rms_norm_backward", &rms_norm_backward);
   m.impl("grad_norm", &grad_norm);
   m.impl("clip_grad_norm", &clip_grad_norm);
+  m.impl("gated_add_rms_norm", &gated_add_rms_norm);
+  m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward);
+  m.impl("linear_log_probs", &linear_log_probs);
+  m.impl("linear_log_probs_backward", &linear_log_probs_backward);
+  m.impl("rms_norm_int8", &rms_norm_int8);
+  m.impl("linear_int8", &linear_int8);
 }
 
 TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
@@ -735,4 +1017,10 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("rms_norm_backward", &rms_norm_backward_meta);
   m.impl("grad_norm", &grad_norm_meta);
   m.impl("clip_grad_norm", &clip_grad_norm_meta);
+  m.impl("gated_add_rms_norm", &gated_add_rms_norm_meta);
+  m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_meta);
+  m.impl("linear_log_probs", &linear_log_probs_meta);
+  m.impl("linear_log_probs_backward", &linear_log_probs_backward_meta);
+  m.impl("rms_norm_int8", &rms_norm_int8_meta);
+  m.impl("linear_int8", &linear_int8_meta);
 }

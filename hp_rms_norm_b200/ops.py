@@ -10,12 +10,17 @@ Extensions (not in the reference): ``rms_norm`` (plain RMSNorm),
 ``fused_add_rms_norm`` (the fused op into a separate output) and
 ``rms_norm_fp8`` (either form with an fp8 e4m3 output, static or per-row
 scale), ``rms_norm_nvfp4`` (NVFP4 output), and the gated activations ``silu_and_mul``, ``gelu_and_mul`` and
-``gelu_tanh_and_mul``; and for training ``gated_linear`` (a feed-forward block's gate and up
+``gelu_tanh_and_mul``; ``gated_add_rms_norm`` (the norms on both sides of a gated block) and its
+backward pass; ``linear_log_probs`` (log probabilities of given tokens, entropy and best
+alternatives) and its backward pass; ``rms_norm_int8``, ``quantize_int8`` and ``linear_int8``
+(products of 8-bit integers and what feeds them); and for training ``gated_linear`` (a feed-forward block's gate and up
 products with the activation), ``linear_cross_entropy`` (the loss of a linear layer over a
 vocabulary, without its logits), their backward passes, ``rms_norm_backward``, and
 ``grad_norm`` / ``clip_grad_norm``.  Everything dispatches through ``torch.ops.hp_rms_norm``, registered
 by this package's compiled ``_C`` extension.
 """
+from typing import NamedTuple, Optional
+
 import torch
 
 _ops = torch.ops.hp_rms_norm
@@ -217,8 +222,121 @@ def clip_grad_norm(grads, max_norm, out=None):
     return norm
 
 
+def gated_add_rms_norm(input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0,
+                       out=None, residual_out=None):
+    """The end of one block and the norm before the next in one pass:
+
+        residual_out = residual_scale * residual + gate * (RMSNorm(input) * post_weight)
+        out = RMSNorm(residual_out) * weight
+
+    ``residual_out`` None updates ``residual`` in place.  ``post_weight`` None leaves the norm after
+    the block out.  ``gate`` None is 1; otherwise its shape is one that broadcasts over
+    ``input``'s trailing leading dimensions: [hidden] (a learned gate for each channel), [batch, 1,
+    hidden] (one for each sequence), input's own shape, or any of these with a last dimension
+    of 1.  The sums are fp32 and ``out`` comes from the unrounded new residual.  Returns ``out``."""
+    if out is None:
+        out = torch.empty_like(input)
+    _ops.gated_add_rms_norm.default(out, residual, residual_out, input, post_weight, weight, gate,
+                                    residual_scale, eps)
+    return out
+
+
+def gated_add_rms_norm_backward(grad_out, input, residual, post_weight, weight, eps, gate=None,
+                                residual_scale=1.0, grad_residual=None):
+    """Gradients (grad_input, grad_residual, grad_post_weight, grad_weight, grad_gate) of
+    ``gated_add_rms_norm`` for a gradient of ``out`` and, with ``grad_residual``, one that reaches
+    the new residual from its other uses.  ``residual`` is the new residual that the forward call
+    wrote.  grad_post_weight and grad_gate are None where their tensors are."""
+    grad_input = _new_like(input)
+    grad_old = _new_like(input)
+    grad_post = None if post_weight is None else _new_like(post_weight)
+    grad_weight = _new_like(weight)
+    grad_gate = None
+    if gate is not None:
+        grad_gate = _new_like(gate)
+        if input.numel() == 0:
+            grad_gate.zero_()
+    _ops.gated_add_rms_norm_backward.default(grad_input, grad_old, grad_post, grad_weight, grad_gate,
+                                             grad_out, grad_residual, input, residual, post_weight,
+                                             weight, gate, residual_scale, eps)
+    return grad_input, grad_old, grad_post, grad_weight, grad_gate
+
+
+class LogProbs(NamedTuple):
+    """What ``linear_log_probs`` returns; the last two are None without ``top``."""
+    log_prob: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_log_probs: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+def linear_log_probs(input, weight, target, top=0, temperature=1.0, ignore_index=-100):
+    """Log probabilities under softmax(input weight^T / temperature) without holding the logits:
+    ``input`` [..., hidden], ``weight`` [vocab, hidden], ``target`` int64 [...].  Returns a
+    ``LogProbs``: log_prob and entropy, float32 [...] (0 where the target is ``ignore_index``; the
+    log probability of any other target outside the vocabulary is NaN), lse, the log-sum-exp
+    that ``linear_log_probs_backward`` takes, and for ``top`` > 0 (at most 64) the largest log
+    probabilities of every row, float32 [..., top], with their int64 indices: the largest first,
+    equal ones by their indices."""
+    lead = input.shape[:-1]
+    log_prob = torch.empty(lead, dtype=torch.float32, device=input.device)
+    entropy = torch.empty_like(log_prob)
+    lse = torch.empty_like(log_prob)
+    values = indices = None
+    if top:
+        values = torch.empty(lead + (top,), dtype=torch.float32, device=input.device)
+        indices = torch.empty(lead + (top,), dtype=torch.int64, device=input.device)
+    _ops.linear_log_probs.default(log_prob, entropy, lse, values, indices, input, weight, target,
+                                  temperature, ignore_index)
+    return LogProbs(log_prob, entropy, lse, values, indices)
+
+
+def linear_log_probs_backward(grad_log_prob, input, weight, target, lse, entropy=None,
+                              grad_entropy=None, temperature=1.0, ignore_index=-100):
+    """Gradients (grad_input, grad_weight) of ``linear_log_probs`` for gradients of the rows' log
+    probabilities and, where ``grad_entropy`` is given (with the forward call's ``entropy``), of
+    their entropies, float32 [...]; the logits are computed again, one piece of the vocabulary at
+    a time."""
+    grad_input = _new_like(input)
+    grad_weight = _new_like(weight)
+    _ops.linear_log_probs_backward.default(grad_input, grad_weight, grad_log_prob, grad_entropy,
+                                           input, weight, target, lse, entropy, temperature,
+                                           ignore_index)
+    return grad_input, grad_weight
+
+
+def rms_norm_int8(input, weight, eps, residual=None, residual_out=None):
+    """RMSNorm (with a residual: of residual + input, which goes to ``residual_out``, or to
+    ``residual`` itself without one) with an int8 output and one scale a row: returns (codes,
+    scales), codes int8 of input's shape, scales float32 [...] = max|y| / 127, y ~ codes *
+    scale.  ``linear_int8`` takes both."""
+    codes = torch.empty(input.shape, dtype=torch.int8, device=input.device)
+    scales = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
+    _ops.rms_norm_int8.default(codes, scales, input, weight, residual, residual_out, eps)
+    return codes, scales
+
+
+def quantize_int8(input):
+    """``input`` itself as int8 codes with one scale a row: (codes, scales) as ``rms_norm_int8``."""
+    return rms_norm_int8(input, None, 0.0)
+
+
+def linear_int8(input, input_scale, weight, weight_scale, bias=None, dtype=torch.bfloat16, out=None):
+    """out = (input weight^T) * input_scale * weight_scale + bias in 8-bit integers: ``input`` int8
+    [..., hidden] with a float32 scale for each row (``rms_norm_int8``, ``quantize_int8``),
+    ``weight`` int8 [channels, hidden] with a float32 scale for each channel, ``bias`` [channels]
+    of type ``dtype`` (bfloat16 or float16).  The sums are exact.  Returns ``out`` [..., channels]
+    of type ``dtype``."""
+    if out is None:
+        out = torch.empty(input.shape[:-1] + weight.shape[:1], dtype=dtype, device=input.device)
+    _ops.linear_int8.default(out, input, input_scale, weight, weight_scale, bias)
+    return out
+
+
 __all__ = ["hp_rms_norm", "relu", "rms_norm", "fused_add_rms_norm", "rms_norm_fp8", "rms_norm_nvfp4",
            "rms_norm_fp8_group", "silu_and_mul", "gelu_and_mul", "gelu_tanh_and_mul",
            "gated_linear", "gated_linear_backward", "linear_cross_entropy",
            "linear_cross_entropy_backward", "rms_norm_backward", "grad_norm", "clip_grad_norm",
-           "torch"]
+           "gated_add_rms_norm", "gated_add_rms_norm_backward", "LogProbs", "linear_log_probs",
+           "linear_log_probs_backward", "rms_norm_int8", "quantize_int8", "linear_int8", "torch"]

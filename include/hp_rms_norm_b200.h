@@ -339,6 +339,129 @@ HPRN_API int hprn_clip_grad_norm(float* norm, const hprn_grad* grads, int64_t co
                                  double max_norm, void* workspace, int64_t* workspace_bytes,
                                  void* stream, unsigned flags);
 
+/*
+ * The norms before and after a gated block in one pass (extension):
+ *   y   = input inv_x post_weight, inv_x = rsqrt(eps + mean(input^2))
+ *         (y = input where post_weight is NULL)
+ *   t   = residual_scale residual + gate y       (fp32; residual_out = round_T(t))
+ *   out = round_T(t inv_t weight), inv_t = rsqrt(eps + mean(t^2))  (t unrounded)
+ * input is a block's output, out what the next block reads.  gate: NULL (1), or
+ * rows / rows_per_gate rows of gate_width values, gate_width 1 or hidden; gate
+ * row k serves rows k rows_per_gate to (k + 1) rows_per_gate - 1.  out may be
+ * input, and residual_out residual, with the same stride; outputs must not
+ * otherwise overlap anything.
+ */
+HPRN_API int hprn_gated_add_rms_norm(void* out, void* residual_out, const void* input,
+                                     const void* residual, const void* post_weight,
+                                     const void* weight, const void* gate, int64_t rows,
+                                     int64_t hidden, int64_t rows_per_gate, int64_t gate_width,
+                                     int64_t out_row_stride, int64_t residual_out_row_stride,
+                                     int64_t input_row_stride, int64_t residual_row_stride,
+                                     int64_t gate_row_stride, double residual_scale, double eps,
+                                     int dtype, void* stream, unsigned flags);
+
+/*
+ * Gradients of hprn_gated_add_rms_norm for gradients D of out and E
+ * (grad_residual_out; NULL for none) of residual_out.  residual_out is what the
+ * forward call wrote.  With n = residual_out inv_t, m = input inv_x (m = input,
+ * post_weight = 1 where that is NULL), g the gate, means over a row:
+ *   dt = inv_t (weight D - n mean(weight D n)) + E
+ *   grad_residual    = round_T(residual_scale dt)
+ *   grad_gate        = round_T(sum of dt m post_weight over what shares a value)
+ *   grad_input       = round_T(inv_x (g post_weight dt - m mean(g post_weight dt m)))
+ *                      (round_T(g dt) without post_weight)
+ *   grad_post_weight = round_T(sum over rows of g dt m)    (not without post_weight)
+ *   grad_weight      = round_T(sum over rows of D n)
+ * grad_gate has the gate's rows and width.
+ */
+HPRN_API int hprn_gated_add_rms_norm_backward(
+    void* grad_input, void* grad_residual, void* grad_post_weight, void* grad_weight,
+    void* grad_gate, const void* grad_out, const void* grad_residual_out, const void* input,
+    const void* residual_out, const void* post_weight, const void* weight, const void* gate,
+    int64_t rows, int64_t hidden, int64_t rows_per_gate, int64_t gate_width,
+    int64_t grad_input_row_stride, int64_t grad_residual_row_stride, int64_t grad_gate_row_stride,
+    int64_t grad_out_row_stride, int64_t grad_residual_out_row_stride, int64_t input_row_stride,
+    int64_t residual_out_row_stride, int64_t gate_row_stride, double residual_scale, double eps,
+    int dtype, void* workspace, int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Log probabilities under the softmax of a linear layer over a vocabulary
+ * (extension): with L = input weight^T / temperature (fp32 sums), t = target[i],
+ *   lse[i]      = log sum_j exp(L_ij)
+ *   log_prob[i] = L_{i, t} - lse[i]; 0 where t == ignore_index; NaN where t is
+ *                 otherwise outside [0, vocab)
+ *   entropy[i]  = -sum_j p_ij log p_ij, p_ij = exp(L_ij - lse[i]); 0 where
+ *                 t == ignore_index
+ *   top_log_probs[i, k], top_indices[i, k], k < top: the largest L_ij - lse[i] of
+ *                 every row, the largest first, and their j.  They are ordered by
+ *                 logits summed in 64 bits, equal ones by their indices; a logit
+ *                 is missed only where more than four others lie between it and
+ *                 the last place within the rounding of an fp32 sum.  In rows with a
+ *                 NaN logit the values are NaN and the indices any.
+ * 0 <= top <= 64, top <= vocab; top_* may be NULL where top is 0.  The outputs of
+ * rows are dense.  With top > 0 the workspace holds the logits of a block of rows,
+ * 1 GiB at most where 256 rows fit in that.
+ */
+HPRN_API int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse,
+                                   float* top_log_probs, int64_t* top_indices, const void* input,
+                                   const void* weight, const int64_t* target, int64_t ignore_index,
+                                   double temperature, int64_t top, int64_t rows, int64_t hidden,
+                                   int64_t vocab, int64_t input_row_stride,
+                                   int64_t weight_row_stride, int dtype, void* workspace,
+                                   int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Gradients of hprn_linear_log_probs for gradients g of log_prob and h of entropy
+ * (fp32; grad_entropy NULL for none, entropy is then not read); lse and entropy
+ * from the forward call:
+ *   S_ij = (g_i ([j == t_i] - p_ij) - h_i p_ij (log p_ij + entropy_i)) / temperature
+ *          to 16 bits; 0 in rows with target_i == ignore_index, NaN in rows with any
+ *          other invalid target
+ *   grad_input [rows, hidden]   = round_T(S weight)
+ *   grad_weight [vocab, hidden] = round_T(S^T input)
+ * S is held divided by the largest finite |g_i| or |h_i| (and in fp16 times 2^14, or
+ * 2^13 with grad_entropy).  Where g_i or h_i is infinite or NaN, so are row i of
+ * grad_input and grad_weight.
+ */
+HPRN_API int hprn_linear_log_probs_backward(
+    void* grad_input, void* grad_weight, const float* grad_log_prob, const float* grad_entropy,
+    const void* input, const void* weight, const int64_t* target, const float* lse,
+    const float* entropy, int64_t ignore_index, double temperature, int64_t rows, int64_t hidden,
+    int64_t vocab, int64_t grad_input_row_stride, int64_t grad_weight_row_stride,
+    int64_t input_row_stride, int64_t weight_row_stride, int dtype, void* workspace,
+    int64_t* workspace_bytes, void* stream, unsigned flags);
+
+/*
+ * Rows quantised to 8-bit integers with one scale each (extension):
+ *   t = input, or input + residual (fp32; residual_out = round_T of it)
+ *   y = t weight rsqrt(eps + mean(t^2)), or y = t where weight is NULL
+ *   scales[i] = max(max_j |y_ij|, 1e-12) / 127,  out_ij = round(y_ij (1 / scales[i])),
+ * to nearest even, in [-127, 127]; t is not rounded in between.  residual and
+ * residual_out go together and may be one tensor; a row with a NaN has a NaN scale,
+ * one with an infinity an infinite or NaN scale.
+ */
+HPRN_API int hprn_rms_norm_int8(int8_t* out, float* scales, void* residual_out, const void* input,
+                                const void* weight, const void* residual, int64_t rows,
+                                int64_t hidden, int64_t out_row_stride,
+                                int64_t residual_out_row_stride, int64_t input_row_stride,
+                                int64_t residual_row_stride, double eps, int dtype, void* stream,
+                                unsigned flags);
+
+/*
+ * Linear layer in 8-bit integers (extension):
+ *   out_ij = round_T(S_ij input_scale[i] weight_scale[j] + bias[j]),
+ *   S_ij = sum_k input_ik weight_jk, exact in 32 bits (hidden <= 131071) and
+ * rounded to fp32 once.  input int8 [rows, hidden], weight int8 [channels, hidden],
+ * scales fp32, bias (NULL for none) and out of type `dtype`.  Rows of an even
+ * length on 16-byte boundaries are read as they are, others are copied first.
+ */
+HPRN_API int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale,
+                              const int8_t* weight, const float* weight_scale, const void* bias,
+                              int64_t rows, int64_t hidden, int64_t channels,
+                              int64_t out_row_stride, int64_t input_row_stride,
+                              int64_t weight_row_stride, int dtype, void* workspace,
+                              int64_t* workspace_bytes, void* stream, unsigned flags);
+
 /* Message for the last non-OK status returned on this thread ("" if none). */
 HPRN_API const char* hprn_last_error(void);
 
@@ -388,14 +511,14 @@ HPRN_API int hprn_set_plan_override(const char* plan);
  * No reference counterpart.  Kernels that wait on mbarriers for asynchronous
  * copies and matrix instructions do so with a bound (one second): those that
  * stage rows of hprn_rms_norm* through TMA bulk copies (plan kind tma, reached
- * only through a plan override), the matrix products of hprn_gated_linear* and
- * hprn_linear_cross_entropy*, and hprn_rms_norm_backward.  A CTA that gives up
+ * only through a plan override), the matrix products of hprn_gated_linear*,
+ * hprn_linear_cross_entropy*, hprn_linear_log_probs* and hprn_linear_int8, and
+ * hprn_rms_norm_backward.  A CTA that gives up
  * a wait stops, once its copies in flight have landed, and counts itself here,
  * on its device: in the tma plans it leaves the row it gave up on and its
  * remaining rows untouched (input and residual as they were), in the others
  * the outputs it had not written.  The call that launched it still returns
- * HPRN_OK; later calls of hprn_gated_linear*, hprn_linear_cross_entropy* and
- * hprn_rms_norm_backward on that device return HPRN_ERR_CUDA once a launch of
+ * HPRN_OK; later calls of these operators on that device return HPRN_ERR_CUDA once a launch of
  * these has given up a wait, until the count is reset.  No wait gives up on a
  * GPU that works.
  * Writes the current device's count into *count and, if `reset` is non-zero,
