@@ -1,0 +1,973 @@
+// Gradients of the norms on both sides of a gated block (gated_norm.cu):
+//   t = a r + g y,  y_j = x_j inv_x p_j (y = x without p),  out_j = t_j inv_t w_j
+// With D the gradient of out, E that of t from its other uses, n = t inv_t,
+// m = x inv_x (m = x and p = 1 without p), means over a row:
+//   dt = inv_t (w D - n mean(w D n)) + E
+//   dr = a dt,  dg = sum of dt m p over what shares the gate,
+//   dx = inv_x (p g dt - m mean(p g dt m)),  dp = sum over rows of g dt m,
+//   dw = sum over rows of D n
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "bulk.cuh"
+#include "gated_norm.cuh"
+#include "rows.cuh"
+#include "runtime.cuh"
+#include "vec.cuh"
+
+namespace hprn {
+
+struct BlockGradArgs {
+  uint16_t *dx, *dr, *dp, *dw, *dg;  // dp, dg: or null
+  const uint16_t *d, *e, *x, *t, *p, *w, *g;  // e, p, g: or null
+  int64_t dx_stride, dr_stride, dg_stride, d_stride, e_stride, x_stride, t_stride, g_stride;
+  int64_t rows, hidden;
+  int64_t rows_per_gate, gates;
+  bool gate_row;  // the gate is a row of `hidden` values
+  bool gate_each;  // ... of its own for every row
+  float scale, eps;
+  float4* stats;      // per row: {inv_t, mean(w D n), inv_x, mean(p g dt m)}
+  float* gate_sums;   // per row: sum of dt m p, where the gate is one value
+  // Sums over the rows of a part (`parts` for each gate where the gate is a
+  // shared row, else `parts` in all): of D n, and of dt m where the gate is a
+  // shared row, else of g dt m.
+  float *dw_parts, *m_parts;
+  int64_t parts, part_rows, parts_ld;
+  // Of block_grad_rows: what a row's buffer holds (t, D, and x, E, g where they are
+  // needed; their places in it, or -1), and how its threads are dealt out.
+  const uint16_t* src[5];
+  int64_t src_stride[5];
+  int tensors, x_at, e_at, g_at;
+  int row_threads, row_groups, slots;
+  uint32_t ring_at, join_at;  // in shared memory: the ring, and where the groups' sums meet
+  bool staged;  // w, p and a shared gate row are in shared memory
+  int64_t ctas;
+  bool dense;  // every tensor's rows follow each other
+  Waits waits;
+};
+
+// ---------------------------------------------------------------------------
+// Rows read once: memory-bound, 8 bytes of an element in and 4 out with E and x.
+//
+// A CTA works on a run of neighbouring rows, `row_groups` at a time, each by
+// row_threads threads, a thread always on the same W words (pairs of elements).
+// One warp more brings the rows into a ring of `slots` buffers in shared memory by
+// bulk copies.  Two sums over the row's threads lie between three passes over the
+// buffer: the means of squares and of w D n; then dt, and with it dr, dg, the sums
+// over rows, and the mean of p g dt m; then dx.  The second sum and the next row's
+// first one meet at one barrier (4096 x 8192 with E: TIME_ONE us; with two, 87).  The sums over rows (D n, and dt m
+// or g dt m) stay in registers, 4 W floats, as do w, p and a gate row that rows
+// share up to 8 words a thread.  Where a run reaches into another gate's rows, the
+// sums for the gate are written out and started anew.
+//   kVectors: every row of every tensor starts on a 16-byte boundary and hidden is
+// a multiple of 8; threads take vectors of eight elements.  Else a row is copied
+// with the 16-byte granules it lies in (elements in granules that reach out of the
+// tensor one by one), and threads take single words, neighbouring threads
+// neighbouring ones, put together from two where the row starts on an odd element.
+//
+// A wait that runs out (mbar_wait_bounded) ends its group after the copies in
+// flight, and says so (report_give_up).
+// Few threads of many registers: 512 workers had 96 each and spilled 300 bytes.
+constexpr int kBlockThreads = 352;
+constexpr int kBlockSmem = 220 * 1024;
+constexpr int kBlockSlots = 4;
+constexpr int kBlockGroups = 16;
+
+__device__ __forceinline__ void team_barrier(int barrier, int threads) {
+  if (threads == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
+
+// The sums of N values over the warps that hold a row, which meet at hardware
+// barrier `barrier`; `part` alternates between two buffers.
+template <int N>
+__device__ __forceinline__ void team_sums(float (&v)[N], float (*part)[32], int warp, int warps, int first_warp,
+                                          int barrier) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = warp_total(v[k]);
+  if (warps == 1) {
+    __syncwarp();
+    return;
+  }
+  const int lane = threadIdx.x % 32;
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[k][warp] = v[k];
+  }
+  team_barrier(barrier, warps * 32);
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = warp_total(lane < warps ? part[k][first_warp + lane] : 0.f);
+}
+
+__device__ __forceinline__ uint32_t shared_word(uint32_t addr) {
+  uint32_t w;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(addr));
+  return w;
+}
+__device__ __forceinline__ void shared_words(uint32_t (&w)[4], uint32_t addr) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void set_shared_words(uint32_t addr, const uint32_t (&w)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+__device__ __forceinline__ void set_shared_half(uint32_t addr, uint16_t h) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(h) : "memory");
+}
+
+// The first row of CTA c's run; row i lies in the run of CTA
+// ((i + 1) ctas - 1) / rows.
+__device__ __forceinline__ int64_t run_start(const BlockGradArgs& a, int64_t c) { return a.rows * c / a.ctas; }
+__device__ __forceinline__ int64_t run_of(const BlockGradArgs& a, int64_t i) { return ((i + 1) * a.ctas - 1) / a.rows; }
+
+// kGate: kOneGate a gate of one value a row, or none (1); kGateRow a row of values
+// that rows share; kGateEach one for every row.
+enum GateKind { kOneGate, kGateRow, kGateEach };
+
+template <typename T, int W, bool kVectors, bool kPost, int kGate>
+__global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGradArgs a) {
+  constexpr int kVecs = W / 4;
+  constexpr bool kHold = W <= 12;
+  static_assert(kHold || kVectors, "words of unaligned rows are read by two threads");
+  extern __shared__ __align__(128) unsigned char row_mem[];
+  __shared__ __align__(8) uint64_t full[kBlockSlots], empty[kBlockSlots];
+  __shared__ float part[2][4][32];
+  __shared__ int gave_up[kBlockGroups];
+  const int tid = threadIdx.x, row_threads = a.row_threads, groups = a.row_groups;
+  const int workers = groups * row_threads;
+  const bool copier = tid >= workers;
+  const int group = copier ? 0 : tid / row_threads, in = copier ? 0 : tid - group * row_threads;
+  const int warps = row_threads / 32, barrier = 1 + group;
+  const int hidden = static_cast<int>(a.hidden), nvec = (hidden + 7) / 8, words = (hidden + 1) / 2;
+  // A buffer: `groups` rows of each tensor in turn, `pitch` bytes a row.
+  const uint32_t row_bytes = static_cast<uint32_t>(nvec) * 16, pitch = row_bytes + (kVectors ? 0 : 16);
+  const uint32_t tensor_bytes = pitch * groups, slot_bytes = tensor_bytes * a.tensors;
+  const uint32_t staged = smem_u32(row_mem), ring = staged + a.ring_at;
+  const int begin = static_cast<int>(run_start(a, blockIdx.x)), end = static_cast<int>(run_start(a, blockIdx.x + 1));
+  const int rows_per_gate = static_cast<int>(a.rows_per_gate);
+  constexpr bool shared_row = kGate == kGateRow;
+  // A run's rows up to the next gate's.
+  auto segment_end = [&](int i) { return shared_row ? min(end, (i / rows_per_gate + 1) * rows_per_gate) : end; };
+  const int lane = tid % 32;
+  if (copier) {
+    if (lane < groups) gave_up[lane] = 0;
+    if (lane == 0) {
+      for (int s = 0; s < a.slots; ++s) {
+        mbar_init(smem_u32(&full[s]), 1);
+        mbar_init(smem_u32(&empty[s]), groups * warps);
+      }
+      mbar_init_fence();
+    }
+    // The first rows, into L2, while the preceding grid drains.
+    const int first = begin + lane;
+    if (lane < groups * a.slots && first < end)
+      for (int t = 0; t < a.tensors; ++t)
+        prefetch_l2(a.src[t] + static_cast<int64_t>(first) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
+  }
+  __syncthreads();
+  pdl_wait();
+
+  if (copier) {
+    const uint64_t pol = policy_evict_first();
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i0 = a.waits.stall ? end : begin; i0 < end && ok; i0 = segment_end(i0)) {
+      const int last = segment_end(i0);
+      for (int base = i0; base < last; base += groups) {
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1, a.waits.limit_ns));
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&full[slot]), to = ring + slot * slot_bytes;
+        const int here = min(groups, last - base);
+        // With few buffers a later round's rows are asked into L2.
+        const int next = base + a.slots * groups;
+        if (kVectors && a.dense) {
+          const uint32_t bytes = static_cast<uint32_t>(here) * row_bytes;
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes * a.tensors);
+          __syncwarp();
+          if (lane < a.tensors) {
+            bulk_load(to + lane * tensor_bytes, a.src[lane] + base * a.src_stride[lane], bytes, bar, pol);
+            if (a.slots < 3 && next < end)
+              prefetch_l2(a.src[lane] + next * a.src_stride[lane],
+                          static_cast<uint64_t>(min(groups, end - next)) * row_bytes);
+          }
+        } else {
+          const bool mine = lane < here;
+          const int64_t i = base + lane;
+          const unsigned char* from[5];
+          uint32_t bytes[5], at[5], total = 0;
+#pragma unroll
+          for (int t = 0; t < 5; ++t) {
+            bytes[t] = 0;
+            if (!mine || t >= a.tensors) continue;
+            const int64_t stride = a.src_stride[t];
+            const unsigned char* p = reinterpret_cast<const unsigned char*>(a.src[t] + i * stride);
+            const uint32_t off = kVectors ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
+            at[t] = to + t * tensor_bytes + lane * pitch;
+            // Granules [lo, hi) of the row's span, from its first one; those that
+            // reach out of the tensor are left out, their elements of this row stored
+            // one by one.
+            const uint32_t stop = off + static_cast<uint32_t>(hidden) * 2;
+            uint32_t lo = 0, hi = (stop + 15) & ~15u;
+            if (off > i * stride * 2) lo = 16;
+            if (hi - stop > (a.rows - 1 - i) * stride * 2) hi -= 16;
+            hi = max(hi, lo);
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+            if (lo > 0)
+              for (int j = 0; j < hidden && off + 2 * j < lo; ++j) set_shared_half(at[t] + off + 2 * j, q[j]);
+            if (hi < stop)
+              for (int j = hi > off ? static_cast<int>(hi - off) / 2 : 0; j < hidden; ++j)
+                set_shared_half(at[t] + off + 2 * j, q[j]);
+            from[t] = p - off + lo, at[t] += lo, bytes[t] = hi - lo, total += bytes[t];
+          }
+          // The stores above, in this round and in earlier ones of this buffer, before
+          // the bulk copies that write there by another proxy.
+          if constexpr (!kVectors) fence_proxy_async_smem();
+          total = __reduce_add_sync(~0u, total);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(bar, total);
+          __syncwarp();
+#pragma unroll
+          for (int t = 0; t < 5; ++t) {
+            if (bytes[t] > 0) bulk_load(at[t], from[t], bytes[t], bar, pol);
+            if (a.slots < 3 && t < a.tensors && lane < groups && next + lane < end)
+              prefetch_l2(a.src[t] + (next + lane) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
+          }
+        }
+        if (++slot == a.slots) slot = 0, phase ^= 1;
+      }
+    }
+    if (!ok) {
+      if (lane == 0) report_give_up(a.waits);
+      for (int k = 0; k < a.slots; ++k) {  // copies still in flight
+        if (--slot < 0) slot = a.slots - 1, phase ^= 1;
+        mbar_wait_bounded(smem_u32(&full[slot]), phase, kWaitLimitNs / 16);
+      }
+    }
+    return;
+  }
+  pdl_trigger();
+
+  // Words 4 k to 4 k + 3 of this thread's: one vector, or one word every row_threads.
+  // (Of words, what the whole warp has some of: lanes past the end work on zeros.)
+  auto inside = [&](int k) {
+    return kVectors ? in + k * row_threads < nvec : in - lane + 4 * k * row_threads < words;
+  };
+  auto word_at = [&](int k, int e) { return in + (4 * k + e) * row_threads; };
+  const uint64_t keep = policy_evict_last();
+  // Of a row in memory (a weight, or a gate row).
+  auto load_weight = [&](uint32_t (&w)[4], const uint16_t* p, int k) {
+    if constexpr (kVectors) {
+      const Vec<16> q = ld_weight<16>(p + (in + k * row_threads) * 8, keep);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = q.w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 2 * word_at(k, e);
+        const uint32_t lo = j < hidden ? ld_weight<2>(p + j, keep).h : 0;
+        const uint32_t hi = j + 1 < hidden ? ld_weight<2>(p + j + 1, keep).h : 0;
+        w[e] = lo | hi << 16;
+      }
+    }
+  };
+  // Of a row in shared memory that starts at `at`.
+  auto load_row = [&](uint32_t (&w)[4], uint32_t at, int k) {
+    if constexpr (kVectors) {
+      shared_words(w, at + (in + k * row_threads) * 16);
+    } else {
+      // All loads first, past the row's end the last word again.  (The word behind
+      // the last one lies in the buffer's spare granule.)
+      const uint32_t from = at & ~3u;
+      uint32_t next[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = shared_word(from + min(word_at(k, e), words - 1) * 4);
+      if (at & 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next[e] = shared_word(from + min(word_at(k, e), words - 1) * 4 + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(w[e], next[e], 16);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (2 * word_at(k, e) + 1 == hidden) w[e] &= 0xffffu;
+        if (word_at(k, e) >= words) w[e] = 0;
+      }
+    }
+  };
+  auto store_row = [&](uint16_t* row, int k, const uint32_t (&w)[4]) {
+    if constexpr (kVectors) {
+      *reinterpret_cast<uint4*>(row + (in + k * row_threads) * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = word_at(k, e);
+        uint16_t* q = row + 2 * j;
+        const bool second = 2 * j + 1 < hidden;
+        if ((reinterpret_cast<uintptr_t>(row) & 2) == 0) {
+          if (j >= words) continue;
+          if (second) *reinterpret_cast<uint32_t*>(q) = w[e];
+          else q[0] = static_cast<uint16_t>(w[e]);
+          continue;
+        }
+        // An element off the words of memory: a lane stores the word of its first
+        // element and the last one of the lane before.
+        const uint32_t before = __shfl_up_sync(~0u, w[e], 1);
+        if (j >= words) continue;
+        if (lane > 0) *reinterpret_cast<uint32_t*>(q - 1) = before >> 16 | w[e] << 16;
+        else q[0] = static_cast<uint16_t>(w[e]);
+        if (second && (lane == 31 || j + 1 >= words)) q[1] = static_cast<uint16_t>(w[e] >> 16);
+      }
+    }
+  };
+
+  constexpr bool post = kPost;
+  const bool one_gate = kGate == kOneGate && a.g;
+  float2 acc_w[W], acc_m[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) acc_w[k] = acc_m[k] = make_float2(0.f, 0.f);
+  // Row `which` of w, p and a shared gate row into shared memory, by all threads.
+  const int gate_place = post ? 2 : 1;
+  auto stage = [&](int which, const uint16_t* p) {
+    uint32_t* to = reinterpret_cast<uint32_t*>(row_mem) + which * (row_bytes / 4);
+    for (int j = tid; j < nvec * 4; j += workers) {
+      const uint32_t lo = 2 * j < hidden ? ld_weight<2>(p + 2 * j, keep).h : 0;
+      const uint32_t hi = 2 * j + 1 < hidden ? ld_weight<2>(p + 2 * j + 1, keep).h : 0;
+      to[j] = lo | hi << 16;
+    }
+  };
+  auto weight = [&](uint32_t (&w)[4], int which, const uint16_t* p, int k) {
+    if (!a.staged) return load_weight(w, p, k);
+    const uint32_t at = staged + which * row_bytes;
+    if constexpr (kVectors) {
+      shared_words(w, at + (in + k * row_threads) * 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = word_at(k, e) < words ? shared_word(at + word_at(k, e) * 4) : 0;
+    }
+  };
+  if (a.staged) {
+    stage(0, a.w);
+    if (post) stage(1, a.p);
+    if (!shared_row) team_barrier(15, workers);
+  }
+  const float scale = 1.0f / static_cast<float>(hidden);
+  const float2 residual_scale = make_float2(a.scale, a.scale);
+  // A CTA's sums over the rows so far: the groups' meet in shared memory, the first
+  // group writes them.
+  auto write_sums = [&](float2 (&acc)[W], float* out) {
+    if (groups > 1) {
+      float2* sums = reinterpret_cast<float2*>(row_mem + a.join_at);
+      team_barrier(15, workers);
+#pragma unroll
+      for (int k = 0; k < W; ++k) sums[k * workers + tid] = acc[k];
+      team_barrier(15, workers);
+      if (group > 0) return;
+      for (int g = 1; g < groups; ++g) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[k] = __fadd2_rn(acc[k], sums[k * workers + g * row_threads + tid]);
+      }
+    }
+    // (Rows of sums are padded to whole vectors.)
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      if (!inside(k)) break;
+      if constexpr (kVectors) {
+        Vec<32> q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          q.w[2 * e] = __float_as_uint(acc[4 * k + e].x);
+          q.w[2 * e + 1] = __float_as_uint(acc[4 * k + e].y);
+        }
+        st_global<32>(out + (in + k * row_threads) * 8, q);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (word_at(k, e) < words) reinterpret_cast<float2*>(out)[word_at(k, e)] = acc[4 * k + e];
+      }
+    }
+  };
+
+  auto start_of = [&](int t, int64_t i, uint32_t at) {
+    return at + t * tensor_bytes +
+           (kVectors ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.src[t] + i * a.src_stride[t]) & 15));
+  };
+  // Row i's sums of t^2, w D t and x^2, once its buffer at `at` has arrived.
+  auto first_pass = [&](int64_t i, uint32_t at, int of_slot, uint32_t of_phase, float& s_t, float& s_d, float& s_x) {
+    const uint32_t ts = start_of(0, i, at), ds = start_of(1, i, at), xs = post ? start_of(a.x_at, i, at) : 0;
+    if (!mbar_wait_bounded(smem_u32(&full[of_slot]), of_phase, a.waits.limit_ns)) gave_up[group] = 1;
+    float2 st = make_float2(0.f, 0.f), sd = st, sx = st;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      if (!inside(k)) break;
+      uint32_t t[4], d[4], w[4], x[4];
+      load_row(t, ts, k);
+      load_row(d, ds, k);
+      weight(w, 0, a.w, k);
+      if constexpr (post) load_row(x, xs, k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 tf = unpack2<T>(t[e]);
+        st = __ffma2_rn(tf, tf, st);
+        sd = __ffma2_rn(mul_pair<T>(w[e], d[e]), tf, sd);
+        if constexpr (post) sx = fma_pair<T>(x[e], x[e], sx);
+      }
+    }
+    s_t = st.x + st.y, s_d = sd.x + sd.y, s_x = sx.x + sx.y;
+  };
+  int slot = 0, turn = 0;
+  uint32_t phase = 0;
+  bool stopped = false, have = false;  // have: `sums` are the next row's
+  float sums[3];
+  for (int i0 = begin; i0 < end; i0 = segment_end(i0)) {
+    const int last = segment_end(i0);
+    const uint16_t* gate_row = shared_row ? a.g + i0 / rows_per_gate * a.g_stride : nullptr;
+    if (a.staged && shared_row) {
+      if (i0 > begin) team_barrier(15, workers);  // every group is done with the last one
+      stage(gate_place, gate_row);
+      team_barrier(15, workers);
+    }
+    for (int base = i0; base < last && !stopped; base += groups) {
+      const int64_t i = base + group;
+      const uint32_t at = ring + slot * slot_bytes + group * pitch, slot_bar = smem_u32(&empty[slot]);
+      const int this_slot = slot;
+      const uint32_t this_phase = phase;
+      if (++slot == a.slots) slot = 0, phase ^= 1;
+      if (i >= last) {  // fewer rows left than groups
+        __syncwarp();
+        if (lane == 0) mbar_arrive(slot_bar);
+        continue;
+      }
+      float gate_one = 1.f;
+      if (one_gate) gate_one = unpack1<T>(a.g[(static_cast<uint32_t>(i) / static_cast<uint32_t>(a.rows_per_gate)) * a.g_stride]);
+      if (!have) {
+        first_pass(i, at, this_slot, this_phase, sums[0], sums[1], sums[2]);
+        team_sums(sums, part[turn], tid / 32, warps, group * warps, barrier);
+        turn ^= 1;
+      }
+      have = false;
+      if (*static_cast<volatile int*>(&gave_up[group])) {
+        // The copier may have issued its last row and left without a wait.
+        if (in == 0) report_give_up(a.waits);
+        stopped = true;
+        break;
+      }
+      const uint32_t ts = start_of(0, i, at), ds = start_of(1, i, at), xs = a.x_at >= 0 ? start_of(a.x_at, i, at) : 0;
+      const uint32_t es = a.e_at >= 0 ? start_of(a.e_at, i, at) : 0, gs = a.g_at >= 0 ? start_of(a.g_at, i, at) : 0;
+      const float inv_t = rsqrtf(sums[0] * scale + a.eps), mean = sums[1] * inv_t * scale;
+      const float inv_x = post ? rsqrtf(sums[2] * scale + a.eps) : 1.f;
+      // dt = w D inv_t + (E - t mean inv_t^2); the sums over a row leave inv_x out.
+      const float2 inv_t2 = make_float2(inv_t, inv_t), minus = make_float2(-mean * inv_t * inv_t, -mean * inv_t * inv_t);
+      const float by = (kGate == kOneGate ? gate_one : 1.f) * inv_x;
+      const float2 m_by = make_float2(by, by);
+      uint16_t* dr = a.dr + i * a.dr_stride;
+      uint16_t* dx = a.dx + i * a.dx_stride;
+      // Held or put back: p dt, times g where that is a row.
+      float2 u[kHold ? W : 1], su = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        if (!inside(k)) break;
+        uint32_t t[4], d[4], w[4], x[4] = {}, e4[4] = {}, g[4], p[4], out_r[4], out_g[4];
+        load_row(t, ts, k);
+        load_row(d, ds, k);
+        weight(w, 0, a.w, k);
+        if (a.x_at >= 0) load_row(x, xs, k);
+        if (a.e_at >= 0) load_row(e4, es, k);
+        if constexpr (post) weight(p, 1, a.p, k);
+        if constexpr (kGate == kGateEach) load_row(g, gs, k);
+        if constexpr (kGate == kGateRow) weight(g, gate_place, gate_row, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 dt = __ffma2_rn(mul_pair<T>(w[e], d[e]), inv_t2, __ffma2_rn(unpack2<T>(t[e]), minus, unpack2<T>(e4[e])));
+          acc_w[4 * k + e] = __ffma2_rn(mul_pair<T>(d[e], t[e]), inv_t2, acc_w[4 * k + e]);
+          const float2 xf = unpack2<T>(x[e]), q = __fmul2_rn(dt, xf);
+          float2 pdt = dt;
+          if constexpr (kGate == kOneGate) {
+            acc_m[4 * k + e] = __ffma2_rn(q, m_by, acc_m[4 * k + e]);
+            if constexpr (post) pdt = __fmul2_rn(dt, unpack2<T>(p[e]));
+          } else {
+            if constexpr (kGate == kGateEach)
+              acc_m[4 * k + e] = __ffma2_rn(__fmul2_rn(q, unpack2<T>(g[e])), m_by, acc_m[4 * k + e]);
+            else
+              acc_m[4 * k + e] = __ffma2_rn(q, m_by, acc_m[4 * k + e]);
+            if constexpr (post) pdt = __fmul2_rn(dt, mul_pair<T>(p[e], g[e]));
+            else pdt = __fmul2_rn(dt, unpack2<T>(g[e]));
+          }
+          su = __ffma2_rn(pdt, xf, su);
+          const float2 r = __fmul2_rn(dt, residual_scale);
+          out_r[e] = pack2<T>(r.x, r.y);
+          if constexpr (kGate == kGateEach) {
+            float2 v = __fmul2_rn(q, m_by);
+            if constexpr (post) v = __fmul2_rn(v, unpack2<T>(p[e]));
+            out_g[e] = pack2<T>(v.x, v.y);
+          }
+          if constexpr (!post) {
+            const float2 v = kGate == kOneGate ? __fmul2_rn(pdt, m_by) : pdt;
+            t[e] = pack2<T>(v.x, v.y);
+          } else if constexpr (kHold) {
+            u[4 * k + e] = pdt;
+          } else {
+            t[e] = __float_as_uint(pdt.x), d[e] = __float_as_uint(pdt.y);
+          }
+        }
+        store_row(dr, k, out_r);
+        if constexpr (kGate == kGateEach) store_row(a.dg + i * a.dg_stride, k, out_g);
+        if constexpr (!post) {
+          store_row(dx, k, t);
+        } else if constexpr (!kHold) {
+          set_shared_words(ts + (in + k * row_threads) * 16, t);
+          set_shared_words(ds + (in + k * row_threads) * 16, d);
+        }
+      }
+      // The group's row of the next round goes through its first pass now, so that
+      // both rows' sums meet at one barrier.
+      const int next_last = base + groups < last ? last : last < end ? segment_end(last) : 0;
+      const int next = (base + groups < last ? base + groups : last) + group;
+      float s[4] = {0.f, 0.f, 0.f, su.x + su.y};
+      if (a.slots > 1 && next < next_last) {
+        first_pass(next, ring + slot * slot_bytes + group * pitch, slot, phase, s[0], s[1], s[2]);
+        have = true;
+      }
+      if (have || post || one_gate) {
+        team_sums(s, part[turn], tid / 32, warps, group * warps, barrier);
+        turn ^= 1;
+        sums[0] = s[0], sums[1] = s[1], sums[2] = s[2];
+        if (one_gate && in == 0) a.gate_sums[i] = s[3] * inv_x;
+        if constexpr (post) {
+          // dx = inv_x (p g dt - m mean(p g dt m)) = u by - x inv_x^2 mean(u x by).
+          const float b = -s[3] * by * inv_x * inv_x * scale;
+          const float2 back = make_float2(b, b);
+#pragma unroll
+          for (int k = 0; k < kVecs; ++k) {
+            if (!inside(k)) break;
+            uint32_t x[4], ux[4], uy[4], o[4];
+            load_row(x, xs, k);
+            if constexpr (!kHold) {
+              shared_words(ux, ts + (in + k * row_threads) * 16);
+              shared_words(uy, ds + (in + k * row_threads) * 16);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float2 pdt;
+              if constexpr (kHold) pdt = u[4 * k + e];
+              else pdt = make_float2(__uint_as_float(ux[e]), __uint_as_float(uy[e]));
+              const float2 v = __ffma2_rn(pdt, m_by, __fmul2_rn(unpack2<T>(x[e]), back));
+              o[e] = pack2<T>(v.x, v.y);
+            }
+            store_row(dx, k, o);
+          }
+          // The words put into the buffer, before the next copies into it.
+          if constexpr (!kHold) fence_proxy_async_smem();
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(slot_bar);
+    }
+    if (shared_row) {
+      write_sums(acc_m, a.m_parts + static_cast<int64_t>(blockIdx.x + i0 / rows_per_gate) * a.parts_ld);
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc_m[k] = make_float2(0.f, 0.f);
+    }
+  }
+  write_sums(acc_w, a.dw_parts + blockIdx.x * a.parts_ld);
+  if (!shared_row) write_sums(acc_m, a.m_parts + blockIdx.x * a.parts_ld);
+}
+
+// The weights' and a shared gate row's gradients from block_grad_rows' sums: 32
+// columns a CTA.  Its 8 warps share out the CTAs' sums; where rows of the gate
+// are few they share out each one's sums as well, else they take gates in turn.
+template <typename T>
+__global__ void __launch_bounds__(256) block_grad_runs(BlockGradArgs a) {
+  __shared__ float sums[2][8][32];
+  pdl_wait();
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + tx;
+  const bool shared_row = a.gate_row && !a.gate_each, in = j < a.hidden;
+  float sw = 0.f, sp = 0.f;
+  if (in) {
+#pragma unroll 8
+    for (int64_t c = ty; c < a.ctas; c += 8) sw += a.dw_parts[c * a.parts_ld + j];
+  }
+  if (!shared_row) {
+    if (in) {
+#pragma unroll 8
+      for (int64_t c = ty; c < a.ctas; c += 8) sp += a.m_parts[c * a.parts_ld + j];
+    }
+  } else {
+    const float p = in && a.p ? unpack1<T>(a.p[j]) : 1.f;
+    const bool together = a.gates < 8;
+    for (int64_t k = together ? 0 : ty; k < a.gates; k += together ? 1 : 8) {
+      const int64_t first = run_of(a, k * a.rows_per_gate), last = run_of(a, (k + 1) * a.rows_per_gate - 1);
+      float sm = 0.f;
+      if (in) {
+#pragma unroll 4
+        for (int64_t c = first + (together ? ty : 0); c <= last; c += together ? 8 : 1)
+          sm += a.m_parts[(c + k) * a.parts_ld + j];
+      }
+      if (together) {
+        __syncthreads();
+        sums[0][ty][tx] = sm;
+        __syncthreads();
+        if (ty > 0) continue;
+        for (int q = 1; q < 8; ++q) sm += sums[0][q][tx];
+      }
+      if (!in) continue;
+      sp = fmaf(unpack1<T>(a.g[k * a.g_stride + j]), sm, sp);
+      a.dg[k * a.dg_stride + j] = pack1<T>(sm * p);
+    }
+    __syncthreads();
+  }
+  sums[0][ty][tx] = sw, sums[1][ty][tx] = sp;
+  __syncthreads();
+  if (ty > 0 || !in) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sw += sums[0][k][tx], sp += sums[1][k][tx];
+  a.dw[j] = pack1<T>(sw);
+  if (a.dp) a.dp[j] = pack1<T>(sp);
+}
+
+// ---------------------------------------------------------------------------
+// Rows too long for that, read twice, element by element.
+
+// The values of one element of row i that the sums and outputs are made of.
+template <typename T>
+struct BlockGradElement {
+  float d, e, n, m, p, g, wd;
+  __device__ __forceinline__ BlockGradElement(const BlockGradArgs& a, int64_t i, int64_t j, const uint16_t* gate,
+                                         float inv_t, float inv_x) {
+    d = unpack1<T>(a.d[i * a.d_stride + j]);
+    e = a.e ? unpack1<T>(a.e[i * a.e_stride + j]) : 0.f;
+    n = unpack1<T>(a.t[i * a.t_stride + j]) * inv_t;
+    m = unpack1<T>(a.x[i * a.x_stride + j]) * inv_x;
+    p = a.p ? unpack1<T>(a.p[j]) : 1.f;
+    g = gate ? unpack1<T>(gate[a.gate_row ? j : 0]) : 1.f;
+    wd = unpack1<T>(a.w[j]) * d;
+  }
+  __device__ __forceinline__ float dt(float inv_t, float mean) const { return inv_t * (wd - n * mean) + e; }
+};
+
+template <typename T>
+__device__ __forceinline__ const uint16_t* gate_of(const BlockGradArgs& a, int64_t i) {
+  return a.g ? a.g + (static_cast<uint32_t>(i) / static_cast<uint32_t>(a.rows_per_gate)) * a.g_stride : nullptr;
+}
+
+// One CTA per row: the row's means.
+template <typename T>
+__global__ void __launch_bounds__(256) block_grad_stats(BlockGradArgs a) {
+  __shared__ float part[4][32];
+  pdl_wait();
+  const int64_t i = blockIdx.x;
+  const uint16_t* gate = gate_of<T>(a, i);
+  const float inv_hidden = 1.f / static_cast<float>(a.hidden);
+  float st = 0.f, sx = 0.f, sd = 0.f;
+  for (int64_t j = threadIdx.x; j < a.hidden; j += 256) {
+    const BlockGradElement<T> v(a, i, j, gate, 1.f, 1.f);
+    st = fmaf(v.n, v.n, st), sx = fmaf(v.m, v.m, sx), sd = fmaf(v.wd, v.n, sd);
+  }
+  st = row_sum(st, part[0], 8, 0), sx = row_sum(sx, part[1], 8, 0), sd = row_sum(sd, part[2], 8, 0);
+  const float inv_t = rsqrtf(st * inv_hidden + a.eps), inv_x = a.p ? rsqrtf(sx * inv_hidden + a.eps) : 1.f;
+  const float mean = sd * inv_t * inv_hidden;
+  float s = 0.f;
+  for (int64_t j = threadIdx.x; j < a.hidden; j += 256) {
+    const BlockGradElement<T> v(a, i, j, gate, inv_t, inv_x);
+    s = fmaf(v.dt(inv_t, mean) * v.p * (a.gate_row ? v.g : 1.f), v.m, s);
+  }
+  s = row_sum(s, part[3], 8, 0);
+  if (threadIdx.x != 0) return;
+  if (a.gate_sums) a.gate_sums[i] = s;
+  if (gate && !a.gate_row) s *= unpack1<T>(gate[0]);
+  a.stats[i] = make_float4(inv_t, mean, inv_x, a.p ? s * inv_hidden : 0.f);
+}
+
+// A part of the rows x 256 columns per CTA: the rows' outputs, the part's sums.
+template <typename T>
+__global__ void __launch_bounds__(256) block_grad_columns(BlockGradArgs a) {
+  pdl_wait();
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (j >= a.hidden) return;
+  const bool shared_row = a.gate_row && !a.gate_each;
+  const int64_t gates = shared_row ? a.gates : 1, rows = shared_row ? a.rows_per_gate : a.rows;
+  for (int64_t part = blockIdx.y; part < gates * a.parts; part += gridDim.y) {
+    const int64_t first = part / a.parts * rows, in = part % a.parts * a.part_rows;
+    const int64_t end = first + min(rows, in + a.part_rows);
+    float sw = 0.f, sm = 0.f;
+    for (int64_t i = first + in; i < end; ++i) {
+      const float4 st = a.stats[i];
+      const BlockGradElement<T> v(a, i, j, gate_of<T>(a, i), st.x, st.z);
+      const float dt = v.dt(st.x, st.y);
+      a.dr[i * a.dr_stride + j] = pack1<T>(a.scale * dt);
+      a.dx[i * a.dx_stride + j] = pack1<T>(a.p ? st.z * (v.p * v.g * dt - v.m * st.w) : v.g * dt);
+      sw = fmaf(v.d, v.n, sw);
+      sm = fmaf(shared_row ? dt : v.g * dt, v.m, sm);
+      if (a.gate_each) a.dg[i * a.dg_stride + j] = pack1<T>(dt * v.m * v.p);
+    }
+    a.dw_parts[part * a.parts_ld + j] = sw;
+    a.m_parts[part * a.parts_ld + j] = sm;
+  }
+}
+
+// The weights' and a shared gate row's gradients from the parts' sums: 32
+// columns a CTA, its 8 warps taking gates (or, where there are none, parts) in
+// turn.
+template <typename T>
+__global__ void __launch_bounds__(256) block_grad_join(BlockGradArgs a) {
+  __shared__ float sums[2][8][32];
+  pdl_wait();
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + tx;
+  const bool shared_row = a.gate_row && !a.gate_each;
+  float sw = 0.f, sp = 0.f;
+  if (j < a.hidden) {
+    if (shared_row) {
+      const float p = a.p ? unpack1<T>(a.p[j]) : 1.f;
+      for (int64_t k = ty; k < a.gates; k += 8) {
+        float sm = 0.f;
+        for (int64_t part = k * a.parts; part < (k + 1) * a.parts; ++part) {
+          sw += a.dw_parts[part * a.parts_ld + j];
+          sm += a.m_parts[part * a.parts_ld + j];
+        }
+        sp = fmaf(unpack1<T>(a.g[k * a.g_stride + j]), sm, sp);
+        a.dg[k * a.dg_stride + j] = pack1<T>(sm * p);
+      }
+    } else {
+      for (int64_t part = ty; part < a.parts; part += 8) {
+        sw += a.dw_parts[part * a.parts_ld + j];
+        sp += a.m_parts[part * a.parts_ld + j];
+      }
+    }
+  }
+  sums[0][ty][tx] = sw, sums[1][ty][tx] = sp;
+  __syncthreads();
+  if (ty > 0 || j >= a.hidden) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sw += sums[0][k][tx], sp += sums[1][k][tx];
+  a.dw[j] = pack1<T>(sw);
+  if (a.dp) a.dp[j] = pack1<T>(sp);
+}
+
+// The gradients of gates of one value: one CTA adds up the rows that share one.
+template <typename T>
+__global__ void __launch_bounds__(256) block_grad_gates(BlockGradArgs a) {
+  __shared__ float part[32];
+  pdl_wait();
+  for (int64_t k = blockIdx.x; k < a.gates; k += gridDim.x) {
+    float s = 0.f;
+    for (int64_t i = threadIdx.x; i < a.rows_per_gate; i += 256) s += a.gate_sums[k * a.rows_per_gate + i];
+    s = row_sum(s, part, 8, 0);
+    if (threadIdx.x == 0) a.dg[k * a.dg_stride] = pack1<T>(s);
+    __syncthreads();
+  }
+}
+
+namespace {
+
+// How block_grad_rows takes the rows; words 0 where it does not.
+struct BlockGradPlan {
+  int words, smem;
+  bool vectors;
+};
+
+BlockGradPlan plan_block_grad(BlockGradArgs& a) {
+  a.tensors = 0, a.x_at = a.e_at = a.g_at = -1;
+  auto add = [&](const uint16_t* p, int64_t stride) {
+    a.src[a.tensors] = p, a.src_stride[a.tensors] = a.rows > 1 ? stride : a.hidden;
+    return a.tensors++;
+  };
+  add(a.t, a.t_stride);
+  add(a.d, a.d_stride);
+  if (a.p || a.g) a.x_at = add(a.x, a.x_stride);
+  if (a.e) a.e_at = add(a.e, a.e_stride);
+  if (a.gate_each) a.g_at = add(a.g, a.g_stride);
+  BlockGradPlan plan{};
+  plan.vectors = a.hidden % 8 == 0 && tma_rows(a.dx, a.rows, a.dx_stride) && tma_rows(a.dr, a.rows, a.dr_stride) &&
+                 aligned(a.w, 16) && aligned(a.p, 16) && (!a.gate_each || tma_rows(a.dg, a.rows, a.dg_stride));
+  if (a.gate_row && !a.gate_each) plan.vectors = plan.vectors && tma_rows(a.g, a.gates, a.g_stride);
+  a.dense = true;
+  for (int k = 0; k < a.tensors; ++k) {
+    plan.vectors = plan.vectors && tma_rows(a.src[k], a.rows, a.src_stride[k]);
+    a.dense = a.dense && a.src_stride[k] == a.hidden;
+  }
+  if (a.rows <= 0 || a.hidden <= 0 || a.hidden > 32768) return plan;
+  const int64_t nvec = (a.hidden + 7) / 8, pairs = (a.hidden + 1) / 2;
+  const int64_t slot = (nvec * 16 + (plan.vectors ? 0 : 16)) * a.tensors;
+  const bool segments = a.gate_row && !a.gate_each && a.gates > 1;
+  const int64_t weights = 1 + (a.p != nullptr) + (a.gate_row && !a.gate_each);
+  int best = 0;
+  for (int words : {4, 8, 12, 24}) {
+    if (words > 12 && !plan.vectors) break;
+    const int64_t threads = round_up(plan.vectors ? (nvec + words / 4 - 1) / (words / 4) : (pairs + words - 1) / words, 32);
+    const bool few = a.rows <= 4 * 148;
+    if (threads > kBlockThreads || (words == 4 && threads > 128 && !few)) continue;
+    int64_t groups = kBlockThreads / threads;
+    if (groups > 14) groups = 14;  // a hardware barrier each, and one for all
+    if (groups > a.rows) groups = a.rows;
+    auto join_bytes = [&] { return groups > 1 ? words * threads * groups * 8 : 0; };
+    auto ring_bytes = [&](int64_t slots) { return slots * groups * slot; };
+    int64_t before = weights * nvec * 16;  // the ring
+    while (groups > 1 && before + ring_bytes(2) + (segments ? join_bytes() : 0) > kBlockSmem) --groups;
+    const bool staged = before + ring_bytes(2) + (segments ? join_bytes() : 0) <= kBlockSmem;
+    if (!staged) before = 0;
+    int64_t slots = (kBlockSmem - before - (segments ? join_bytes() : 0)) / (groups * slot);
+    if (slots > kBlockSlots) slots = kBlockSlots;
+    if (slots < 1 || threads * groups <= best) continue;
+    best = static_cast<int>(threads * groups);
+    plan.words = words;
+    a.row_threads = static_cast<int>(threads), a.row_groups = static_cast<int>(groups), a.slots = static_cast<int>(slots);
+    // The ring is free when a CTA's only sums are written.
+    a.staged = staged, a.ring_at = static_cast<uint32_t>(before);
+    a.join_at = static_cast<uint32_t>(segments ? before + ring_bytes(slots) : 0);
+    const int64_t ring = before + ring_bytes(slots), joined = a.join_at + join_bytes();
+    plan.smem = static_cast<int>(ring > joined ? ring : joined);
+    const int64_t need = (a.rows + groups - 1) / groups;
+    a.ctas = need < 148 ? need : 148;
+    if (few || best >= 288) break;
+  }
+  return plan;
+}
+
+template <typename T, bool kVectors, bool kPost, int kGate>
+void (*block_grad_kernel(int words))(BlockGradArgs) {
+  switch (words) {
+    case 4: return block_grad_rows<T, 4, kVectors, kPost, kGate>;
+    case 8: return block_grad_rows<T, 8, kVectors, kPost, kGate>;
+    case 12: return block_grad_rows<T, 12, kVectors, kPost, kGate>;
+  }
+  if constexpr (kVectors) return block_grad_rows<T, 24, true, kPost, kGate>;
+  return nullptr;
+}
+template <typename T, bool kVectors>
+void (*block_grad_kernel(const BlockGradArgs& a, int words))(BlockGradArgs) {
+  const int gate = !a.gate_row ? kOneGate : a.gate_each ? kGateEach : kGateRow;
+  if (gate == kOneGate)
+    return a.p ? block_grad_kernel<T, kVectors, true, kOneGate>(words) : block_grad_kernel<T, kVectors, false, kOneGate>(words);
+  if (gate == kGateRow)
+    return a.p ? block_grad_kernel<T, kVectors, true, kGateRow>(words) : block_grad_kernel<T, kVectors, false, kGateRow>(words);
+  return a.p ? block_grad_kernel<T, kVectors, true, kGateEach>(words) : block_grad_kernel<T, kVectors, false, kGateEach>(words);
+}
+
+template <typename T>
+int launch_backward(const BlockGradArgs& a, const BlockGradPlan& plan, const DeviceInfo* dev, cudaStream_t stream,
+                    unsigned flags) {
+  const char* what = "gated_add_rms_norm_backward";
+  int st = HPRN_OK;
+  if (plan.words > 0) {
+    const auto fn = plan.vectors ? block_grad_kernel<T, true>(a, plan.words) : block_grad_kernel<T, false>(a, plan.words);
+    if ((st = allow_smem(dev, reinterpret_cast<const void*>(fn), kBlockSmem, what)) != HPRN_OK) return st;
+    st = launch_rows_smem(fn, dim3(static_cast<unsigned>(a.ctas)),
+                          dim3(static_cast<unsigned>(a.row_threads * a.row_groups + 32)), plan.smem, stream, flags, what, a);
+    if (st != HPRN_OK) return st;
+  } else if (a.rows > 0) {
+    st = launch_rows(block_grad_stats<T>, dim3(static_cast<unsigned>(a.rows)), dim3(256), stream, flags, what, a);
+    if (st != HPRN_OK) return st;
+    const int64_t parts = (a.gate_row && !a.gate_each ? a.gates : 1) * a.parts;
+    st = launch_rows(block_grad_columns<T>,
+                     dim3(static_cast<unsigned>((a.hidden + 255) / 256), static_cast<unsigned>(parts < 65535 ? parts : 65535)),
+                     dim3(256), stream, flags, what, a);
+    if (st != HPRN_OK) return st;
+  }
+  if (a.rows > 0 && a.gate_sums) {
+    st = launch_rows(block_grad_gates<T>, dim3(static_cast<unsigned>(a.gates < 65535 ? a.gates : 65535)), dim3(256),
+                     stream, flags, what, a);
+    if (st != HPRN_OK) return st;
+  }
+  return launch_rows(plan.words > 0 ? block_grad_runs<T> : block_grad_join<T>,
+                     dim3(static_cast<unsigned>((a.hidden + 31) / 32)), dim3(256), stream, flags, what, a);
+}
+
+}  // namespace
+}  // namespace hprn
+
+extern "C" {
+
+int hprn_gated_add_rms_norm_backward(
+    void* grad_input, void* grad_residual, void* grad_post_weight, void* grad_weight, void* grad_gate,
+    const void* grad_out, const void* grad_residual_out, const void* input, const void* residual_out,
+    const void* post_weight, const void* weight, const void* gate, int64_t rows, int64_t hidden,
+    int64_t rows_per_gate, int64_t gate_width, int64_t grad_input_row_stride, int64_t grad_residual_row_stride,
+    int64_t grad_gate_row_stride, int64_t grad_out_row_stride, int64_t grad_residual_out_row_stride,
+    int64_t input_row_stride, int64_t residual_out_row_stride, int64_t gate_row_stride, double residual_scale,
+    double eps, int dtype, void* workspace, int64_t* workspace_bytes, void* stream, unsigned flags) {
+  using namespace hprn;
+  if (flags & ~static_cast<unsigned>(HPRN_LAUNCH_PDL | HPRN_WORKSPACE_QUERY))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "unknown launch flags");
+  int st = check_block_norm(rows, hidden, rows_per_gate, gate_width, gate != nullptr, dtype);
+  if (st != HPRN_OK) return st;
+  if (!workspace_bytes) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace_bytes pointer required");
+  const int64_t gates = gate ? rows / rows_per_gate : 1;
+  if ((rows > 1 && (grad_input_row_stride < hidden || grad_residual_row_stride < hidden ||
+                    grad_out_row_stride < hidden || (grad_residual_out && grad_residual_out_row_stride < hidden) ||
+                    input_row_stride < hidden || residual_out_row_stride < hidden)) ||
+      (gate && gates > 1 && (gate_row_stride < gate_width || grad_gate_row_stride < gate_width)))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  BlockGradArgs a{};
+  a.dx = static_cast<uint16_t*>(grad_input), a.dr = static_cast<uint16_t*>(grad_residual);
+  a.dp = static_cast<uint16_t*>(grad_post_weight), a.dw = static_cast<uint16_t*>(grad_weight);
+  a.dg = static_cast<uint16_t*>(grad_gate);
+  a.d = static_cast<const uint16_t*>(grad_out), a.e = static_cast<const uint16_t*>(grad_residual_out);
+  a.x = static_cast<const uint16_t*>(input), a.t = static_cast<const uint16_t*>(residual_out);
+  a.p = static_cast<const uint16_t*>(post_weight), a.w = static_cast<const uint16_t*>(weight);
+  a.g = static_cast<const uint16_t*>(gate);
+  a.dx_stride = grad_input_row_stride, a.dr_stride = grad_residual_row_stride, a.dg_stride = grad_gate_row_stride;
+  a.d_stride = grad_out_row_stride, a.e_stride = grad_residual_out_row_stride, a.x_stride = input_row_stride;
+  a.t_stride = residual_out_row_stride, a.g_stride = gate_row_stride;
+  a.rows = rows, a.hidden = hidden;
+  a.rows_per_gate = gate ? rows_per_gate : 1, a.gates = gates;
+  // (With hidden 1 a gate of one value is a row of one.)
+  a.gate_row = gate && gate_width == hidden, a.gate_each = a.gate_row && rows_per_gate == 1;
+  a.scale = static_cast<float>(residual_scale), a.eps = static_cast<float>(eps);
+  const bool shared_row = a.gate_row && !a.gate_each;
+  const int64_t share = shared_row ? rows_per_gate : rows;
+  a.parts = shared_row ? (64 + gates - 1) / (gates > 0 ? gates : 1) : 64;
+  if (a.parts > share) a.parts = share > 0 ? share : 1;
+  a.part_rows = (share + a.parts - 1) / a.parts;
+  a.parts = a.part_rows > 0 ? (share + a.part_rows - 1) / a.part_rows : 0;
+  const BlockGradPlan plan = plan_block_grad(a);
+  Workspace ws(workspace, *workspace_bytes);
+  a.stats = ws.take<float4>(plan.words > 0 ? 0 : rows);
+  a.gate_sums = ws.take<float>(gate && !a.gate_row ? rows : 0);
+  if (!gate || a.gate_row) a.gate_sums = nullptr;
+  a.parts_ld = round_up(hidden, 8);
+  // A run and a gate it meets make one row of sums: each step to the next of them
+  // goes on by a run, a gate or both, so that run + gate tells them apart.
+  const int64_t parts = (shared_row ? gates : 1) * a.parts;
+  a.dw_parts = ws.take<float>((plan.words > 0 ? a.ctas : parts) * a.parts_ld);
+  a.m_parts = ws.take<float>((plan.words > 0 ? a.ctas + (shared_row ? gates : 0) : parts) * a.parts_ld);
+  if (flags & HPRN_WORKSPACE_QUERY) {
+    *workspace_bytes = ws.needed();
+    return ok();
+  }
+  if (hidden == 0) return ok();
+  if (!grad_weight || !weight || (post_weight && !grad_post_weight) ||
+      (rows > 0 && (!grad_input || !grad_residual || !grad_out || !input || !residual_out || (gate && !grad_gate))))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!post_weight) a.dp = nullptr;
+  for (const void* p : {static_cast<const void*>(grad_input), static_cast<const void*>(grad_residual),
+                        static_cast<const void*>(grad_post_weight), static_cast<const void*>(grad_weight),
+                        static_cast<const void*>(grad_gate), grad_out, grad_residual_out, input, residual_out,
+                        post_weight, weight, gate})
+    if (!aligned(p, 2)) return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");
+  const Extent outs[] = {extent16(grad_input, rows, hidden, grad_input_row_stride),
+                         extent16(grad_residual, rows, hidden, grad_residual_row_stride),
+                         extent16(a.dp, 1, hidden, hidden), extent16(grad_weight, 1, hidden, hidden),
+                         extent16(gate ? grad_gate : nullptr, gates, gate_width, grad_gate_row_stride)};
+  const Extent ins[] = {extent16(grad_out, rows, hidden, grad_out_row_stride),
+                        extent16(grad_residual_out, rows, hidden, grad_residual_out_row_stride),
+                        extent16(input, rows, hidden, input_row_stride),
+                        extent16(residual_out, rows, hidden, residual_out_row_stride),
+                        extent16(post_weight, 1, hidden, hidden), extent16(weight, 1, hidden, hidden),
+                        extent16(gate, gates, gate_width, gate_row_stride)};
+  if (!disjoint(outs, ins)) return fail(HPRN_ERR_INVALID_ARGUMENT, "outputs must not overlap other tensors");
+  if (!ws.fits()) return fail(HPRN_ERR_INVALID_ARGUMENT, "workspace too small");
+  const DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != HPRN_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if ((st = waits_of(dev, &a.waits, "gated_add_rms_norm_backward")) != HPRN_OK) return st;
+  return dtype == HPRN_DTYPE_BF16 ? launch_backward<__nv_bfloat16>(a, plan, dev, cs, flags)
+                                  : launch_backward<__half>(a, plan, dev, cs, flags);
+}
+
+}  // extern "C"
