@@ -131,7 +131,7 @@ enum GateKind { kOneGate, kGateRow, kGateEach };
 template <typename T, int W, bool kVectors, bool kPost, int kGate>
 __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGradArgs a) {
   constexpr int kVecs = W / 4;
-  constexpr bool kHold = W <= 12;
+  constexpr bool kHold = W <= 12, kKeep = kHold && kVectors;
   static_assert(kHold || kVectors, "words of unaligned rows are read by two threads");
   extern __shared__ __align__(128) unsigned char row_mem[];
   __shared__ __align__(8) uint64_t full[kBlockSlots], empty[kBlockSlots];
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
 #pragma unroll
   for (int k = 0; k < W; ++k) acc_w[k] = acc_m[k] = make_float2(0.f, 0.f);
   // Row `which` of w, p and a shared gate row into shared memory, by all threads.
-  const int gate_place = post ? 2 : 1;
+  constexpr int gate_place = kKeep || post ? 2 : 1;
   auto stage = [&](int which, const uint16_t* p) {
     uint32_t* to = reinterpret_cast<uint32_t*>(row_mem) + which * (row_bytes / 4);
     for (int j = tid; j < nvec * 4; j += workers) {
@@ -340,7 +340,13 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
       to[j] = lo | hi << 16;
     }
   };
+  uint32_t held[kKeep ? 3 : 1][kKeep ? W : 1];
   auto weight = [&](uint32_t (&w)[4], int which, const uint16_t* p, int k) {
+    if constexpr (kKeep) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = held[which][4 * k + e];
+      return;
+    }
     if (!a.staged) return load_weight(w, p, k);
     const uint32_t at = staged + which * row_bytes;
     if constexpr (kVectors) {
@@ -350,7 +356,22 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
       for (int e = 0; e < 4; ++e) w[e] = word_at(k, e) < words ? shared_word(at + word_at(k, e) * 4) : 0;
     }
   };
-  if (a.staged) {
+  auto keep_weight = [&](int which, const uint16_t* p) {
+    if constexpr (kKeep) {
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        if (!inside(k)) break;
+        uint32_t w[4];
+        load_weight(w, p, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) held[which][4 * k + e] = w[e];
+      }
+    }
+  };
+  if constexpr (kKeep) {
+    keep_weight(0, a.w);
+    if constexpr (post) keep_weight(1, a.p);
+  } else if (a.staged) {
     stage(0, a.w);
     if (post) stage(1, a.p);
     if (!shared_row) team_barrier(15, workers);
@@ -426,7 +447,9 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
   for (int i0 = begin; i0 < end; i0 = segment_end(i0)) {
     const int last = segment_end(i0);
     const uint16_t* gate_row = shared_row ? a.g + i0 / rows_per_gate * a.g_stride : nullptr;
-    if (a.staged && shared_row) {
+    if constexpr (kKeep && shared_row) {
+      keep_weight(2, gate_row);
+    } else if (a.staged && shared_row) {
       if (i0 > begin) team_barrier(15, workers);  // every group is done with the last one
       stage(gate_place, gate_row);
       team_barrier(15, workers);
@@ -578,34 +601,38 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
 }
 
 // The weights' and a shared gate row's gradients from block_grad_rows' sums: 32
-// columns a CTA.  Its 8 warps share out the CTAs' sums; where rows of the gate
+// columns a CTA.  Its 16 warps share out the CTAs' sums; where rows of the gate
 // are few they share out each one's sums as well, else they take gates in turn.
+constexpr int kRunWarps = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(256) block_grad_runs(BlockGradArgs a) {
-  __shared__ float sums[2][8][32];
+__global__ void __launch_bounds__(32 * kRunWarps) block_grad_runs(BlockGradArgs a) {
+  __shared__ float sums[2][kRunWarps][32];
   pdl_wait();
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + tx;
   const bool shared_row = a.gate_row && !a.gate_each, in = j < a.hidden;
+  const int ctas = static_cast<int>(a.ctas);
   float sw = 0.f, sp = 0.f;
   if (in) {
-#pragma unroll 8
-    for (int64_t c = ty; c < a.ctas; c += 8) sw += a.dw_parts[c * a.parts_ld + j];
+#pragma unroll 10
+    for (int c = ty; c < ctas; c += kRunWarps) sw += a.dw_parts[c * a.parts_ld + j];
   }
   if (!shared_row) {
     if (in) {
-#pragma unroll 8
-      for (int64_t c = ty; c < a.ctas; c += 8) sp += a.m_parts[c * a.parts_ld + j];
+#pragma unroll 10
+      for (int c = ty; c < ctas; c += kRunWarps) sp += a.m_parts[c * a.parts_ld + j];
     }
   } else {
     const float p = in && a.p ? unpack1<T>(a.p[j]) : 1.f;
-    const bool together = a.gates < 8;
-    for (int64_t k = together ? 0 : ty; k < a.gates; k += together ? 1 : 8) {
-      const int64_t first = run_of(a, k * a.rows_per_gate), last = run_of(a, (k + 1) * a.rows_per_gate - 1);
+    const bool together = a.gates <= 2;
+    for (int64_t k = together ? 0 : ty; k < a.gates; k += together ? 1 : kRunWarps) {
+      const int first = static_cast<int>(run_of(a, k * a.rows_per_gate));
+      const int last = static_cast<int>(run_of(a, (k + 1) * a.rows_per_gate - 1));
       float sm = 0.f;
       if (in) {
-#pragma unroll 4
-        for (int64_t c = first + (together ? ty : 0); c <= last; c += together ? 8 : 1)
+#pragma unroll 10
+        for (int c = first + (together ? ty : 0); c <= last; c += together ? kRunWarps : 1)
           sm += a.m_parts[(c + k) * a.parts_ld + j];
       }
       if (together) {
@@ -613,7 +640,8 @@ __global__ void __launch_bounds__(256) block_grad_runs(BlockGradArgs a) {
         sums[0][ty][tx] = sm;
         __syncthreads();
         if (ty > 0) continue;
-        for (int q = 1; q < 8; ++q) sm += sums[0][q][tx];
+#pragma unroll
+        for (int q = 1; q < kRunWarps; ++q) sm += sums[0][q][tx];
       }
       if (!in) continue;
       sp = fmaf(unpack1<T>(a.g[k * a.g_stride + j]), sm, sp);
@@ -625,7 +653,7 @@ __global__ void __launch_bounds__(256) block_grad_runs(BlockGradArgs a) {
   __syncthreads();
   if (ty > 0 || !in) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) sw += sums[0][k][tx], sp += sums[1][k][tx];
+  for (int k = 1; k < kRunWarps; ++k) sw += sums[0][k][tx], sp += sums[1][k][tx];
   a.dw[j] = pack1<T>(sw);
   if (a.dp) a.dp[j] = pack1<T>(sp);
 }
@@ -795,7 +823,7 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
   const int64_t nvec = (a.hidden + 7) / 8, pairs = (a.hidden + 1) / 2;
   const int64_t slot = (nvec * 16 + (plan.vectors ? 0 : 16)) * a.tensors;
   const bool segments = a.gate_row && !a.gate_each && a.gates > 1;
-  const int64_t weights = 1 + (a.p != nullptr) + (a.gate_row && !a.gate_each);
+  const int64_t staged_rows = 1 + (a.p != nullptr) + (a.gate_row && !a.gate_each);
   int best = 0;
   for (int words : {4, 8, 12, 24}) {
     if (words > 12 && !plan.vectors) break;
@@ -807,9 +835,10 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
     if (groups > a.rows) groups = a.rows;
     auto join_bytes = [&] { return groups > 1 ? words * threads * groups * 8 : 0; };
     auto ring_bytes = [&](int64_t slots) { return slots * groups * slot; };
+    const int64_t weights = plan.vectors && words <= 12 ? 0 : staged_rows;
     int64_t before = weights * nvec * 16;  // the ring
     while (groups > 1 && before + ring_bytes(2) + (segments ? join_bytes() : 0) > kBlockSmem) --groups;
-    const bool staged = before + ring_bytes(2) + (segments ? join_bytes() : 0) <= kBlockSmem;
+    const bool staged = weights > 0 && before + ring_bytes(2) + (segments ? join_bytes() : 0) <= kBlockSmem;
     if (!staged) before = 0;
     int64_t slots = (kBlockSmem - before - (segments ? join_bytes() : 0)) / (groups * slot);
     if (slots > kBlockSlots) slots = kBlockSlots;
@@ -874,8 +903,9 @@ int launch_backward(const BlockGradArgs& a, const BlockGradPlan& plan, const Dev
                      stream, flags, what, a);
     if (st != HPRN_OK) return st;
   }
-  return launch_rows(plan.words > 0 ? block_grad_runs<T> : block_grad_join<T>,
-                     dim3(static_cast<unsigned>((a.hidden + 31) / 32)), dim3(256), stream, flags, what, a);
+  const dim3 columns(static_cast<unsigned>((a.hidden + 31) / 32));
+  return plan.words > 0 ? launch_rows(block_grad_runs<T>, columns, dim3(32 * kRunWarps), stream, flags, what, a)
+                        : launch_rows(block_grad_join<T>, columns, dim3(256), stream, flags, what, a);
 }
 
 }  // namespace
