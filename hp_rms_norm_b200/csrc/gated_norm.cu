@@ -37,74 +37,95 @@ struct BlockNormArgs {
 };
 
 // Rows held in registers: a CTA works on blockDim / row_threads rows, each
-// thread on VPT vectors of VEC bytes.
-template <typename T, int VEC, int VPT>
+// thread on VPT vectors of VEC bytes.  kLoose: rows that start anywhere (rows.cuh).
+// kGateRow: the gate is a row of values; else one value, or none.
+template <typename T, int VEC, int VPT, bool kLoose, bool kPost, bool kGateRow>
 __global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) block_norm_rows(BlockNormArgs a) {
-  constexpr int P = Pairs<VEC>::kCount;
+  static_assert(!kLoose || VEC == 16, "loose rows are read in vectors of eight elements");
+  constexpr int P = VEC / 4;
   __shared__ float part[2][32];
   const int in = threadIdx.x % a.row_threads, group = threadIdx.x / a.row_threads;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.row_threads) + group;
   const int warps = a.row_threads / 32, first_warp = group * warps;
   const bool valid = row < a.rows;
-  auto inside = [&](int k) { return valid && in + k * a.row_threads < a.nvec; };
-  auto at = [&](int k) { return static_cast<int64_t>(in + k * a.row_threads) * Vec<VEC>::kElems; };
+  // (Of a loose row, what a warp has some of: its lanes store together.)
+  const int from = kLoose ? in & ~31 : in;
+  auto inside = [&](int k) { return valid && from + k * a.row_threads < a.nvec; };
+  auto vector = [&](int k) { return in + k * a.row_threads; };
   const uint64_t once = policy_evict_first(), keep = policy_evict_last();
+  auto load = [&](const uint16_t* base, int64_t stride, int k) {
+    Vec<VEC> v;
+    if constexpr (kLoose) load_loose(v.w, loose_row(base, row, a.rows, stride, a.hidden), vector(k));
+    else v = ld_stream<VEC>(base + row * stride + vector(k) * Vec<VEC>::kElems, once);
+    return v;
+  };
+  auto weight = [&](const uint16_t* p, int k) {
+    Vec<VEC> v;
+    if constexpr (kLoose) load_loose(v.w, LooseRow{p, a.hidden, false, false}, vector(k));
+    else v = ld_weight<VEC>(p + vector(k) * Vec<VEC>::kElems, keep);
+    return v;
+  };
+  auto store = [&](uint16_t* base, int64_t stride, int k, const Vec<VEC>& v) {
+    if constexpr (kLoose) store_loose(base + row * stride, a.hidden, vector(k), v.w);
+    else st_global<VEC>(base + row * stride + vector(k) * Vec<VEC>::kElems, v);
+  };
   pdl_wait();
 
   Vec<VEC> x[VPT], r[VPT];
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
-    if (inside(k)) x[k] = ld_stream<VEC>(a.x + row * a.x_stride + at(k), once);
+    if (inside(k)) x[k] = load(a.x, a.x_stride, k);
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
-    if (inside(k)) r[k] = ld_stream<VEC>(a.r + row * a.r_stride + at(k), once);
+    if (inside(k)) r[k] = load(a.r, a.r_stride, k);
   const uint16_t* gate = a.g && valid ? a.g + (static_cast<uint32_t>(row) / a.rows_per_gate) * a.g_stride : nullptr;
-  float gate_one = 1.f;
-  if (gate && !a.gate_row) gate_one = unpack1<T>(gate[0]);
   float inv_x = 1.f;
-  if (a.p) {
+  if constexpr (kPost) {
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       if (!inside(k)) break;
 #pragma unroll
-      for (int e = 0; e < P; ++e) {
-        const float2 v = pair_of<T, VEC>(x[k], e);
-        s = __ffma2_rn(v, v, s);
-      }
+      for (int e = 0; e < P; ++e) s = fma_pair<T>(x[k].w[e], x[k].w[e], s);
     }
     inv_x = rsqrtf(row_sum(s.x + s.y, part[0], warps, first_warp) * a.inv_hidden + a.eps);
   }
+  if constexpr (!kGateRow) {
+    if (gate) inv_x *= unpack1<T>(gate[0]);
+  }
+  const float2 by = make_float2(inv_x, inv_x), scale = make_float2(a.scale, a.scale);
   float2 t[VPT][P], s = make_float2(0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     if (!inside(k)) break;
     Vec<VEC> p, g, o;
-    if (a.p) p = ld_weight<VEC>(a.p + at(k), keep);
-    if (gate && a.gate_row) g = ld_weight<VEC>(gate + at(k), keep);
+    if constexpr (kPost) p = weight(a.p, k);
+    if constexpr (kGateRow) g = weight(gate, k);
 #pragma unroll
     for (int e = 0; e < P; ++e) {
-      float2 y = pair_of<T, VEC>(x[k], e);
-      if (a.p) y = __fmul2_rn(__fmul2_rn(y, make_float2(inv_x, inv_x)), pair_of<T, VEC>(p, e));
-      if (gate && a.gate_row) y = __fmul2_rn(y, pair_of<T, VEC>(g, e));
-      else y = __fmul2_rn(y, make_float2(gate_one, gate_one));
-      t[k][e] = __ffma2_rn(pair_of<T, VEC>(r[k], e), make_float2(a.scale, a.scale), y);
+      float2 y = __fmul2_rn(unpack2<T>(x[k].w[e]), by);
+      if constexpr (kPost && kGateRow) y = __fmul2_rn(y, mul_pair<T>(p.w[e], g.w[e]));
+      else if constexpr (kPost) y = __fmul2_rn(y, unpack2<T>(p.w[e]));
+      else if constexpr (kGateRow) y = __fmul2_rn(y, unpack2<T>(g.w[e]));
+      t[k][e] = __ffma2_rn(unpack2<T>(r[k].w[e]), scale, y);
       s = __ffma2_rn(t[k][e], t[k][e], s);
-      set_pair<T, VEC>(o, e, t[k][e]);
+      o.w[e] = pack2<T>(t[k][e].x, t[k][e].y);
     }
-    st_global<VEC>(a.t + row * a.t_stride + at(k), o);
+    store(a.t, a.t_stride, k, o);
   }
   const float inv_t = rsqrtf(row_sum(s.x + s.y, part[1], warps, first_warp) * a.inv_hidden + a.eps);
   pdl_trigger();
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     if (!inside(k)) break;
-    const Vec<VEC> w = ld_weight<VEC>(a.w + at(k), keep);
+    const Vec<VEC> w = weight(a.w, k);
     Vec<VEC> o;
 #pragma unroll
-    for (int e = 0; e < P; ++e)
-      set_pair<T, VEC>(o, e, __fmul2_rn(__fmul2_rn(t[k][e], make_float2(inv_t, inv_t)), pair_of<T, VEC>(w, e)));
-    st_global<VEC>(a.out + row * a.out_stride + at(k), o);
+    for (int e = 0; e < P; ++e) {
+      const float2 y = __fmul2_rn(__fmul2_rn(t[k][e], make_float2(inv_t, inv_t)), unpack2<T>(w.w[e]));
+      o.w[e] = pack2<T>(y.x, y.y);
+    }
+    store(a.out, a.out_stride, k, o);
   }
 }
 
@@ -174,48 +195,36 @@ __global__ void __launch_bounds__(1024) block_norm_long_rows(BlockNormArgs a) {
 
 namespace {
 
-// The widest vectors that every row of every tensor is made of.
+// The widest vectors that every row of every tensor is made of: 32 or 16 bytes, or 0.
 int vector_bytes(int64_t hidden, std::initializer_list<const void*> rows, std::initializer_list<int64_t> strides) {
-  for (int vec : {32, 16, 4}) {
+  for (int vec : {32, 16}) {
     bool fits = hidden * 2 % vec == 0;
     for (const void* p : rows) fits = fits && aligned(p, vec);
     for (int64_t s : strides) fits = fits && s * 2 % vec == 0;
     if (fits) return vec;
   }
-  return 2;
+  return 0;
 }
 
 using RowsKernel = void (*)(BlockNormArgs);
 
-template <typename T>
+template <typename T, bool kPost, bool kGateRow>
 RowsKernel rows_kernel(int vec, int vpt) {
-  switch (vec * 100 + vpt) {
-    case 3201: return block_norm_rows<T, 32, 1>;
-    case 3202: return block_norm_rows<T, 32, 2>;
-    case 1601: return block_norm_rows<T, 16, 1>;
-    case 1602: return block_norm_rows<T, 16, 2>;
-    case 401: return block_norm_rows<T, 4, 1>;
-    case 402: return block_norm_rows<T, 4, 2>;
-    case 404: return block_norm_rows<T, 4, 4>;
-    case 408: return block_norm_rows<T, 4, 8>;
-    case 201: return block_norm_rows<T, 2, 1>;
-    case 202: return block_norm_rows<T, 2, 2>;
-    case 204: return block_norm_rows<T, 2, 4>;
-    case 208: return block_norm_rows<T, 2, 8>;
-    case 216: return block_norm_rows<T, 2, 16>;
-    default: return nullptr;
-  }
+  if (vec == 32) return vpt == 1 ? block_norm_rows<T, 32, 1, false, kPost, kGateRow> : nullptr;
+  if (vec == 16) return vpt == 1 ? block_norm_rows<T, 16, 1, false, kPost, kGateRow> : block_norm_rows<T, 16, 2, false, kPost, kGateRow>;
+  return vpt == 1 ? block_norm_rows<T, 16, 1, true, kPost, kGateRow> : block_norm_rows<T, 16, 2, true, kPost, kGateRow>;
 }
 
 template <typename T>
 int launch_forward(BlockNormArgs& a, int vec, cudaStream_t stream, unsigned flags) {
   const char* what = "gated_add_rms_norm";
-  a.nvec = static_cast<int32_t>(static_cast<int64_t>(a.hidden) * 2 / vec);
-  for (int vpt = 1; vpt <= 16; vpt *= 2) {
-    const RowsKernel fn = rows_kernel<T>(vec, vpt);
+  const int64_t elems = vec > 0 ? vec / 2 : 8;
+  a.nvec = static_cast<int32_t>((a.hidden + elems - 1) / elems);
+  for (int vpt = 1; vpt <= 2; ++vpt) {
+    const RowsKernel fn = a.p ? (a.gate_row ? rows_kernel<T, true, true>(vec, vpt) : rows_kernel<T, true, false>(vec, vpt))
+                              : (a.gate_row ? rows_kernel<T, false, true>(vec, vpt) : rows_kernel<T, false, false>(vec, vpt));
     const int64_t threads = round_up((a.nvec + vpt - 1) / vpt, 32);
-    // More vectors a thread leave registers for 512 threads only.
-    if (!fn || threads > (vpt * vec > 32 ? 512 : 1024)) continue;
+    if (!fn || threads > 1024) continue;
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
     return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),

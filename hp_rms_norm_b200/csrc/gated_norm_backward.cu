@@ -62,10 +62,10 @@ struct BlockGradArgs {
 // share up to 8 words a thread.  Where a run reaches into another gate's rows, the
 // sums for the gate are written out and started anew.
 //   kVectors: every row of every tensor starts on a 16-byte boundary and hidden is
-// a multiple of 8; threads take vectors of eight elements.  Else a row is copied
-// with the 16-byte granules it lies in (elements in granules that reach out of the
-// tensor one by one), and threads take single words, neighbouring threads
-// neighbouring ones, put together from two where the row starts on an odd element.
+// a multiple of 8.  Else a row is copied with the 16-byte granules it lies in
+// (elements in granules that reach out of the tensor one by one), and a vector put
+// together from two (12 x 257 rows of 1001, fp16: WORDS_US us where threads took
+// single words instead).
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies in
 // flight, and says so (report_give_up).
@@ -131,8 +131,8 @@ enum GateKind { kOneGate, kGateRow, kGateEach };
 template <typename T, int W, bool kVectors, bool kPost, int kGate>
 __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGradArgs a) {
   constexpr int kVecs = W / 4;
-  constexpr bool kHold = W <= 12, kKeep = kHold && kVectors;
-  static_assert(kHold || kVectors, "words of unaligned rows are read by two threads");
+  constexpr bool kHold = W <= 12, kKeep = kHold;
+  static_assert(kHold || kVectors, "vectors of loose rows are read by two threads");
   extern __shared__ __align__(128) unsigned char row_mem[];
   __shared__ __align__(8) uint64_t full[kBlockSlots], empty[kBlockSlots];
   __shared__ float part[2][4][32];
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
   const bool copier = tid >= workers;
   const int group = copier ? 0 : tid / row_threads, in = copier ? 0 : tid - group * row_threads;
   const int warps = row_threads / 32, barrier = 1 + group;
-  const int hidden = static_cast<int>(a.hidden), nvec = (hidden + 7) / 8, words = (hidden + 1) / 2;
+  const int hidden = static_cast<int>(a.hidden), nvec = (hidden + 7) / 8;
   // A buffer: `groups` rows of each tensor in turn, `pitch` bytes a row.
   const uint32_t row_bytes = static_cast<uint32_t>(nvec) * 16, pitch = row_bytes + (kVectors ? 0 : 16);
   const uint32_t tensor_bytes = pitch * groups, slot_bytes = tensor_bytes * a.tensors;
@@ -252,12 +252,9 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
   }
   pdl_trigger();
 
-  // Words 4 k to 4 k + 3 of this thread's: one vector, or one word every row_threads.
-  // (Of words, what the whole warp has some of: lanes past the end work on zeros.)
-  auto inside = [&](int k) {
-    return kVectors ? in + k * row_threads < nvec : in - lane + 4 * k * row_threads < words;
-  };
-  auto word_at = [&](int k, int e) { return in + (4 * k + e) * row_threads; };
+  // This thread's vector k.  (Of loose rows, what the whole warp has some of: lanes
+  // past the end work on zeros.)
+  auto inside = [&](int k) { return (kVectors ? in : in - lane) + k * row_threads < nvec; };
   const uint64_t keep = policy_evict_last();
   // Of a row in memory (a weight, or a gate row).
   auto load_weight = [&](uint32_t (&w)[4], const uint16_t* p, int k) {
@@ -266,13 +263,7 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = q.w[e];
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 2 * word_at(k, e);
-        const uint32_t lo = j < hidden ? ld_weight<2>(p + j, keep).h : 0;
-        const uint32_t hi = j + 1 < hidden ? ld_weight<2>(p + j + 1, keep).h : 0;
-        w[e] = lo | hi << 16;
-      }
+      load_loose(w, LooseRow{p, hidden, false, false}, in + k * row_threads);
     }
   };
   // Of a row in shared memory that starts at `at`.
@@ -280,49 +271,24 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
     if constexpr (kVectors) {
       shared_words(w, at + (in + k * row_threads) * 16);
     } else {
-      // All loads first, past the row's end the last word again.  (The word behind
-      // the last one lies in the buffer's spare granule.)
-      const uint32_t from = at & ~3u;
-      uint32_t next[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = shared_word(from + min(word_at(k, e), words - 1) * 4);
-      if (at & 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) next[e] = shared_word(from + min(word_at(k, e), words - 1) * 4 + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(w[e], next[e], 16);
+      const int v = in + k * row_threads, o = static_cast<int>(at & 15) / 2;
+      if (v >= nvec) {
+        w[0] = w[1] = w[2] = w[3] = 0;
+        return;
       }
+      uint32_t lo[4], hi[4] = {};
+      shared_words(lo, (at & ~15u) + v * 16);
+      if (o > 0) shared_words(hi, (at & ~15u) + v * 16 + 16);
+      uint32_t both[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      shift_down(both, o);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (2 * word_at(k, e) + 1 == hidden) w[e] &= 0xffffu;
-        if (word_at(k, e) >= words) w[e] = 0;
-      }
+      for (int e = 0; e < 4; ++e) w[e] = both[e];
+      clear_tail(w, v, hidden);
     }
   };
   auto store_row = [&](uint16_t* row, int k, const uint32_t (&w)[4]) {
-    if constexpr (kVectors) {
-      *reinterpret_cast<uint4*>(row + (in + k * row_threads) * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = word_at(k, e);
-        uint16_t* q = row + 2 * j;
-        const bool second = 2 * j + 1 < hidden;
-        if ((reinterpret_cast<uintptr_t>(row) & 2) == 0) {
-          if (j >= words) continue;
-          if (second) *reinterpret_cast<uint32_t*>(q) = w[e];
-          else q[0] = static_cast<uint16_t>(w[e]);
-          continue;
-        }
-        // An element off the words of memory: a lane stores the word of its first
-        // element and the last one of the lane before.
-        const uint32_t before = __shfl_up_sync(~0u, w[e], 1);
-        if (j >= words) continue;
-        if (lane > 0) *reinterpret_cast<uint32_t*>(q - 1) = before >> 16 | w[e] << 16;
-        else q[0] = static_cast<uint16_t>(w[e]);
-        if (second && (lane == 31 || j + 1 >= words)) q[1] = static_cast<uint16_t>(w[e] >> 16);
-      }
-    }
+    if constexpr (kVectors) *reinterpret_cast<uint4*>(row + (in + k * row_threads) * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    else store_loose(row, hidden, in + k * row_threads, w);
   };
 
   constexpr bool post = kPost;
@@ -348,13 +314,8 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
       return;
     }
     if (!a.staged) return load_weight(w, p, k);
-    const uint32_t at = staged + which * row_bytes;
-    if constexpr (kVectors) {
-      shared_words(w, at + (in + k * row_threads) * 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = word_at(k, e) < words ? shared_word(at + word_at(k, e) * 4) : 0;
-    }
+    if (in + k * row_threads < nvec) shared_words(w, staged + which * row_bytes + (in + k * row_threads) * 16);
+    else w[0] = w[1] = w[2] = w[3] = 0;
   };
   auto keep_weight = [&](int which, const uint16_t* p) {
     if constexpr (kKeep) {
@@ -397,19 +358,14 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       if (!inside(k)) break;
-      if constexpr (kVectors) {
-        Vec<32> q;
+      if (in + k * row_threads >= nvec) break;
+      Vec<32> q;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          q.w[2 * e] = __float_as_uint(acc[4 * k + e].x);
-          q.w[2 * e + 1] = __float_as_uint(acc[4 * k + e].y);
-        }
-        st_global<32>(out + (in + k * row_threads) * 8, q);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (word_at(k, e) < words) reinterpret_cast<float2*>(out)[word_at(k, e)] = acc[4 * k + e];
+      for (int e = 0; e < 4; ++e) {
+        q.w[2 * e] = __float_as_uint(acc[4 * k + e].x);
+        q.w[2 * e + 1] = __float_as_uint(acc[4 * k + e].y);
       }
+      st_global<32>(out + (in + k * row_threads) * 8, q);
     }
   };
 
@@ -820,14 +776,14 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
     a.dense = a.dense && a.src_stride[k] == a.hidden;
   }
   if (a.rows <= 0 || a.hidden <= 0 || a.hidden > 32768) return plan;
-  const int64_t nvec = (a.hidden + 7) / 8, pairs = (a.hidden + 1) / 2;
+  const int64_t nvec = (a.hidden + 7) / 8;
   const int64_t slot = (nvec * 16 + (plan.vectors ? 0 : 16)) * a.tensors;
   const bool segments = a.gate_row && !a.gate_each && a.gates > 1;
   const int64_t staged_rows = 1 + (a.p != nullptr) + (a.gate_row && !a.gate_each);
   int best = 0;
   for (int words : {4, 8, 12, 24}) {
     if (words > 12 && !plan.vectors) break;
-    const int64_t threads = round_up(plan.vectors ? (nvec + words / 4 - 1) / (words / 4) : (pairs + words - 1) / words, 32);
+    const int64_t threads = round_up((nvec + words / 4 - 1) / (words / 4), 32);
     const bool few = a.rows <= 4 * 148;
     if (threads > kBlockThreads || (words == 4 && threads > 128 && !few)) continue;
     int64_t groups = kBlockThreads / threads;
@@ -835,7 +791,7 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
     if (groups > a.rows) groups = a.rows;
     auto join_bytes = [&] { return groups > 1 ? words * threads * groups * 8 : 0; };
     auto ring_bytes = [&](int64_t slots) { return slots * groups * slot; };
-    const int64_t weights = plan.vectors && words <= 12 ? 0 : staged_rows;
+    const int64_t weights = words <= 12 ? 0 : staged_rows;
     int64_t before = weights * nvec * 16;  // the ring
     while (groups > 1 && before + ring_bytes(2) + (segments ? join_bytes() : 0) > kBlockSmem) --groups;
     const bool staged = weights > 0 && before + ring_bytes(2) + (segments ? join_bytes() : 0) <= kBlockSmem;

@@ -65,8 +65,6 @@ template <int VEC>
 __device__ __forceinline__ void store_codes(int8_t* q, const float2 (&y)[Pairs<VEC>::kCount], float inv) {
   if constexpr (VEC == 2) {
     *q = static_cast<int8_t>(codes_of(y[0], inv));
-  } else if constexpr (VEC == 4) {
-    *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(codes_of(y[0], inv));
   } else {
     Vec<VEC / 2> o;
 #pragma unroll
@@ -75,52 +73,96 @@ __device__ __forceinline__ void store_codes(int8_t* q, const float2 (&y)[Pairs<V
   }
 }
 
+// Codes 8 v to 8 v + 7 of a row of n bytes that starts anywhere, v neighbouring in
+// neighbouring lanes: whole words of eight inside a warp's span, as store_loose.
+__device__ __forceinline__ void store_codes_loose(int8_t* row, int n, int v, const float2 (&y)[4], float inv) {
+  const int o = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 7), lane = threadIdx.x % 32;
+  const uint64_t lo = codes_of(y[0], inv) | codes_of(y[1], inv) << 16, hi = codes_of(y[2], inv) | codes_of(y[3], inv) << 16;
+  const uint64_t own = lo | hi << 32, before = __shfl_up_sync(~0u, own, 1);
+  if (8 * v >= n) return;
+  const uint64_t word = o > 0 ? before >> (64 - 8 * o) | own << (8 * o) : own;
+  int8_t* q = row + 8 * v;
+  if ((lane > 0 || o == 0) && 8 * v - o + 8 <= n) {
+    *reinterpret_cast<uint64_t*>(q - o) = word;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e < 8 - o && 8 * v + e < n) q[e] = static_cast<int8_t>(own >> (8 * e));
+      if (lane > 0 && e < o) q[e - o] = static_cast<int8_t>(word >> (8 * e));
+    }
+  }
+  if (lane == 31 || 8 * (v + 1) >= n) {
+#pragma unroll
+    for (int e = 1; e < 8; ++e)
+      if (e >= 8 - o && 8 * v + e < n) q[e] = static_cast<int8_t>(own >> (8 * e));
+  }
+}
+
 // Rows held in registers, laid out over threads as in gated_norm.cu.
-template <typename T, int VEC, int VPT>
-__global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) quant_rows(QuantArgs a) {
-  constexpr int P = Pairs<VEC>::kCount;
+template <typename T, int VEC, int VPT, bool kLoose, bool kNorm>
+__global__ void __launch_bounds__(1024) quant_rows(QuantArgs a) {
+  static_assert(!kLoose || VEC == 16, "loose rows are read in vectors of eight elements");
+  constexpr int P = VEC / 4;
   __shared__ float part[2][32];
   const int in = threadIdx.x % a.row_threads, group = threadIdx.x / a.row_threads;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.row_threads) + group;
   const int warps = a.row_threads / 32, first_warp = group * warps;
   const bool valid = row < a.rows;
-  auto inside = [&](int k) { return valid && in + k * a.row_threads < a.nvec; };
-  auto at = [&](int k) { return static_cast<int64_t>(in + k * a.row_threads) * Vec<VEC>::kElems; };
+  const int from = kLoose ? in & ~31 : in;
+  auto inside = [&](int k) { return valid && from + k * a.row_threads < a.nvec; };
+  auto vector = [&](int k) { return in + k * a.row_threads; };
   const uint64_t once = policy_evict_first(), keep = policy_evict_last();
+  auto load = [&](const uint16_t* base, int64_t stride, int k) {
+    Vec<VEC> v;
+    if constexpr (kLoose) load_loose(v.w, loose_row(base, row, a.rows, stride, a.hidden), vector(k));
+    else v = ld_stream<VEC>(base + row * stride + vector(k) * Vec<VEC>::kElems, once);
+    return v;
+  };
   pdl_wait();
 
   Vec<VEC> x[VPT], r[VPT];
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
-    if (inside(k)) x[k] = ld_stream<VEC>(a.x + row * a.x_stride + at(k), once);
+    if (inside(k)) x[k] = load(a.x, a.x_stride, k);
   if (a.r) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
-      if (inside(k)) r[k] = ld_stream<VEC>(a.r + row * a.r_stride + at(k), once);
+      if (inside(k)) r[k] = load(a.r, a.r_stride, k);
   }
   float2 y[VPT][P], s = make_float2(0.f, 0.f);
   float most = 0.f;
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     if (!inside(k)) break;
-    Vec<VEC> o, w;
-    if (a.w) w = ld_weight<VEC>(a.w + at(k), keep);
+    Vec<VEC> w;
+    if constexpr (kNorm) {
+      if constexpr (kLoose) load_loose(w.w, LooseRow{a.w, a.hidden, false, false}, vector(k));
+      else w = ld_weight<VEC>(a.w + vector(k) * Vec<VEC>::kElems, keep);
+    }
+    if (a.r) {
+      Vec<VEC> o;
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        y[k][e] = __fadd2_rn(unpack2<T>(x[k].w[e]), unpack2<T>(r[k].w[e]));
+        o.w[e] = pack2<T>(y[k][e].x, y[k][e].y);
+      }
+      if constexpr (kLoose) store_loose(a.t + row * a.t_stride, a.hidden, vector(k), o.w);
+      else st_global<VEC>(a.t + row * a.t_stride + vector(k) * Vec<VEC>::kElems, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < P; ++e) y[k][e] = unpack2<T>(x[k].w[e]);
+    }
 #pragma unroll
     for (int e = 0; e < P; ++e) {
-      float2 v = pair_of<T, VEC>(x[k], e);
-      if (a.r) {
-        v = __fadd2_rn(v, pair_of<T, VEC>(r[k], e));
-        set_pair<T, VEC>(o, e, v);
+      if constexpr (kNorm) {
+        s = __ffma2_rn(y[k][e], y[k][e], s);
+        y[k][e] = __fmul2_rn(y[k][e], unpack2<T>(w.w[e]));
       }
-      s = __ffma2_rn(v, v, s);
-      if (a.w) v = __fmul2_rn(v, pair_of<T, VEC>(w, e));
-      y[k][e] = v;
-      most = amax_nan(most, v.x, v.y);
+      most = amax_nan(most, y[k][e].x, y[k][e].y);
     }
-    if (a.r) st_global<VEC>(a.t + row * a.t_stride + at(k), o);
   }
   float inv = 1.f;
-  if (a.w) inv = rsqrtf(row_sum(s.x + s.y, part[0], warps, first_warp) * a.inv_hidden + a.eps);
+  if constexpr (kNorm) inv = rsqrtf(row_sum(s.x + s.y, part[0], warps, first_warp) * a.inv_hidden + a.eps);
   // max |y inv| = max |y| inv, rounded once: rounding keeps the order.
   most = row_amax(most, part[1], warps, first_warp) * inv;
   pdl_trigger();
@@ -129,9 +171,13 @@ __global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) quant_rows(QuantA
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     if (!inside(k)) break;
+    if constexpr (kNorm) {
 #pragma unroll
-    for (int e = 0; e < P; ++e) y[k][e] = __fmul2_rn(y[k][e], make_float2(inv, inv));
-    store_codes<VEC>(a.q + row * a.q_stride + at(k), y[k], by);
+      for (int e = 0; e < P; ++e) y[k][e] = __fmul2_rn(y[k][e], make_float2(inv, inv));
+    }
+    int8_t* q = a.q + row * a.q_stride;
+    if constexpr (kLoose) store_codes_loose(q, a.hidden, vector(k), y[k], by);
+    else store_codes<VEC>(q + vector(k) * Vec<VEC>::kElems, y[k], by);
   }
 }
 
@@ -273,34 +319,22 @@ struct ScaledEpilogue {
 
 namespace {
 
-template <typename T>
+template <typename T, bool kNorm>
 void (*quant_kernel(int vec, int vpt))(QuantArgs) {
-  switch (vec * 100 + vpt) {
-    case 3201: return quant_rows<T, 32, 1>;
-    case 3202: return quant_rows<T, 32, 2>;
-    case 1601: return quant_rows<T, 16, 1>;
-    case 1602: return quant_rows<T, 16, 2>;
-    case 401: return quant_rows<T, 4, 1>;
-    case 402: return quant_rows<T, 4, 2>;
-    case 404: return quant_rows<T, 4, 4>;
-    case 408: return quant_rows<T, 4, 8>;
-    case 201: return quant_rows<T, 2, 1>;
-    case 202: return quant_rows<T, 2, 2>;
-    case 204: return quant_rows<T, 2, 4>;
-    case 208: return quant_rows<T, 2, 8>;
-    case 216: return quant_rows<T, 2, 16>;
-    default: return nullptr;
-  }
+  if (vec == 32) return vpt == 1 ? quant_rows<T, 32, 1, false, kNorm> : nullptr;
+  if (vec == 16) return vpt == 1 ? quant_rows<T, 16, 1, false, kNorm> : quant_rows<T, 16, 2, false, kNorm>;
+  return vpt == 1 ? quant_rows<T, 16, 1, true, kNorm> : quant_rows<T, 16, 2, true, kNorm>;
 }
 
 template <typename T>
 int launch_quant(QuantArgs& a, int vec, cudaStream_t stream, unsigned flags) {
   const char* what = "rms_norm_int8";
-  a.nvec = static_cast<int32_t>(static_cast<int64_t>(a.hidden) * 2 / vec);
-  for (int vpt = 1; vpt <= 16; vpt *= 2) {
-    const auto fn = quant_kernel<T>(vec, vpt);
+  const int64_t elems = vec > 0 ? vec / 2 : 8;
+  a.nvec = static_cast<int32_t>((a.hidden + elems - 1) / elems);
+  for (int vpt = 1; vpt <= 2; ++vpt) {
+    const auto fn = a.w ? quant_kernel<T, true>(vec, vpt) : quant_kernel<T, false>(vec, vpt);
     const int64_t threads = round_up((a.nvec + vpt - 1) / vpt, 32);
-    if (!fn || threads > (vpt * vec > 32 ? 512 : 1024)) continue;
+    if (!fn || threads > 1024) continue;
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
     return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),
@@ -360,8 +394,8 @@ int hprn_rms_norm_int8(int8_t* out, float* scales, void* residual_out, const voi
   a.r_stride = residual_row_stride;
   a.rows = static_cast<int32_t>(rows), a.hidden = static_cast<int32_t>(hidden);
   a.eps = static_cast<float>(eps), a.inv_hidden = 1.f / static_cast<float>(hidden);
-  int vec = 2;
-  for (int v : {32, 16, 4}) {
+  int vec = 0;  // rows that start anywhere
+  for (int v : {32, 16}) {
     auto fits = [&](const void* p, int64_t stride, int bytes) {
       return aligned(p, v * bytes / 2) && (rows <= 1 || !p || stride * bytes % (v * bytes / 2) == 0);
     };

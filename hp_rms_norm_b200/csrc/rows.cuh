@@ -1,5 +1,6 @@
 // What the row kernels of gated_norm.cu and int8.cu share: vectors of 16-bit
-// elements as pairs of floats, and sums over the threads that hold a row.
+// elements as pairs of floats, sums over the threads that hold a row, and rows that
+// start anywhere.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -50,6 +51,117 @@ __device__ __forceinline__ float row_sum(float v, float* part, int warps, int fi
   if (lane == 0) part[threadIdx.x / 32] = v;
   __syncthreads();
   return warp_total(lane < warps ? part[first_warp + lane] : 0.f);
+}
+
+// ---------------------------------------------------------------------------
+// Rows that start anywhere: vectors of eight elements by the 16-byte granules of
+// memory that they lie in, two loads and a shift instead of eight loads.
+
+// Elements o to o + 7 of the sixteen in w, into w[0..3]; o the same in a warp.
+__device__ __forceinline__ void shift_down(uint32_t (&w)[8], int o) {
+  if (o & 4) {
+#pragma unroll
+    for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+  }
+  if (o & 2) {
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+  }
+  if (o & 1) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+  }
+}
+
+__device__ __forceinline__ int granule_offset(const void* row) {
+  return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / 2;
+}
+
+// Zeros for the elements of vector v behind a row of n.
+__device__ __forceinline__ void clear_tail(uint32_t (&w)[4], int v, int n) {
+  const int left = n - 8 * v;
+  if (left >= 8) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = 2 * k >= left ? 0 : 2 * k + 1 >= left ? w[k] & 0xffffu : w[k];
+}
+
+// A row of n elements and whether the granules its ends lie in may be read whole.
+struct LooseRow {
+  const uint16_t* p;
+  int n;
+  bool low, high;
+};
+// Row i of `rows` with a stride between them: the granules reach into the rows
+// beside it, but not out of the tensor.
+__device__ __forceinline__ LooseRow loose_row(const uint16_t* base, int64_t i, int64_t rows, int64_t stride, int n) {
+  const uint16_t* p = base + i * stride;
+  return LooseRow{p, n, granule_offset(p) <= i * stride, (rows - 1 - i) * stride >= 8};
+}
+
+// Elements 8 v to 8 v + 7, zeros past the row's end.
+__device__ __forceinline__ void load_loose(uint32_t (&out)[4], const LooseRow& r, int v) {
+  const int o = granule_offset(r.p);
+  const uint4* g = reinterpret_cast<const uint4*>(r.p - o) + v;
+  // (What a granule behind the row's last whole one holds of the next row, or of
+  // nothing.)
+  const bool whole = (v > 0 || o == 0 || r.low) && (r.high || 8 * (v + (o > 0 ? 2 : 1)) - o <= r.n);
+  if (whole) {
+    const uint4 a = *g;
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
+    if (o > 0) {
+      if (8 * (v + 1) - o < r.n) {
+        const uint4 b = g[1];
+        w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+      }
+      shift_down(w, o);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = w[k];
+    clear_tail(out, v, r.n);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int j = 8 * v + 2 * k;
+    const uint32_t lo = j < r.n ? r.p[j] : 0, hi = j + 1 < r.n ? r.p[j + 1] : 0;
+    out[k] = lo | hi << 16;
+  }
+}
+
+// Elements 8 v to 8 v + 7 of a row of n, v neighbouring in neighbouring lanes: the
+// granules inside a warp's span whole, put together with the lane before, what is
+// over at its ends element by element.  Whole warps; v may lie past the row.
+__device__ __forceinline__ void store_loose(uint16_t* row, int n, int v, const uint32_t (&w)[4]) {
+  const int o = granule_offset(row), lane = threadIdx.x % 32;
+  auto element = [&](int e) { return static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))); };
+  uint32_t both[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) both[4 + k] = w[k], both[k] = o > 0 ? __shfl_up_sync(~0u, w[k], 1) : 0;
+  if (8 * v >= n) return;
+  if (o > 0) shift_down(both, 8 - o);
+  else both[0] = w[0], both[1] = w[1], both[2] = w[2], both[3] = w[3];
+  uint16_t* q = row + 8 * v;
+  if ((lane > 0 || o == 0) && 8 * v - o + 8 <= n) {
+    *reinterpret_cast<uint4*>(q - o) = make_uint4(both[0], both[1], both[2], both[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < 8 - o && 8 * v + e < n) q[e] = element(e);
+    if (lane > 0) {  // the lane before's last elements: their granule is not whole
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // Elements 2 e and 2 e + 1 of the granule, those before this lane's own.
+        if (2 * e < o) q[2 * e - o] = static_cast<uint16_t>(both[e]);
+        if (2 * e + 1 < o) q[2 * e + 1 - o] = static_cast<uint16_t>(both[e] >> 16);
+      }
+    }
+  }
+  // The last elements, where no lane follows that would store them.
+  if (lane == 31 || 8 * (v + 1) >= n) {
+#pragma unroll
+    for (int e = 1; e < 8; ++e)
+      if (e >= 8 - o && 8 * v + e < n) q[e] = element(e);
+  }
 }
 
 }  // namespace hprn
