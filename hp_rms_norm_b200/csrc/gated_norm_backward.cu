@@ -41,8 +41,9 @@ struct BlockGradArgs {
   int64_t src_stride[5];
   int tensors, x_at, e_at, g_at;
   int row_threads, row_groups, slots;
-  uint32_t ring_at, join_at;  // in shared memory: the ring, and where the groups' sums meet
-  bool staged;  // w, p and a shared gate row are in shared memory
+  uint32_t ring_at;  // in shared memory
+  bool staged;       // w and p are in shared memory, before the ring
+  bool e_direct;     // E is read where it is, not through the ring
   int64_t ctas;
   bool dense;  // every tensor's rows follow each other
   Waits waits;
@@ -80,32 +81,35 @@ __device__ __forceinline__ void team_barrier(int barrier, int threads) {
   else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 }
 
-// The sums of N values over the warps that hold a row, which meet at hardware
-// barrier `barrier`; `part` alternates between two buffers.
-template <int N>
-__device__ __forceinline__ void team_sums(float (&v)[N], float (*part)[32], int warp, int warps, int first_warp,
-                                          int barrier) {
+// The sums of four values over the `warps` warps from `first_warp` that hold a row,
+// which meet at hardware barrier `barrier`; `part` alternates between two buffers.
+// In a warp each lane goes on with half of its values twice, 6 shuffles for the 20
+// of four sums by themselves.
+__device__ __forceinline__ void team_sums(float (&v)[4], float4* part, int warps, int first_warp, int barrier) {
+  const int lane = threadIdx.x % 32;
+  const bool upper = lane & 16, odd = lane & 8;
+  float a = upper ? v[2] : v[0], b = upper ? v[3] : v[1];
+  a += __shfl_xor_sync(~0u, upper ? v[0] : v[2], 16);
+  b += __shfl_xor_sync(~0u, upper ? v[1] : v[3], 16);
+  float s = odd ? b : a;
+  s += __shfl_xor_sync(~0u, odd ? a : b, 8);
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = warp_total(v[k]);
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   if (warps == 1) {
-    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(~0u, s, 8 * k);
     return;
   }
-  const int lane = threadIdx.x % 32;
-  if (lane == 0) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) part[k][warp] = v[k];
-  }
+  if (lane % 8 == 0) reinterpret_cast<float*>(part + threadIdx.x / 32)[lane / 8] = s;
   team_barrier(barrier, warps * 32);
-#pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = warp_total(lane < warps ? part[k][first_warp + lane] : 0.f);
+  float4 sum = part[first_warp];
+  for (int w = 1; w < warps; ++w) {
+    const float4 q = part[first_warp + w];
+    sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+  }
+  v[0] = sum.x, v[1] = sum.y, v[2] = sum.z, v[3] = sum.w;
 }
 
-__device__ __forceinline__ uint32_t shared_word(uint32_t addr) {
-  uint32_t w;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(addr));
-  return w;
-}
 __device__ __forceinline__ void shared_words(uint32_t (&w)[4], uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
@@ -124,18 +128,18 @@ __device__ __forceinline__ void set_shared_half(uint32_t addr, uint16_t h) {
 __device__ __forceinline__ int64_t run_start(const BlockGradArgs& a, int64_t c) { return a.rows * c / a.ctas; }
 __device__ __forceinline__ int64_t run_of(const BlockGradArgs& a, int64_t i) { return ((i + 1) * a.ctas - 1) / a.rows; }
 
-// kGate: kOneGate a gate of one value a row, or none (1); kGateRow a row of values
-// that rows share; kGateEach one for every row.
-enum GateKind { kOneGate, kGateRow, kGateEach };
+// kGate: kOneGate a gate of one value a row, or none (1); kChannels one row of values
+// for all rows; kGateRow rows of values that rows share; kGateEach one for every row.
+enum GateKind { kOneGate, kChannels, kGateRow, kGateEach };
 
 template <typename T, int W, bool kVectors, bool kPost, int kGate>
 __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGradArgs a) {
   constexpr int kVecs = W / 4;
-  constexpr bool kHold = W <= 12, kKeep = kHold;
+  constexpr bool kHold = W <= 12;
   static_assert(kHold || kVectors, "vectors of loose rows are read by two threads");
   extern __shared__ __align__(128) unsigned char row_mem[];
   __shared__ __align__(8) uint64_t full[kBlockSlots], empty[kBlockSlots];
-  __shared__ float part[2][4][32];
+  __shared__ float4 part[2][kBlockThreads / 32];
   __shared__ int gave_up[kBlockGroups];
   const int tid = threadIdx.x, row_threads = a.row_threads, groups = a.row_groups;
   const int workers = groups * row_threads;
@@ -148,10 +152,6 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
   const uint32_t tensor_bytes = pitch * groups, slot_bytes = tensor_bytes * a.tensors;
   const uint32_t staged = smem_u32(row_mem), ring = staged + a.ring_at;
   const int begin = static_cast<int>(run_start(a, blockIdx.x)), end = static_cast<int>(run_start(a, blockIdx.x + 1));
-  const int rows_per_gate = static_cast<int>(a.rows_per_gate);
-  constexpr bool shared_row = kGate == kGateRow;
-  // A run's rows up to the next gate's.
-  auto segment_end = [&](int i) { return shared_row ? min(end, (i / rows_per_gate + 1) * rows_per_gate) : end; };
   const int lane = tid % 32;
   if (copier) {
     if (lane < groups) gave_up[lane] = 0;
@@ -176,70 +176,69 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int i0 = a.waits.stall ? end : begin; i0 < end && ok; i0 = segment_end(i0)) {
-      const int last = segment_end(i0);
-      for (int base = i0; base < last; base += groups) {
-        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1, a.waits.limit_ns));
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&full[slot]), to = ring + slot * slot_bytes;
-        const int here = min(groups, last - base);
-        // With few buffers a later round's rows are asked into L2.
-        const int next = base + a.slots * groups;
-        if (kVectors && a.dense) {
-          const uint32_t bytes = static_cast<uint32_t>(here) * row_bytes;
-          if (lane == 0) mbar_arrive_expect_tx(bar, bytes * a.tensors);
-          __syncwarp();
-          if (lane < a.tensors) {
-            bulk_load(to + lane * tensor_bytes, a.src[lane] + base * a.src_stride[lane], bytes, bar, pol);
-            if (a.slots < 3 && next < end)
-              prefetch_l2(a.src[lane] + next * a.src_stride[lane],
-                          static_cast<uint64_t>(min(groups, end - next)) * row_bytes);
-          }
-        } else {
-          const bool mine = lane < here;
-          const int64_t i = base + lane;
-          const unsigned char* from[5];
-          uint32_t bytes[5], at[5], total = 0;
-#pragma unroll
-          for (int t = 0; t < 5; ++t) {
-            bytes[t] = 0;
-            if (!mine || t >= a.tensors) continue;
-            const int64_t stride = a.src_stride[t];
-            const unsigned char* p = reinterpret_cast<const unsigned char*>(a.src[t] + i * stride);
-            const uint32_t off = kVectors ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
-            at[t] = to + t * tensor_bytes + lane * pitch;
-            // Granules [lo, hi) of the row's span, from its first one; those that
-            // reach out of the tensor are left out, their elements of this row stored
-            // one by one.
-            const uint32_t stop = off + static_cast<uint32_t>(hidden) * 2;
-            uint32_t lo = 0, hi = (stop + 15) & ~15u;
-            if (off > i * stride * 2) lo = 16;
-            if (hi - stop > (a.rows - 1 - i) * stride * 2) hi -= 16;
-            hi = max(hi, lo);
-            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-            if (lo > 0)
-              for (int j = 0; j < hidden && off + 2 * j < lo; ++j) set_shared_half(at[t] + off + 2 * j, q[j]);
-            if (hi < stop)
-              for (int j = hi > off ? static_cast<int>(hi - off) / 2 : 0; j < hidden; ++j)
-                set_shared_half(at[t] + off + 2 * j, q[j]);
-            from[t] = p - off + lo, at[t] += lo, bytes[t] = hi - lo, total += bytes[t];
-          }
-          // The stores above, in this round and in earlier ones of this buffer, before
-          // the bulk copies that write there by another proxy.
-          if constexpr (!kVectors) fence_proxy_async_smem();
-          total = __reduce_add_sync(~0u, total);
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(bar, total);
-          __syncwarp();
-#pragma unroll
-          for (int t = 0; t < 5; ++t) {
-            if (bytes[t] > 0) bulk_load(at[t], from[t], bytes[t], bar, pol);
-            if (a.slots < 3 && t < a.tensors && lane < groups && next + lane < end)
-              prefetch_l2(a.src[t] + (next + lane) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
-          }
+    for (int base = a.waits.stall ? end : begin; base < end; base += groups) {
+      ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1, a.waits.limit_ns));
+      if (!ok) break;
+      const uint32_t bar = smem_u32(&full[slot]), to = ring + slot * slot_bytes;
+      const int here = min(groups, end - base);
+      // With few buffers a later round's rows are asked into L2.
+      const int next = base + a.slots * groups;
+      if (kVectors && a.dense) {
+        const uint32_t bytes = static_cast<uint32_t>(here) * row_bytes;
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes * a.tensors);
+        __syncwarp();
+        if (lane < a.tensors) {
+          bulk_load(to + lane * tensor_bytes, a.src[lane] + base * a.src_stride[lane], bytes, bar, pol);
+          if (a.slots < 3 && next < end)
+            prefetch_l2(a.src[lane] + next * a.src_stride[lane],
+                        static_cast<uint64_t>(min(groups, end - next)) * row_bytes);
         }
-        if (++slot == a.slots) slot = 0, phase ^= 1;
+      } else {
+        const bool mine = lane < here;
+        const int64_t i = base + lane;
+        const unsigned char* from[5];
+        uint32_t bytes[5], at[5], total = 0;
+#pragma unroll
+        for (int t = 0; t < 5; ++t) {
+          bytes[t] = 0;
+          if (!mine || t >= a.tensors) continue;
+          const int64_t stride = a.src_stride[t];
+          const unsigned char* p = reinterpret_cast<const unsigned char*>(a.src[t] + i * stride);
+          const uint32_t off = kVectors ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
+          at[t] = to + t * tensor_bytes + lane * pitch;
+          // Granules [lo, hi) of the row's span, from its first one; those that
+          // reach out of the tensor are left out, their elements of this row stored
+          // one by one.
+          const uint32_t stop = off + static_cast<uint32_t>(hidden) * 2;
+          uint32_t lo = 0, hi = (stop + 15) & ~15u;
+          if (off > i * stride * 2) lo = 16;
+          if (hi - stop > (a.rows - 1 - i) * stride * 2) hi -= 16;
+          hi = max(hi, lo);
+          const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+          if (lo > 0)
+            for (int j = 0; j < hidden && off + 2 * j < lo; ++j) set_shared_half(at[t] + off + 2 * j, q[j]);
+          if (hi < stop)
+            for (int j = hi > off ? static_cast<int>(hi - off) / 2 : 0; j < hidden; ++j)
+              set_shared_half(at[t] + off + 2 * j, q[j]);
+          from[t] = p - off + lo, at[t] += lo, bytes[t] = hi - lo, total += bytes[t];
+        }
+        // The stores above, in this round and in earlier ones of this buffer, before
+        // the bulk copies that write there by another proxy.
+        if constexpr (!kVectors) fence_proxy_async_smem();
+        total = __reduce_add_sync(~0u, total);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bar, total);
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < 5; ++t) {
+          if (bytes[t] > 0) bulk_load(at[t], from[t], bytes[t], bar, pol);
+          if (a.slots < 3 && t < a.tensors && lane < groups && next + lane < end)
+            prefetch_l2(a.src[t] + (next + lane) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
+        }
       }
+      if (a.e_direct && lane < here)
+        prefetch_l2(a.e + (base + lane) * a.e_stride, static_cast<uint64_t>(hidden) * 2);
+      if (++slot == a.slots) slot = 0, phase ^= 1;
     }
     if (!ok) {
       if (lane == 0) report_give_up(a.waits);
@@ -256,7 +255,7 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
   // past the end work on zeros.)
   auto inside = [&](int k) { return (kVectors ? in : in - lane) + k * row_threads < nvec; };
   const uint64_t keep = policy_evict_last();
-  // Of a row in memory (a weight, or a gate row).
+  // Of a row in memory.
   auto load_weight = [&](uint32_t (&w)[4], const uint16_t* p, int k) {
     if constexpr (kVectors) {
       const Vec<16> q = ld_weight<16>(p + (in + k * row_threads) * 8, keep);
@@ -291,34 +290,11 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
     else store_loose(row, hidden, in + k * row_threads, w);
   };
 
-  constexpr bool post = kPost;
-  const bool one_gate = kGate == kOneGate && a.g;
-  float2 acc_w[W], acc_m[W];
-#pragma unroll
-  for (int k = 0; k < W; ++k) acc_w[k] = acc_m[k] = make_float2(0.f, 0.f);
-  // Row `which` of w, p and a shared gate row into shared memory, by all threads.
-  constexpr int gate_place = kKeep || post ? 2 : 1;
-  auto stage = [&](int which, const uint16_t* p) {
-    uint32_t* to = reinterpret_cast<uint32_t*>(row_mem) + which * (row_bytes / 4);
-    for (int j = tid; j < nvec * 4; j += workers) {
-      const uint32_t lo = 2 * j < hidden ? ld_weight<2>(p + 2 * j, keep).h : 0;
-      const uint32_t hi = 2 * j + 1 < hidden ? ld_weight<2>(p + 2 * j + 1, keep).h : 0;
-      to[j] = lo | hi << 16;
-    }
-  };
-  uint32_t held[kKeep ? 3 : 1][kKeep ? W : 1];
-  auto weight = [&](uint32_t (&w)[4], int which, const uint16_t* p, int k) {
-    if constexpr (kKeep) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = held[which][4 * k + e];
-      return;
-    }
-    if (!a.staged) return load_weight(w, p, k);
-    if (in + k * row_threads < nvec) shared_words(w, staged + which * row_bytes + (in + k * row_threads) * 16);
-    else w[0] = w[1] = w[2] = w[3] = 0;
-  };
-  auto keep_weight = [&](int which, const uint16_t* p) {
-    if constexpr (kKeep) {
+  // Weights (0 w, 1 p, 2 a shared gate row): in registers, in shared memory, or (the
+  // gate row of many words a thread) where they are.
+  uint32_t held[kHold ? 3 : 1][kHold ? W : 1];
+  auto take_weight = [&](int which, const uint16_t* p) {
+    if constexpr (kHold) {
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
         if (!inside(k)) break;
@@ -327,37 +303,33 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
 #pragma unroll
         for (int e = 0; e < 4; ++e) held[which][4 * k + e] = w[e];
       }
+    } else if (a.staged && (which < 2 || kGate == kChannels)) {
+      for (int v = tid; v < nvec; v += workers)
+        reinterpret_cast<uint4*>(row_mem)[which * nvec + v] = *reinterpret_cast<const uint4*>(p + v * 8);
     }
   };
-  if constexpr (kKeep) {
-    keep_weight(0, a.w);
-    if constexpr (post) keep_weight(1, a.p);
-  } else if (a.staged) {
-    stage(0, a.w);
-    if (post) stage(1, a.p);
-    if (!shared_row) team_barrier(15, workers);
-  }
-  const float scale = 1.0f / static_cast<float>(hidden);
-  const float2 residual_scale = make_float2(a.scale, a.scale);
-  // A CTA's sums over the rows so far: the groups' meet in shared memory, the first
-  // group writes them.
-  auto write_sums = [&](float2 (&acc)[W], float* out) {
-    if (groups > 1) {
-      float2* sums = reinterpret_cast<float2*>(row_mem + a.join_at);
-      team_barrier(15, workers);
+  auto weight = [&](uint32_t (&w)[4], int which, const uint16_t* p, int k) {
+    if constexpr (kHold) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) sums[k * workers + tid] = acc[k];
-      team_barrier(15, workers);
-      if (group > 0) return;
-      for (int g = 1; g < groups; ++g) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) acc[k] = __fadd2_rn(acc[k], sums[k * workers + g * row_threads + tid]);
-      }
+      for (int e = 0; e < 4; ++e) w[e] = held[which][4 * k + e];
+    } else if (a.staged && (which < 2 || kGate == kChannels)) {
+      shared_words(w, staged + (which * nvec + in + k * row_threads) * 16);
+    } else {
+      load_weight(w, p, k);
     }
-    // (Rows of sums are padded to whole vectors.)
+  };
+  take_weight(0, a.w);
+  if constexpr (kPost) take_weight(1, a.p);
+  if constexpr (kGate == kChannels) take_weight(2, a.g);
+  if (!kHold && a.staged) team_barrier(15, workers);
+
+  float2 acc_w[W], acc_m[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) acc_w[k] = acc_m[k] = make_float2(0.f, 0.f);
+  // Sums over rows, to a row of vectors.
+  auto write_sums = [&](const float2 (&acc)[W], float* out) {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-      if (!inside(k)) break;
       if (in + k * row_threads >= nvec) break;
       Vec<32> q;
 #pragma unroll
@@ -368,192 +340,207 @@ __global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGr
       st_global<32>(out + (in + k * row_threads) * 8, q);
     }
   };
-
-  auto start_of = [&](int t, int64_t i, uint32_t at) {
-    return at + t * tensor_bytes +
-           (kVectors ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.src[t] + i * a.src_stride[t]) & 15));
-  };
-  // Row i's sums of t^2, w D t and x^2, once its buffer at `at` has arrived.
-  auto first_pass = [&](int64_t i, uint32_t at, int of_slot, uint32_t of_phase, float& s_t, float& s_d, float& s_x) {
-    const uint32_t ts = start_of(0, i, at), ds = start_of(1, i, at), xs = post ? start_of(a.x_at, i, at) : 0;
-    if (!mbar_wait_bounded(smem_u32(&full[of_slot]), of_phase, a.waits.limit_ns)) gave_up[group] = 1;
-    float2 st = make_float2(0.f, 0.f), sd = st, sx = st;
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      if (!inside(k)) break;
-      uint32_t t[4], d[4], w[4], x[4];
-      load_row(t, ts, k);
-      load_row(d, ds, k);
-      weight(w, 0, a.w, k);
-      if constexpr (post) load_row(x, xs, k);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 tf = unpack2<T>(t[e]);
-        st = __ffma2_rn(tf, tf, st);
-        sd = __ffma2_rn(mul_pair<T>(w[e], d[e]), tf, sd);
-        if constexpr (post) sx = fma_pair<T>(x[e], x[e], sx);
-      }
-    }
-    s_t = st.x + st.y, s_d = sd.x + sd.y, s_x = sx.x + sx.y;
-  };
-  int slot = 0, turn = 0;
-  uint32_t phase = 0;
-  bool stopped = false, have = false;  // have: `sums` are the next row's
-  float sums[3];
-  for (int i0 = begin; i0 < end; i0 = segment_end(i0)) {
-    const int last = segment_end(i0);
-    const uint16_t* gate_row = shared_row ? a.g + i0 / rows_per_gate * a.g_stride : nullptr;
-    if constexpr (kKeep && shared_row) {
-      keep_weight(2, gate_row);
-    } else if (a.staged && shared_row) {
-      if (i0 > begin) team_barrier(15, workers);  // every group is done with the last one
-      stage(gate_place, gate_row);
+  // The groups' sums meet in shared memory (the ring, done with), the first group
+  // writes them.
+  auto join_sums = [&](float2 (&acc)[W], float* out) {
+    if (groups > 1) {
+      float2* sums = reinterpret_cast<float2*>(row_mem);
       team_barrier(15, workers);
+#pragma unroll
+      for (int k = 0; k < W; ++k) sums[k * workers + tid] = acc[k];
+      team_barrier(15, workers);
+      if (group > 0) return;
+      for (int g = 1; g < groups; ++g) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[k] = __fadd2_rn(acc[k], sums[k * workers + g * row_threads + tid]);
+      }
     }
-    for (int base = i0; base < last && !stopped; base += groups) {
-      const int64_t i = base + group;
-      const uint32_t at = ring + slot * slot_bytes + group * pitch, slot_bar = smem_u32(&empty[slot]);
-      const int this_slot = slot;
-      const uint32_t this_phase = phase;
-      if (++slot == a.slots) slot = 0, phase ^= 1;
-      if (i >= last) {  // fewer rows left than groups
-        __syncwarp();
-        if (lane == 0) mbar_arrive(slot_bar);
-        continue;
-      }
-      float gate_one = 1.f;
-      if (one_gate) gate_one = unpack1<T>(a.g[(static_cast<uint32_t>(i) / static_cast<uint32_t>(a.rows_per_gate)) * a.g_stride]);
-      if (!have) {
-        first_pass(i, at, this_slot, this_phase, sums[0], sums[1], sums[2]);
-        team_sums(sums, part[turn], tid / 32, warps, group * warps, barrier);
-        turn ^= 1;
-      }
-      have = false;
-      if (*static_cast<volatile int*>(&gave_up[group])) {
-        // The copier may have issued its last row and left without a wait.
-        if (in == 0) report_give_up(a.waits);
-        stopped = true;
-        break;
-      }
-      const uint32_t ts = start_of(0, i, at), ds = start_of(1, i, at), xs = a.x_at >= 0 ? start_of(a.x_at, i, at) : 0;
-      const uint32_t es = a.e_at >= 0 ? start_of(a.e_at, i, at) : 0, gs = a.g_at >= 0 ? start_of(a.g_at, i, at) : 0;
-      const float inv_t = rsqrtf(sums[0] * scale + a.eps), mean = sums[1] * inv_t * scale;
-      const float inv_x = post ? rsqrtf(sums[2] * scale + a.eps) : 1.f;
-      // dt = w D inv_t + (E - t mean inv_t^2); the sums over a row leave inv_x out.
-      const float2 inv_t2 = make_float2(inv_t, inv_t), minus = make_float2(-mean * inv_t * inv_t, -mean * inv_t * inv_t);
-      const float by = (kGate == kOneGate ? gate_one : 1.f) * inv_x;
-      const float2 m_by = make_float2(by, by);
-      uint16_t* dr = a.dr + i * a.dr_stride;
-      uint16_t* dx = a.dx + i * a.dx_stride;
-      // Held or put back: p dt, times g where that is a row.
-      float2 u[kHold ? W : 1], su = make_float2(0.f, 0.f);
+    write_sums(acc, out);
+  };
+
+  const float scale = 1.0f / static_cast<float>(hidden);
+  const float2 residual_scale = make_float2(a.scale, a.scale);
+  const bool one_gate = kGate == kOneGate && a.g;
+  const int rows_per_gate = static_cast<int>(a.rows_per_gate);
+  int slot = 0, turn = 0, held_gate = -1, gate_at = begin / rows_per_gate;
+  uint32_t phase = 0;
+  float sums[4] = {0.f, 0.f, 0.f, 0.f};  // of t^2, w D t and x^2 of the coming row, of p g dt x of the last one
+  // A group's sums for the gates of its run before gate k: those for the one that its
+  // rows had, zeros for the others.
+  auto finish_gates = [&](int k) {
+    for (; gate_at < k; ++gate_at) {
+      write_sums(acc_m, a.m_parts + (static_cast<int64_t>(blockIdx.x + gate_at) * groups + group) * a.parts_ld);
+#pragma unroll
+      for (int q = 0; q < W; ++q) acc_m[q] = make_float2(0.f, 0.f);
+    }
+  };
+  // Held or put back: p dt, times g where that is a row.
+  float2 u[kHold ? W : 1];
+  int64_t last = -1;  // the row whose last pass is due; its buffer, and what its sums are multiplied by
+  uint32_t last_at = 0, last_bar = 0;
+  float last_by = 0.f, last_inv = 0.f;
+  for (int64_t i = begin + group;; i += groups) {
+    const bool more = i < end;
+    const uint32_t at = ring + slot * slot_bytes + group * pitch;
+    auto start_of = [&](int t) {
+      return at + t * tensor_bytes +
+             (kVectors ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.src[t] + i * a.src_stride[t]) & 15));
+    };
+    uint32_t ts = 0, ds = 0, xs = 0;
+    if (more) {
+      // First pass.
+      ts = start_of(0), ds = start_of(1);
+      if (a.x_at >= 0) xs = start_of(a.x_at);
+      if (!mbar_wait_bounded(smem_u32(&full[slot]), phase, a.waits.limit_ns)) gave_up[group] = 1;
+      float2 st = make_float2(0.f, 0.f), sd = st, sx = st;
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
         if (!inside(k)) break;
-        uint32_t t[4], d[4], w[4], x[4] = {}, e4[4] = {}, g[4], p[4], out_r[4], out_g[4];
+        uint32_t t[4], d[4], w[4], x[4];
         load_row(t, ts, k);
         load_row(d, ds, k);
         weight(w, 0, a.w, k);
-        if (a.x_at >= 0) load_row(x, xs, k);
-        if (a.e_at >= 0) load_row(e4, es, k);
-        if constexpr (post) weight(p, 1, a.p, k);
-        if constexpr (kGate == kGateEach) load_row(g, gs, k);
-        if constexpr (kGate == kGateRow) weight(g, gate_place, gate_row, k);
+        if constexpr (kPost) load_row(x, xs, k);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 dt = __ffma2_rn(mul_pair<T>(w[e], d[e]), inv_t2, __ffma2_rn(unpack2<T>(t[e]), minus, unpack2<T>(e4[e])));
-          acc_w[4 * k + e] = __ffma2_rn(mul_pair<T>(d[e], t[e]), inv_t2, acc_w[4 * k + e]);
-          const float2 xf = unpack2<T>(x[e]), q = __fmul2_rn(dt, xf);
-          float2 pdt = dt;
-          if constexpr (kGate == kOneGate) {
-            acc_m[4 * k + e] = __ffma2_rn(q, m_by, acc_m[4 * k + e]);
-            if constexpr (post) pdt = __fmul2_rn(dt, unpack2<T>(p[e]));
-          } else {
-            if constexpr (kGate == kGateEach)
-              acc_m[4 * k + e] = __ffma2_rn(__fmul2_rn(q, unpack2<T>(g[e])), m_by, acc_m[4 * k + e]);
-            else
-              acc_m[4 * k + e] = __ffma2_rn(q, m_by, acc_m[4 * k + e]);
-            if constexpr (post) pdt = __fmul2_rn(dt, mul_pair<T>(p[e], g[e]));
-            else pdt = __fmul2_rn(dt, unpack2<T>(g[e]));
-          }
-          su = __ffma2_rn(pdt, xf, su);
-          const float2 r = __fmul2_rn(dt, residual_scale);
-          out_r[e] = pack2<T>(r.x, r.y);
-          if constexpr (kGate == kGateEach) {
-            float2 v = __fmul2_rn(q, m_by);
-            if constexpr (post) v = __fmul2_rn(v, unpack2<T>(p[e]));
-            out_g[e] = pack2<T>(v.x, v.y);
-          }
-          if constexpr (!post) {
-            const float2 v = kGate == kOneGate ? __fmul2_rn(pdt, m_by) : pdt;
-            t[e] = pack2<T>(v.x, v.y);
-          } else if constexpr (kHold) {
-            u[4 * k + e] = pdt;
-          } else {
-            t[e] = __float_as_uint(pdt.x), d[e] = __float_as_uint(pdt.y);
-          }
-        }
-        store_row(dr, k, out_r);
-        if constexpr (kGate == kGateEach) store_row(a.dg + i * a.dg_stride, k, out_g);
-        if constexpr (!post) {
-          store_row(dx, k, t);
-        } else if constexpr (!kHold) {
-          set_shared_words(ts + (in + k * row_threads) * 16, t);
-          set_shared_words(ds + (in + k * row_threads) * 16, d);
+          const float2 tf = unpack2<T>(t[e]);
+          st = __ffma2_rn(tf, tf, st);
+          sd = __ffma2_rn(mul_pair<T>(w[e], d[e]), tf, sd);
+          if constexpr (kPost) sx = fma_pair<T>(x[e], x[e], sx);
         }
       }
-      // The group's row of the next round goes through its first pass now, so that
-      // both rows' sums meet at one barrier.
-      const int next_last = base + groups < last ? last : last < end ? segment_end(last) : 0;
-      const int next = (base + groups < last ? base + groups : last) + group;
-      float s[4] = {0.f, 0.f, 0.f, su.x + su.y};
-      if (a.slots > 1 && next < next_last) {
-        first_pass(next, ring + slot * slot_bytes + group * pitch, slot, phase, s[0], s[1], s[2]);
-        have = true;
-      }
-      if (have || post || one_gate) {
-        team_sums(s, part[turn], tid / 32, warps, group * warps, barrier);
-        turn ^= 1;
-        sums[0] = s[0], sums[1] = s[1], sums[2] = s[2];
-        if (one_gate && in == 0) a.gate_sums[i] = s[3] * inv_x;
-        if constexpr (post) {
-          // dx = inv_x (p g dt - m mean(p g dt m)) = u by - x inv_x^2 mean(u x by).
-          const float b = -s[3] * by * inv_x * inv_x * scale;
-          const float2 back = make_float2(b, b);
+      sums[0] = st.x + st.y, sums[1] = sd.x + sd.y, sums[2] = sx.x + sx.y;
+    }
+    if (more || (last >= 0 && (kPost || one_gate))) {
+      team_sums(sums, part[turn], warps, group * warps, barrier);
+      turn ^= 1;
+    }
+    if (last >= 0) {
+      // The row before's last pass:
+      //   dx = inv_x (p g dt - m mean(p g dt m)) = u by - x inv_x^2 mean(u x by)
+      if (one_gate && in == 0) a.gate_sums[last] = sums[3] * last_inv;
+      if constexpr (kPost) {
+        const float b = -sums[3] * last_by * last_inv * last_inv * scale;
+        const float2 back = make_float2(b, b), by = make_float2(last_by, last_by);
+        uint16_t* dx = a.dx + last * a.dx_stride;
+        const uint32_t x_at = last_at + a.x_at * tensor_bytes +
+            (kVectors ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.src[a.x_at] + last * a.src_stride[a.x_at]) & 15));
 #pragma unroll
-          for (int k = 0; k < kVecs; ++k) {
-            if (!inside(k)) break;
-            uint32_t x[4], ux[4], uy[4], o[4];
-            load_row(x, xs, k);
-            if constexpr (!kHold) {
-              shared_words(ux, ts + (in + k * row_threads) * 16);
-              shared_words(uy, ds + (in + k * row_threads) * 16);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float2 pdt;
-              if constexpr (kHold) pdt = u[4 * k + e];
-              else pdt = make_float2(__uint_as_float(ux[e]), __uint_as_float(uy[e]));
-              const float2 v = __ffma2_rn(pdt, m_by, __fmul2_rn(unpack2<T>(x[e]), back));
-              o[e] = pack2<T>(v.x, v.y);
-            }
-            store_row(dx, k, o);
+        for (int k = 0; k < kVecs; ++k) {
+          if (!inside(k)) break;
+          uint32_t x[4], ux[4], uy[4], o[4];
+          load_row(x, x_at, k);
+          if constexpr (!kHold) {
+            shared_words(ux, last_at + (in + k * row_threads) * 16);
+            shared_words(uy, last_at + tensor_bytes + (in + k * row_threads) * 16);
           }
-          // The words put into the buffer, before the next copies into it.
-          if constexpr (!kHold) fence_proxy_async_smem();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float2 pgdt;
+            if constexpr (kHold) pgdt = u[4 * k + e];
+            else pgdt = make_float2(__uint_as_float(ux[e]), __uint_as_float(uy[e]));
+            const float2 v = __ffma2_rn(pgdt, by, __fmul2_rn(unpack2<T>(x[e]), back));
+            o[e] = pack2<T>(v.x, v.y);
+          }
+          store_row(dx, k, o);
         }
+        // The words put into the buffer, before the next copies into it.
+        if constexpr (!kHold) fence_proxy_async_smem();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(slot_bar);
+      if (lane == 0) mbar_arrive(last_bar);
     }
-    if (shared_row) {
-      write_sums(acc_m, a.m_parts + static_cast<int64_t>(blockIdx.x + i0 / rows_per_gate) * a.parts_ld);
+    if (!more) break;
+    if (*static_cast<volatile int*>(&gave_up[group])) {
+      // The copier may have issued its last row and left without a wait.
+      if (in == 0) report_give_up(a.waits);
+      break;
+    }
+    const uint16_t* gate_row = a.g;
+    if constexpr (kGate == kGateRow) {
+      const int k = static_cast<int>(i) / rows_per_gate;
+      gate_row = a.g + k * a.g_stride;
+      if (k != held_gate) {
+        finish_gates(k);
+        take_weight(2, gate_row);
+        held_gate = k;
+      }
+    }
+    // Second pass: dt = w D inv_t + (E - t mean inv_t^2); the sums over a row leave
+    // inv_x out.
+    const float inv_t = rsqrtf(sums[0] * scale + a.eps), mean = sums[1] * inv_t * scale;
+    const float inv_x = kPost ? rsqrtf(sums[2] * scale + a.eps) : 1.f;
+    float by = inv_x;
+    if constexpr (kGate == kOneGate) {
+      if (a.g) by *= unpack1<T>(a.g[(static_cast<uint32_t>(i) / static_cast<uint32_t>(rows_per_gate)) * a.g_stride]);
+    }
+    const float2 inv_t2 = make_float2(inv_t, inv_t), minus = make_float2(-mean * inv_t * inv_t, -mean * inv_t * inv_t);
+    const float2 m_by = make_float2(by, by);
+    float2 su = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < W; ++k) acc_m[k] = make_float2(0.f, 0.f);
+    for (int k = 0; k < kVecs; ++k) {
+      if (!inside(k)) break;
+      uint32_t t[4], d[4], w[4], x[4] = {}, e4[4] = {}, g[4], p[4], out_r[4], out_g[4];
+      if (a.e_direct) load_loose(e4, loose_row(a.e, i, a.rows, a.e_stride, hidden), in + k * row_threads);
+      load_row(t, ts, k);
+      load_row(d, ds, k);
+      weight(w, 0, a.w, k);
+      if (a.x_at >= 0) load_row(x, xs, k);
+      if (a.e_at >= 0) load_row(e4, start_of(a.e_at), k);
+      if constexpr (kPost) weight(p, 1, a.p, k);
+      if constexpr (kGate == kGateEach) load_row(g, start_of(a.g_at), k);
+      if constexpr (kGate == kGateRow || kGate == kChannels) weight(g, 2, gate_row, k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 dt = __ffma2_rn(mul_pair<T>(w[e], d[e]), inv_t2, __ffma2_rn(unpack2<T>(t[e]), minus, unpack2<T>(e4[e])));
+        acc_w[4 * k + e] = __ffma2_rn(mul_pair<T>(d[e], t[e]), inv_t2, acc_w[4 * k + e]);
+        const float2 xf = unpack2<T>(x[e]), q = __fmul2_rn(dt, xf);
+        float2 pdt = dt;
+        if constexpr (kGate == kOneGate) {
+          acc_m[4 * k + e] = __ffma2_rn(q, m_by, acc_m[4 * k + e]);
+          if constexpr (kPost) pdt = __fmul2_rn(dt, unpack2<T>(p[e]));
+        } else {
+          if constexpr (kGate == kGateEach)
+            acc_m[4 * k + e] = __ffma2_rn(__fmul2_rn(q, unpack2<T>(g[e])), m_by, acc_m[4 * k + e]);
+          else
+            acc_m[4 * k + e] = __ffma2_rn(q, m_by, acc_m[4 * k + e]);
+          if constexpr (kPost) pdt = __fmul2_rn(dt, mul_pair<T>(p[e], g[e]));
+          else pdt = __fmul2_rn(dt, unpack2<T>(g[e]));
+        }
+        su = __ffma2_rn(pdt, xf, su);
+        const float2 r = __fmul2_rn(dt, residual_scale);
+        out_r[e] = pack2<T>(r.x, r.y);
+        if constexpr (kGate == kGateEach) {
+          float2 v = __fmul2_rn(q, m_by);
+          if constexpr (kPost) v = __fmul2_rn(v, unpack2<T>(p[e]));
+          out_g[e] = pack2<T>(v.x, v.y);
+        }
+        if constexpr (!kPost) {
+          const float2 v = kGate == kOneGate ? __fmul2_rn(pdt, m_by) : pdt;
+          t[e] = pack2<T>(v.x, v.y);
+        } else if constexpr (kHold) {
+          u[4 * k + e] = pdt;
+        } else {
+          t[e] = __float_as_uint(pdt.x), d[e] = __float_as_uint(pdt.y);
+        }
+      }
+      store_row(a.dr + i * a.dr_stride, k, out_r);
+      if constexpr (kGate == kGateEach) store_row(a.dg + i * a.dg_stride, k, out_g);
+      if constexpr (!kPost) {
+        store_row(a.dx + i * a.dx_stride, k, t);
+      } else if constexpr (!kHold) {
+        set_shared_words(ts + (in + k * row_threads) * 16, t);
+        set_shared_words(ds + (in + k * row_threads) * 16, d);
+      }
     }
+    sums[3] = su.x + su.y;
+    last = i, last_at = at, last_bar = smem_u32(&empty[slot]), last_by = by, last_inv = inv_x;
+    if (++slot == a.slots) slot = 0, phase ^= 1;
   }
-  write_sums(acc_w, a.dw_parts + blockIdx.x * a.parts_ld);
-  if (!shared_row) write_sums(acc_m, a.m_parts + blockIdx.x * a.parts_ld);
+  // Buffers of a last round with fewer rows than groups are nobody's any more.
+  if constexpr (kGate == kGateRow) finish_gates((end - 1) / rows_per_gate + 1);
+  else join_sums(acc_m, a.m_parts + blockIdx.x * a.parts_ld);
+  join_sums(acc_w, a.dw_parts + blockIdx.x * a.parts_ld);
 }
 
 // The weights' and a shared gate row's gradients from block_grad_rows' sums: 32
@@ -582,14 +569,15 @@ __global__ void __launch_bounds__(32 * kRunWarps) block_grad_runs(BlockGradArgs 
   } else {
     const float p = in && a.p ? unpack1<T>(a.p[j]) : 1.f;
     const bool together = a.gates <= 2;
+    const int groups = a.gates > 1 ? a.row_groups : 1;
     for (int64_t k = together ? 0 : ty; k < a.gates; k += together ? 1 : kRunWarps) {
-      const int first = static_cast<int>(run_of(a, k * a.rows_per_gate));
-      const int last = static_cast<int>(run_of(a, (k + 1) * a.rows_per_gate - 1));
+      // The sums of the runs that the gate's rows lie in follow each other.
+      const int64_t first = (run_of(a, k * a.rows_per_gate) + k) * groups;
+      const int64_t end = (run_of(a, (k + 1) * a.rows_per_gate - 1) + k + 1) * groups;
       float sm = 0.f;
       if (in) {
 #pragma unroll 10
-        for (int c = first + (together ? ty : 0); c <= last; c += together ? kRunWarps : 1)
-          sm += a.m_parts[(c + k) * a.parts_ld + j];
+        for (int64_t e = first + (together ? ty : 0); e < end; e += together ? kRunWarps : 1) sm += a.m_parts[e * a.parts_ld + j];
       }
       if (together) {
         __syncthreads();
@@ -756,60 +744,58 @@ struct BlockGradPlan {
 };
 
 BlockGradPlan plan_block_grad(BlockGradArgs& a) {
-  a.tensors = 0, a.x_at = a.e_at = a.g_at = -1;
-  auto add = [&](const uint16_t* p, int64_t stride) {
-    a.src[a.tensors] = p, a.src_stride[a.tensors] = a.rows > 1 ? stride : a.hidden;
-    return a.tensors++;
-  };
-  add(a.t, a.t_stride);
-  add(a.d, a.d_stride);
-  if (a.p || a.g) a.x_at = add(a.x, a.x_stride);
-  if (a.e) a.e_at = add(a.e, a.e_stride);
-  if (a.gate_each) a.g_at = add(a.g, a.g_stride);
   BlockGradPlan plan{};
   plan.vectors = a.hidden % 8 == 0 && tma_rows(a.dx, a.rows, a.dx_stride) && tma_rows(a.dr, a.rows, a.dr_stride) &&
-                 aligned(a.w, 16) && aligned(a.p, 16) && (!a.gate_each || tma_rows(a.dg, a.rows, a.dg_stride));
-  if (a.gate_row && !a.gate_each) plan.vectors = plan.vectors && tma_rows(a.g, a.gates, a.g_stride);
-  a.dense = true;
-  for (int k = 0; k < a.tensors; ++k) {
-    plan.vectors = plan.vectors && tma_rows(a.src[k], a.rows, a.src_stride[k]);
-    a.dense = a.dense && a.src_stride[k] == a.hidden;
-  }
+                 tma_rows(a.t, a.rows, a.t_stride) && tma_rows(a.d, a.rows, a.d_stride) &&
+                 tma_rows(a.x, a.rows, a.x_stride) && (!a.e || tma_rows(a.e, a.rows, a.e_stride)) &&
+                 aligned(a.w, 16) && aligned(a.p, 16) &&
+                 (!a.gate_each || (tma_rows(a.dg, a.rows, a.dg_stride) && tma_rows(a.g, a.rows, a.g_stride))) &&
+                 (!a.gate_row || a.gate_each || tma_rows(a.g, a.gates, a.g_stride));
   if (a.rows <= 0 || a.hidden <= 0 || a.hidden > 32768) return plan;
   const int64_t nvec = (a.hidden + 7) / 8;
-  const int64_t slot = (nvec * 16 + (plan.vectors ? 0 : 16)) * a.tensors;
-  const bool segments = a.gate_row && !a.gate_each && a.gates > 1;
-  const int64_t staged_rows = 1 + (a.p != nullptr) + (a.gate_row && !a.gate_each);
-  int best = 0;
-  for (int words : {4, 8, 12, 24}) {
-    if (words > 12 && !plan.vectors) break;
-    const int64_t threads = round_up((nvec + words / 4 - 1) / (words / 4), 32);
-    const bool few = a.rows <= 4 * 148;
-    if (threads > kBlockThreads || (words == 4 && threads > 128 && !few)) continue;
-    int64_t groups = kBlockThreads / threads;
-    if (groups > 14) groups = 14;  // a hardware barrier each, and one for all
-    if (groups > a.rows) groups = a.rows;
-    auto join_bytes = [&] { return groups > 1 ? words * threads * groups * 8 : 0; };
-    auto ring_bytes = [&](int64_t slots) { return slots * groups * slot; };
-    const int64_t weights = words <= 12 ? 0 : staged_rows;
-    int64_t before = weights * nvec * 16;  // the ring
-    while (groups > 1 && before + ring_bytes(2) + (segments ? join_bytes() : 0) > kBlockSmem) --groups;
-    const bool staged = weights > 0 && before + ring_bytes(2) + (segments ? join_bytes() : 0) <= kBlockSmem;
-    if (!staged) before = 0;
-    int64_t slots = (kBlockSmem - before - (segments ? join_bytes() : 0)) / (groups * slot);
-    if (slots > kBlockSlots) slots = kBlockSlots;
-    if (slots < 1 || threads * groups <= best) continue;
-    best = static_cast<int>(threads * groups);
-    plan.words = words;
-    a.row_threads = static_cast<int>(threads), a.row_groups = static_cast<int>(groups), a.slots = static_cast<int>(slots);
-    // The ring is free when a CTA's only sums are written.
-    a.staged = staged, a.ring_at = static_cast<uint32_t>(before);
-    a.join_at = static_cast<uint32_t>(segments ? before + ring_bytes(slots) : 0);
-    const int64_t ring = before + ring_bytes(slots), joined = a.join_at + join_bytes();
-    plan.smem = static_cast<int>(ring > joined ? ring : joined);
-    const int64_t need = (a.rows + groups - 1) / groups;
-    a.ctas = need < 148 ? need : 148;
-    if (few || best >= 288) break;
+  // Two buffers at least: a row's last pass waits for the next one's first.  Where E
+  // leaves no room for them it stays outside.
+  for (int direct = 0; direct < (a.e ? 2 : 1); ++direct) {
+    a.tensors = 0, a.x_at = a.e_at = a.g_at = -1, a.e_direct = direct;
+    auto add = [&](const uint16_t* p, int64_t stride) {
+      a.src[a.tensors] = p, a.src_stride[a.tensors] = a.rows > 1 ? stride : a.hidden;
+      return a.tensors++;
+    };
+    add(a.t, a.t_stride);
+    add(a.d, a.d_stride);
+    if (a.p || a.g) a.x_at = add(a.x, a.x_stride);
+    if (a.e && !direct) a.e_at = add(a.e, a.e_stride);
+    if (a.gate_each) a.g_at = add(a.g, a.g_stride);
+    a.dense = true;
+    for (int k = 0; k < a.tensors; ++k) a.dense = a.dense && a.src_stride[k] == a.hidden;
+    const int64_t slot = (nvec * 16 + (plan.vectors ? 0 : 16)) * a.tensors;
+    int best = 0;
+    for (int words : {4, 8, 12, 24}) {
+      if (words > 12 && (!plan.vectors || best > 0)) break;
+      const int64_t threads = round_up((nvec + words / 4 - 1) / (words / 4), 32);
+      const bool few = a.rows <= 4 * 148;
+      if (threads > kBlockThreads || (words == 4 && threads > 128 && !few)) continue;
+      int64_t groups = kBlockThreads / threads;
+      if (groups > 14) groups = 14;  // a hardware barrier each, and one for all
+      if (groups > a.rows) groups = a.rows;
+      // (Places for w, p and the gate's row.)
+      const int64_t weights = words <= 12 ? 0 : (a.gate_row && a.gates == 1 ? 3 : 2) * nvec * 16;
+      while (groups > 1 && weights + 2 * groups * slot > kBlockSmem) --groups;
+      const bool staged = weights > 0 && weights + 2 * groups * slot <= kBlockSmem;
+      int64_t slots = (kBlockSmem - (staged ? weights : 0)) / (groups * slot);
+      if (slots > kBlockSlots) slots = kBlockSlots;
+      if (slots < 2 || threads * groups <= best) continue;
+      best = static_cast<int>(threads * groups);
+      plan.words = words;
+      a.row_threads = static_cast<int>(threads), a.row_groups = static_cast<int>(groups), a.slots = static_cast<int>(slots);
+      a.staged = staged, a.ring_at = static_cast<uint32_t>(staged ? weights : 0);
+      const int64_t ring = a.ring_at + slots * groups * slot, joined = groups > 1 ? words * threads * groups * 8 : 0;
+      plan.smem = static_cast<int>(ring > joined ? ring : joined);
+      const int64_t need = (a.rows + groups - 1) / groups;
+      a.ctas = need < 148 ? need : 148;
+      if (few || best >= 224) break;
+    }
+    if (plan.words > 0) break;
   }
   return plan;
 }
@@ -826,7 +812,9 @@ void (*block_grad_kernel(int words))(BlockGradArgs) {
 }
 template <typename T, bool kVectors>
 void (*block_grad_kernel(const BlockGradArgs& a, int words))(BlockGradArgs) {
-  const int gate = !a.gate_row ? kOneGate : a.gate_each ? kGateEach : kGateRow;
+  const int gate = !a.gate_row ? kOneGate : a.gate_each ? kGateEach : a.gates == 1 ? kChannels : kGateRow;
+  if (gate == kChannels)
+    return a.p ? block_grad_kernel<T, kVectors, true, kChannels>(words) : block_grad_kernel<T, kVectors, false, kChannels>(words);
   if (gate == kOneGate)
     return a.p ? block_grad_kernel<T, kVectors, true, kOneGate>(words) : block_grad_kernel<T, kVectors, false, kOneGate>(words);
   if (gate == kGateRow)
@@ -917,11 +905,12 @@ int hprn_gated_add_rms_norm_backward(
   a.gate_sums = ws.take<float>(gate && !a.gate_row ? rows : 0);
   if (!gate || a.gate_row) a.gate_sums = nullptr;
   a.parts_ld = round_up(hidden, 8);
-  // A run and a gate it meets make one row of sums: each step to the next of them
-  // goes on by a run, a gate or both, so that run + gate tells them apart.
+  // A run and a gate it meets make one row of sums (for each group of threads): each
+  // step to the next of them goes on by a run, a gate or both, so that run + gate tells
+  // them apart.
   const int64_t parts = (shared_row ? gates : 1) * a.parts;
   a.dw_parts = ws.take<float>((plan.words > 0 ? a.ctas : parts) * a.parts_ld);
-  a.m_parts = ws.take<float>((plan.words > 0 ? a.ctas + (shared_row ? gates : 0) : parts) * a.parts_ld);
+  a.m_parts = ws.take<float>((plan.words == 0 ? parts : shared_row && gates > 1 ? (a.ctas + gates) * a.row_groups : a.ctas) * a.parts_ld);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();
