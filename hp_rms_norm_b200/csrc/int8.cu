@@ -285,6 +285,102 @@ class ByteRows {
   uint8_t* copy_ = nullptr;
 };
 
+// Few rows: the weight's bytes bound the product, so it is read straight into
+// registers, without the tensor cores' pipeline of stages whose filling and
+// draining costs 6 us.  A CTA takes 16 channels, its warps shares of the sums in
+// blocks of 128 bytes, all of a warp's loads of several blocks in flight; the
+// products are mma.sync's 16 channels x 8 rows x 32 terms.  A lane's 32 bytes of a
+// block are the terms that the instruction wants of it in some order, the same for
+// both operands, which is all that a sum needs.  The shares meet in shared memory.
+struct FewArgs {
+  uint16_t* out;
+  const int8_t* x;
+  const int8_t* w;
+  const float* row_scale;
+  const float* channel_scale;
+  const uint16_t* bias;  // or null
+  int64_t out_ld, x_ld, w_ld;
+  int32_t rows, hidden, channels;
+  int32_t first_wave;  // CTAs that are resident at once
+};
+constexpr int kFewWarps = 8;
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// kTiles: tiles of 8 rows.
+template <typename T, int kTiles>
+__global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 4 : kTiles == 2 ? 3 : 2) few_rows(FewArgs a) {
+  constexpr int kChannels = 16, kBlocks = 2;  // blocks whose loads are in flight together
+  __shared__ int sums[kFewWarps][8 * kTiles][kChannels + 1];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  const int channel = blockIdx.x * kChannels;
+  if (blockIdx.x < a.first_wave && threadIdx.x < kChannels && channel + threadIdx.x < a.channels)
+    prefetch_l2(a.w + (channel + threadIdx.x) * a.w_ld, a.hidden);
+  pdl_wait();
+  const uint64_t once = policy_evict_first(), keep = policy_evict_last();
+  const int8_t* w0 = a.w + (channel + g) * a.w_ld;
+  int acc[kTiles][4] = {};
+  auto load = [&](uint32_t (&v)[8], const int8_t* p, int at, bool there, bool stream) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Vec<16> q;
+      q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
+      if (there && at + 16 * h < a.hidden) {
+        if (stream) q = ld_stream<16>(p + at + 16 * h, once);
+        else q = ld_weight<16>(p + at + 16 * h, keep);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * h + k] = q.w[k];
+    }
+  };
+  for (int block = warp; block * 128 < a.hidden; block += kFewWarps * kBlocks) {
+    uint32_t w[kBlocks][2][8];
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        load(w[u][m], w0 + 8 * m * a.w_ld, (block + u * kFewWarps) * 128 + 32 * t, channel + g + 8 * m < a.channels, true);
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      uint32_t x[kBlocks][8];
+#pragma unroll
+      for (int u = 0; u < kBlocks; ++u)
+        load(x[u], a.x + (8 * i + g) * a.x_ld, (block + u * kFewWarps) * 128 + 32 * t, 8 * i + g < a.rows, false);
+#pragma unroll
+      for (int u = 0; u < kBlocks; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t q[4] = {w[u][0][2 * j], w[u][1][2 * j], w[u][0][2 * j + 1], w[u][1][2 * j + 1]};
+          mma_s8(acc[i], q, x[u][2 * j], x[u][2 * j + 1]);
+        }
+      }
+    }
+  }
+  pdl_trigger();
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sums[warp][8 * i + 2 * t + k % 2][g + k / 2 * 8] = acc[i][k];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < kChannels * 8 * kTiles; e += 32 * kFewWarps) {
+    const int c = e % kChannels, i = e / kChannels, j = channel + c;
+    if (i >= a.rows || j >= a.channels) continue;
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < kFewWarps; ++k) sum += sums[k][i][c];
+    float y = static_cast<float>(sum) * a.row_scale[i] * a.channel_scale[j];
+    if (a.bias) y += unpack1<T>(a.bias[j]);
+    a.out[i * a.out_ld + j] = pack1<T>(y);
+  }
+}
+
 template <typename T>
 struct ScaledEpilogue {
   static constexpr bool kPaired = false;
@@ -299,25 +395,39 @@ struct ScaledEpilogue {
     float scale;
   };
   __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const { return Row{l.inside ? row_scale[i] : 0.f}; }
+  // A lane reads one column's scale and hands it round: a load a chunk, its latency
+  // under the tensor memory's.
   __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
+    const bool mine = j + l.lane < out.n;
+    const float scale = mine ? channel_scale[j + l.lane] : 0.f;
+    const float add = mine && bias ? unpack1<T>(bias[j + l.lane]) : 0.f;
 #pragma unroll
     for (int k = 0; k < kChunk; ++k) {
-      const int64_t c = j + k < out.n ? j + k : out.n - 1;
-      v[k] = value(v[k], r.scale, c);
+      v[k] = static_cast<float>(__float_as_int(v[k])) * r.scale * __shfl_sync(~0u, scale, k);
+      if (bias) v[k] += __shfl_sync(~0u, add, k);
     }
     out.template store<T>(l, i, j, v);
   }
-  __device__ __forceinline__ float value(float bits, float scale, int64_t j) const {
-    const float y = static_cast<float>(__float_as_int(bits)) * scale * channel_scale[j];
-    return bias ? y + unpack1<T>(bias[j]) : y;
-  }
   __device__ __forceinline__ void end(Row&, const Lane&, int64_t, int64_t) const {}
   __device__ __forceinline__ void point(int64_t i, int64_t j, float v) const {
-    out.p[i * out.ld + j] = pack1<T>(value(v, row_scale[i], j));
+    float y = static_cast<float>(__float_as_int(v)) * row_scale[i] * channel_scale[j];
+    if (bias) y += unpack1<T>(bias[j]);
+    out.p[i * out.ld + j] = pack1<T>(y);
   }
 };
 
 namespace {
+
+// Products that few_rows takes: rows of both operands in vectors of 16 bytes, and
+// up to 8 rows; more where the weight is small, since every CTA reads all of x
+// (us, few_rows against the tiles: 28672 x 4096, 1 row 20.1 / 25.2, 8 rows 21.8 /
+// 25.6, 16 rows 29 / 25.8; 6144 x 4096, 1 row 6.2 / 10.9, 16 rows 7.8 / 10.9, 24
+// rows 11.8 / 10.8; 1024 x 1024, 1 row 2.2 / 4.7, 32 rows 2.8 / 4.7).
+bool few_product(const void* x, const void* w, int64_t rows, int64_t hidden, int64_t channels, int64_t x_ld, int64_t w_ld) {
+  const int64_t most = rows <= 8 ? INT64_MAX : rows <= 16 ? int64_t{32} << 20 : rows <= 32 ? int64_t{8} << 20 : 0;
+  return rows >= 1 && hidden >= 1 && channels * hidden <= most && hidden % 16 == 0 && aligned(x, 16) && aligned(w, 16) &&
+         (rows <= 1 || x_ld % 16 == 0) && (channels <= 1 || w_ld % 16 == 0);
+}
 
 template <typename T, bool kNorm>
 void (*quant_kernel(int vec, int vpt))(QuantArgs) {
@@ -428,6 +538,7 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
   if ((rows > 1 && (input_row_stride < hidden || out_row_stride < channels)) ||
       (channels > 1 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
+  const bool few = few_product(input, weight, rows, hidden, channels, input_row_stride, weight_row_stride);
   Workspace ws(workspace, *workspace_bytes);
   const ByteRows x(ws, input, rows, hidden, input_row_stride);
   const ByteRows w(ws, weight, channels, hidden, weight_row_stride);
@@ -462,12 +573,23 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
                      copies);
     if (st != HPRN_OK) return st;
   }
-  Product q;
-  q.a = {x.data(), x.ld()};
-  q.b = {w.data(), w.ld()};
-  q.m = rows, q.n = channels, q.depth = pairs;
   auto launch = [&](auto t) {
     using T = decltype(t);
+    if (few) {
+      FewArgs f{};
+      f.out = static_cast<uint16_t*>(out), f.x = input, f.w = weight;
+      f.row_scale = input_scale, f.channel_scale = weight_scale, f.bias = static_cast<const uint16_t*>(bias);
+      f.out_ld = out_row_stride, f.x_ld = rows > 1 ? input_row_stride : hidden, f.w_ld = channels > 1 ? weight_row_stride : hidden;
+      f.rows = static_cast<int32_t>(rows), f.hidden = static_cast<int32_t>(hidden);
+      f.channels = static_cast<int32_t>(channels);
+      const auto fn = rows <= 8 ? few_rows<T, 1> : rows <= 16 ? few_rows<T, 2> : few_rows<T, 4>;
+      f.first_wave = static_cast<int32_t>(first_wave_ctas(dev, reinterpret_cast<const void*>(fn), 32 * kFewWarps));
+      return launch_rows(fn, dim3(static_cast<unsigned>((channels + 15) / 16)), dim3(32 * kFewWarps), cs, flags, what, f);
+    }
+    Product q;
+    q.a = {x.data(), x.ld()};
+    q.b = {w.data(), w.ld()};
+    q.m = rows, q.n = channels, q.depth = pairs;
     ScaledEpilogue<T> e;
     e.out = Out16(out, out_row_stride, channels);
     e.row_scale = input_scale, e.channel_scale = weight_scale, e.bias = static_cast<const uint16_t*>(bias);
