@@ -138,38 +138,58 @@ struct LogProbJoin {
   float *log_prob, *entropy, *lse;
 };
 
-// Joins a row's parts, one warp a row.
-__global__ void __launch_bounds__(256) log_prob_join(LogProbJoin q) {
-  pdl_wait();
-  const int lane = threadIdx.x % 32;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
-  if (i >= q.rows) return;
-  float m = -INFINITY, s = 0.f, a = 0.f;
-  auto join = [&](float pm, float ps, float pa) {
-    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
-    const float x0 = max_nan((m - ref) * q.to_log2, kLeastExponent), f0 = exp2_fast(x0);
-    const float x1 = max_nan((pm - ref) * q.to_log2, kLeastExponent), f1 = exp2_fast(x1);
-    a = f0 * fmaf(s, x0, a) + f1 * fmaf(ps, x1, pa);
-    s = s * f0 + ps * f1;
-    m = top;
-  };
-  for (int64_t k = lane; k < q.parts; k += 32) {
-    const float4 p = q.partial[i * q.parts + k];
-    join(p.x, p.y, p.z);
+// Joins the parts of row i, by a CTA of kThreads: the largest first, then the sums
+// relative to it, so that no term waits for another.  Returns the row's lse in every
+// thread.
+template <int kThreads>
+__device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ float most[kWarps], sums[2][kWarps];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const float4* parts = q.partial + i * q.parts;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int64_t k = threadIdx.x; k < q.parts; k += kThreads) m = fmaxf(m, parts[k].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (lane == 0) most[warp] = m;
+  __syncthreads();
+  m = most[0];
+#pragma unroll
+  for (int k = 1; k < kWarps; ++k) m = fmaxf(m, most[k]);
+  float top = m == -INFINITY ? 0.f : m, s = 0.f, a = 0.f;
+#pragma unroll 4
+  for (int64_t k = threadIdx.x; k < q.parts; k += kThreads) {
+    const float4 p = parts[k];
+    const float x = max_nan((p.x - top) * q.to_log2, kLeastExponent), f = exp2_fast(x);
+    s = fmaf(p.y, f, s);
+    a = fmaf(f, fmaf(p.y, x, p.z), a);
   }
-  for (int o = 16; o > 0; o >>= 1)
-    join(__shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), __shfl_xor_sync(~0u, a, o));
-  if (lane != 0) return;
-  if (q.parts == 0 && q.vocab > 0) m = 0.f, s = static_cast<float>(q.vocab), a = 0.f;
-  const float top = m == -INFINITY ? 0.f : m, log_s = logf(s);
-  q.lse[i] = fmaf(top, q.inv_t, log_s);
-  const int64_t t = target_of(q.target, i, q.ignore, q.vocab);
-  // The two logits first: where the target is the largest one the log probability
-  // is -log s, which a sum with a logit of 30 would round to multiples of 2^-19.
-  q.log_prob[i] = t == kIgnored   ? 0.f
-                  : t == kInvalid ? __int_as_float(0x7fc00000)
-                                  : ((q.parts > 0 ? q.target_logit[i] : 0.f) - top) * q.inv_t - log_s;
-  q.entropy[i] = t == kIgnored ? 0.f : log_s - 0.693147180559945f * (a / s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o), a += __shfl_xor_sync(~0u, a, o);
+  if (lane == 0) sums[0][warp] = s, sums[1][warp] = a;
+  __syncthreads();
+  s = sums[0][0], a = sums[1][0];
+#pragma unroll
+  for (int k = 1; k < kWarps; ++k) s += sums[0][k], a += sums[1][k];
+  if (q.parts == 0 && q.vocab > 0) top = 0.f, s = static_cast<float>(q.vocab), a = 0.f;
+  const float log_s = logf(s), lse = fmaf(top, q.inv_t, log_s);
+  if (threadIdx.x == 0) {
+    q.lse[i] = lse;
+    const int64_t t = target_of(q.target, i, q.ignore, q.vocab);
+    // The two logits first: where the target is the largest one the log probability
+    // is -log s, which a sum with a logit of 30 would round to multiples of 2^-19.
+    q.log_prob[i] = t == kIgnored   ? 0.f
+                    : t == kInvalid ? __int_as_float(0x7fc00000)
+                                    : ((q.parts > 0 ? q.target_logit[i] : 0.f) - top) * q.inv_t - log_s;
+    q.entropy[i] = t == kIgnored ? 0.f : log_s - 0.693147180559945f * (a / s);
+  }
+  return lse;
+}
+
+__global__ void __launch_bounds__(128) log_prob_join(LogProbJoin q) {
+  pdl_wait();
+  join_row<128>(q, blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -190,7 +210,7 @@ struct TopArgs {
   const uint16_t* x;
   const uint16_t* w;
   int64_t x_ld, w_ld;
-  const float* lse;
+  LogProbJoin join;
   double inv_t;
   int32_t top, candidates;
   float* values;
@@ -231,80 +251,129 @@ __device__ __forceinline__ uint64_t block_most(uint64_t key, uint64_t* part) {
 template <typename T>
 __device__ __forceinline__ double exact_dot(const uint16_t* x, const uint16_t* w, int64_t n) {
   const int lane = threadIdx.x % 32;
-  double s = 0.0;
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 2
   for (int64_t k = lane * 8; k < n; k += 256) {
     if (k + 8 <= n) {
       const uint4 a = *reinterpret_cast<const uint4*>(x + k), b = *reinterpret_cast<const uint4*>(w + k);
       const float2 p[4] = {mul_pair<T>(a.x, b.x), mul_pair<T>(a.y, b.y), mul_pair<T>(a.z, b.z), mul_pair<T>(a.w, b.w)};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += static_cast<double>(p[e].x), s += static_cast<double>(p[e].y);
+      for (int e = 0; e < 4; ++e) part[e] += static_cast<double>(p[e].x), part[e] += static_cast<double>(p[e].y);
     } else {
-      for (int64_t e = k; e < n; ++e) s += static_cast<double>(unpack1<T>(x[e]) * unpack1<T>(w[e]));
+      for (int64_t e = k; e < n; ++e) part[0] += static_cast<double>(unpack1<T>(x[e]) * unpack1<T>(w[e]));
     }
   }
+  double s = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   return s;
 }
 
-// One CTA per row.
+// One CTA per row.  A thread holds the largest of its share of the group maxima;
+// the `candidates` largest of those 256 have a last one, and no candidate lies below
+// it.  Groups that reach it, and then their logits that do, are collected (few more
+// than wanted, of logits in no particular order) and each one's place is counted.
+// Where more than kCollect reach it, groups and logits are picked one by one.
+constexpr int kCollect = 512;
+
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
-  __shared__ uint64_t part[2][kTopThreads / 32];
-  __shared__ uint32_t group_at[kMostCandidates], column[kMostCandidates];
+  __shared__ uint64_t part[2][kTopThreads / 32], best_of[kTopThreads], collected[kCollect], bound;
+  __shared__ uint32_t group_at[kCollect], column[kMostCandidates];
+  __shared__ int group_count, count;
   __shared__ double exact[kMostCandidates];
   pdl_wait();
   const int64_t i = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid % 32;
   float* values = a.values + i * a.top;
   int64_t* indices = a.indices + i * a.top;
+  if (tid == 0) group_count = count = 0;
+  if (tid < kMostCandidates) column[tid] = 0;
+  const float lse = join_row<kTopThreads>(a.join, i);
   if (a.hidden == 0) {  // logits that are sums of no terms
-    if (tid < a.top) values[tid] = -a.lse[i], indices[tid] = tid;
+    if (tid < a.top) values[tid] = -lse, indices[tid] = tid;
     return;
   }
-  const int groups = static_cast<int>(a.groups);
+  const int groups = static_cast<int>(a.groups), wanted = min(a.candidates, groups);
   const float* maxima = a.group_max + i * a.groups;
-  int turn = 0;
-  // The groups with the largest maxima.
+  const float* row = a.logits + i * a.groups * kChunk;
+  // The largest key below `limit` of the thread's groups.
   auto best_below = [&](uint64_t limit) {
     uint64_t best = 0;
+#pragma unroll 4
     for (int k = tid; k < groups; k += kTopThreads) {
       const uint64_t key = order_key(maxima[k], static_cast<uint32_t>(k));
       if (key < limit && key > best) best = key;
     }
     return best;
   };
-  const int wanted = min(a.candidates, groups);
   uint64_t mine = best_below(~uint64_t{0});
-  for (int c = 0; c < wanted; ++c) {
-    const uint64_t best = block_most(mine, part[turn]);
-    turn ^= 1;
-    if (mine == best) group_at[c] = key_index(best), mine = best_below(best);
+  best_of[tid] = mine;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int k = 0; k < kTopThreads; ++k) above += best_of[k] > mine;
+  if (above == wanted - 1) bound = mine;  // keys differ, but for those of threads without groups
+  __syncthreads();
+  const uint64_t least = bound;
+  if (mine >= least) {
+    for (int k = tid; k < groups; k += kTopThreads) {
+      if (order_key(maxima[k], static_cast<uint32_t>(k)) < least) continue;
+      const int at = atomicAdd(&group_count, 1);
+      if (at < kCollect) group_at[at] = k;
+    }
   }
   __syncthreads();
-  // The largest of their logits.
-  const float* row = a.logits + i * a.groups * kChunk;
-  uint64_t keys[kHeld];
-  mine = 0;
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) {
-    const int slot = tid + k * kTopThreads;
-    keys[k] = 0;
-    if (slot < wanted * kChunk) {
-      const uint32_t j = group_at[slot / kChunk] * kChunk + slot % kChunk;
-      if (j < a.vocab) keys[k] = order_key(row[j], j);
-    }
-    mine = keys[k] > mine ? keys[k] : mine;
+  // (A logit as large as the least group's maximum counts whatever its index; every
+  // logit where the groups are fewer than the candidates.)
+  const uint64_t least_logit = wanted < a.candidates ? 0 : least >> 32 << 32;
+  for (int g = tid / 32; g < min(group_count, kCollect); g += kTopThreads / 32) {
+    const uint32_t j = group_at[g] * kChunk + lane;
+    if (j >= a.vocab) continue;
+    const uint64_t key = order_key(row[j], j);
+    if (key < least_logit) continue;
+    const int at = atomicAdd(&count, 1);
+    if (at < kCollect) collected[at] = key;
   }
-  for (int c = 0; c < a.candidates; ++c) {
-    const uint64_t best = block_most(mine, part[turn]);
-    turn ^= 1;
-    if (mine == best) {
-      column[c] = key_index(best);
-      mine = 0;
+  __syncthreads();
+  if (group_count <= kCollect && count <= kCollect) {
+    for (int e = tid; e < count; e += kTopThreads) {
+      const uint64_t key = collected[e];
+      int place = 0;
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) place += collected[k] > key;
+      if (place < a.candidates) column[place] = key_index(key);
+    }
+  } else {
+    int turn = 0;
+    for (int c = 0; c < wanted; ++c) {
+      const uint64_t best = block_most(mine, part[turn]);
+      turn ^= 1;
+      if (mine == best) group_at[c] = key_index(best), mine = best_below(best);
+    }
+    __syncthreads();
+    uint64_t keys[kHeld];
+    mine = 0;
 #pragma unroll
-      for (int k = 0; k < kHeld; ++k) {
-        if (keys[k] < best) mine = keys[k] > mine ? keys[k] : mine;
+    for (int k = 0; k < kHeld; ++k) {
+      const int slot = tid + k * kTopThreads;
+      keys[k] = 0;
+      if (slot < wanted * kChunk) {
+        const uint32_t j = group_at[slot / kChunk] * kChunk + slot % kChunk;
+        if (j < a.vocab) keys[k] = order_key(row[j], j);
+      }
+      mine = keys[k] > mine ? keys[k] : mine;
+    }
+    for (int c = 0; c < a.candidates; ++c) {
+      const uint64_t best = block_most(mine, part[turn]);
+      turn ^= 1;
+      if (mine == best) {
+        column[c] = key_index(best);
+        mine = 0;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+          if (keys[k] < best) mine = keys[k] > mine ? keys[k] : mine;
+        }
       }
     }
   }
@@ -322,7 +391,7 @@ __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
     rank += other > bits || (other == bits && column[c] < column[tid]);
   }
   if (rank >= a.top) return;
-  values[rank] = static_cast<float>(exact[tid] * a.inv_t - static_cast<double>(a.lse[i]));
+  values[rank] = static_cast<float>(exact[tid] * a.inv_t - static_cast<double>(lse));
   indices[rank] = column[tid];
 }
 
@@ -479,13 +548,15 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       q.inv_t = static_cast<float>(1.0 / temperature);
       q.to_log2 = static_cast<float>(1.4426950408889634 / temperature);
       q.log_prob = log_prob + first, q.entropy = entropy + first, q.lse = lse + first;
-      r = launch_rows(log_prob_join, dim3(static_cast<unsigned>((count + 7) / 8)), dim3(256), cs, flags, what, q);
-      if (r != HPRN_OK) return r;
-      if (top == 0) continue;
+      if (top == 0) {
+        r = launch_rows(log_prob_join, dim3(static_cast<unsigned>(count)), dim3(128), cs, flags, what, q);
+        if (r != HPRN_OK) return r;
+        continue;
+      }
       TopArgs a{};
       a.logits = logits, a.group_max = group_max, a.groups = groups, a.vocab = vocab, a.hidden = hidden;
       a.x = x.data() + first * x.ld(), a.x_ld = x.ld(), a.w = w.data(), a.w_ld = w.ld();
-      a.lse = lse + first, a.inv_t = 1.0 / temperature;
+      a.join = q, a.inv_t = 1.0 / temperature;
       a.top = static_cast<int32_t>(top);
       a.candidates = static_cast<int32_t>(top + kSpareTop < vocab ? top + kSpareTop : vocab);
       a.values = top_log_probs + first * top, a.indices = top_indices + first * top;
