@@ -33,6 +33,8 @@ struct BlockNormArgs {
   uint32_t rows_per_gate;
   int32_t gate_row;  // the gate is a row of `hidden` values
   int32_t row_threads, nvec;
+  // Rows that are worked on at once where the grid is larger than that, else 0.
+  int32_t wave_rows;
   float scale, eps, inv_hidden;
 };
 
@@ -69,6 +71,14 @@ __global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) block_norm_rows(B
     if constexpr (kLoose) store_loose(base + row * stride, a.hidden, vector(k), v.w);
     else st_global<VEC>(base + row * stride + vector(k) * Vec<VEC>::kElems, v);
   };
+  // The first rows into L2 while the preceding grid drains, and then the row that
+  // will take this one's place.
+  auto ahead = [&](int64_t i) {
+    if (in != 0 || i >= a.rows) return;
+    prefetch_l2(a.x + i * a.x_stride, static_cast<uint64_t>(a.hidden) * 2);
+    prefetch_l2(a.r + i * a.r_stride, static_cast<uint64_t>(a.hidden) * 2);
+  };
+  if (a.wave_rows == 0 || row < a.wave_rows) ahead(row);
   pdl_wait();
 
   Vec<VEC> x[VPT], r[VPT];
@@ -78,6 +88,10 @@ __global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) block_norm_rows(B
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
     if (inside(k)) r[k] = load(a.r, a.r_stride, k);
+  if (a.wave_rows > 0) {
+    ahead(row + a.wave_rows);
+    pdl_trigger();
+  }
   const uint16_t* gate = a.g && valid ? a.g + (static_cast<uint32_t>(row) / a.rows_per_gate) * a.g_stride : nullptr;
   float inv_x = 1.f;
   if constexpr (kPost) {
@@ -114,7 +128,7 @@ __global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) block_norm_rows(B
     store(a.t, a.t_stride, k, o);
   }
   const float inv_t = rsqrtf(row_sum(s.x + s.y, part[1], warps, first_warp) * a.inv_hidden + a.eps);
-  pdl_trigger();
+  if (a.wave_rows == 0) pdl_trigger();
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     if (!inside(k)) break;
@@ -216,7 +230,7 @@ RowsKernel rows_kernel(int vec, int vpt) {
 }
 
 template <typename T>
-int launch_forward(BlockNormArgs& a, int vec, cudaStream_t stream, unsigned flags) {
+int launch_forward(BlockNormArgs& a, int vec, const DeviceInfo* dev, cudaStream_t stream, unsigned flags) {
   const char* what = "gated_add_rms_norm";
   const int64_t elems = vec > 0 ? vec / 2 : 8;
   a.nvec = static_cast<int32_t>((a.hidden + elems - 1) / elems);
@@ -227,6 +241,8 @@ int launch_forward(BlockNormArgs& a, int vec, cudaStream_t stream, unsigned flag
     if (!fn || threads > 1024) continue;
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
+    const int64_t wave = first_wave_ctas(dev, reinterpret_cast<const void*>(fn), static_cast<int>(threads) * groups) * groups;
+    a.wave_rows = wave > 0 && a.rows > wave ? static_cast<int32_t>(wave) : 0;
     return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),
                        dim3(static_cast<unsigned>(threads * groups)), stream, flags, what, a);
   }
@@ -301,8 +317,8 @@ int hprn_gated_add_rms_norm(void* out, void* residual_out, const void* input, co
                                 rows > 1 ? input_row_stride : 0, rows > 1 ? residual_row_stride : 0,
                                 gate_rows && gates > 1 ? gate_row_stride : 0});
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  return dtype == HPRN_DTYPE_BF16 ? launch_forward<__nv_bfloat16>(a, vec, cs, flags)
-                                  : launch_forward<__half>(a, vec, cs, flags);
+  return dtype == HPRN_DTYPE_BF16 ? launch_forward<__nv_bfloat16>(a, vec, dev, cs, flags)
+                                  : launch_forward<__half>(a, vec, dev, cs, flags);
 }
 
 }  // extern "C"

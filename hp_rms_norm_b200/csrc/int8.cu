@@ -29,6 +29,7 @@ struct QuantArgs {
   int64_t q_stride, t_stride, x_stride, r_stride;
   int32_t rows, hidden;
   int32_t row_threads, nvec;
+  int32_t wave_rows;  // as in gated_norm.cu
   float eps, inv_hidden;
 };
 
@@ -118,6 +119,12 @@ __global__ void __launch_bounds__(1024) quant_rows(QuantArgs a) {
     else v = ld_stream<VEC>(base + row * stride + vector(k) * Vec<VEC>::kElems, once);
     return v;
   };
+  auto ahead = [&](int64_t i) {
+    if (in != 0 || i >= a.rows) return;
+    prefetch_l2(a.x + i * a.x_stride, static_cast<uint64_t>(a.hidden) * 2);
+    if (a.r) prefetch_l2(a.r + i * a.r_stride, static_cast<uint64_t>(a.hidden) * 2);
+  };
+  if (a.wave_rows == 0 || row < a.wave_rows) ahead(row);
   pdl_wait();
 
   Vec<VEC> x[VPT], r[VPT];
@@ -128,6 +135,10 @@ __global__ void __launch_bounds__(1024) quant_rows(QuantArgs a) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
       if (inside(k)) r[k] = load(a.r, a.r_stride, k);
+  }
+  if (a.wave_rows > 0) {
+    ahead(row + a.wave_rows);
+    pdl_trigger();
   }
   float2 y[VPT][P], s = make_float2(0.f, 0.f);
   float most = 0.f;
@@ -165,7 +176,7 @@ __global__ void __launch_bounds__(1024) quant_rows(QuantArgs a) {
   if constexpr (kNorm) inv = rsqrtf(row_sum(s.x + s.y, part[0], warps, first_warp) * a.inv_hidden + a.eps);
   // max |y inv| = max |y| inv, rounded once: rounding keeps the order.
   most = row_amax(most, part[1], warps, first_warp) * inv;
-  pdl_trigger();
+  if (a.wave_rows == 0) pdl_trigger();
   const float scale = amax_nan(1e-12f, most, 0.f) / 127.f, by = 1.f / scale;
   if (valid && in == 0) a.scales[row] = scale;
 #pragma unroll
@@ -242,21 +253,49 @@ struct ByteCopies {
   ByteCopy c[2];
 };
 
+// A warp copies kByteSpan bytes of a row at a time: the words of memory that they
+// lie in, all of a lane's loads in flight, put together with the next lane's.  (517 x
+// 2731 and 1001 x 2731: BYTES_NEW us, 9.2 with single bytes.)
+constexpr int kByteSpan = 512;
+
 __global__ void __launch_bounds__(256) copy_byte_rows(ByteCopies both) {
   pdl_wait();
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const ByteCopy& c = both.c[k];
-    const int64_t per_row = c.dst_ld / 4, all = c.rows * per_row;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < all;
-         e += static_cast<int64_t>(gridDim.x) * 256) {
-      const int64_t i = e / per_row, j = (e - i * per_row) * 4;
-      const uint8_t* p = c.src + i * c.src_ld + j;
+  pdl_trigger();
+  const int lane = threadIdx.x % 32;
+  auto spans_of = [](const ByteCopy& c) { return c.rows * ((c.dst_ld + kByteSpan - 1) / kByteSpan); };
+  const int64_t first = spans_of(both.c[0]), all = first + spans_of(both.c[1]);
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; e < all;
+       e += static_cast<int64_t>(gridDim.x) * 8) {
+    const ByteCopy& c = e < first ? both.c[0] : both.c[1];
+    const int64_t span = e < first ? e : e - first, per_row = (c.dst_ld + kByteSpan - 1) / kByteSpan;
+    const int64_t i = span / per_row, j0 = (span - i * per_row) * kByteSpan;
+    const uint8_t* row = c.src + i * c.src_ld;
+    const uint8_t* end = c.src + (c.rows - 1) * c.src_ld + c.cols;  // of the tensor
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3);
+    // Word k of the span and those behind the row's start, whole where memory allows.
+    auto word = [&](int k) {
+      const uint8_t* p = row - shift + j0 + 4 * k;
+      if (p >= row + c.cols) return 0u;
+      if (p >= c.src && p + 4 <= end) return *reinterpret_cast<const uint32_t*>(p);
       uint32_t w = 0;
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        if (j + b < c.cols) w |= static_cast<uint32_t>(p[b]) << (8 * b);
-      *reinterpret_cast<uint32_t*>(c.dst + i * c.dst_ld + j) = w;
+        if (p + b >= c.src && p + b < end) w |= static_cast<uint32_t>(p[b]) << (8 * b);
+      return w;
+    };
+    uint32_t w[4], last[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = word(32 * k + lane);
+      last[k] = lane == 31 ? word(32 * k + 32) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t after = __shfl_down_sync(~0u, w[k], 1);
+      uint32_t v = __funnelshift_r(w[k], lane == 31 ? last[k] : after, 8 * shift);
+      const int64_t j = j0 + 4 * (32 * k + lane), left = c.cols - j;
+      if (left < 4) v = left <= 0 ? 0 : v & (0xffffffffu >> (8 * (4 - left)));
+      if (j < c.dst_ld) *reinterpret_cast<uint32_t*>(c.dst + i * c.dst_ld + j) = v;
     }
   }
 }
@@ -437,7 +476,7 @@ void (*quant_kernel(int vec, int vpt))(QuantArgs) {
 }
 
 template <typename T>
-int launch_quant(QuantArgs& a, int vec, cudaStream_t stream, unsigned flags) {
+int launch_quant(QuantArgs& a, int vec, const DeviceInfo* dev, cudaStream_t stream, unsigned flags) {
   const char* what = "rms_norm_int8";
   const int64_t elems = vec > 0 ? vec / 2 : 8;
   a.nvec = static_cast<int32_t>((a.hidden + elems - 1) / elems);
@@ -447,6 +486,8 @@ int launch_quant(QuantArgs& a, int vec, cudaStream_t stream, unsigned flags) {
     if (!fn || threads > 1024) continue;
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
+    const int64_t wave = first_wave_ctas(dev, reinterpret_cast<const void*>(fn), static_cast<int>(threads) * groups) * groups;
+    a.wave_rows = wave > 0 && a.rows > wave ? static_cast<int32_t>(wave) : 0;
     return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),
                        dim3(static_cast<unsigned>(threads * groups)), stream, flags, what, a);
   }
@@ -516,8 +557,8 @@ int hprn_rms_norm_int8(int8_t* out, float* scales, void* residual_out, const voi
     }
   }
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  return dtype == HPRN_DTYPE_BF16 ? launch_quant<__nv_bfloat16>(a, vec, cs, flags)
-                                  : launch_quant<__half>(a, vec, cs, flags);
+  return dtype == HPRN_DTYPE_BF16 ? launch_quant<__nv_bfloat16>(a, vec, dev, cs, flags)
+                                  : launch_quant<__half>(a, vec, dev, cs, flags);
 }
 
 int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, const int8_t* weight,
@@ -566,9 +607,10 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_int8";
   const ByteCopies copies{{x.copy(), w.copy()}};
-  const int64_t words = (copies.c[0].rows * copies.c[0].dst_ld + copies.c[1].rows * copies.c[1].dst_ld) / 4;
-  if (words > 0) {
-    const int64_t ctas = (words + 255) / 256, most = 32 * dev->sm_count;
+  int64_t spans = 0;
+  for (const ByteCopy& c : copies.c) spans += c.rows * ((c.dst_ld + kByteSpan - 1) / kByteSpan);
+  if (spans > 0) {
+    const int64_t ctas = (spans + 7) / 8, most = 16 * dev->sm_count;
     st = launch_rows(copy_byte_rows, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), cs, flags, what,
                      copies);
     if (st != HPRN_OK) return st;
