@@ -70,8 +70,9 @@ struct BlockGradArgs {
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies in
 // flight, and says so (report_give_up).
-// Few threads of many registers: 512 workers had 96 each and spilled 300 bytes.
-constexpr int kBlockThreads = 352;
+// Threads that work on rows, by their words: what their registers leave room for (96,
+// 128 and 168 each).
+__host__ __device__ constexpr int block_threads(int words) { return words <= 4 ? 608 : words <= 8 ? 480 : 352; }
 constexpr int kBlockSmem = 220 * 1024;
 constexpr int kBlockSlots = 4;
 constexpr int kBlockGroups = 16;
@@ -81,10 +82,11 @@ __device__ __forceinline__ void team_barrier(int barrier, int threads) {
   else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 }
 
-// The sums of four values over the `warps` warps from `first_warp` that hold a row,
-// which meet at hardware barrier `barrier`; `part` alternates between two buffers.
-// In a warp each lane goes on with half of its values twice, 6 shuffles for the 20
-// of four sums by themselves.
+// The sums of four values over the `warps` (at most 24) warps from `first_warp` that
+// hold a row, which meet at hardware barrier `barrier`; `part` alternates between two
+// buffers.  In a warp each lane goes on with half of its values twice, 6 shuffles for
+// the 20 of four sums by themselves; eight lanes each add up one value's sums of the
+// warps.
 __device__ __forceinline__ void team_sums(float (&v)[4], float4* part, int warps, int first_warp, int barrier) {
   const int lane = threadIdx.x % 32;
   const bool upper = lane & 16, odd = lane & 8;
@@ -95,19 +97,20 @@ __device__ __forceinline__ void team_sums(float (&v)[4], float4* part, int warps
   s += __shfl_xor_sync(~0u, odd ? a : b, 8);
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  if (warps == 1) {
+  if (warps > 1) {
+    float* sums = reinterpret_cast<float*>(part);
+    if (lane % 8 == 0) sums[threadIdx.x / 32 * 4 + lane / 8] = s;
+    team_barrier(barrier, warps * 32);
+    const int k = lane % 8;
+    const float* q = sums + (first_warp + k) * 4 + lane / 8;
+    s = k < warps ? q[0] : 0.f;
+    if (k + 8 < warps) s += q[32];
+    if (k + 16 < warps) s += q[64];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(~0u, s, 8 * k);
-    return;
+    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   }
-  if (lane % 8 == 0) reinterpret_cast<float*>(part + threadIdx.x / 32)[lane / 8] = s;
-  team_barrier(barrier, warps * 32);
-  float4 sum = part[first_warp];
-  for (int w = 1; w < warps; ++w) {
-    const float4 q = part[first_warp + w];
-    sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
-  }
-  v[0] = sum.x, v[1] = sum.y, v[2] = sum.z, v[3] = sum.w;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(~0u, s, 8 * k);
 }
 
 __device__ __forceinline__ void shared_words(uint32_t (&w)[4], uint32_t addr) {
@@ -133,13 +136,13 @@ __device__ __forceinline__ int64_t run_of(const BlockGradArgs& a, int64_t i) { r
 enum GateKind { kOneGate, kChannels, kGateRow, kGateEach };
 
 template <typename T, int W, bool kVectors, bool kPost, int kGate>
-__global__ void __launch_bounds__(kBlockThreads + 32, 1) block_grad_rows(BlockGradArgs a) {
+__global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(BlockGradArgs a) {
   constexpr int kVecs = W / 4;
   constexpr bool kHold = W <= 12;
   static_assert(kHold || kVectors, "vectors of loose rows are read by two threads");
   extern __shared__ __align__(128) unsigned char row_mem[];
   __shared__ __align__(8) uint64_t full[kBlockSlots], empty[kBlockSlots];
-  __shared__ float4 part[2][kBlockThreads / 32];
+  __shared__ float4 part[2][block_threads(W) / 32];
   __shared__ int gave_up[kBlockGroups];
   const int tid = threadIdx.x, row_threads = a.row_threads, groups = a.row_groups;
   const int workers = groups * row_threads;
@@ -769,13 +772,11 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
     a.dense = true;
     for (int k = 0; k < a.tensors; ++k) a.dense = a.dense && a.src_stride[k] == a.hidden;
     const int64_t slot = (nvec * 16 + (plan.vectors ? 0 : 16)) * a.tensors;
-    int best = 0;
     for (int words : {4, 8, 12, 24}) {
-      if (words > 12 && (!plan.vectors || best > 0)) break;
+      if (words > 12 && !plan.vectors) break;
       const int64_t threads = round_up((nvec + words / 4 - 1) / (words / 4), 32);
-      const bool few = a.rows <= 4 * 148;
-      if (threads > kBlockThreads || (words == 4 && threads > 128 && !few)) continue;
-      int64_t groups = kBlockThreads / threads;
+      if (threads > block_threads(words) || (words == 4 && threads > 128)) continue;
+      int64_t groups = block_threads(words) / threads;
       if (groups > 14) groups = 14;  // a hardware barrier each, and one for all
       if (groups > a.rows) groups = a.rows;
       // (Places for w, p and the gate's row.)
@@ -784,8 +785,7 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
       const bool staged = weights > 0 && weights + 2 * groups * slot <= kBlockSmem;
       int64_t slots = (kBlockSmem - (staged ? weights : 0)) / (groups * slot);
       if (slots > kBlockSlots) slots = kBlockSlots;
-      if (slots < 2 || threads * groups <= best) continue;
-      best = static_cast<int>(threads * groups);
+      if (slots < 2) continue;
       plan.words = words;
       a.row_threads = static_cast<int>(threads), a.row_groups = static_cast<int>(groups), a.slots = static_cast<int>(slots);
       a.staged = staged, a.ring_at = static_cast<uint32_t>(staged ? weights : 0);
@@ -793,7 +793,7 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
       plan.smem = static_cast<int>(ring > joined ? ring : joined);
       const int64_t need = (a.rows + groups - 1) / groups;
       a.ctas = need < 148 ? need : 148;
-      if (few || best >= 224) break;
+      break;
     }
     if (plan.words > 0) break;
   }
