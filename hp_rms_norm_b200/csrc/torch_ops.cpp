@@ -13,6 +13,8 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -875,21 +877,138 @@ void linear_int8(at::Tensor& out, const at::Tensor& input, const at::Tensor& inp
   });
 }
 
+// The operators that make their outputs: a call from Python spends 2 to 5 us less on
+// each than on a torch.empty of its own.
+at::Tensor dense_like(const at::Tensor& t) { return at::empty_like(t, at::MemoryFormat::Contiguous); }
+
+// One entry, or `last` of them, for each row of input.
+at::Tensor rows_like(const at::Tensor& input, at::ScalarType type, int64_t last = -1) {
+  c10::SymDimVector sizes(input.sym_sizes().begin(), input.sym_sizes().end() - (input.dim() > 0));
+  if (last >= 0) sizes.push_back(last);
+  return at::empty_symint(sizes, input.options().dtype(type));
+}
+
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, c10::optional<at::Tensor>>
+block_grads_like(const at::Tensor& input, const c10::optional<at::Tensor>& post_weight, const at::Tensor& weight,
+                 const c10::optional<at::Tensor>& gate) {
+  c10::optional<at::Tensor> grad_post, grad_gate;
+  if (post_weight.has_value()) grad_post = dense_like(*post_weight);
+  if (gate.has_value()) grad_gate = dense_like(*gate);
+  return {dense_like(input), dense_like(input), grad_post, dense_like(weight), grad_gate};
+}
+
+// Absent gradients are returned as tensors without elements.
+using BlockGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+BlockGrads gated_add_rms_norm_backward_new(const at::Tensor& grad_out, c10::optional<at::Tensor> grad_residual_out,
+                                           const at::Tensor& input, const at::Tensor& residual_out,
+                                           c10::optional<at::Tensor> post_weight, const at::Tensor& weight,
+                                           c10::optional<at::Tensor> gate, double residual_scale, double eps) {
+  auto [gi, gr, gp, gw, gg] = block_grads_like(input, post_weight, weight, gate);
+  if (gg.has_value() && input.numel() == 0) gg->zero_();  // a gate without rows
+  gated_add_rms_norm_backward(gi, gr, gp, gw, gg, grad_out, grad_residual_out, input, residual_out, post_weight,
+                              weight, gate, residual_scale, eps);
+  const at::Tensor none = gp.has_value() && gg.has_value() ? at::Tensor() : at::empty({0}, input.options());
+  return {gi, gr, gp.has_value() ? *gp : none, gw, gg.has_value() ? *gg : none};
+}
+
+BlockGrads gated_add_rms_norm_backward_new_meta(const at::Tensor&, c10::optional<at::Tensor>, const at::Tensor& input,
+                                                const at::Tensor&, c10::optional<at::Tensor> post_weight,
+                                                const at::Tensor& weight, c10::optional<at::Tensor> gate, double,
+                                                double) {
+  auto [gi, gr, gp, gw, gg] = block_grads_like(input, post_weight, weight, gate);
+  auto or_none = [&](const c10::optional<at::Tensor>& t) {
+    return t.has_value() ? *t : at::empty({0}, input.options());
+  };
+  return {gi, gr, or_none(gp), gw, or_none(gg)};
+}
+
+using LogProbOutputs = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+LogProbOutputs log_prob_outputs(const at::Tensor& input, int64_t top) {
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(top >= 0 && top <= 64, "top must be between 0 and 64 and at most vocab");
+  const at::Tensor log_prob = rows_like(input, at::kFloat);
+  return {log_prob, dense_like(log_prob), dense_like(log_prob), rows_like(input, at::kFloat, top),
+          rows_like(input, at::kLong, top)};
+}
+
+LogProbOutputs linear_log_probs_new(const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
+                                    int64_t top, double temperature, int64_t ignore_index) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  auto [log_prob, entropy, lse, values, indices] = log_prob_outputs(input, top);
+  c10::optional<at::Tensor> v, k;
+  if (top > 0) v = values, k = indices;
+  linear_log_probs(log_prob, entropy, lse, v, k, input, weight, target, temperature, ignore_index);
+  return {log_prob, entropy, lse, values, indices};
+}
+
+LogProbOutputs linear_log_probs_new_meta(const at::Tensor& input, const at::Tensor&, const at::Tensor&, int64_t top,
+                                         double, int64_t) {
+  return log_prob_outputs(input, top);
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_log_probs_backward_new(
+    const at::Tensor& grad_log_prob, c10::optional<at::Tensor> grad_entropy, const at::Tensor& input,
+    const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse, c10::optional<at::Tensor> entropy,
+    double temperature, int64_t ignore_index) {
+  at::Tensor gi = dense_like(input), gw = dense_like(weight);
+  linear_log_probs_backward(gi, gw, grad_log_prob, grad_entropy, input, weight, target, lse, entropy, temperature,
+                            ignore_index);
+  return {gi, gw};
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_log_probs_backward_new_meta(
+    const at::Tensor&, c10::optional<at::Tensor>, const at::Tensor& input, const at::Tensor& weight,
+    const at::Tensor&, const at::Tensor&, c10::optional<at::Tensor>, double, int64_t) {
+  return {dense_like(input), dense_like(weight)};
+}
+
+std::tuple<at::Tensor, at::Tensor> int8_outputs(const at::Tensor& input) {
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  return {at::empty_like(input, input.options().dtype(at::kChar), at::MemoryFormat::Contiguous),
+          rows_like(input, at::kFloat)};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_int8_new(const at::Tensor& input, c10::optional<at::Tensor> weight,
+                                                     c10::optional<at::Tensor> residual,
+                                                     c10::optional<at::Tensor> residual_out, double eps) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  auto [codes, scales] = int8_outputs(input);
+  rms_norm_int8(codes, scales, input, weight, residual, residual_out, eps);
+  return {codes, scales};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_int8_new_meta(const at::Tensor& input, c10::optional<at::Tensor>,
+                                                          c10::optional<at::Tensor>, c10::optional<at::Tensor>,
+                                                          double) {
+  return int8_outputs(input);
+}
+
+at::Tensor int8_product_like(const at::Tensor& input, const at::Tensor& weight, at::ScalarType dtype) {
+  TORCH_CHECK(input.dim() >= 1, "input.dim() >= 1");
+  TORCH_CHECK(weight.dim() == 2, "weight must be [channels, hidden]");
+  c10::SymDimVector sizes(input.sym_sizes().begin(), input.sym_sizes().end() - 1);
+  sizes.push_back(weight.sym_size(0));
+  return at::empty_symint(sizes, input.options().dtype(dtype));
+}
+
+at::Tensor linear_int8_new(const at::Tensor& input, const at::Tensor& input_scale, const at::Tensor& weight,
+                           const at::Tensor& weight_scale, c10::optional<at::Tensor> bias, at::ScalarType dtype) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  at::Tensor out = int8_product_like(input, weight, dtype);
+  linear_int8(out, input, input_scale, weight, weight_scale, bias);
+  return out;
+}
+
+at::Tensor linear_int8_new_meta(const at::Tensor& input, const at::Tensor&, const at::Tensor& weight,
+                                const at::Tensor&, c10::optional<at::Tensor>, at::ScalarType dtype) {
+  return int8_product_like(input, weight, dtype);
+}
+
 void gated_add_rms_norm_meta(at::Tensor&, at::Tensor&, c10::optional<at::Tensor>, const at::Tensor&,
                              c10::optional<at::Tensor>, const at::Tensor&, c10::optional<at::Tensor>,
                              double, double) {}
-void gated_add_rms_norm_backward_meta(at::Tensor&, at::Tensor&, c10::optional<at::Tensor>, at::Tensor&,
-                                      c10::optional<at::Tensor>, const at::Tensor&,
-                                      c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
-                                      c10::optional<at::Tensor>, const at::Tensor&,
-                                      c10::optional<at::Tensor>, double, double) {}
-void linear_log_probs_meta(at::Tensor&, at::Tensor&, at::Tensor&, c10::optional<at::Tensor>,
-                           c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
-                           const at::Tensor&, double, int64_t) {}
-void linear_log_probs_backward_meta(at::Tensor&, at::Tensor&, const at::Tensor&,
-                                    c10::optional<at::Tensor>, const at::Tensor&, const at::Tensor&,
-                                    const at::Tensor&, const at::Tensor&, c10::optional<at::Tensor>,
-                                    double, int64_t) {}
 void rms_norm_int8_meta(at::Tensor&, at::Tensor&, const at::Tensor&, c10::optional<at::Tensor>,
                         c10::optional<at::Tensor>, c10::optional<at::Tensor>, double) {}
 void linear_int8_meta(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
@@ -956,20 +1075,25 @@ TORCH_LIBRARY(hp_rms_norm, m) {
         "Tensor input, Tensor weight, Tensor? grad_residual, float eps) -> ()");
   m.def("gated_add_rms_norm(Tensor(a!) out, Tensor(b!) residual, Tensor(c!)? residual_out, Tensor input, "
         "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
-  m.def("gated_add_rms_norm_backward(Tensor(a!) grad_input, Tensor(b!) grad_residual, "
-        "Tensor(c!)? grad_post_weight, Tensor(d!) grad_weight, Tensor(e!)? grad_gate, Tensor grad_out, "
-        "Tensor? grad_residual_out, Tensor input, Tensor residual_out, Tensor? post_weight, "
-        "Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
-  m.def("linear_log_probs(Tensor(a!) log_prob, Tensor(b!) entropy, Tensor(c!) lse, "
-        "Tensor(d!)? top_log_probs, Tensor(e!)? top_indices, Tensor input, Tensor weight, Tensor target, "
-        "float temperature, int ignore_index) -> ()");
-  m.def("linear_log_probs_backward(Tensor(a!) grad_input, Tensor(b!) grad_weight, Tensor grad_log_prob, "
-        "Tensor? grad_entropy, Tensor input, Tensor weight, Tensor target, Tensor lse, Tensor? entropy, "
-        "float temperature, int ignore_index) -> ()");
+  // (Gradients of what is absent come back without elements, as do alternatives with top 0.)
+  m.def("gated_add_rms_norm_backward(Tensor grad_out, Tensor? grad_residual_out, Tensor input, "
+        "Tensor residual_out, Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, "
+        "float eps) -> (Tensor grad_input, Tensor grad_residual, Tensor grad_post_weight, "
+        "Tensor grad_weight, Tensor grad_gate)");
+  m.def("linear_log_probs(Tensor input, Tensor weight, Tensor target, int top, float temperature, "
+        "int ignore_index) -> (Tensor log_prob, Tensor entropy, Tensor lse, Tensor top_log_probs, "
+        "Tensor top_indices)");
+  m.def("linear_log_probs_backward(Tensor grad_log_prob, Tensor? grad_entropy, Tensor input, Tensor weight, "
+        "Tensor target, Tensor lse, Tensor? entropy, float temperature, int ignore_index) -> "
+        "(Tensor grad_input, Tensor grad_weight)");
   // Extensions: 8-bit integers.
-  m.def("rms_norm_int8(Tensor(a!) out, Tensor(b!) scales, Tensor input, Tensor? weight, "
+  m.def("rms_norm_int8(Tensor input, Tensor? weight, Tensor(a!)? residual, Tensor(b!)? residual_out, "
+        "float eps) -> (Tensor codes, Tensor scales)");
+  m.def("rms_norm_int8.out(Tensor(a!) out, Tensor(b!) scales, Tensor input, Tensor? weight, "
         "Tensor(c!)? residual, Tensor(d!)? residual_out, float eps) -> ()");
-  m.def("linear_int8(Tensor(a!) out, Tensor input, Tensor input_scale, Tensor weight, "
+  m.def("linear_int8(Tensor input, Tensor input_scale, Tensor weight, Tensor weight_scale, Tensor? bias, "
+        "ScalarType dtype) -> Tensor");
+  m.def("linear_int8.out(Tensor(a!) out, Tensor input, Tensor input_scale, Tensor weight, "
         "Tensor weight_scale, Tensor? bias) -> ()");
   m.def("grad_norm(Tensor(a!) norm, Tensor[] grads) -> ()");
   m.def("clip_grad_norm(Tensor(a!)[] out, Tensor(b!) norm, Tensor[] grads, float max_norm) -> ()");
@@ -993,11 +1117,13 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("grad_norm", &grad_norm);
   m.impl("clip_grad_norm", &clip_grad_norm);
   m.impl("gated_add_rms_norm", &gated_add_rms_norm);
-  m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward);
-  m.impl("linear_log_probs", &linear_log_probs);
-  m.impl("linear_log_probs_backward", &linear_log_probs_backward);
-  m.impl("rms_norm_int8", &rms_norm_int8);
-  m.impl("linear_int8", &linear_int8);
+  m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_new);
+  m.impl("linear_log_probs", &linear_log_probs_new);
+  m.impl("linear_log_probs_backward", &linear_log_probs_backward_new);
+  m.impl("rms_norm_int8", &rms_norm_int8_new);
+  m.impl("rms_norm_int8.out", &rms_norm_int8);
+  m.impl("linear_int8", &linear_int8_new);
+  m.impl("linear_int8.out", &linear_int8);
 }
 
 TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
@@ -1018,9 +1144,21 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("grad_norm", &grad_norm_meta);
   m.impl("clip_grad_norm", &clip_grad_norm_meta);
   m.impl("gated_add_rms_norm", &gated_add_rms_norm_meta);
-  m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_meta);
-  m.impl("linear_log_probs", &linear_log_probs_meta);
-  m.impl("linear_log_probs_backward", &linear_log_probs_backward_meta);
-  m.impl("rms_norm_int8", &rms_norm_int8_meta);
-  m.impl("linear_int8", &linear_int8_meta);
+  m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_new_meta);
+  m.impl("linear_log_probs", &linear_log_probs_new_meta);
+  m.impl("linear_log_probs_backward", &linear_log_probs_backward_new_meta);
+  m.impl("rms_norm_int8", &rms_norm_int8_new_meta);
+  m.impl("rms_norm_int8.out", &rms_norm_int8_meta);
+  m.impl("linear_int8", &linear_int8_new_meta);
+  m.impl("linear_int8.out", &linear_int8_meta);
+}
+
+// No gradients of their own (hp_rms_norm_b200.autograd has the differentiable forms):
+// outputs of these have no history, whatever their inputs ask for.
+TORCH_LIBRARY_IMPL(hp_rms_norm, Autograd, m) {
+  m.impl("gated_add_rms_norm_backward", torch::CppFunction::makeFallthrough());
+  m.impl("linear_log_probs", torch::CppFunction::makeFallthrough());
+  m.impl("linear_log_probs_backward", torch::CppFunction::makeFallthrough());
+  m.impl("rms_norm_int8", torch::CppFunction::makeFallthrough());
+  m.impl("linear_int8", torch::CppFunction::makeFallthrough());
 }

@@ -247,19 +247,10 @@ def gated_add_rms_norm_backward(grad_out, input, residual, post_weight, weight, 
     ``gated_add_rms_norm`` for a gradient of ``out`` and, with ``grad_residual``, one that reaches
     the new residual from its other uses.  ``residual`` is the new residual that the forward call
     wrote.  grad_post_weight and grad_gate are None where their tensors are."""
-    grad_input = _new_like(input)
-    grad_old = _new_like(input)
-    grad_post = None if post_weight is None else _new_like(post_weight)
-    grad_weight = _new_like(weight)
-    grad_gate = None
-    if gate is not None:
-        grad_gate = _new_like(gate)
-        if input.numel() == 0:
-            grad_gate.zero_()
-    _ops.gated_add_rms_norm_backward.default(grad_input, grad_old, grad_post, grad_weight, grad_gate,
-                                             grad_out, grad_residual, input, residual, post_weight,
-                                             weight, gate, residual_scale, eps)
-    return grad_input, grad_old, grad_post, grad_weight, grad_gate
+    grad_input, grad_old, grad_post, grad_weight, grad_gate = _ops.gated_add_rms_norm_backward.default(
+        grad_out, grad_residual, input, residual, post_weight, weight, gate, residual_scale, eps)
+    return (grad_input, grad_old, None if post_weight is None else grad_post, grad_weight,
+            None if gate is None else grad_gate)
 
 
 class LogProbs(NamedTuple):
@@ -279,17 +270,9 @@ def linear_log_probs(input, weight, target, top=0, temperature=1.0, ignore_index
     that ``linear_log_probs_backward`` takes, and for ``top`` > 0 (at most 64) the largest log
     probabilities of every row, float32 [..., top], with their int64 indices: the largest first,
     equal ones by their indices."""
-    lead = input.shape[:-1]
-    log_prob = torch.empty(lead, dtype=torch.float32, device=input.device)
-    entropy = torch.empty_like(log_prob)
-    lse = torch.empty_like(log_prob)
-    values = indices = None
-    if top:
-        values = torch.empty(lead + (top,), dtype=torch.float32, device=input.device)
-        indices = torch.empty(lead + (top,), dtype=torch.int64, device=input.device)
-    _ops.linear_log_probs.default(log_prob, entropy, lse, values, indices, input, weight, target,
-                                  temperature, ignore_index)
-    return LogProbs(log_prob, entropy, lse, values, indices)
+    log_prob, entropy, lse, values, indices = _ops.linear_log_probs.default(
+        input, weight, target, top, temperature, ignore_index)
+    return LogProbs(log_prob, entropy, lse, values if top else None, indices if top else None)
 
 
 def linear_log_probs_backward(grad_log_prob, input, weight, target, lse, entropy=None,
@@ -298,12 +281,8 @@ def linear_log_probs_backward(grad_log_prob, input, weight, target, lse, entropy
     probabilities and, where ``grad_entropy`` is given (with the forward call's ``entropy``), of
     their entropies, float32 [...]; the logits are computed again, one piece of the vocabulary at
     a time."""
-    grad_input = _new_like(input)
-    grad_weight = _new_like(weight)
-    _ops.linear_log_probs_backward.default(grad_input, grad_weight, grad_log_prob, grad_entropy,
-                                           input, weight, target, lse, entropy, temperature,
-                                           ignore_index)
-    return grad_input, grad_weight
+    return _ops.linear_log_probs_backward.default(grad_log_prob, grad_entropy, input, weight, target, lse,
+                                                  entropy, temperature, ignore_index)
 
 
 def rms_norm_int8(input, weight, eps, residual=None, residual_out=None):
@@ -311,10 +290,7 @@ def rms_norm_int8(input, weight, eps, residual=None, residual_out=None):
     ``residual`` itself without one) with an int8 output and one scale a row: returns (codes,
     scales), codes int8 of input's shape, scales float32 [...] = max|y| / 127, y ~ codes *
     scale.  ``linear_int8`` takes both."""
-    codes = torch.empty(input.shape, dtype=torch.int8, device=input.device)
-    scales = torch.empty(input.shape[:-1], dtype=torch.float32, device=input.device)
-    _ops.rms_norm_int8.default(codes, scales, input, weight, residual, residual_out, eps)
-    return codes, scales
+    return _ops.rms_norm_int8.default(input, weight, residual, residual_out, eps)
 
 
 def quantize_int8(input):
@@ -329,8 +305,8 @@ def linear_int8(input, input_scale, weight, weight_scale, bias=None, dtype=torch
     of type ``dtype`` (bfloat16 or float16).  The sums are exact.  Returns ``out`` [..., channels]
     of type ``dtype``."""
     if out is None:
-        out = torch.empty(input.shape[:-1] + weight.shape[:1], dtype=dtype, device=input.device)
-    _ops.linear_int8.default(out, input, input_scale, weight, weight_scale, bias)
+        return _ops.linear_int8.default(input, input_scale, weight, weight_scale, bias, dtype)
+    _ops.linear_int8.out(out, input, input_scale, weight, weight_scale, bias)
     return out
 
 

@@ -136,7 +136,7 @@ def test_quantised_strides_and_values(cuda):
         x = wide[:, offset:offset + hidden]
         out = torch.full((40, hidden + 40), 55, dtype=torch.int8, device=cuda)
         scale = torch.empty(40, device=cuda)
-        torch.ops.hp_rms_norm.rms_norm_int8.default(out[:, 8:8 + hidden], scale, x, None, None, None, 0.0)
+        torch.ops.hp_rms_norm.rms_norm_int8.out(out[:, 8:8 + hidden], scale, x, None, None, None, 0.0)
         want, want_scale = hp.quantize_int8(x.contiguous())
         assert torch.equal(out[:, 8:8 + hidden], want) and torch.equal(scale, want_scale)
         assert (out[:, :8] == 55).all() and (out[:, 8 + hidden:] == 55).all()
