@@ -31,7 +31,7 @@ CUDA_SOURCES = ["rms_norm.cu", "relu.cu", "act_and_mul.cu", "matmul.cu", "gated_
                 "linear_cross_entropy.cu", "linear_log_probs.cu", "rms_norm_backward.cu", "gated_norm.cu",
                 "gated_norm_backward.cu", "int8.cu", "grad_clip.cu", "runtime.cu"]
 HEADERS = ["vec.cuh", "bulk.cuh", "runtime.cuh", "rms_norm_kernels.cuh", "tcgen05.cuh", "matmul.cuh",
-           "gated.cuh", "gated_norm.cuh", "rows.cuh", "vocabulary.cuh"]
+           "gated.cuh", "few_rows.cuh", "gated_norm.cuh", "rows.cuh", "vocabulary.cuh"]
 
 # HPRN_DEBUG=1 (or the reference's own DEBUG=1, setup.py:23-28 there) builds
 # host code without optimisation and with debug symbols (device code keeps -O3

@@ -10,6 +10,7 @@
 
 #include <string>
 
+#include "few_rows.cuh"
 #include "matmul.cuh"
 #include "rows.cuh"
 #include "runtime.cuh"
@@ -253,50 +254,53 @@ struct ByteCopies {
   ByteCopy c[2];
 };
 
-// A warp copies kByteSpan bytes of a row at a time: the words of memory that they
-// lie in, all of a lane's loads in flight, put together with the next lane's.  (517 x
-// 2731 and 1001 x 2731: BYTES_NEW us, 9.2 with single bytes.)
+// A warp copies kByteSpan bytes of a row: the words of memory that they lie in, all
+// of a lane's loads in flight, put together with the next lane's.  blockIdx.y is the
+// span, z the operand.  (517 x 2731 and 1001 x 2731, nothing in L2: BYTES_NEW us, 9.2
+// with single bytes.)
 constexpr int kByteSpan = 512;
 
 __global__ void __launch_bounds__(256) copy_byte_rows(ByteCopies both) {
+  const ByteCopy& c = both.c[blockIdx.z];
+  const int lane = threadIdx.x % 32;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32, j0 = static_cast<int64_t>(blockIdx.y) * kByteSpan;
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x % 32;
-  auto spans_of = [](const ByteCopy& c) { return c.rows * ((c.dst_ld + kByteSpan - 1) / kByteSpan); };
-  const int64_t first = spans_of(both.c[0]), all = first + spans_of(both.c[1]);
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; e < all;
-       e += static_cast<int64_t>(gridDim.x) * 8) {
-    const ByteCopy& c = e < first ? both.c[0] : both.c[1];
-    const int64_t span = e < first ? e : e - first, per_row = (c.dst_ld + kByteSpan - 1) / kByteSpan;
-    const int64_t i = span / per_row, j0 = (span - i * per_row) * kByteSpan;
-    const uint8_t* row = c.src + i * c.src_ld;
-    const uint8_t* end = c.src + (c.rows - 1) * c.src_ld + c.cols;  // of the tensor
-    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3);
-    // Word k of the span and those behind the row's start, whole where memory allows.
-    auto word = [&](int k) {
-      const uint8_t* p = row - shift + j0 + 4 * k;
-      if (p >= row + c.cols) return 0u;
-      if (p >= c.src && p + 4 <= end) return *reinterpret_cast<const uint32_t*>(p);
-      uint32_t w = 0;
+  if (i >= c.rows || j0 >= c.dst_ld) return;
+  const uint8_t* row = c.src + i * c.src_ld;
+  const uint8_t* end = c.src + (c.rows - 1) * c.src_ld + c.cols;  // of the tensor
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3);
+  const uint8_t* from = row - shift + j0;
+  uint32_t w[5];  // words lane, 32 + lane, ...; the last one lane 31's alone
+  if (from >= c.src && from + kByteSpan + 4 <= end) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(from) + lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = p[32 * k];
+    w[4] = lane == 0 ? p[128] : 0;
+  } else {
+    // Words that reach out of the tensor byte by byte.
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      const uint8_t* p = from + 4 * (32 * k + lane);
+      w[k] = 0;
+      if ((k == 4 && lane > 0) || p >= end || p + 4 <= c.src) continue;
+      if (p >= c.src && p + 4 <= end) {
+        w[k] = *reinterpret_cast<const uint32_t*>(p);
+        continue;
+      }
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        if (p + b >= c.src && p + b < end) w |= static_cast<uint32_t>(p[b]) << (8 * b);
-      return w;
-    };
-    uint32_t w[4], last[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = word(32 * k + lane);
-      last[k] = lane == 31 ? word(32 * k + 32) : 0;
+        if (p + b >= c.src && p + b < end) w[k] |= static_cast<uint32_t>(p[b]) << (8 * b);
     }
+  }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t after = __shfl_down_sync(~0u, w[k], 1);
-      uint32_t v = __funnelshift_r(w[k], lane == 31 ? last[k] : after, 8 * shift);
-      const int64_t j = j0 + 4 * (32 * k + lane), left = c.cols - j;
-      if (left < 4) v = left <= 0 ? 0 : v & (0xffffffffu >> (8 * (4 - left)));
-      if (j < c.dst_ld) *reinterpret_cast<uint32_t*>(c.dst + i * c.dst_ld + j) = v;
-    }
+  for (int k = 0; k < 4; ++k) {
+    // The next lane's word; behind the last lane's comes the first one's next.
+    const uint32_t next = __shfl_sync(~0u, lane == 0 ? w[k + 1] : w[k], (lane + 1) % 32);
+    uint32_t v = __funnelshift_r(w[k], next, 8 * shift);
+    const int64_t j = j0 + 4 * (32 * k + lane), left = c.cols - j;
+    if (left < 4) v = left <= 0 ? 0 : v & (0xffffffffu >> (8 * (4 - left)));
+    if (j < c.dst_ld) *reinterpret_cast<uint32_t*>(c.dst + i * c.dst_ld + j) = v;
   }
 }
 
@@ -324,93 +328,24 @@ class ByteRows {
   uint8_t* copy_ = nullptr;
 };
 
-// Few rows: the weight's bytes bound the product, so it is read straight into
-// registers, without the tensor cores' pipeline of stages whose filling and
-// draining costs 6 us.  A CTA takes 16 channels, its warps shares of the sums in
-// blocks of 128 bytes, all of a warp's loads of several blocks in flight; the
-// products are mma.sync's 16 channels x 8 rows x 32 terms.  A lane's 32 bytes of a
-// block are the terms that the instruction wants of it in some order, the same for
-// both operands, which is all that a sum needs.  The shares meet in shared memory.
+// Few rows (few_rows.cuh), a CTA for 16 channels.
 struct FewArgs {
+  FewOperands in;
   uint16_t* out;
-  const int8_t* x;
-  const int8_t* w;
   const float* row_scale;
   const float* channel_scale;
   const uint16_t* bias;  // or null
-  int64_t out_ld, x_ld, w_ld;
-  int32_t rows, hidden, channels;
-  int32_t first_wave;  // CTAs that are resident at once
+  int64_t out_ld;
 };
-constexpr int kFewWarps = 8;
 
-__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// kTiles: tiles of 8 rows.
 template <typename T, int kTiles>
-__global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 4 : kTiles == 2 ? 3 : 2) few_rows(FewArgs a) {
-  constexpr int kChannels = 16, kBlocks = 2;  // blocks whose loads are in flight together
-  __shared__ int sums[kFewWarps][8 * kTiles][kChannels + 1];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
-  const int channel = blockIdx.x * kChannels;
-  if (blockIdx.x < a.first_wave && threadIdx.x < kChannels && channel + threadIdx.x < a.channels)
-    prefetch_l2(a.w + (channel + threadIdx.x) * a.w_ld, a.hidden);
-  pdl_wait();
-  const uint64_t once = policy_evict_first(), keep = policy_evict_last();
-  const int8_t* w0 = a.w + (channel + g) * a.w_ld;
-  int acc[kTiles][4] = {};
-  auto load = [&](uint32_t (&v)[8], const int8_t* p, int at, bool there, bool stream) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      Vec<16> q;
-      q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
-      if (there && at + 16 * h < a.hidden) {
-        if (stream) q = ld_stream<16>(p + at + 16 * h, once);
-        else q = ld_weight<16>(p + at + 16 * h, keep);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * h + k] = q.w[k];
-    }
-  };
-  for (int block = warp; block * 128 < a.hidden; block += kFewWarps * kBlocks) {
-    uint32_t w[kBlocks][2][8];
-#pragma unroll
-    for (int u = 0; u < kBlocks; ++u) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-        load(w[u][m], w0 + 8 * m * a.w_ld, (block + u * kFewWarps) * 128 + 32 * t, channel + g + 8 * m < a.channels, true);
-    }
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      uint32_t x[kBlocks][8];
-#pragma unroll
-      for (int u = 0; u < kBlocks; ++u)
-        load(x[u], a.x + (8 * i + g) * a.x_ld, (block + u * kFewWarps) * 128 + 32 * t, 8 * i + g < a.rows, false);
-#pragma unroll
-      for (int u = 0; u < kBlocks; ++u) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t q[4] = {w[u][0][2 * j], w[u][1][2 * j], w[u][0][2 * j + 1], w[u][1][2 * j + 1]};
-          mma_s8(acc[i], q, x[u][2 * j], x[u][2 * j + 1]);
-        }
-      }
-    }
-  }
-  pdl_trigger();
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) sums[warp][8 * i + 2 * t + k % 2][g + k / 2 * 8] = acc[i][k];
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < kChannels * 8 * kTiles; e += 32 * kFewWarps) {
-    const int c = e % kChannels, i = e / kChannels, j = channel + c;
-    if (i >= a.rows || j >= a.channels) continue;
+__global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 4 : kTiles == 2 ? 3 : 2) few_int8(FewArgs a) {
+  __shared__ FewSums<int8_t, kTiles, 1> sums;
+  const int channel = blockIdx.x * 16;
+  few_products<int8_t, kTiles, 1>(a.in, channel, sums);
+  for (int e = threadIdx.x; e < 16 * 8 * kTiles; e += 32 * kFewWarps) {
+    const int c = e % 16, i = e / 16, j = channel + c;
+    if (i >= a.in.rows || j >= a.in.channels) continue;
     int sum = 0;
 #pragma unroll
     for (int k = 0; k < kFewWarps; ++k) sum += sums[k][i][c];
@@ -457,9 +392,9 @@ struct ScaledEpilogue {
 
 namespace {
 
-// Products that few_rows takes: rows of both operands in vectors of 16 bytes, and
+// Products that few_int8 takes: rows of both operands in vectors of 16 bytes, and
 // up to 8 rows; more where the weight is small, since every CTA reads all of x
-// (us, few_rows against the tiles: 28672 x 4096, 1 row 20.1 / 25.2, 8 rows 21.8 /
+// (us, few_int8 against the tiles: 28672 x 4096, 1 row 20.1 / 25.2, 8 rows 21.8 /
 // 25.6, 16 rows 29 / 25.8; 6144 x 4096, 1 row 6.2 / 10.9, 16 rows 7.8 / 10.9, 24
 // rows 11.8 / 10.8; 1024 x 1024, 1 row 2.2 / 4.7, 32 rows 2.8 / 4.7).
 bool few_product(const void* x, const void* w, int64_t rows, int64_t hidden, int64_t channels, int64_t x_ld, int64_t w_ld) {
@@ -607,25 +542,27 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_int8";
   const ByteCopies copies{{x.copy(), w.copy()}};
-  int64_t spans = 0;
-  for (const ByteCopy& c : copies.c) spans += c.rows * ((c.dst_ld + kByteSpan - 1) / kByteSpan);
-  if (spans > 0) {
-    const int64_t ctas = (spans + 7) / 8, most = 16 * dev->sm_count;
-    st = launch_rows(copy_byte_rows, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), cs, flags, what,
-                     copies);
-    if (st != HPRN_OK) return st;
+  int64_t most_rows = 0, most_bytes = 0;
+  for (const ByteCopy& c : copies.c) {
+    if (c.rows > most_rows) most_rows = c.rows;
+    if (c.dst_ld > most_bytes) most_bytes = c.dst_ld;
+  }
+  if (most_rows > 0) {
+    const dim3 grid(static_cast<unsigned>((most_rows + 7) / 8), static_cast<unsigned>((most_bytes + kByteSpan - 1) / kByteSpan), 2);
+    if ((st = launch_rows(copy_byte_rows, grid, dim3(256), cs, flags, what, copies)) != HPRN_OK) return st;
   }
   auto launch = [&](auto t) {
     using T = decltype(t);
     if (few) {
       FewArgs f{};
-      f.out = static_cast<uint16_t*>(out), f.x = input, f.w = weight;
+      f.in.x = reinterpret_cast<const uint8_t*>(input), f.in.w = reinterpret_cast<const uint8_t*>(weight);
+      f.in.x_ld = rows > 1 ? input_row_stride : hidden, f.in.w_ld = channels > 1 ? weight_row_stride : hidden;
+      f.in.rows = static_cast<int32_t>(rows), f.in.bytes = static_cast<int32_t>(hidden);
+      f.in.channels = static_cast<int32_t>(channels);
+      f.out = static_cast<uint16_t*>(out), f.out_ld = out_row_stride;
       f.row_scale = input_scale, f.channel_scale = weight_scale, f.bias = static_cast<const uint16_t*>(bias);
-      f.out_ld = out_row_stride, f.x_ld = rows > 1 ? input_row_stride : hidden, f.w_ld = channels > 1 ? weight_row_stride : hidden;
-      f.rows = static_cast<int32_t>(rows), f.hidden = static_cast<int32_t>(hidden);
-      f.channels = static_cast<int32_t>(channels);
-      const auto fn = rows <= 8 ? few_rows<T, 1> : rows <= 16 ? few_rows<T, 2> : few_rows<T, 4>;
-      f.first_wave = static_cast<int32_t>(first_wave_ctas(dev, reinterpret_cast<const void*>(fn), 32 * kFewWarps));
+      const auto fn = rows <= 8 ? few_int8<T, 1> : rows <= 16 ? few_int8<T, 2> : few_int8<T, 4>;
+      f.in.first_wave = static_cast<int32_t>(first_wave_ctas(dev, reinterpret_cast<const void*>(fn), 32 * kFewWarps));
       return launch_rows(fn, dim3(static_cast<unsigned>((channels + 15) / 16)), dim3(32 * kFewWarps), cs, flags, what, f);
     }
     Product q;

@@ -33,6 +33,7 @@
 
 #include <string>
 
+#include "few_rows.cuh"
 #include "matmul.cuh"
 #include "runtime.cuh"
 #include "vocabulary.cuh"
@@ -192,6 +193,42 @@ __global__ void __launch_bounds__(128) log_prob_join(LogProbJoin q) {
   join_row<128>(q, blockIdx.x);
 }
 
+// Few rows (few_rows.cuh): a CTA computes 32 columns' logits, which are a group and
+// a part; a warp each takes a row of them.
+struct FewLogits {
+  FewOperands in;
+  LogProbEpilogue<true> out;  // logits and group_max null where they are not wanted
+};
+
+template <typename T, int kTiles>
+__global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 3 : 2) few_logits(FewLogits a) {
+  __shared__ FewSums<T, kTiles, 2> sums;
+  const int first = blockIdx.x * kChunk;
+  few_products<T, kTiles, 2>(a.in, first, sums);
+  const int lane = threadIdx.x % 32;
+  const LogProbEpilogue<true>& o = a.out;
+  for (int i = threadIdx.x / 32; i < a.in.rows; i += kFewWarps) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kFewWarps; ++k) v += sums[k][i][lane];
+    const int64_t j = first + lane;
+    const bool inside = j < o.vocab;
+    if (!inside) v = -INFINITY;
+    if (inside && target_of(o.target, i, o.ignore, o.vocab) == j) o.target_logit[i] = v;
+    if (o.logits) o.logits[i * (o.groups * kChunk) + j] = v;
+    float m = v;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, s));
+    const float x = max_nan((v - (m == -INFINITY ? 0.f : m)) * o.to_log2, kLeastExponent), e = exp2_fast(x);
+    float s = e, t = e * x;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(~0u, s, k), t += __shfl_xor_sync(~0u, t, k);
+    if (lane > 0) continue;
+    o.partial[i * o.parts + blockIdx.x] = make_float4(m, s, t, 0.f);
+    if (o.group_max) o.group_max[i * o.groups + blockIdx.x] = m;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // The largest logits of a row.
 
@@ -246,23 +283,33 @@ __device__ __forceinline__ uint64_t block_most(uint64_t key, uint64_t* part) {
   return key;
 }
 
-// sum_k x_k w_k in 64 bits, by a warp: the product of two 16-bit numbers is exact
-// in 32.  Both rows start on 16-byte boundaries.
+// sum_k x_k w_k over first <= k < n in 64 bits, by a warp: the product of two 16-bit
+// numbers is exact in 32.  Both rows start on 16-byte boundaries, first is a multiple
+// of 8.
 template <typename T>
-__device__ __forceinline__ double exact_dot(const uint16_t* x, const uint16_t* w, int64_t n) {
+__device__ __forceinline__ double exact_dot(const uint16_t* x, const uint16_t* w, int64_t first, int64_t n) {
   const int lane = threadIdx.x % 32;
+  // Loads of 1024 elements in flight; four sums a lane.
+  constexpr int kAhead = 4;
   double part[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 2
-  for (int64_t k = lane * 8; k < n; k += 256) {
-    if (k + 8 <= n) {
-      const uint4 a = *reinterpret_cast<const uint4*>(x + k), b = *reinterpret_cast<const uint4*>(w + k);
-      const float2 p[4] = {mul_pair<T>(a.x, b.x), mul_pair<T>(a.y, b.y), mul_pair<T>(a.z, b.z), mul_pair<T>(a.w, b.w)};
+  const int64_t whole = n & ~int64_t{7};
+  for (int64_t k0 = first; k0 < whole; k0 += kAhead * 256) {
+    uint4 a[kAhead], b[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t k = k0 + u * 256 + lane * 8;
+      a[u] = b[u] = make_uint4(0, 0, 0, 0);
+      if (k < whole) a[u] = *reinterpret_cast<const uint4*>(x + k), b[u] = *reinterpret_cast<const uint4*>(w + k);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float2 p[4] = {mul_pair<T>(a[u].x, b[u].x), mul_pair<T>(a[u].y, b[u].y), mul_pair<T>(a[u].z, b[u].z),
+                           mul_pair<T>(a[u].w, b[u].w)};
 #pragma unroll
       for (int e = 0; e < 4; ++e) part[e] += static_cast<double>(p[e].x), part[e] += static_cast<double>(p[e].y);
-    } else {
-      for (int64_t e = k; e < n; ++e) part[0] += static_cast<double>(unpack1<T>(x[e]) * unpack1<T>(w[e]));
     }
   }
+  if (whole >= first && whole + lane < n) part[0] += static_cast<double>(unpack1<T>(x[whole + lane]) * unpack1<T>(w[whole + lane]));
   double s = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
@@ -278,10 +325,11 @@ constexpr int kCollect = 512;
 
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
-  __shared__ uint64_t part[2][kTopThreads / 32], best_of[kTopThreads], collected[kCollect], bound;
+  constexpr int kWarps = kTopThreads / 32;
+  __shared__ uint64_t part[2][kWarps], best_of[kTopThreads], collected[kCollect], bound;
   __shared__ uint32_t group_at[kCollect], column[kMostCandidates];
   __shared__ int group_count, count;
-  __shared__ double exact[kMostCandidates];
+  __shared__ double exact[kMostCandidates], shares[kWarps];
   pdl_wait();
   const int64_t i = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32;
@@ -289,6 +337,7 @@ __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
   int64_t* indices = a.indices + i * a.top;
   if (tid == 0) group_count = count = 0;
   if (tid < kMostCandidates) column[tid] = 0;
+  const uint16_t* x = a.x + i * a.x_ld;
   const float lse = join_row<kTopThreads>(a.join, i);
   if (a.hidden == 0) {  // logits that are sums of no terms
     if (tid < a.top) values[tid] = -lse, indices[tid] = tid;
@@ -327,7 +376,7 @@ __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
   // (A logit as large as the least group's maximum counts whatever its index; every
   // logit where the groups are fewer than the candidates.)
   const uint64_t least_logit = wanted < a.candidates ? 0 : least >> 32 << 32;
-  for (int g = tid / 32; g < min(group_count, kCollect); g += kTopThreads / 32) {
+  for (int g = tid / 32; g < min(group_count, kCollect); g += kWarps) {
     const uint32_t j = group_at[g] * kChunk + lane;
     if (j >= a.vocab) continue;
     const uint64_t key = order_key(row[j], j);
@@ -378,9 +427,24 @@ __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
     }
   }
   __syncthreads();
-  for (int c = tid / 32; c < a.candidates; c += kTopThreads / 32) {
-    const double s = exact_dot<T>(a.x + i * a.x_ld, a.w + static_cast<int64_t>(column[c]) * a.w_ld, a.hidden);
-    if (tid % 32 == 0) exact[c] = s;
+  // The candidates' weights into L2 at once: 8 warps take them in turn.
+  if (tid < a.candidates)
+    prefetch_l2(a.w + static_cast<int64_t>(column[tid]) * a.w_ld, static_cast<uint64_t>(a.hidden) * 2);
+  // Several warps a candidate where there are more.
+  const int parts = max(1, kWarps / a.candidates), warp = tid / 32;
+  const int64_t length = (a.hidden + 8 * parts - 1) / (8 * parts) * 8;
+  for (int task = warp; task < a.candidates * parts; task += kWarps) {
+    const int c = task / parts;
+    const int64_t first = (task - c * parts) * length;
+    const double s = exact_dot<T>(x, a.w + static_cast<int64_t>(column[c]) * a.w_ld, first,
+                                  min(first + length, a.hidden));
+    if (lane == 0) (parts > 1 ? shares[task] : exact[c]) = s;
+  }
+  __syncthreads();
+  if (parts > 1 && tid < a.candidates) {
+    double s = 0.0;
+    for (int k = 0; k < parts; ++k) s += shares[tid * parts + k];
+    exact[tid] = s;
   }
   __syncthreads();
   if (tid >= a.candidates) return;
@@ -493,7 +557,14 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
   const int64_t groups = top > 0 ? (vocab + kChunk - 1) / kChunk : 0;
   const int64_t block = top > 0 ? rows_of_block(rows, groups) : rows;
   const PlannedProduct<false, true, true> product(ws, block, vocab, hidden, false);
-  const int64_t parts = product.parts(vocab);
+  // few_logits, of rows that are read where they are, against the tiles (us, no
+  // alternatives): 1 row of 1024 x 32768 17.1 / 18.5, of 2048 x 50000 39.0 / 40.6, of
+  // 4096 x 131072 176 / 170; 8 rows 18.5 / 19.3, 40.7 / 40.5; 12 rows 23.3 / 19.3; of 512
+  // x 2000 1 row 5.2 / 7.6, 16 rows 5.8 / 7.7.
+  const int64_t few_most = rows <= 8 ? int64_t{1} << 27 : rows <= 16 ? int64_t{1} << 22 : 0;
+  const bool few = vocab > 0 && hidden > 0 && vocab * hidden <= few_most && hidden % 8 == 0 &&
+                   tma_rows(input, rows, input_row_stride) && tma_rows(weight, vocab, weight_row_stride);
+  const int64_t parts = few ? (vocab + kChunk - 1) / kChunk : product.parts(vocab);
   float4* partial = ws.take<float4>(parts * block);
   float* target_logit = ws.take<float>(block);
   float* group_max = ws.take<float>(groups * block);
@@ -521,7 +592,7 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_log_probs";
-  if ((st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
+  if (!few && (st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
   auto all = [&](auto t) {
     using T = decltype(t);
     auto launch = [&](auto epilogue, int64_t first, int64_t count) {
@@ -533,13 +604,27 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       epilogue.ignore = ignore_index, epilogue.parts = parts, epilogue.vocab = vocab;
       epilogue.to_log2 = static_cast<float>(1.4426950408889634 / temperature);
       epilogue.logits = logits, epilogue.group_max = group_max, epilogue.groups = groups;
+      if constexpr (std::is_same<decltype(epilogue), LogProbEpilogue<true>>::value) {
+        if (few) {
+          FewLogits f{};
+          f.out = epilogue;
+          if (top == 0) f.out.logits = f.out.group_max = nullptr;
+          f.in.x = static_cast<const uint8_t*>(input), f.in.w = static_cast<const uint8_t*>(weight);
+          f.in.x_ld = rows > 1 ? input_row_stride * 2 : 0, f.in.w_ld = vocab > 1 ? weight_row_stride * 2 : 0;
+          f.in.rows = static_cast<int32_t>(rows), f.in.channels = static_cast<int32_t>(vocab);
+          f.in.bytes = static_cast<int32_t>(hidden * 2);
+          const auto fn = rows <= 8 ? few_logits<T, 1> : few_logits<T, 2>;
+          f.in.first_wave = static_cast<int32_t>(first_wave_ctas(dev, reinterpret_cast<const void*>(fn), 32 * kFewWarps));
+          return launch_rows(fn, dim3(static_cast<unsigned>(parts)), dim3(32 * kFewWarps), cs, flags, what, f);
+        }
+      }
       return product.launch_whole<T>(q, epilogue, cs, flags, what);
     };
     int r = HPRN_OK;
     for (int64_t first = 0; first < rows; first += block) {
       const int64_t count = rows - first < block ? rows - first : block;
       if (hidden > 0) {
-        r = top > 0 ? launch(LogProbEpilogue<true>{}, first, count) : launch(LogProbEpilogue<false>{}, first, count);
+        r = top > 0 || few ? launch(LogProbEpilogue<true>{}, first, count) : launch(LogProbEpilogue<false>{}, first, count);
         if (r != HPRN_OK) return r;
       }
       LogProbJoin q{};
@@ -556,6 +641,8 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       TopArgs a{};
       a.logits = logits, a.group_max = group_max, a.groups = groups, a.vocab = vocab, a.hidden = hidden;
       a.x = x.data() + first * x.ld(), a.x_ld = x.ld(), a.w = w.data(), a.w_ld = w.ld();
+      if (few) a.x = static_cast<const uint16_t*>(input), a.w = static_cast<const uint16_t*>(weight);
+      if (few) a.x_ld = rows > 1 ? input_row_stride : hidden, a.w_ld = vocab > 1 ? weight_row_stride : hidden;
       a.join = q, a.inv_t = 1.0 / temperature;
       a.top = static_cast<int32_t>(top);
       a.candidates = static_cast<int32_t>(top + kSpareTop < vocab ? top + kSpareTop : vocab);
