@@ -455,7 +455,8 @@ int hprn_rms_norm_int8(int8_t* out, float* scales, void* residual_out, const voi
   if (rows > 1 && (out_row_stride < hidden || input_row_stride < hidden ||
                    (residual && (residual_row_stride < hidden || residual_out_row_stride < hidden))))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
-  if (rows == 0 || hidden == 0) return ok();
+  if (rows > 0 && hidden == 0) return fail(HPRN_ERR_INVALID_ARGUMENT, "hidden must be at least 1: a row of nothing has no scale");
+  if (rows == 0) return ok();
   if (!out || !scales || !input) return fail(HPRN_ERR_INVALID_ARGUMENT, "null tensor pointer");
   for (const void* p : {static_cast<const void*>(residual_out), input, weight, residual})
     if (!aligned(p, 2)) return fail(HPRN_ERR_INVALID_ARGUMENT, "tensor pointers must be aligned to their elements");

@@ -523,6 +523,9 @@ struct LogProbGradEpilogue {
 
 namespace {
 
+// Temperatures whose inverses fp32 holds with room for log2(e).
+constexpr double kLeastTemperature = 1e-30, kMostTemperature = 1e30;
+
 // What a block of rows may take for its logits.
 constexpr int64_t kLogitBytes = int64_t{1} << 30;
 
@@ -547,8 +550,8 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
   if (st != HPRN_OK) return st;
   if ((rows > 1 && input_row_stride < hidden) || (vocab > 1 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
-  if (!(temperature > 0.0) || !(temperature < INFINITY))
-    return fail(HPRN_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (!(temperature >= kLeastTemperature) || !(temperature <= kMostTemperature))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "temperature must be between 1e-30 and 1e30");
   if (top < 0 || top > kMostTop || top > vocab)
     return fail(HPRN_ERR_INVALID_ARGUMENT, "top must be between 0 and 64 and at most vocab");
   Workspace ws(workspace, *workspace_bytes);
@@ -668,8 +671,8 @@ int hprn_linear_log_probs_backward(void* grad_input, void* grad_weight, const fl
   if ((rows > 1 && (input_row_stride < hidden || grad_input_row_stride < hidden)) ||
       (vocab > 1 && (weight_row_stride < hidden || grad_weight_row_stride < hidden)))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
-  if (!(temperature > 0.0) || !(temperature < INFINITY))
-    return fail(HPRN_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (!(temperature >= kLeastTemperature) || !(temperature <= kMostTemperature))
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "temperature must be between 1e-30 and 1e30");
   Workspace ws(workspace, *workspace_bytes);
   const int64_t x_ld = round_up(hidden, 16);
   uint16_t* x = ws.take<uint16_t>(rows * x_ld);  // X without the ignored rows

@@ -845,7 +845,7 @@ void rms_norm_int8(at::Tensor& out, at::Tensor& scales, const at::Tensor& input,
     r = rows_arg(*residual, "residual", hidden, input, type);
     t = rows_arg(total, "residual_out", hidden, input, type);
   }
-  if (rows == 0 || hidden == 0) return;
+  if (rows == 0) return;
   const c10::cuda::CUDAGuard guard(input.device());
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(input.device().index()).stream();
   check_status(hprn_rms_norm_int8(static_cast<int8_t*>(q.p), sp, t.p, x.p, w.p, r.p, rows, hidden, q.stride,

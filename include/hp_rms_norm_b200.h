@@ -398,7 +398,8 @@ HPRN_API int hprn_gated_add_rms_norm_backward(
  *                 is missed only where more than four others lie between it and
  *                 the last place within the rounding of an fp32 sum.  In rows with a
  *                 NaN logit the values are NaN and the indices any.
- * 0 <= top <= 64, top <= vocab; top_* may be NULL where top is 0.  The outputs of
+ * 1e-30 <= temperature <= 1e30; 0 <= top <= 64, top <= vocab; top_* may be NULL
+ * where top is 0.  The outputs of
  * rows are dense.  With top > 0 the workspace holds the logits of a block of rows,
  * 1 GiB at most where 256 rows fit in that.
  */
@@ -436,7 +437,7 @@ HPRN_API int hprn_linear_log_probs_backward(
  *   t = input, or input + residual (fp32; residual_out = round_T of it)
  *   y = t weight rsqrt(eps + mean(t^2)), or y = t where weight is NULL
  *   scales[i] = max(max_j |y_ij|, 1e-12) / 127,  out_ij = round(y_ij (1 / scales[i])),
- * to nearest even, in [-127, 127]; t is not rounded in between.  residual and
+ * to nearest even, in [-127, 127]; t is not rounded in between; hidden >= 1.  residual and
  * residual_out go together and may be one tensor; a row with a NaN has a NaN scale,
  * one with an infinity an infinite or NaN scale.
  */
@@ -513,7 +514,7 @@ HPRN_API int hprn_set_plan_override(const char* plan);
  * stage rows of hprn_rms_norm* through TMA bulk copies (plan kind tma, reached
  * only through a plan override), the matrix products of hprn_gated_linear*,
  * hprn_linear_cross_entropy*, hprn_linear_log_probs* and hprn_linear_int8, and
- * hprn_rms_norm_backward.  A CTA that gives up
+ * hprn_rms_norm_backward and hprn_gated_add_rms_norm_backward.  A CTA that gives up
  * a wait stops, once its copies in flight have landed, and counts itself here,
  * on its device: in the tma plans it leaves the row it gave up on and its
  * remaining rows untouched (input and residual as they were), in the others
@@ -547,7 +548,7 @@ HPRN_API int hprn_test_stall_bulk_copy(int64_t row, uint64_t wait_limit_ns);
 /*
  * No reference counterpart.  Test hook for the same waits of the training
  * operators: while `on` is non-zero, every launch of their matrix products and
- * of hprn_rms_norm_backward loads nothing, so that its waits run out, after
+ * of the norms' backward kernels loads nothing, so that its waits run out, after
  * `wait_limit_ns` nanoseconds each (at most one second; 0 keeps that), and its
  * CTAs take their give-up path.  No fault and no hang: every wait stays
  * bounded.  Process-global; for tests only.
