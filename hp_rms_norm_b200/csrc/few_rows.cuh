@@ -19,7 +19,7 @@ namespace hprn {
 constexpr int kFewWarps = 8;
 
 struct FewOperands {
-  const uint8_t* x;  // rows of 16-byte vectors, `bytes` of them each
+  const uint8_t* x;  // rows of `bytes`
   const uint8_t* w;
   int64_t x_ld, w_ld;  // in bytes
   int32_t rows, channels, bytes;
@@ -69,7 +69,8 @@ using FewSums = typename FewMma<T>::Sum[kFewWarps][8 * kTiles][16 * kWide + 1];
 // The CTA's products with the 16 kWide weight rows from `channel` on: each warp's
 // share into `sums`, which the caller adds up after this (a barrier is its end).
 // kTiles: tiles of 8 rows of x.
-template <typename T, int kTiles, int kWide>
+// kAlign: what every row's start and length are multiples of, 16 or 8 bytes.
+template <typename T, int kTiles, int kWide, int kAlign>
 __device__ __forceinline__ void few_products(const FewOperands& a, int channel, FewSums<T, kTiles, kWide>& sums) {
   using Sum = typename FewMma<T>::Sum;
   constexpr int kBlocks = kWide == 1 ? 2 : 1;  // blocks whose loads are in flight together
@@ -83,16 +84,16 @@ __device__ __forceinline__ void few_products(const FewOperands& a, int channel, 
   const uint8_t* w0 = a.w + (channel + g) * a.w_ld;
   Sum acc[kTiles][kWide][4] = {}, total[kTiles][kWide][4] = {};
   auto load = [&](uint32_t (&v)[8], const uint8_t* p, int at, bool there, bool stream) {
+    constexpr int kWords = kAlign / 4;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      Vec<16> q;
-      q.w[0] = q.w[1] = q.w[2] = q.w[3] = 0;
-      if (there && at + 16 * h < a.bytes) {
-        if (stream) q = ld_stream<16>(p + at + 16 * h, once);
-        else q = ld_weight<16>(p + at + 16 * h, keep);
+    for (int h = 0; h < 8 / kWords; ++h) {
+      Vec<kAlign> q = {};
+      if (there && at + kAlign * h < a.bytes) {
+        if (stream) q = ld_stream<kAlign>(p + at + kAlign * h, once);
+        else q = ld_weight<kAlign>(p + at + kAlign * h, keep);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * h + k] = q.w[k];
+      for (int k = 0; k < kWords; ++k) v[kWords * h + k] = q.w[k];
     }
   };
   auto join = [&] {

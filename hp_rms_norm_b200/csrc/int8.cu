@@ -254,47 +254,45 @@ struct ByteCopies {
   ByteCopy c[2];
 };
 
-// A warp copies kByteSpan bytes of a row: the words of memory that they lie in, all
-// of a lane's loads in flight, put together with the next lane's.  blockIdx.y is the
-// span, z the operand.  (517 x 2731 and 1001 x 2731, nothing in L2: BYTES_NEW us, 9.2
-// with single bytes.)
-constexpr int kByteSpan = 512;
+// A warp copies kByteSpan bytes of a row at a time: the words of memory that they
+// lie in, all of a lane's loads in flight, put together with the next lane's.  Half
+// of a grid that stays resident takes each operand.  (64 x 3287 and 15814 x 3287,
+// nothing in L2: 30 us; 96 with a span of 512 bytes a warp and its end.)
+constexpr int kByteSpan = 1024;
 
-__global__ void __launch_bounds__(256) copy_byte_rows(ByteCopies both) {
-  const ByteCopy& c = both.c[blockIdx.z];
+__device__ __forceinline__ void copy_byte_span(const ByteCopy& c, int64_t i, int64_t j0) {
+  constexpr int kWords = kByteSpan / 128;
   const int lane = threadIdx.x % 32;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32, j0 = static_cast<int64_t>(blockIdx.y) * kByteSpan;
-  pdl_wait();
-  pdl_trigger();
-  if (i >= c.rows || j0 >= c.dst_ld) return;
   const uint8_t* row = c.src + i * c.src_ld;
   const uint8_t* end = c.src + (c.rows - 1) * c.src_ld + c.cols;  // of the tensor
   const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3);
   const uint8_t* from = row - shift + j0;
-  uint32_t w[5];  // words lane, 32 + lane, ...; the last one lane 31's alone
+  uint32_t w[kWords + 1];  // words lane, 32 + lane, ...; the last one the first lane's alone
   if (from >= c.src && from + kByteSpan + 4 <= end) {
     const uint32_t* p = reinterpret_cast<const uint32_t*>(from) + lane;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = p[32 * k];
-    w[4] = lane == 0 ? p[128] : 0;
+    for (int k = 0; k < kWords; ++k) w[k] = p[32 * k];
+    w[kWords] = lane == 0 ? p[32 * kWords] : 0;
   } else {
     // Words that reach out of the tensor byte by byte.
-#pragma unroll
-    for (int k = 0; k < 5; ++k) {
+#pragma unroll 1
+    for (int k = 0; k <= kWords; ++k) {
       const uint8_t* p = from + 4 * (32 * k + lane);
-      w[k] = 0;
-      if ((k == 4 && lane > 0) || p >= end || p + 4 <= c.src) continue;
-      if (p >= c.src && p + 4 <= end) {
-        w[k] = *reinterpret_cast<const uint32_t*>(p);
-        continue;
+      uint32_t v = 0;
+      if (!(k == kWords && lane > 0) && p < end && p + 4 > c.src) {
+        if (p >= c.src && p + 4 <= end) {
+          v = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+          for (int b = 0; b < 4; ++b)
+            if (p + b >= c.src && p + b < end) v |= static_cast<uint32_t>(p[b]) << (8 * b);
+        }
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (p + b >= c.src && p + b < end) w[k] |= static_cast<uint32_t>(p[b]) << (8 * b);
+      for (int q = 0; q <= kWords; ++q) w[q] = q == k ? v : w[q];
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < kWords; ++k) {
     // The next lane's word; behind the last lane's comes the first one's next.
     const uint32_t next = __shfl_sync(~0u, lane == 0 ? w[k + 1] : w[k], (lane + 1) % 32);
     uint32_t v = __funnelshift_r(w[k], next, 8 * shift);
@@ -302,6 +300,27 @@ __global__ void __launch_bounds__(256) copy_byte_rows(ByteCopies both) {
     if (left < 4) v = left <= 0 ? 0 : v & (0xffffffffu >> (8 * (4 - left)));
     if (j < c.dst_ld) *reinterpret_cast<uint32_t*>(c.dst + i * c.dst_ld + j) = v;
   }
+}
+
+__global__ void __launch_bounds__(256) copy_byte_rows(ByteCopies both, uint32_t x_ctas) {
+  pdl_wait();
+  const bool second = blockIdx.x >= x_ctas;
+  const ByteCopy c = second ? both.c[1] : both.c[0];
+  const uint32_t spans = static_cast<uint32_t>((c.dst_ld + kByteSpan - 1) / kByteSpan);
+  if (spans > 0) {
+    // Spans in the rows' order, a warp every `step`-th; row and span by steps, without
+    // a division each.
+    const uint32_t first = (blockIdx.x - (second ? x_ctas : 0)) * 8 + threadIdx.x / 32;
+    const uint32_t step = (second ? gridDim.x - x_ctas : x_ctas) * 8;
+    const uint32_t step_rows = step / spans, step_spans = step % spans;
+    uint32_t span = first % spans;
+    for (int64_t i = first / spans; i < c.rows;) {
+      copy_byte_span(c, i, static_cast<int64_t>(span) * kByteSpan);
+      i += step_rows, span += step_spans;
+      if (span >= spans) span -= spans, ++i;
+    }
+  }
+  pdl_trigger();
 }
 
 // An operand as TMA reads it: rows on 16-byte boundaries and of an even length
@@ -338,11 +357,11 @@ struct FewArgs {
   int64_t out_ld;
 };
 
-template <typename T, int kTiles>
+template <typename T, int kTiles, int kAlign>
 __global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 4 : kTiles == 2 ? 3 : 2) few_int8(FewArgs a) {
   __shared__ FewSums<int8_t, kTiles, 1> sums;
   const int channel = blockIdx.x * 16;
-  few_products<int8_t, kTiles, 1>(a.in, channel, sums);
+  few_products<int8_t, kTiles, 1, kAlign>(a.in, channel, sums);
   for (int e = threadIdx.x; e < 16 * 8 * kTiles; e += 32 * kFewWarps) {
     const int c = e % 16, i = e / 16, j = channel + c;
     if (i >= a.in.rows || j >= a.in.channels) continue;
@@ -392,15 +411,21 @@ struct ScaledEpilogue {
 
 namespace {
 
-// Products that few_int8 takes: rows of both operands in vectors of 16 bytes, and
-// up to 8 rows; more where the weight is small, since every CTA reads all of x
+// Products that few_int8 takes: rows of both operands in vectors of 16 or 8 bytes,
+// and up to 8 rows; more where the weight is small, since every CTA reads all of x
 // (us, few_int8 against the tiles: 28672 x 4096, 1 row 20.1 / 25.2, 8 rows 21.8 /
 // 25.6, 16 rows 29 / 25.8; 6144 x 4096, 1 row 6.2 / 10.9, 16 rows 7.8 / 10.9, 24
 // rows 11.8 / 10.8; 1024 x 1024, 1 row 2.2 / 4.7, 32 rows 2.8 / 4.7).
-bool few_product(const void* x, const void* w, int64_t rows, int64_t hidden, int64_t channels, int64_t x_ld, int64_t w_ld) {
+// Returns what the rows are multiples of (rows of 8 bytes would have to be copied for
+// the tiles), or 0.
+int few_product(const void* x, const void* w, int64_t rows, int64_t hidden, int64_t channels, int64_t x_ld, int64_t w_ld) {
   const int64_t most = rows <= 8 ? INT64_MAX : rows <= 16 ? int64_t{32} << 20 : rows <= 32 ? int64_t{8} << 20 : 0;
-  return rows >= 1 && hidden >= 1 && channels * hidden <= most && hidden % 16 == 0 && aligned(x, 16) && aligned(w, 16) &&
-         (rows <= 1 || x_ld % 16 == 0) && (channels <= 1 || w_ld % 16 == 0);
+  if (rows < 1 || hidden < 1 || channels * hidden > most) return 0;
+  for (int align : {16, 8})
+    if (hidden % align == 0 && aligned(x, align) && aligned(w, align) && (rows <= 1 || x_ld % align == 0) &&
+        (channels <= 1 || w_ld % align == 0))
+      return align;
+  return 0;
 }
 
 template <typename T, bool kNorm>
@@ -515,10 +540,10 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
   if ((rows > 1 && (input_row_stride < hidden || out_row_stride < channels)) ||
       (channels > 1 && weight_row_stride < hidden))
     return fail(HPRN_ERR_INVALID_ARGUMENT, "row strides must be at least the row lengths");
-  const bool few = few_product(input, weight, rows, hidden, channels, input_row_stride, weight_row_stride);
+  const int few = few_product(input, weight, rows, hidden, channels, input_row_stride, weight_row_stride);
   Workspace ws(workspace, *workspace_bytes);
-  const ByteRows x(ws, input, rows, hidden, input_row_stride);
-  const ByteRows w(ws, weight, channels, hidden, weight_row_stride);
+  const ByteRows x(ws, input, few ? 0 : rows, hidden, input_row_stride);
+  const ByteRows w(ws, weight, few ? 0 : channels, hidden, weight_row_stride);
   const int64_t pairs = (hidden + 1) / 2;
   const PlannedProduct<false, true, true> product(ws, rows, channels, pairs);
   if (flags & HPRN_WORKSPACE_QUERY) {
@@ -543,14 +568,14 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_int8";
   const ByteCopies copies{{x.copy(), w.copy()}};
-  int64_t most_rows = 0, most_bytes = 0;
-  for (const ByteCopy& c : copies.c) {
-    if (c.rows > most_rows) most_rows = c.rows;
-    if (c.dst_ld > most_bytes) most_bytes = c.dst_ld;
-  }
-  if (most_rows > 0) {
-    const dim3 grid(static_cast<unsigned>((most_rows + 7) / 8), static_cast<unsigned>((most_bytes + kByteSpan - 1) / kByteSpan), 2);
-    if ((st = launch_rows(copy_byte_rows, grid, dim3(256), cs, flags, what, copies)) != HPRN_OK) return st;
+  auto ctas_of = [&](const ByteCopy& c) {
+    const int64_t n = (c.rows * ((c.dst_ld + kByteSpan - 1) / kByteSpan) + 7) / 8, most = 6 * dev->sm_count;
+    return static_cast<uint32_t>(n < most ? n : most);
+  };
+  const uint32_t x_ctas = ctas_of(copies.c[0]), w_ctas = ctas_of(copies.c[1]);
+  if (x_ctas + w_ctas > 0) {
+    st = launch_rows(copy_byte_rows, dim3(x_ctas + w_ctas), dim3(256), cs, flags, what, copies, x_ctas);
+    if (st != HPRN_OK) return st;
   }
   auto launch = [&](auto t) {
     using T = decltype(t);
@@ -562,7 +587,11 @@ int hprn_linear_int8(void* out, const int8_t* input, const float* input_scale, c
       f.in.channels = static_cast<int32_t>(channels);
       f.out = static_cast<uint16_t*>(out), f.out_ld = out_row_stride;
       f.row_scale = input_scale, f.channel_scale = weight_scale, f.bias = static_cast<const uint16_t*>(bias);
-      const auto fn = rows <= 8 ? few_int8<T, 1> : rows <= 16 ? few_int8<T, 2> : few_int8<T, 4>;
+      const auto kernel = [&](auto align) {
+        constexpr int kAlign = decltype(align)::value;
+        return rows <= 8 ? few_int8<T, 1, kAlign> : rows <= 16 ? few_int8<T, 2, kAlign> : few_int8<T, 4, kAlign>;
+      };
+      const auto fn = few == 16 ? kernel(std::integral_constant<int, 16>{}) : kernel(std::integral_constant<int, 8>{});
       f.in.first_wave = static_cast<int32_t>(first_wave_ctas(dev, reinterpret_cast<const void*>(fn), 32 * kFewWarps));
       return launch_rows(fn, dim3(static_cast<unsigned>((channels + 15) / 16)), dim3(32 * kFewWarps), cs, flags, what, f);
     }

@@ -204,7 +204,7 @@ template <typename T, int kTiles>
 __global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 3 : 2) few_logits(FewLogits a) {
   __shared__ FewSums<T, kTiles, 2> sums;
   const int first = blockIdx.x * kChunk;
-  few_products<T, kTiles, 2>(a.in, first, sums);
+  few_products<T, kTiles, 2, 16>(a.in, first, sums);
   const int lane = threadIdx.x % 32;
   const LogProbEpilogue<true>& o = a.out;
   for (int i = threadIdx.x / 32; i < a.in.rows; i += kFewWarps) {
