@@ -79,25 +79,13 @@ __device__ __forceinline__ void store_codes(int8_t* q, const float2 (&y)[Pairs<V
 // neighbouring lanes: whole words of eight inside a warp's span, as store_loose.
 __device__ __forceinline__ void store_codes_loose(int8_t* row, int n, int v, const float2 (&y)[4], float inv) {
   const int o = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 7), lane = threadIdx.x % 32;
+  const LooseEdge edge = loose_edge(n, v, o);
   const uint64_t lo = codes_of(y[0], inv) | codes_of(y[1], inv) << 16, hi = codes_of(y[2], inv) | codes_of(y[3], inv) << 16;
   const uint64_t own = lo | hi << 32, before = __shfl_up_sync(~0u, own, 1);
-  if (8 * v >= n) return;
-  const uint64_t word = o > 0 ? before >> (64 - 8 * o) | own << (8 * o) : own;
-  int8_t* q = row + 8 * v;
-  if ((lane > 0 || o == 0) && 8 * v - o + 8 <= n) {
-    *reinterpret_cast<uint64_t*>(q - o) = word;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e < 8 - o && 8 * v + e < n) q[e] = static_cast<int8_t>(own >> (8 * e));
-      if (lane > 0 && e < o) q[e - o] = static_cast<int8_t>(word >> (8 * e));
-    }
-  }
-  if (lane == 31 || 8 * (v + 1) >= n) {
-#pragma unroll
-    for (int e = 1; e < 8; ++e)
-      if (e >= 8 - o && 8 * v + e < n) q[e] = static_cast<int8_t>(own >> (8 * e));
-  }
+  const uint64_t over = __shfl_sync(~0u, own, edge.lane);
+  if (edge.mine) row[edge.unit] = static_cast<int8_t>(over >> (8 * edge.at));
+  if ((lane > 0 || o == 0) && 8 * v - o + 8 <= n)
+    *reinterpret_cast<uint64_t*>(row + 8 * v - o) = o > 0 ? before >> (64 - 8 * o) | own << (8 * o) : own;
 }
 
 // Rows held in registers, laid out over threads as in gated_norm.cu.
