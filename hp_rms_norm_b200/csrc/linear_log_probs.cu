@@ -139,28 +139,35 @@ struct LogProbJoin {
   float *log_prob, *entropy, *lse;
 };
 
-// Joins the parts of row i, by a CTA of kThreads: the largest first, then the sums
-// relative to it, so that no term waits for another.  Returns the row's lse in every
-// thread.
+// Threads kThreads of a CTA's that meet at hardware barrier `barrier`.
 template <int kThreads>
-__device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i) {
-  constexpr int kWarps = kThreads / 32;
+__device__ __forceinline__ void meet(int barrier) {
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory");
+}
+
+// Joins the parts of row i, by kJoinThreads threads `thread`: the largest first, then
+// the sums relative to it, so that no term waits for another.  Returns the row's lse
+// in each of them.
+constexpr int kJoinThreads = 128;
+
+__device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i, int thread) {
+  constexpr int kThreads = kJoinThreads, kWarps = kThreads / 32;
   __shared__ float most[kWarps], sums[2][kWarps];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int lane = thread % 32, warp = thread / 32;
   const float4* parts = q.partial + i * q.parts;
   float m = -INFINITY;
 #pragma unroll 4
-  for (int64_t k = threadIdx.x; k < q.parts; k += kThreads) m = fmaxf(m, parts[k].x);
+  for (int64_t k = thread; k < q.parts; k += kThreads) m = fmaxf(m, parts[k].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   if (lane == 0) most[warp] = m;
-  __syncthreads();
+  meet<kThreads>(2);
   m = most[0];
 #pragma unroll
   for (int k = 1; k < kWarps; ++k) m = fmaxf(m, most[k]);
   float top = m == -INFINITY ? 0.f : m, s = 0.f, a = 0.f;
 #pragma unroll 4
-  for (int64_t k = threadIdx.x; k < q.parts; k += kThreads) {
+  for (int64_t k = thread; k < q.parts; k += kThreads) {
     const float4 p = parts[k];
     const float x = max_nan((p.x - top) * q.to_log2, kLeastExponent), f = exp2_fast(x);
     s = fmaf(p.y, f, s);
@@ -169,13 +176,13 @@ __device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o), a += __shfl_xor_sync(~0u, a, o);
   if (lane == 0) sums[0][warp] = s, sums[1][warp] = a;
-  __syncthreads();
+  meet<kThreads>(2);
   s = sums[0][0], a = sums[1][0];
 #pragma unroll
   for (int k = 1; k < kWarps; ++k) s += sums[0][k], a += sums[1][k];
   if (q.parts == 0 && q.vocab > 0) top = 0.f, s = static_cast<float>(q.vocab), a = 0.f;
   const float log_s = logf(s), lse = fmaf(top, q.inv_t, log_s);
-  if (threadIdx.x == 0) {
+  if (thread == 0) {
     q.lse[i] = lse;
     const int64_t t = target_of(q.target, i, q.ignore, q.vocab);
     // The two logits first: where the target is the largest one the log probability
@@ -188,9 +195,9 @@ __device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i) {
   return lse;
 }
 
-__global__ void __launch_bounds__(128) log_prob_join(LogProbJoin q) {
+__global__ void __launch_bounds__(kJoinThreads) log_prob_join(LogProbJoin q) {
   pdl_wait();
-  join_row<128>(q, blockIdx.x);
+  join_row(q, blockIdx.x, threadIdx.x);
 }
 
 // Few rows (few_rows.cuh): a CTA computes 32 columns' logits, which are a group and
@@ -267,7 +274,7 @@ __device__ __forceinline__ uint64_t order_bits(double v) {
   return v != v ? ~uint64_t{0} : (u >> 63) ? ~u : u | uint64_t{1} << 63;
 }
 
-// The largest key of the CTA, in every thread.  `part`: one of two buffers that
+// The largest key of the searching threads, in each of them.  `part`: one of two buffers that
 // calls alternate between.
 __device__ __forceinline__ uint64_t block_most(uint64_t key, uint64_t* part) {
 #pragma unroll
@@ -276,7 +283,7 @@ __device__ __forceinline__ uint64_t block_most(uint64_t key, uint64_t* part) {
     key = other > key ? other : key;
   }
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = key;
-  __syncthreads();
+  meet<kTopThreads>(1);
   key = part[0];
 #pragma unroll
   for (int k = 1; k < kTopThreads / 32; ++k) key = part[k] > key ? part[k] : key;
@@ -316,36 +323,35 @@ __device__ __forceinline__ double exact_dot(const uint16_t* x, const uint16_t* w
   return s;
 }
 
-// One CTA per row.  A thread holds the largest of its share of the group maxima;
-// the `candidates` largest of those 256 have a last one, and no candidate lies below
-// it.  Groups that reach it, and then their logits that do, are collected (few more
-// than wanted, of logits in no particular order) and each one's place is counted.
-// Where more than kCollect reach it, groups and logits are picked one by one.
+// One CTA per row; four of its warps join the row's parts while eight search.  A
+// searching thread holds the largest of its share of the group maxima, 4, 2 or 1 lanes
+// together the largest of theirs: 64, 128 or 256 of them, over twice the candidates.
+// The `candidates` largest of those have a last one, and no candidate lies below it.
+// Groups that reach it, and then their logits that do, are collected (few more than
+// wanted, of logits in no particular order) and each one's place is counted.  Where
+// more than kCollect reach it, groups and logits are picked one by one.  (7 x 32768
+// logits, 5 wanted, hidden 1024: with the product 22.9 us; 27.1 with the join first, in all warps, and 256
+// of them whatever was wanted.)
 constexpr int kCollect = 512;
 
 template <typename T>
-__global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
-  constexpr int kWarps = kTopThreads / 32;
+__global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopArgs a) {
+  constexpr int kWarps = kTopThreads / 32, kAllWarps = kWarps + kJoinThreads / 32;
   __shared__ uint64_t part[2][kWarps], best_of[kTopThreads], collected[kCollect], bound;
   __shared__ uint32_t group_at[kCollect], column[kMostCandidates];
   __shared__ int group_count, count;
-  __shared__ double exact[kMostCandidates], shares[kWarps];
-  pdl_wait();
+  __shared__ double exact[kMostCandidates], shares[kAllWarps];
+  __shared__ float row_lse;
   const int64_t i = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32;
   float* values = a.values + i * a.top;
   int64_t* indices = a.indices + i * a.top;
-  if (tid == 0) group_count = count = 0;
-  if (tid < kMostCandidates) column[tid] = 0;
   const uint16_t* x = a.x + i * a.x_ld;
-  const float lse = join_row<kTopThreads>(a.join, i);
-  if (a.hidden == 0) {  // logits that are sums of no terms
-    if (tid < a.top) values[tid] = -lse, indices[tid] = tid;
-    return;
-  }
   const int groups = static_cast<int>(a.groups), wanted = min(a.candidates, groups);
   const float* maxima = a.group_max + i * a.groups;
   const float* row = a.logits + i * a.groups * kChunk;
+  if (tid == 0) group_count = count = 0;
+  if (tid < kMostCandidates) column[tid] = 0;
   // The largest key below `limit` of the thread's groups.
   auto best_below = [&](uint64_t limit) {
     uint64_t best = 0;
@@ -356,84 +362,108 @@ __global__ void __launch_bounds__(kTopThreads) log_prob_top(TopArgs a) {
     }
     return best;
   };
-  uint64_t mine = best_below(~uint64_t{0});
-  best_of[tid] = mine;
-  __syncthreads();
-  int above = 0;
+  auto search = [&] {
+    uint64_t mine = best_below(~uint64_t{0});
+    // 2^shift lanes hold a key together, and share the keys it is compared with.
+    const int shift = wanted <= 24 ? 2 : wanted <= 48 ? 1 : 0;
+    uint64_t shared = mine;
+    for (int o = 1; o < 1 << shift; o <<= 1) {
+      const uint64_t other = __shfl_xor_sync(~0u, shared, o);
+      shared = other > shared ? other : shared;
+    }
+    const int own = tid >> shift, keys = kTopThreads >> shift;
+    best_of[own] = shared;
+    meet<kTopThreads>(1);
+    int above = 0;
 #pragma unroll 8
-  for (int k = 0; k < kTopThreads; ++k) above += best_of[k] > mine;
-  if (above == wanted - 1) bound = mine;  // keys differ, but for those of threads without groups
-  __syncthreads();
-  const uint64_t least = bound;
-  if (mine >= least) {
-    for (int k = tid; k < groups; k += kTopThreads) {
-      if (order_key(maxima[k], static_cast<uint32_t>(k)) < least) continue;
-      const int at = atomicAdd(&group_count, 1);
-      if (at < kCollect) group_at[at] = k;
-    }
-  }
-  __syncthreads();
-  // (A logit as large as the least group's maximum counts whatever its index; every
-  // logit where the groups are fewer than the candidates.)
-  const uint64_t least_logit = wanted < a.candidates ? 0 : least >> 32 << 32;
-  for (int g = tid / 32; g < min(group_count, kCollect); g += kWarps) {
-    const uint32_t j = group_at[g] * kChunk + lane;
-    if (j >= a.vocab) continue;
-    const uint64_t key = order_key(row[j], j);
-    if (key < least_logit) continue;
-    const int at = atomicAdd(&count, 1);
-    if (at < kCollect) collected[at] = key;
-  }
-  __syncthreads();
-  if (group_count <= kCollect && count <= kCollect) {
-    for (int e = tid; e < count; e += kTopThreads) {
-      const uint64_t key = collected[e];
-      int place = 0;
-#pragma unroll 4
-      for (int k = 0; k < count; ++k) place += collected[k] > key;
-      if (place < a.candidates) column[place] = key_index(key);
-    }
-  } else {
-    int turn = 0;
-    for (int c = 0; c < wanted; ++c) {
-      const uint64_t best = block_most(mine, part[turn]);
-      turn ^= 1;
-      if (mine == best) group_at[c] = key_index(best), mine = best_below(best);
-    }
-    __syncthreads();
-    uint64_t keys[kHeld];
-    mine = 0;
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int slot = tid + k * kTopThreads;
-      keys[k] = 0;
-      if (slot < wanted * kChunk) {
-        const uint32_t j = group_at[slot / kChunk] * kChunk + slot % kChunk;
-        if (j < a.vocab) keys[k] = order_key(row[j], j);
+    for (int k = tid - (own << shift); k < keys; k += 1 << shift) above += best_of[k] > shared;
+    for (int o = 1; o < 1 << shift; o <<= 1) above += __shfl_xor_sync(~0u, above, o);
+    if (above == wanted - 1) bound = shared;  // keys differ, but for those of threads without groups
+    meet<kTopThreads>(1);
+    const uint64_t least = bound;
+    if (mine >= least) {
+      for (int k = tid; k < groups; k += kTopThreads) {
+        if (order_key(maxima[k], static_cast<uint32_t>(k)) < least) continue;
+        const int at = atomicAdd(&group_count, 1);
+        if (at < kCollect) group_at[at] = k;
       }
-      mine = keys[k] > mine ? keys[k] : mine;
     }
-    for (int c = 0; c < a.candidates; ++c) {
-      const uint64_t best = block_most(mine, part[turn]);
-      turn ^= 1;
-      if (mine == best) {
-        column[c] = key_index(best);
-        mine = 0;
+    meet<kTopThreads>(1);
+    // (A logit as large as the least group's maximum counts whatever its index; every
+    // logit where the groups are fewer than the candidates.)
+    const uint64_t least_logit = wanted < a.candidates ? 0 : least >> 32 << 32;
+    for (int g = tid / 32; g < min(group_count, kCollect); g += kWarps) {
+      const uint32_t j = group_at[g] * kChunk + lane;
+      if (j >= a.vocab) continue;
+      const uint64_t key = order_key(row[j], j);
+      if (key < least_logit) continue;
+      const int at = atomicAdd(&count, 1);
+      if (at < kCollect) collected[at] = key;
+    }
+    meet<kTopThreads>(1);
+    if (group_count <= kCollect && count <= kCollect) {
+      for (int e = tid; e < count; e += kTopThreads) {
+        const uint64_t key = collected[e];
+        int place = 0;
+#pragma unroll 4
+        for (int k = 0; k < count; ++k) place += collected[k] > key;
+        if (place < a.candidates) column[place] = key_index(key);
+      }
+    } else {
+      int turn = 0;
+      for (int c = 0; c < wanted; ++c) {
+        const uint64_t best = block_most(mine, part[turn]);
+        turn ^= 1;
+        if (mine == best) group_at[c] = key_index(best), mine = best_below(best);
+      }
+      meet<kTopThreads>(1);
+      uint64_t held[kHeld];
+      mine = 0;
 #pragma unroll
-        for (int k = 0; k < kHeld; ++k) {
-          if (keys[k] < best) mine = keys[k] > mine ? keys[k] : mine;
+      for (int k = 0; k < kHeld; ++k) {
+        const int slot = tid + k * kTopThreads;
+        held[k] = 0;
+        if (slot < wanted * kChunk) {
+          const uint32_t j = group_at[slot / kChunk] * kChunk + slot % kChunk;
+          if (j < a.vocab) held[k] = order_key(row[j], j);
+        }
+        mine = held[k] > mine ? held[k] : mine;
+      }
+      for (int c = 0; c < a.candidates; ++c) {
+        const uint64_t best = block_most(mine, part[turn]);
+        turn ^= 1;
+        if (mine == best) {
+          column[c] = key_index(best);
+          mine = 0;
+#pragma unroll
+          for (int k = 0; k < kHeld; ++k) {
+            if (held[k] < best) mine = held[k] > mine ? held[k] : mine;
+          }
         }
       }
     }
+  };
+  pdl_wait();
+  __syncthreads();
+  if (tid >= kTopThreads) {
+    const float lse = join_row(a.join, i, tid - kTopThreads);
+    if (tid == kTopThreads) row_lse = lse;
+  } else if (a.hidden > 0) {
+    search();
   }
   __syncthreads();
-  // The candidates' weights into L2 at once: 8 warps take them in turn.
+  const float lse = row_lse;
+  if (a.hidden == 0) {  // logits that are sums of no terms
+    if (tid < a.top) values[tid] = -lse, indices[tid] = tid;
+    return;
+  }
+  // The candidates' weights into L2 at once: the warps take them in turn.
   if (tid < a.candidates)
     prefetch_l2(a.w + static_cast<int64_t>(column[tid]) * a.w_ld, static_cast<uint64_t>(a.hidden) * 2);
   // Several warps a candidate where there are more.
-  const int parts = max(1, kWarps / a.candidates), warp = tid / 32;
+  const int parts = max(1, kAllWarps / a.candidates), warp = tid / 32;
   const int64_t length = (a.hidden + 8 * parts - 1) / (8 * parts) * 8;
-  for (int task = warp; task < a.candidates * parts; task += kWarps) {
+  for (int task = warp; task < a.candidates * parts; task += kAllWarps) {
     const int c = task / parts;
     const int64_t first = (task - c * parts) * length;
     const double s = exact_dot<T>(x, a.w + static_cast<int64_t>(column[c]) * a.w_ld, first,
@@ -637,7 +667,7 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       q.to_log2 = static_cast<float>(1.4426950408889634 / temperature);
       q.log_prob = log_prob + first, q.entropy = entropy + first, q.lse = lse + first;
       if (top == 0) {
-        r = launch_rows(log_prob_join, dim3(static_cast<unsigned>(count)), dim3(128), cs, flags, what, q);
+        r = launch_rows(log_prob_join, dim3(static_cast<unsigned>(count)), dim3(kJoinThreads), cs, flags, what, q);
         if (r != HPRN_OK) return r;
         continue;
       }
@@ -650,7 +680,7 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       a.top = static_cast<int32_t>(top);
       a.candidates = static_cast<int32_t>(top + kSpareTop < vocab ? top + kSpareTop : vocab);
       a.values = top_log_probs + first * top, a.indices = top_indices + first * top;
-      r = launch_rows(log_prob_top<T>, dim3(static_cast<unsigned>(count)), dim3(kTopThreads), cs, flags, what, a);
+      r = launch_rows(log_prob_top<T>, dim3(static_cast<unsigned>(count)), dim3(kTopThreads + kJoinThreads), cs, flags, what, a);
       if (r != HPRN_OK) return r;
     }
     return r;
