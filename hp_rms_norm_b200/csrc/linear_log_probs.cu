@@ -14,10 +14,11 @@
 // also leave the logits of a block of rows and the largest of every 32
 // neighbouring ones (LogProbEpilogue<true>); the `top` largest logits lie among the `top`
 // groups of 32 with the largest maxima, so that a row's search reads a 32nd of
-// its logits' number and a few groups.  A few more than `top` are taken, their
-// logits summed again in 64 bits, and ordered by those; equal ones go to the
-// lowest index.  So the order does not hang on how the tensor cores' sums fall
-// out in their last bits.
+// its logits' number and a few groups.  Of many rows a first part of the vocabulary
+// bounds the largest maxima from below, and only groups that reach the bound leave
+// their logits.  A few more than `top` are taken, their logits summed again in 64
+// bits, and ordered by those; equal ones go to the lowest index.  So the order does
+// not hang on how the tensor cores' sums fall out in their last bits.
 //
 // Backward, g_i and h_i the gradients of log_prob_i and entropy_i:
 //   S_ij = (g_i ([j == t_i] - p_ij) - h_i p_ij (log p_ij + entropy_i)) / T
@@ -64,18 +65,21 @@ struct LogProbEpilogue {
   const int64_t* target = nullptr;
   int64_t ignore = 0;
   int64_t parts = 0;
-  int64_t vocab = 0;
+  int64_t vocab = 0;  // of these columns, which are those from `first` of `all`
+  int64_t first = 0, all = 0;
   float to_log2 = kLog2e;  // log2(e) / T
-  float* logits = nullptr;     // [rows, 32 groups]
-  float* group_max = nullptr;  // [rows, groups]
+  float* logits = nullptr;       // [rows, 32 groups]
+  float* group_max = nullptr;    // [rows, groups]
+  const float* bound = nullptr;  // or: groups with a maximum below it leave no logits
   int64_t groups = 0;
 
   struct Row {
-    float m, s, a;
+    float m, s, a, bound;
     int64_t t;
   };
   __device__ __forceinline__ Row begin(const Lane& l, int64_t i) const {
-    return Row{-INFINITY, 0.f, 0.f, l.inside ? target_of(target, i, ignore, vocab) : kIgnored};
+    return Row{-INFINITY, 0.f, 0.f, kTop && bound && l.inside ? bound[i] : -INFINITY,
+               l.inside ? target_of(target, i, ignore, all) - first : kIgnored};
   }
   __device__ __forceinline__ void chunk(Row& r, const Lane& l, int64_t i, int64_t j, float (&v)[kChunk]) const {
     if (j + kChunk > vocab) {
@@ -97,13 +101,15 @@ struct LogProbEpilogue {
     const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     if constexpr (kTop) {
       if (l.inside) {
-        float* q = logits + i * (groups * kChunk) + j;
+        if (!(most < r.bound)) {
+          float* q = logits + i * (groups * kChunk) + j;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          Vec<32> o;
+          for (int h = 0; h < 4; ++h) {
+            Vec<32> o;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o.w[k] = __float_as_uint(v[8 * h + k]);
-          st_global<32>(q + 8 * h, o);
+            for (int k = 0; k < 8; ++k) o.w[k] = __float_as_uint(v[8 * h + k]);
+            st_global<32>(q + 8 * h, o);
+          }
         }
         group_max[i * groups + j / kChunk] = most;
       }
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, kTiles == 1 ? 3 : 2) few_logit
     const int64_t j = first + lane;
     const bool inside = j < o.vocab;
     if (!inside) v = -INFINITY;
-    if (inside && target_of(o.target, i, o.ignore, o.vocab) == j) o.target_logit[i] = v;
+    if (inside && target_of(o.target, i, o.ignore, o.all) == j) o.target_logit[i] = v;
     if (o.logits) o.logits[i * (o.groups * kChunk) + j] = v;
     float m = v;
 #pragma unroll
@@ -250,6 +256,7 @@ constexpr int kHeld = (kMostCandidates * kChunk + kTopThreads - 1) / kTopThreads
 struct TopArgs {
   const float* logits;
   const float* group_max;
+  const float* bound;  // as in LogProbEpilogue, or null
   int64_t groups, vocab, hidden;
   const uint16_t* x;
   const uint16_t* w;
@@ -323,13 +330,60 @@ __device__ __forceinline__ double exact_dot(const uint16_t* x, const uint16_t* w
   return s;
 }
 
-// One CTA per row; four of its warps join the row's parts while eight search.  A
-// searching thread holds the largest of its share of the group maxima, 4, 2 or 1 lanes
-// together the largest of theirs: 64, 128 or 256 of them, over twice the candidates.
-// The `candidates` largest of those have a last one, and no candidate lies below it.
-// Groups that reach it, and then their logits that do, are collected (few more than
-// wanted, of logits in no particular order) and each one's place is counted.  Where
-// more than kCollect reach it, groups and logits are picked one by one.  (7 x 32768
+// The largest key below `limit` of the thread's share of a row's group maxima.
+__device__ __forceinline__ uint64_t best_below(const float* maxima, int groups, uint64_t limit) {
+  uint64_t best = 0;
+#pragma unroll 4
+  for (int k = threadIdx.x; k < groups; k += kTopThreads) {
+    const uint64_t key = order_key(maxima[k], static_cast<uint32_t>(k));
+    if (key < limit && key > best) best = key;
+  }
+  return best;
+}
+
+// A key that `wanted` of the row's group maxima reach, from the largest one of each
+// of the kTopThreads threads: 4, 2 or 1 lanes together hold the largest of theirs, 64,
+// 128 or 256 of them, over twice as many as wanted, and those have a wanted-th one.
+__device__ __forceinline__ uint64_t least_wanted(uint64_t mine, int wanted) {
+  __shared__ uint64_t best_of[kTopThreads], least;
+  const int tid = threadIdx.x, shift = wanted <= 24 ? 2 : wanted <= 48 ? 1 : 0;
+  for (int o = 1; o < 1 << shift; o <<= 1) {
+    const uint64_t other = __shfl_xor_sync(~0u, mine, o);
+    mine = other > mine ? other : mine;
+  }
+  const int own = tid >> shift, keys = kTopThreads >> shift;
+  best_of[own] = mine;
+  meet<kTopThreads>(1);
+  // The lanes share the keys that theirs is compared with.
+  int above = 0;
+#pragma unroll 8
+  for (int k = tid - (own << shift); k < keys; k += 1 << shift) above += best_of[k] > mine;
+  for (int o = 1; o < 1 << shift; o <<= 1) above += __shfl_xor_sync(~0u, above, o);
+  if (above == wanted - 1) least = mine;  // keys differ, but for those of threads without groups
+  meet<kTopThreads>(1);
+  return least;
+}
+
+struct BoundArgs {
+  float* bound;
+  const float* group_max;
+  int64_t groups, sample;  // of which so many are there
+  int32_t wanted;
+};
+
+// Bounds of the rows' largest logits from a sample of their groups.
+__global__ void __launch_bounds__(kTopThreads) log_prob_bound(BoundArgs a) {
+  pdl_wait();
+  const float* maxima = a.group_max + blockIdx.x * a.groups;
+  const uint64_t least = least_wanted(best_below(maxima, static_cast<int>(a.sample), ~uint64_t{0}), a.wanted);
+  if (threadIdx.x == 0) a.bound[blockIdx.x] = maxima[key_index(least)];
+}
+
+// One CTA per row; four of its warps join the row's parts while eight search.  No
+// candidate lies below least_wanted's bound.  Groups that reach it, and then their
+// logits that do, are collected (few more than wanted, of logits in no particular
+// order) and each one's place is counted.  Where more than kCollect reach it, groups
+// and logits are picked one by one.  (7 x 32768
 // logits, 5 wanted, hidden 1024: with the product 22.9 us; 27.1 with the join first, in all warps, and 256
 // of them whatever was wanted.)
 constexpr int kCollect = 512;
@@ -337,7 +391,7 @@ constexpr int kCollect = 512;
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopArgs a) {
   constexpr int kWarps = kTopThreads / 32, kAllWarps = kWarps + kJoinThreads / 32;
-  __shared__ uint64_t part[2][kWarps], best_of[kTopThreads], collected[kCollect], bound;
+  __shared__ uint64_t part[2][kWarps], collected[kCollect];
   __shared__ uint32_t group_at[kCollect], column[kMostCandidates];
   __shared__ int group_count, count;
   __shared__ double exact[kMostCandidates], shares[kAllWarps];
@@ -352,35 +406,13 @@ __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopAr
   const float* row = a.logits + i * a.groups * kChunk;
   if (tid == 0) group_count = count = 0;
   if (tid < kMostCandidates) column[tid] = 0;
-  // The largest key below `limit` of the thread's groups.
-  auto best_below = [&](uint64_t limit) {
-    uint64_t best = 0;
-#pragma unroll 4
-    for (int k = tid; k < groups; k += kTopThreads) {
-      const uint64_t key = order_key(maxima[k], static_cast<uint32_t>(k));
-      if (key < limit && key > best) best = key;
-    }
-    return best;
-  };
   auto search = [&] {
-    uint64_t mine = best_below(~uint64_t{0});
-    // 2^shift lanes hold a key together, and share the keys it is compared with.
-    const int shift = wanted <= 24 ? 2 : wanted <= 48 ? 1 : 0;
-    uint64_t shared = mine;
-    for (int o = 1; o < 1 << shift; o <<= 1) {
-      const uint64_t other = __shfl_xor_sync(~0u, shared, o);
-      shared = other > shared ? other : shared;
+    uint64_t mine = best_below(maxima, groups, ~uint64_t{0});
+    uint64_t least = least_wanted(mine, wanted);
+    if (a.bound) {
+      const uint64_t known = order_key(a.bound[i], 0xffffffffu);
+      least = known > least ? known : least;
     }
-    const int own = tid >> shift, keys = kTopThreads >> shift;
-    best_of[own] = shared;
-    meet<kTopThreads>(1);
-    int above = 0;
-#pragma unroll 8
-    for (int k = tid - (own << shift); k < keys; k += 1 << shift) above += best_of[k] > shared;
-    for (int o = 1; o < 1 << shift; o <<= 1) above += __shfl_xor_sync(~0u, above, o);
-    if (above == wanted - 1) bound = shared;  // keys differ, but for those of threads without groups
-    meet<kTopThreads>(1);
-    const uint64_t least = bound;
     if (mine >= least) {
       for (int k = tid; k < groups; k += kTopThreads) {
         if (order_key(maxima[k], static_cast<uint32_t>(k)) < least) continue;
@@ -414,7 +446,7 @@ __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopAr
       for (int c = 0; c < wanted; ++c) {
         const uint64_t best = block_most(mine, part[turn]);
         turn ^= 1;
-        if (mine == best) group_at[c] = key_index(best), mine = best_below(best);
+        if (mine == best) group_at[c] = key_index(best), mine = best_below(maxima, groups, best);
       }
       meet<kTopThreads>(1);
       uint64_t held[kHeld];
@@ -559,6 +591,25 @@ constexpr double kLeastTemperature = 1e-30, kMostTemperature = 1e30;
 // What a block of rows may take for its logits.
 constexpr int64_t kLogitBytes = int64_t{1} << 30;
 
+int32_t candidates_of(int64_t top, int64_t vocab) {
+  return static_cast<int32_t>(top + kSpareTop < vocab ? top + kSpareTop : vocab);
+}
+
+// Columns whose logits are computed before the others', for a bound below which those
+// need not be written (0: none): a wave of tiles, and 8 groups for each candidate, of
+// which one in 8 others is still written.  Whole and with a sample (us): 131072 x 512
+// of 5, 128 rows 54.4 / 56.7, 256 rows 79.4 / 67.0, 512 rows 137 / 100; 131072 x 4096 of
+// 20, 128 rows 217 / 217, 256 rows 279 / 263; with a sample of more than a quarter,
+// 20000 x 1024 of 1, 300 rows 35.0 / 39.0.
+constexpr int64_t kLeastSampled = 256;
+
+int64_t sample_of(int64_t rows, int64_t vocab, int64_t top) {
+  if (top == 0 || rows < kLeastSampled) return 0;
+  const int64_t wave = 74 / ((rows + 255) / 256) * 256, least = round_up(8 * kChunk * candidates_of(top, vocab), 256);
+  const int64_t sample = wave > least ? wave : least;
+  return 4 * sample <= vocab ? sample : 0;
+}
+
 int64_t rows_of_block(int64_t rows, int64_t groups) {
   int64_t most = kLogitBytes / (groups > 0 ? groups * kChunk * 4 : 1) / 256 * 256;
   if (most < 256) most = 256;
@@ -589,7 +640,9 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
   const AlignedRows w(ws, weight, vocab, hidden, weight_row_stride, rows);
   const int64_t groups = top > 0 ? (vocab + kChunk - 1) / kChunk : 0;
   const int64_t block = top > 0 ? rows_of_block(rows, groups) : rows;
-  const PlannedProduct<false, true, true> product(ws, block, vocab, hidden, false);
+  const int64_t sample = sample_of(block, vocab, top);
+  const PlannedProduct<false, true, true> of_sample(ws, block, sample > 0 ? sample : vocab, hidden, false),
+      product(ws, block, vocab - sample, hidden, false);
   // few_logits, of rows that are read where they are, against the tiles (us, no
   // alternatives): 1 row of 1024 x 32768 17.1 / 18.5, of 2048 x 50000 39.0 / 40.6, of
   // 4096 x 131072 176 / 170; 8 rows 18.5 / 19.3, 40.7 / 40.5; 12 rows 23.3 / 19.3; of 512
@@ -597,7 +650,9 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
   const int64_t few_most = rows <= 8 ? int64_t{1} << 27 : rows <= 16 ? int64_t{1} << 22 : 0;
   const bool few = vocab > 0 && hidden > 0 && vocab * hidden <= few_most && hidden % 8 == 0 &&
                    tma_rows(input, rows, input_row_stride) && tma_rows(weight, vocab, weight_row_stride);
-  const int64_t parts = few ? (vocab + kChunk - 1) / kChunk : product.parts(vocab);
+  const int64_t sample_parts = of_sample.parts(sample);
+  const int64_t parts = few ? (vocab + kChunk - 1) / kChunk : sample_parts + product.parts(vocab - sample);
+  float* bound = ws.take<float>(sample > 0 ? block : 0);
   float4* partial = ws.take<float4>(parts * block);
   float* target_logit = ws.take<float>(block);
   float* group_max = ws.take<float>(groups * block);
@@ -625,6 +680,7 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
   if ((st = current_device(&dev)) != HPRN_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const char* what = "linear_log_probs";
+  const int32_t candidates = candidates_of(top, vocab);
   if (!few && (st = AlignedRows::prepare(x, w, cs, flags)) != HPRN_OK) return st;
   auto all = [&](auto t) {
     using T = decltype(t);
@@ -634,7 +690,7 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       q.b = {w.data(), w.ld()};
       q.m = count, q.n = vocab, q.depth = hidden;
       epilogue.partial = partial, epilogue.target_logit = target_logit, epilogue.target = target + first;
-      epilogue.ignore = ignore_index, epilogue.parts = parts, epilogue.vocab = vocab;
+      epilogue.ignore = ignore_index, epilogue.parts = parts, epilogue.vocab = epilogue.all = vocab;
       epilogue.to_log2 = static_cast<float>(1.4426950408889634 / temperature);
       epilogue.logits = logits, epilogue.group_max = group_max, epilogue.groups = groups;
       if constexpr (std::is_same<decltype(epilogue), LogProbEpilogue<true>>::value) {
@@ -651,6 +707,17 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
           return launch_rows(fn, dim3(static_cast<unsigned>(parts)), dim3(32 * kFewWarps), cs, flags, what, f);
         }
       }
+      if (sample == 0) return product.launch_whole<T>(q, epilogue, cs, flags, what);
+      q.n = epilogue.vocab = sample;
+      int r = of_sample.launch_whole<T>(q, epilogue, cs, flags, what);
+      if (r != HPRN_OK) return r;
+      BoundArgs b{bound, group_max, groups, sample / kChunk, candidates};
+      r = launch_rows(log_prob_bound, dim3(static_cast<unsigned>(count)), dim3(kTopThreads), cs, flags, what, b);
+      if (r != HPRN_OK) return r;
+      q.b.p = w.data() + sample * w.ld();
+      q.n = epilogue.vocab = vocab - sample;
+      epilogue.first = sample, epilogue.bound = bound;
+      epilogue.partial += sample_parts, epilogue.logits += sample, epilogue.group_max += sample / kChunk;
       return product.launch_whole<T>(q, epilogue, cs, flags, what);
     };
     int r = HPRN_OK;
@@ -673,12 +740,13 @@ int hprn_linear_log_probs(float* log_prob, float* entropy, float* lse, float* to
       }
       TopArgs a{};
       a.logits = logits, a.group_max = group_max, a.groups = groups, a.vocab = vocab, a.hidden = hidden;
+      a.bound = sample > 0 && hidden > 0 ? bound : nullptr;
       a.x = x.data() + first * x.ld(), a.x_ld = x.ld(), a.w = w.data(), a.w_ld = w.ld();
       if (few) a.x = static_cast<const uint16_t*>(input), a.w = static_cast<const uint16_t*>(weight);
       if (few) a.x_ld = rows > 1 ? input_row_stride : hidden, a.w_ld = vocab > 1 ? weight_row_stride : hidden;
       a.join = q, a.inv_t = 1.0 / temperature;
       a.top = static_cast<int32_t>(top);
-      a.candidates = static_cast<int32_t>(top + kSpareTop < vocab ? top + kSpareTop : vocab);
+      a.candidates = candidates;
       a.values = top_log_probs + first * top, a.indices = top_indices + first * top;
       r = launch_rows(log_prob_top<T>, dim3(static_cast<unsigned>(count)), dim3(kTopThreads + kJoinThreads), cs, flags, what, a);
       if (r != HPRN_OK) return r;

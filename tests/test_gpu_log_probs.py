@@ -120,6 +120,30 @@ def test_blocks_of_rows(cuda):
         check_forward(part, x[k], w, t[k], 1.0, 7, f"rows {k}")
 
 
+@pytest.mark.parametrize("rows,vocab,top", [(2600, 20003, 1), (2601, 20003, 5), (300, 90001, 20), (19000, 10300, 1)])
+def test_many_rows_of_a_long_vocabulary(cuda, rows, vocab, top):
+    """Rows and vocabularies large enough that a first part of the columns tells which logits of the
+    others matter; the largest ones in the first part, in the last, equal in both, and one value."""
+    x, w, t, _, _ = make(rows, 40, vocab, torch.bfloat16, cuda)
+    w[-700:-350] = w[:350]
+    w[:, 39] = 0
+    x[:, 39] = 8
+    w[:64, 39] = (torch.arange(64, device=cuda) % 8).to(w.dtype)
+    w[-64:, 39] = (torch.arange(64, device=cuda) % 16).to(w.dtype)
+    x[:50, 39] = -8
+    x[50:60] = 0
+    found = hp.linear_log_probs(x, w, t, top=top)
+    x64 = torch.cat([x[:120], x[-120:]])
+    part = hp.LogProbs(*(None if v is None else torch.cat([v[:120], v[-120:]]) for v in found))
+    check_forward(part, x64, w, torch.cat([t[:120], t[-120:]]), 1.0, top, f"{rows} rows, {top}")
+    x[7] = float("nan")
+    x[8, 3] = float("inf")
+    again = hp.linear_log_probs(x, w, t, top=top)
+    assert again.top_log_probs[7:9].isnan().all()
+    for a, b in zip(found, again):
+        assert torch.equal(a[9:], b[9:]) and torch.equal(a[:7], b[:7])
+
+
 @pytest.mark.parametrize("dt", list(DTYPES))
 def test_sharp_and_flat_logits(cuda, dt):
     """Logits of several hundred, where nearly all probability is one token's, and equal ones."""
