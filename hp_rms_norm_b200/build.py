@@ -119,7 +119,7 @@ def build_torch_binding(force: bool = False) -> str:
     cmd += [src, "-o", out, f"-L{PKG}", "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN"]
     for d in libdirs:
         cmd += [f"-L{d}", f"-Wl,-rpath,{d}"]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda"]
     _run(cmd, os.path.join(BUILD, "torch_ops.log"))
     return out
 
