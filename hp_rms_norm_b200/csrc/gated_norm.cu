@@ -242,6 +242,11 @@ int launch_forward(BlockNormArgs& a, int vec, const DeviceInfo* dev, cudaStream_
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
     const int64_t wave = first_wave_ctas(dev, reinterpret_cast<const void*>(fn), static_cast<int>(threads) * groups) * groups;
+    // Rows that start anywhere are bound by issue: many of them by two vectors a thread,
+    // half the sums over threads for each (us, one / two): 3084 x 2001 22.6 / 20.1, x 5001
+    // 55 / 48; of fewer waves 592 x 2001 5.4 / 6.5, x 5001 11.3 / 12.5; where that leaves more
+    // threads idle, 3084 x 515 8.9 / 10.7.
+    if (vec == 0 && vpt == 1 && wave > 0 && a.rows > 4 * wave && 2 * round_up((a.nvec + 1) / 2, 32) <= threads) continue;
     a.wave_rows = wave > 0 && a.rows > wave ? static_cast<int32_t>(wave) : 0;
     return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),
                        dim3(static_cast<unsigned>(threads * groups)), stream, flags, what, a);

@@ -72,6 +72,7 @@ def test_many_rows(cuda):
     check(make((2500, 2), 512, torch.bfloat16, cuda, gate="sequence"), 1.0, "5000 rows, 2500 gates")
     check(make((5, 1000), 768, torch.bfloat16, cuda, gate="sequence"), 1.0, "5000 rows, 5 gates")
     check(make((5000,), 1024, torch.float16, cuda, gate="token"), 1.0, "5000 rows, a gate each")
+    check(make((6, 1000), 2003, torch.float16, cuda, gate="sequence"), 0.5, "6000 odd rows")
 
 
 def test_strides_and_offsets(cuda):
