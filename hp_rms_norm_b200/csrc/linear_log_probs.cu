@@ -341,12 +341,13 @@ __device__ __forceinline__ uint64_t best_below(const float* maxima, int groups, 
   return best;
 }
 
-// A key that `wanted` of the row's group maxima reach, from the largest one of each
-// of the kTopThreads threads: 4, 2 or 1 lanes together hold the largest of theirs, 64,
-// 128 or 256 of them, over twice as many as wanted, and those have a wanted-th one.
-__device__ __forceinline__ uint64_t least_wanted(uint64_t mine, int wanted) {
+// A key that `wanted` of a row's group maxima reach (`groups` of them, as many as wanted
+// at least), from the largest one of each of the kTopThreads threads: 4, 2 or 1 lanes
+// together hold the largest of theirs, 64, 128 or 256 of them, over twice as many as
+// wanted, and those have a wanted-th one.  Each thread by itself where some have none.
+__device__ __forceinline__ uint64_t least_wanted(uint64_t mine, int groups, int wanted) {
   __shared__ uint64_t best_of[kTopThreads], least;
-  const int tid = threadIdx.x, shift = wanted <= 24 ? 2 : wanted <= 48 ? 1 : 0;
+  const int tid = threadIdx.x, shift = groups < kTopThreads || wanted > 48 ? 0 : wanted > 24 ? 1 : 2;
   for (int o = 1; o < 1 << shift; o <<= 1) {
     const uint64_t other = __shfl_xor_sync(~0u, mine, o);
     mine = other > mine ? other : mine;
@@ -375,7 +376,8 @@ struct BoundArgs {
 __global__ void __launch_bounds__(kTopThreads) log_prob_bound(BoundArgs a) {
   pdl_wait();
   const float* maxima = a.group_max + blockIdx.x * a.groups;
-  const uint64_t least = least_wanted(best_below(maxima, static_cast<int>(a.sample), ~uint64_t{0}), a.wanted);
+  const int groups = static_cast<int>(a.sample);
+  const uint64_t least = least_wanted(best_below(maxima, groups, ~uint64_t{0}), groups, a.wanted);
   if (threadIdx.x == 0) a.bound[blockIdx.x] = maxima[key_index(least)];
 }
 
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopAr
   if (tid < kMostCandidates) column[tid] = 0;
   auto search = [&] {
     uint64_t mine = best_below(maxima, groups, ~uint64_t{0});
-    uint64_t least = least_wanted(mine, wanted);
+    uint64_t least = least_wanted(mine, groups, wanted);
     if (a.bound) {
       const uint64_t known = order_key(a.bound[i], 0xffffffffu);
       least = known > least ? known : least;

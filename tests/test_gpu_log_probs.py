@@ -120,6 +120,18 @@ def test_blocks_of_rows(cuda):
         check_forward(part, x[k], w, t[k], 1.0, 7, f"rows {k}")
 
 
+@pytest.mark.parametrize("vocab", [33, 70, 257, 600, 1500, 4001, 8160, 8192, 8200])
+def test_few_groups(cuda, vocab):
+    """Vocabularies of fewer groups of 32 than threads search them, after a call whose logits are
+    larger, so that what a CTA finds in shared memory is of no use."""
+    big = make(500, 64, 40000, torch.bfloat16, cuda, scale=50.0)
+    for rows in (5, 300):
+        x, w, t, _, _ = make(rows, 64, vocab, torch.bfloat16, cuda)
+        for top in (1, 3, 20, min(vocab, 64)):
+            hp.linear_log_probs(*big[:3], top=20)
+            check_forward(hp.linear_log_probs(x, w, t, top=top), x, w, t, 1.0, top, f"{rows} x {vocab} top {top}")
+
+
 @pytest.mark.parametrize("rows,vocab,top", [(2600, 20003, 1), (2601, 20003, 5), (300, 90001, 20), (19000, 10300, 1)])
 def test_many_rows_of_a_long_vocabulary(cuda, rows, vocab, top):
     """Rows and vocabularies large enough that a first part of the columns tells which logits of the
