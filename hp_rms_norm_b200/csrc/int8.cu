@@ -435,6 +435,10 @@ int launch_quant(QuantArgs& a, int vec, const DeviceInfo* dev, cudaStream_t stre
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
     const int64_t wave = first_wave_ctas(dev, reinterpret_cast<const void*>(fn), static_cast<int>(threads) * groups) * groups;
+    // Rows that start anywhere are bound by issue: more than a wave of them by two vectors
+    // a thread, half the sums over threads for each (us, one / two): 3084 x 1001 10.5 / 9.5,
+    // x 5001 66 / 38, 592 x 3001 7.3 / 5.9; of less than a wave 592 x 1001 3.4 / 4.3.
+    if (vec == 0 && vpt == 1 && wave > 0 && a.rows > wave && 2 * round_up((a.nvec + 1) / 2, 32) <= threads) continue;
     a.wave_rows = wave > 0 && a.rows > wave ? static_cast<int32_t>(wave) : 0;
     return launch_rows(fn, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)),
                        dim3(static_cast<unsigned>(threads * groups)), stream, flags, what, a);
