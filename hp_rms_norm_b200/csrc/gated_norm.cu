@@ -40,9 +40,10 @@ struct BlockNormArgs {
 
 // Rows held in registers: a CTA works on blockDim / row_threads rows, each
 // thread on VPT vectors of VEC bytes.  kLoose: rows that start anywhere (rows.cuh).
-// kGateRow: the gate is a row of values; else one value, or none.
-template <typename T, int VEC, int VPT, bool kLoose, bool kPost, bool kGateRow>
-__global__ void __launch_bounds__(VPT * VEC > 32 ? 512 : 1024) block_norm_rows(BlockNormArgs a) {
+// kGateRow: the gate is a row of values; else one value, or none.  kMost: the threads
+// of a CTA at most, two of which share an SM where they are fewer than 1024.
+template <typename T, int VEC, int VPT, bool kLoose, bool kPost, bool kGateRow, int kMost = 1024>
+__global__ void __launch_bounds__(kMost, kMost < 1024 ? 2 : 1) block_norm_rows(BlockNormArgs a) {
   static_assert(!kLoose || VEC == 16, "loose rows are read in vectors of eight elements");
   constexpr int P = VEC / 4;
   __shared__ float part[2][32];
@@ -223,7 +224,13 @@ int vector_bytes(int64_t hidden, std::initializer_list<const void*> rows, std::i
 using RowsKernel = void (*)(BlockNormArgs);
 
 template <typename T, bool kPost, bool kGateRow>
-RowsKernel rows_kernel(int vec, int vpt) {
+RowsKernel rows_kernel(int vec, int vpt, int64_t threads) {
+  // The sums of a row leave an SM idle meanwhile unless it has a second CTA: in the
+  // 48 or 40 registers that 640 or 768 threads have then (4096 x 10240 72.7 us with one,
+  // 52.2 with two; x 12288 83.4 and 65.2, for all of 24 bytes spilled).
+  if (vec == 32 && vpt == 1 && threads > 512 && threads <= 768)
+    return threads <= 640 ? block_norm_rows<T, 32, 1, false, kPost, kGateRow, 640>
+                          : block_norm_rows<T, 32, 1, false, kPost, kGateRow, 768>;
   if (vec == 32) return vpt == 1 ? block_norm_rows<T, 32, 1, false, kPost, kGateRow> : nullptr;
   if (vec == 16) return vpt == 1 ? block_norm_rows<T, 16, 1, false, kPost, kGateRow> : block_norm_rows<T, 16, 2, false, kPost, kGateRow>;
   return vpt == 1 ? block_norm_rows<T, 16, 1, true, kPost, kGateRow> : block_norm_rows<T, 16, 2, true, kPost, kGateRow>;
@@ -235,9 +242,9 @@ int launch_forward(BlockNormArgs& a, int vec, const DeviceInfo* dev, cudaStream_
   const int64_t elems = vec > 0 ? vec / 2 : 8;
   a.nvec = static_cast<int32_t>((a.hidden + elems - 1) / elems);
   for (int vpt = 1; vpt <= 2; ++vpt) {
-    const RowsKernel fn = a.p ? (a.gate_row ? rows_kernel<T, true, true>(vec, vpt) : rows_kernel<T, true, false>(vec, vpt))
-                              : (a.gate_row ? rows_kernel<T, false, true>(vec, vpt) : rows_kernel<T, false, false>(vec, vpt));
     const int64_t threads = round_up((a.nvec + vpt - 1) / vpt, 32);
+    const RowsKernel fn = a.p ? (a.gate_row ? rows_kernel<T, true, true>(vec, vpt, threads) : rows_kernel<T, true, false>(vec, vpt, threads))
+                              : (a.gate_row ? rows_kernel<T, false, true>(vec, vpt, threads) : rows_kernel<T, false, false>(vec, vpt, threads));
     if (!fn || threads > 1024) continue;
     a.row_threads = static_cast<int32_t>(threads);
     const int groups = threads <= 64 ? static_cast<int>(128 / threads) : 1;
