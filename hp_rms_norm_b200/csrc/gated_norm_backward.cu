@@ -58,14 +58,15 @@ struct BlockGradArgs {
 // bulk copies.  Two sums over the row's threads lie between three passes over the
 // buffer: the means of squares and of w D n; then dt, and with it dr, dg, the sums
 // over rows, and the mean of p g dt m; then dx.  The second sum and the next row's
-// first one meet at one barrier (4096 x 8192 with E: 80 us, its bytes at a copy's rate 61).  The sums over rows (D n, and dt m
-// or g dt m) stay in registers, 4 W floats, as do w, p and a gate row that rows
-// share up to 8 words a thread.  Where a run reaches into another gate's rows, the
-// sums for the gate are written out and started anew.
+// first one meet at one barrier (4096 x 8192 with E: 80 us, its bytes at a copy's rate
+// 61).  The sums over rows (D n, and dt m or g dt m) stay in registers, 4 W floats, as
+// do w, p and a gate row that rows share up to 12 words a thread (of more they are in
+// shared memory).  Where a run reaches into another gate's rows, the sums for the gate
+// are written out and started anew.
 //   kVectors: every row of every tensor starts on a 16-byte boundary and hidden is
 // a multiple of 8.  Else a row is copied with the 16-byte granules it lies in
 // (elements in granules that reach out of the tensor one by one), and a vector put
-// together from two (12 x 257 rows of 1001, fp16: 36 us).
+// together from two (12 x 257 rows of 1001, fp16: 33 us).
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies in
 // flight, and says so (report_give_up).

@@ -12,7 +12,8 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 EPS = 1e-6
 # (leading dimensions, hidden)
 SHAPES = [((1,), 1), ((3,), 7), ((5,), 32), ((2, 9), 64), ((33,), 250), ((4, 17), 1001), ((1,), 4096), ((70,), 1024),
-          ((12, 11), 2056), ((9,), 5001), ((150,), 8192), ((6,), 16384), ((3,), 16383), ((2,), 20000), ((2, 2), 33001)]
+          ((12, 11), 2056), ((9,), 5001), ((150,), 8192), ((6,), 16384), ((3,), 16383), ((2,), 20000), ((2, 2), 33001),
+          ((400,), 10240), ((3,), 9216), ((170, 2), 12288)]
 GATES = ["none", "channel", "token", "sequence", "one for each sequence", "full", "one"]
 
 

@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 EPS = 1e-6
 ROWS = [(1, 1), (3, 7), (5, 32), (40, 250), (33, 1001), (1, 4096), (70, 1024), (9, 5001), (150, 8192), (5, 16384),
-        (3, 16383), (2, 20000), (2, 33001), (3000, 1001), (700, 5001)]
+        (3, 16383), (2, 20000), (2, 33001), (3000, 1001), (700, 5001),
+        (400, 12288), (3, 10240)]
 # (rows, hidden, channels)
 PRODUCTS = [(1, 1, 1), (1, 16, 32), (2, 15, 7), (3, 32, 64), (7, 33, 100), (16, 4096, 512), (1, 8192, 100), (33, 128, 129),
             (128, 256, 256), (130, 160, 1001), (257, 1000, 333), (300, 2731, 520), (520, 512, 1500), (1, 131071, 40),
