@@ -68,6 +68,7 @@ EXPORTED = (
     "hprn_linear_log_probs_backward",
     "hprn_rms_norm_int8",
     "hprn_linear_int8",
+    "hprn_test_loose_reads",
     "hprn_test_loss_backward_piece",
     "hprn_test_stall_loads",
 )
@@ -157,6 +158,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.hprn_linear_int8.argtypes = [vp] * 6 + [i64] * 6 + [c_int, vp, wsp, vp, u32]
     lib.hprn_test_loss_backward_piece.argtypes = [i64] * 4 + [wsp]
     lib.hprn_test_loss_backward_piece.restype = c_int
+    lib.hprn_test_loose_reads.argtypes = [i64] * 4 + [wsp]
+    lib.hprn_test_loose_reads.restype = c_int
     lib.hprn_test_stall_loads.argtypes = [c_int, ctypes.c_uint64]
     lib.hprn_test_stall_loads.restype = c_int
     for fn in (lib.hprn_gated_linear, lib.hprn_gated_linear_backward, lib.hprn_linear_cross_entropy,

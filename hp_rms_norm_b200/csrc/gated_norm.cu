@@ -333,4 +333,33 @@ int hprn_gated_add_rms_norm(void* out, void* residual_out, const void* input, co
                                   : launch_forward<__half>(a, vec, dev, cs, flags);
 }
 
+int hprn_test_loose_reads(int64_t rows, int64_t hidden, int64_t row_stride, int64_t start, int64_t* out) {
+  using namespace hprn;
+  if (rows < 1 || hidden < 1 || rows > 4096 || hidden > 65536 || row_stride < hidden || row_stride > 65536 || start < 0 ||
+      start > 7 || !out)
+    return fail(HPRN_ERR_INVALID_ARGUMENT, "rows, hidden, strides and starts of a small tensor");
+  // (Only addresses: nothing is read.)
+  const uint16_t* base = reinterpret_cast<const uint16_t*>(uintptr_t{1} << 30) + start;
+  const int n = static_cast<int>(hidden), lanes = (n + 255) / 256 * 32;
+  const int64_t end = (rows - 1) * row_stride + hidden;
+  out[0] = out[1] = out[2] = 0;
+  for (int64_t i = 0; i < rows; ++i) {
+    const LooseRow r = loose_row(base, i, rows, row_stride, n);
+    const int o = granule_offset(r.p);
+    for (int v = 0; v < lanes; ++v) {
+      int64_t from = 8 * v, to = from + 8 < hidden ? from + 8 : hidden;  // of the row
+      if (reads_granule(r, o, v)) from -= o, to = from + (reads_next(r, o, v) ? 16 : 8);
+      if (to > from) {
+        const int64_t before = -(i * row_stride + from), behind = i * row_stride + to - end;
+        if (before > out[0]) out[0] = before;
+        if (behind > out[1]) out[1] = behind;
+      }
+      // Elements of the row that the vector has and that were not read.
+      const int64_t last = 8 * v + 8 < hidden ? 8 * v + 8 : hidden;
+      if (8 * v < last && (to < last || from > 8 * v)) ++out[2];
+    }
+  }
+  return ok();
+}
+
 }  // extern "C"

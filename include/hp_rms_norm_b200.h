@@ -565,6 +565,16 @@ HPRN_API int hprn_test_stall_loads(int on, uint64_t wait_limit_ns);
 HPRN_API int hprn_test_loss_backward_piece(int64_t rows, int64_t hidden, int64_t vocab,
                                            int64_t piece, int64_t* out);
 
+/*
+ * No reference counterpart.  Test hook, launches and reads nothing: what the row
+ * kernels of hprn_gated_add_rms_norm and hprn_rms_norm_int8 read of a tensor whose
+ * rows lie off 16-byte boundaries, `start` elements behind one.  Writes to out[0..2]
+ * the most elements read before the tensor, the most behind it, and the vectors of
+ * which an element is not read.
+ */
+HPRN_API int hprn_test_loose_reads(int64_t rows, int64_t hidden, int64_t row_stride, int64_t start,
+                                   int64_t* out);
+
 #ifdef __cplusplus
 }
 #endif
