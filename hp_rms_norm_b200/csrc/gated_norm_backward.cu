@@ -44,7 +44,8 @@ struct BlockGradArgs {
   uint32_t ring_at;  // in shared memory
   bool staged;       // w and p are in shared memory, before the ring
   bool e_direct;     // E is read where it is, not through the ring
-  int64_t ctas;
+  int64_t ctas, runs;
+  bool own_runs;  // of the groups of a CTA
   bool dense;  // every tensor's rows follow each other
   Waits waits;
 };
@@ -54,6 +55,12 @@ struct BlockGradArgs {
 //
 // A CTA works on a run of neighbouring rows, `row_groups` at a time, each by
 // row_threads threads, a thread always on the same W words (pairs of elements).
+//   Where a gate's row is shared by few rows, more than two gates a CTA, each group has
+// a run of its own: the sums for a gate are then one row for each run that meets it,
+// where groups that share a run each write a row for every gate of it (gates of two rows,
+// 65536 x 512: 67 MiB of workspace for 579, 3.9 ms for 10.3; of 64 rows 246 us for 347).
+// With more rows a gate a CTA's rows are better copied together (65536 x 128, gates of
+// 512 rows: 85 us, with runs of their own 127).
 // One warp more brings the rows into a ring of `slots` buffers in shared memory by
 // bulk copies.  Two sums over the row's threads lie between three passes over the
 // buffer: the means of squares and of w D n; then dt, and with it dr, dg, the sums
@@ -126,18 +133,22 @@ __device__ __forceinline__ void set_shared_half(uint32_t addr, uint16_t h) {
   asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(h) : "memory");
 }
 
-// The first row of CTA c's run; row i lies in the run of CTA
-// ((i + 1) ctas - 1) / rows.
-__device__ __forceinline__ int64_t run_start(const BlockGradArgs& a, int64_t c) { return a.rows * c / a.ctas; }
-__device__ __forceinline__ int64_t run_of(const BlockGradArgs& a, int64_t i) { return ((i + 1) * a.ctas - 1) / a.rows; }
+// The first row of run c (no more runs than rows: none is empty); row i lies in run
+// ((i + 1) runs - 1) / rows.
+__device__ __forceinline__ int run_start(const BlockGradArgs& a, int64_t c) {
+  return static_cast<int>(a.rows * min(c, a.runs) / a.runs);
+}
+__device__ __forceinline__ int64_t run_of(const BlockGradArgs& a, int64_t i) { return ((i + 1) * a.runs - 1) / a.rows; }
 
 // kGate: kOneGate a gate of one value a row, or none (1); kChannels one row of values
-// for all rows; kGateRow rows of values that rows share; kGateEach one for every row.
-enum GateKind { kOneGate, kChannels, kGateRow, kGateEach };
+// for all rows; kGateRow rows of values that rows share, kGateRuns with own runs;
+// kGateEach one for every row.
+enum GateKind { kOneGate, kChannels, kGateRow, kGateRuns, kGateEach };
 
 template <typename T, int W, bool kVectors, bool kPost, int kGate>
 __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(BlockGradArgs a) {
   constexpr int kVecs = W / 4;
+  constexpr bool kOwnRuns = kGate == kGateRuns, kSharedRow = kGate == kGateRow || kOwnRuns;
   constexpr bool kHold = W <= 12;
   static_assert(kHold || kVectors, "vectors of loose rows are read by two threads");
   extern __shared__ __align__(128) unsigned char row_mem[];
@@ -154,8 +165,12 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
   const uint32_t row_bytes = static_cast<uint32_t>(nvec) * 16, pitch = row_bytes + (kVectors ? 0 : 16);
   const uint32_t tensor_bytes = pitch * groups, slot_bytes = tensor_bytes * a.tensors;
   const uint32_t staged = smem_u32(row_mem), ring = staged + a.ring_at;
-  const int begin = static_cast<int>(run_start(a, blockIdx.x)), end = static_cast<int>(run_start(a, blockIdx.x + 1));
-  const int lane = tid % 32;
+  // A group's rows, `step` apart; its run, its own or the CTA's.  A lane of the copying
+  // warp has a group's.
+  const int lane = tid % 32, member = copier ? lane : group, step = kOwnRuns ? 1 : groups;
+  const int64_t run = kOwnRuns ? static_cast<int64_t>(blockIdx.x) * groups + min(member, groups - 1) : blockIdx.x;
+  const int begin = run_start(a, run), end = run_start(a, run + 1);
+  const int first = kOwnRuns ? begin : begin + member;
   if (copier) {
     if (lane < groups) gave_up[lane] = 0;
     if (lane == 0) {
@@ -166,10 +181,11 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
       mbar_init_fence();
     }
     // The first rows, into L2, while the preceding grid drains.
-    const int first = begin + lane;
-    if (lane < groups * a.slots && first < end)
-      for (int t = 0; t < a.tensors; ++t)
-        prefetch_l2(a.src[t] + static_cast<int64_t>(first) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
+    const int ahead = kOwnRuns ? min(end, first + a.slots) : min(end, first + 1);
+    if (lane < (kOwnRuns ? groups : groups * a.slots))
+      for (int i = first; i < ahead; ++i)
+        for (int t = 0; t < a.tensors; ++t)
+          prefetch_l2(a.src[t] + static_cast<int64_t>(i) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
   }
   __syncthreads();
   pdl_wait();
@@ -179,14 +195,19 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int base = a.waits.stall ? end : begin; base < end; base += groups) {
+    // (Runs differ by a row at most: only a last round has groups without one.)
+    // The lane's row: `base` and, in a run that groups share, its own behind it.
+    const int longest = kOwnRuns ? __reduce_max_sync(~0u, end - begin) : end - begin;
+    const int behind = kOwnRuns ? 0 : lane;
+    for (int done = a.waits.stall ? longest : 0; done < longest; done += step) {
       ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), phase ^ 1, a.waits.limit_ns));
       if (!ok) break;
       const uint32_t bar = smem_u32(&full[slot]), to = ring + slot * slot_bytes;
-      const int here = min(groups, end - base);
       // With few buffers a later round's rows are asked into L2.
-      const int next = base + a.slots * groups;
-      if (kVectors && a.dense) {
+      const int base = begin + done, next = base + a.slots * step;
+      const bool mine = lane < groups && base + behind < end;
+      if (kVectors && !kOwnRuns && a.dense) {
+        const int here = min(groups, end - base);
         const uint32_t bytes = static_cast<uint32_t>(here) * row_bytes;
         if (lane == 0) mbar_arrive_expect_tx(bar, bytes * a.tensors);
         __syncwarp();
@@ -197,8 +218,7 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
                         static_cast<uint64_t>(min(groups, end - next)) * row_bytes);
         }
       } else {
-        const bool mine = lane < here;
-        const int64_t i = base + lane;
+        const int64_t i = base + behind;
         const unsigned char* from[5];
         uint32_t bytes[5], at[5], total = 0;
 #pragma unroll
@@ -235,12 +255,12 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
 #pragma unroll
         for (int t = 0; t < 5; ++t) {
           if (bytes[t] > 0) bulk_load(at[t], from[t], bytes[t], bar, pol);
-          if (a.slots < 3 && t < a.tensors && lane < groups && next + lane < end)
-            prefetch_l2(a.src[t] + (next + lane) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
+          if (a.slots < 3 && t < a.tensors && lane < groups && next + behind < end)
+            prefetch_l2(a.src[t] + (next + behind) * a.src_stride[t], static_cast<uint64_t>(hidden) * 2);
         }
       }
-      if (a.e_direct && lane < here)
-        prefetch_l2(a.e + (base + lane) * a.e_stride, static_cast<uint64_t>(hidden) * 2);
+      if (a.e_direct && mine)
+        prefetch_l2(a.e + (base + behind) * a.e_stride, static_cast<uint64_t>(hidden) * 2);
       if (++slot == a.slots) slot = 0, phase ^= 1;
     }
     if (!ok) {
@@ -372,7 +392,8 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
   // rows had, zeros for the others.
   auto finish_gates = [&](int k) {
     for (; gate_at < k; ++gate_at) {
-      write_sums(acc_m, a.m_parts + (static_cast<int64_t>(blockIdx.x + gate_at) * groups + group) * a.parts_ld);
+      const int64_t at = run + gate_at;
+      write_sums(acc_m, a.m_parts + (kOwnRuns ? at : at * groups + group) * a.parts_ld);
 #pragma unroll
       for (int q = 0; q < W; ++q) acc_m[q] = make_float2(0.f, 0.f);
     }
@@ -382,7 +403,7 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
   int64_t last = -1;  // the row whose last pass is due; its buffer, and what its sums are multiplied by
   uint32_t last_at = 0, last_bar = 0;
   float last_by = 0.f, last_inv = 0.f;
-  for (int64_t i = begin + group;; i += groups) {
+  for (int64_t i = first;; i += step) {
     const bool more = i < end;
     const uint32_t at = ring + slot * slot_bytes + group * pitch;
     auto start_of = [&](int t) {
@@ -460,7 +481,7 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
       break;
     }
     const uint16_t* gate_row = a.g;
-    if constexpr (kGate == kGateRow) {
+    if constexpr (kSharedRow) {
       const int k = static_cast<int>(i) / rows_per_gate;
       gate_row = a.g + k * a.g_stride;
       if (k != held_gate) {
@@ -492,7 +513,7 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
       if (a.e_at >= 0) load_row(e4, start_of(a.e_at), k);
       if constexpr (kPost) weight(p, 1, a.p, k);
       if constexpr (kGate == kGateEach) load_row(g, start_of(a.g_at), k);
-      if constexpr (kGate == kGateRow || kGate == kChannels) weight(g, 2, gate_row, k);
+      if constexpr (kSharedRow || kGate == kChannels) weight(g, 2, gate_row, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 dt = __ffma2_rn(mul_pair<T>(w[e], d[e]), inv_t2, __ffma2_rn(unpack2<T>(t[e]), minus, unpack2<T>(e4[e])));
@@ -541,7 +562,7 @@ __global__ void __launch_bounds__(block_threads(W) + 32, 1) block_grad_rows(Bloc
     if (++slot == a.slots) slot = 0, phase ^= 1;
   }
   // Buffers of a last round with fewer rows than groups are nobody's any more.
-  if constexpr (kGate == kGateRow) finish_gates((end - 1) / rows_per_gate + 1);
+  if constexpr (kSharedRow) finish_gates((end - 1) / rows_per_gate + 1);
   else join_sums(acc_m, a.m_parts + blockIdx.x * a.parts_ld);
   join_sums(acc_w, a.dw_parts + blockIdx.x * a.parts_ld);
 }
@@ -572,7 +593,7 @@ __global__ void __launch_bounds__(32 * kRunWarps) block_grad_runs(BlockGradArgs 
   } else {
     const float p = in && a.p ? unpack1<T>(a.p[j]) : 1.f;
     const bool together = a.gates <= 2;
-    const int groups = a.gates > 1 ? a.row_groups : 1;
+    const int groups = a.gates > 1 && !a.own_runs ? a.row_groups : 1;
     for (int64_t k = together ? 0 : ty; k < a.gates; k += together ? 1 : kRunWarps) {
       // The sums of the runs that the gate's rows lie in follow each other.
       const int64_t first = (run_of(a, k * a.rows_per_gate) + k) * groups;
@@ -793,6 +814,9 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
       plan.smem = static_cast<int>(ring > joined ? ring : joined);
       const int64_t need = (a.rows + groups - 1) / groups;
       a.ctas = need < 148 ? need : 148;
+      a.runs = a.ctas;
+      a.own_runs = a.gate_row && !a.gate_each && a.gates > 2 * a.ctas;
+      if (a.own_runs) a.runs = a.ctas * groups < a.rows ? a.ctas * groups : a.rows;
       break;
     }
     if (plan.words > 0) break;
@@ -812,11 +836,13 @@ void (*block_grad_kernel(int words))(BlockGradArgs) {
 }
 template <typename T, bool kVectors>
 void (*block_grad_kernel(const BlockGradArgs& a, int words))(BlockGradArgs) {
-  const int gate = !a.gate_row ? kOneGate : a.gate_each ? kGateEach : a.gates == 1 ? kChannels : kGateRow;
+  const int gate = !a.gate_row ? kOneGate : a.gate_each ? kGateEach : a.gates == 1 ? kChannels : a.own_runs ? kGateRuns : kGateRow;
   if (gate == kChannels)
     return a.p ? block_grad_kernel<T, kVectors, true, kChannels>(words) : block_grad_kernel<T, kVectors, false, kChannels>(words);
   if (gate == kOneGate)
     return a.p ? block_grad_kernel<T, kVectors, true, kOneGate>(words) : block_grad_kernel<T, kVectors, false, kOneGate>(words);
+  if (gate == kGateRuns)
+    return a.p ? block_grad_kernel<T, kVectors, true, kGateRuns>(words) : block_grad_kernel<T, kVectors, false, kGateRuns>(words);
   if (gate == kGateRow)
     return a.p ? block_grad_kernel<T, kVectors, true, kGateRow>(words) : block_grad_kernel<T, kVectors, false, kGateRow>(words);
   return a.p ? block_grad_kernel<T, kVectors, true, kGateEach>(words) : block_grad_kernel<T, kVectors, false, kGateEach>(words);
@@ -905,12 +931,12 @@ int hprn_gated_add_rms_norm_backward(
   a.gate_sums = ws.take<float>(gate && !a.gate_row ? rows : 0);
   if (!gate || a.gate_row) a.gate_sums = nullptr;
   a.parts_ld = round_up(hidden, 8);
-  // A run and a gate it meets make one row of sums (for each group of threads): each
-  // step to the next of them goes on by a run, a gate or both, so that run + gate tells
-  // them apart.
+  // A run and a gate it meets make one row of sums (for each group of threads that shares
+  // it): each step to the next of them goes on by a run, a gate or both, so that run +
+  // gate tells them apart.
   const int64_t parts = (shared_row ? gates : 1) * a.parts;
   a.dw_parts = ws.take<float>((plan.words > 0 ? a.ctas : parts) * a.parts_ld);
-  a.m_parts = ws.take<float>((plan.words == 0 ? parts : shared_row && gates > 1 ? (a.ctas + gates) * a.row_groups : a.ctas) * a.parts_ld);
+  a.m_parts = ws.take<float>((plan.words == 0 ? parts : shared_row && gates > 1 ? (a.runs + gates) * (a.own_runs ? 1 : a.row_groups) : a.runs) * a.parts_ld);
   if (flags & HPRN_WORKSPACE_QUERY) {
     *workspace_bytes = ws.needed();
     return ok();

@@ -123,6 +123,18 @@ def test_workspaces_stay_bounded():
     assert capi.workspace_bytes(*probs(rows=4096, vocab=1 << 22, hidden=64)[1]) <= 256 * (1 << 24) * 1.2
 
 
+@pytest.mark.parametrize("hidden", [64, 512, 1001, 4096, 8192, 16384])
+@pytest.mark.parametrize("rows,per", [(65536, 2), (65536, 3 * 2 ** 4), (5000, 2), (1 << 20, 4), (30, 15), (4096, 2048)])
+def test_gates_that_rows_share_stay_bounded(rows, per, hidden):
+    """The sums for a gate are one row of floats and one more for each run of rows that ends inside
+    it, a run for each of at most 14 groups of 148 CTAs; or, of at most two gates a CTA, a row for each
+    group.  With gates of two rows that is the size of the rows themselves."""
+    per = per if rows % per == 0 else 2
+    strides = {k: hidden for k in ("dxs", "drs", "dgs", "ds", "es", "xs", "ts", "gs")}
+    need = capi.workspace_bytes(*norm_backward(rows=rows, hidden=hidden, per=per, width=hidden, **strides)[1])
+    assert need <= 4 * -(-hidden // 8) * 8 * (rows // per + 148 * (3 * 14 + 1)) + 1024
+
+
 def test_signatures():
     import inspect
 
