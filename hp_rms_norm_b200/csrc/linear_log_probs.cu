@@ -152,11 +152,11 @@ __device__ __forceinline__ void meet(int barrier) {
 }
 
 // Joins the parts of row i, by kJoinThreads threads `thread`: the largest first, then
-// the sums relative to it, so that no term waits for another.  Returns the row's lse
-// in each of them.
+// the sums relative to it, so that no term waits for another.  Returns m and log s in
+// each of them.
 constexpr int kJoinThreads = 128;
 
-__device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i, int thread) {
+__device__ __forceinline__ float2 join_row(const LogProbJoin& q, int64_t i, int thread) {
   constexpr int kThreads = kJoinThreads, kWarps = kThreads / 32;
   __shared__ float most[kWarps], sums[2][kWarps];
   const int lane = thread % 32, warp = thread / 32;
@@ -198,7 +198,7 @@ __device__ __forceinline__ float join_row(const LogProbJoin& q, int64_t i, int t
                                     : ((q.parts > 0 ? q.target_logit[i] : 0.f) - top) * q.inv_t - log_s;
     q.entropy[i] = t == kIgnored ? 0.f : log_s - 0.693147180559945f * (a / s);
   }
-  return lse;
+  return make_float2(top, log_s);
 }
 
 __global__ void __launch_bounds__(kJoinThreads) log_prob_join(LogProbJoin q) {
@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopAr
   __shared__ uint64_t part[2][kWarps], collected[kCollect];
   __shared__ uint32_t group_at[kCollect], column[kMostCandidates];
   __shared__ int group_count, count;
-  __shared__ double exact[kMostCandidates], shares[kAllWarps];
-  __shared__ float row_lse;
+  __shared__ double exact[kMostCandidates], off[kMostCandidates], shares[kAllWarps];
+  __shared__ float2 joined;
   const int64_t i = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32;
   float* values = a.values + i * a.top;
@@ -480,15 +480,15 @@ __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopAr
   pdl_wait();
   __syncthreads();
   if (tid >= kTopThreads) {
-    const float lse = join_row(a.join, i, tid - kTopThreads);
-    if (tid == kTopThreads) row_lse = lse;
+    const float2 q = join_row(a.join, i, tid - kTopThreads);
+    if (tid == kTopThreads) joined = q;
   } else if (a.hidden > 0) {
     search();
   }
   __syncthreads();
-  const float lse = row_lse;
+  const float most = joined.x, log_s = joined.y;
   if (a.hidden == 0) {  // logits that are sums of no terms
-    if (tid < a.top) values[tid] = -lse, indices[tid] = tid;
+    if (tid < a.top) values[tid] = -log_s, indices[tid] = tid;
     return;
   }
   // The candidates' weights into L2 at once: the warps take them in turn.
@@ -504,22 +504,36 @@ __global__ void __launch_bounds__(kTopThreads + kJoinThreads) log_prob_top(TopAr
                                   min(first + length, a.hidden));
     if (lane == 0) (parts > 1 ? shares[task] : exact[c]) = s;
   }
+  // How far the logit that is in s is off, times its share of s.
+  const float summed = tid < a.candidates ? row[column[tid]] : 0.f;
   __syncthreads();
-  if (parts > 1 && tid < a.candidates) {
-    double s = 0.0;
-    for (int k = 0; k < parts; ++k) s += shares[tid * parts + k];
-    exact[tid] = s;
+  if (tid < a.candidates) {
+    double s = exact[tid];
+    if (parts > 1) {
+      s = 0.0;
+      for (int k = 0; k < parts; ++k) s += shares[tid * parts + k];
+      exact[tid] = s;
+    }
+    const float p = expf((summed - most) * a.join.inv_t - log_s);
+    off[tid] = p > 0.f ? (s - static_cast<double>(summed)) * static_cast<double>(p) : 0.0;
   }
   __syncthreads();
   if (tid >= a.candidates) return;
   const uint64_t bits = order_bits(exact[tid]);
   int rank = 0;
+  double all_off = 0.0;
   for (int c = 0; c < a.candidates; ++c) {
     const uint64_t other = order_bits(exact[c]);
     rank += other > bits || (other == bits && column[c] < column[tid]);
+    all_off += off[c];
   }
   if (rank >= a.top) return;
-  values[rank] = static_cast<float>(exact[tid] * a.inv_t - static_cast<double>(lse));
+  // lse in 64 bits, moved by what the candidates' logits are off (its derivatives by
+  // logits are the shares).  As an fp32 number, near 30 a multiple of 2^-19, it left
+  // values above 0 in rows whose largest logit has all the weight, 4e-5 off with logits of
+  // 100 where this is 1e-6.
+  const double value = (exact[tid] - static_cast<double>(most) - all_off) * a.inv_t - static_cast<double>(log_s);
+  values[rank] = value > 0.0 ? 0.f : static_cast<float>(value);
   indices[rank] = column[tid];
 }
 

@@ -1,5 +1,6 @@
 """linear_log_probs and its backward pass on the GPU against the 64-bit formulas."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -108,6 +109,27 @@ def test_neighbours_in_the_last_bits(cuda):
     w[:, 100] = torch.randint(-64, 65, (2000,), generator=g, device=cuda).to(w.dtype) / 64
     _, order = ranked(x.double() @ w.double().T, 12)
     assert torch.equal(hp.linear_log_probs(x, w, t, top=12).top_indices, order)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("rows,vocab", [(1, 300), (8, 5000), (64, 5000), (300, 40001)], ids=str)
+def test_rows_whose_largest_has_the_weight(cuda, rows, vocab, temperature):
+    """No alternative's value is above 0, in rows with nearly all weight on one token, rows that are
+    flat, rows of zeros.  Where one has all of it but 2^-30, its value is 0 to 2^-23, whatever the
+    rounding of lse, and so is its log probability."""
+    x, w, _, _, _ = make(rows, 128, vocab, torch.bfloat16, cuda, scale=20.0)
+    x[rows // 2] = 0
+    x[:rows // 3] /= 16
+    x[-1] = 4 * w[7]
+    logits = x.double() @ w.double().T / temperature
+    best = logits.topk(2, dim=-1)
+    # The others are at most vocab - 1 times the second.
+    sharp = best.values[:, 0] - best.values[:, 1] > 21 + math.log(vocab)
+    assert sharp.any()
+    found = hp.linear_log_probs(x, w, best.indices[:, 0].contiguous(), top=5, temperature=temperature)
+    assert torch.equal(found.top_indices[sharp, 0], best.indices[sharp, 0])
+    assert (found.top_log_probs <= 0).all()
+    assert (found.top_log_probs[sharp, 0] >= -(2.0 ** -23)).all() and (found.log_prob[sharp].abs() <= 2.0 ** -23).all()
 
 
 def test_blocks_of_rows(cuda):
