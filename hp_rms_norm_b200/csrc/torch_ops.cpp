@@ -925,9 +925,11 @@ template <typename M>
 BlockGrads block_grads_like(const at::Tensor& input, const c10::optional<at::Tensor>& post_weight,
                             const at::Tensor& weight, const c10::optional<at::Tensor>& gate) {
   auto like = [](const at::Tensor& t) { return M::dense_like(t, t.scalar_type()); };
-  const at::Tensor none = post_weight.has_value() && gate.has_value() ? at::Tensor() : at::empty({0}, input.options());
-  return {like(input), like(input), post_weight.has_value() ? like(*post_weight) : none, like(weight),
-          gate.has_value() ? like(*gate) : none};
+  // (One each: outputs of an operator are not the same tensor.)
+  auto like_or_none = [&](const c10::optional<at::Tensor>& t) {
+    return t.has_value() ? like(*t) : at::empty({0}, input.options());
+  };
+  return {like(input), like(input), like_or_none(post_weight), like(weight), like_or_none(gate)};
 }
 
 BlockGrads gated_add_rms_norm_backward_new(const at::Tensor& grad_out, c10::optional<at::Tensor> grad_residual_out,

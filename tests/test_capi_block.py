@@ -164,6 +164,15 @@ def test_shapes_without_a_device():
     assert dx.shape == x.shape and dw.shape == v.shape
 
 
+def test_outputs_are_tensors_of_their_own():
+    """Gradients of what is absent too: the schema declares five outputs that alias nothing."""
+    x, w = torch.empty(4, 64, device="meta", dtype=torch.bfloat16), torch.empty(64, device="meta", dtype=torch.bfloat16)
+    for post, gate in ((None, None), (w, None), (None, w), (w, w)):
+        grads = torch.ops.hp_rms_norm.gated_add_rms_norm_backward.default(x, None, x, x, post, w, gate, 1.0, 1e-6)
+        assert len({id(g) for g in grads}) == 5
+        assert [g.numel() for g in grads] == [256, 256, 0 if post is None else 64, 64, 0 if gate is None else 64]
+
+
 def test_no_cpu_kernels():
     x, w = torch.zeros(4, 8).bfloat16(), torch.ones(8).bfloat16()
     for call in (lambda: hp.gated_add_rms_norm(x, x.clone(), w, w, 1e-6), lambda: hp.rms_norm_int8(x, w, 1e-6),
