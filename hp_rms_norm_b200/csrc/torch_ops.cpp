@@ -692,13 +692,13 @@ BlockNorm check_block_norm(const at::Tensor& input, const c10::optional<at::Tens
   return c;
 }
 
-void gated_add_rms_norm(at::Tensor& out, at::Tensor& residual, c10::optional<at::Tensor> residual_out,
-                        const at::Tensor& input, c10::optional<at::Tensor> post_weight,
-                        const at::Tensor& weight, c10::optional<at::Tensor> gate,
-                        double residual_scale, double eps) {
+// The new residual in a tensor of its own.
+void gated_add_rms_norm_sum(at::Tensor& out, at::Tensor& total, const at::Tensor& input,
+                            const at::Tensor& residual, c10::optional<at::Tensor> post_weight,
+                            const at::Tensor& weight, c10::optional<at::Tensor> gate,
+                            double residual_scale, double eps) {
   const BlockNorm c = check_block_norm(input, post_weight, weight, gate);
   const at::ScalarType type = input.scalar_type();
-  const at::Tensor& total = residual_out.has_value() ? *residual_out : residual;
   TORCH_CHECK(out.sizes() == input.sizes(), "out must have the input's shape");
   TORCH_CHECK(residual.sizes() == input.sizes(), "residual must have the input's shape");
   TORCH_CHECK(total.sizes() == input.sizes(), "residual_out must have the input's shape");
@@ -712,6 +712,14 @@ void gated_add_rms_norm(at::Tensor& out, at::Tensor& residual, c10::optional<at:
                                        c.rows_per_gate, c.gate_width, o.stride, t.stride, c.x.stride,
                                        r.stride, c.g.stride, residual_scale, eps, c.dtype, stream,
                                        HPRN_LAUNCH_DEFAULT));
+}
+
+void gated_add_rms_norm(at::Tensor& out, at::Tensor& residual, c10::optional<at::Tensor> residual_out,
+                        const at::Tensor& input, c10::optional<at::Tensor> post_weight,
+                        const at::Tensor& weight, c10::optional<at::Tensor> gate,
+                        double residual_scale, double eps) {
+  gated_add_rms_norm_sum(out, residual_out.has_value() ? *residual_out : residual, input, residual, post_weight,
+                         weight, gate, residual_scale, eps);
 }
 
 void gated_add_rms_norm_backward(at::Tensor& grad_input, at::Tensor& grad_residual,
@@ -1015,6 +1023,17 @@ std::tuple<at::Tensor, at::Tensor> rms_norm_int8_new(const at::Tensor& input, c1
   return outputs;
 }
 
+std::tuple<at::Tensor, at::Tensor> rms_norm_int8_sum(const at::Tensor& input, c10::optional<at::Tensor> weight,
+                                                     const at::Tensor& residual, at::Tensor& residual_out,
+                                                     double eps) {
+  return rms_norm_int8_new(input, weight, residual, residual_out, eps);
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_int8_sum_meta(const at::Tensor& input, c10::optional<at::Tensor>,
+                                                          const at::Tensor&, at::Tensor&, double) {
+  return int8_outputs<Shapes>(input);
+}
+
 std::tuple<at::Tensor, at::Tensor> rms_norm_int8_new_meta(const at::Tensor& input, c10::optional<at::Tensor>,
                                                           c10::optional<at::Tensor>, c10::optional<at::Tensor>,
                                                           double) {
@@ -1044,6 +1063,9 @@ at::Tensor linear_int8_new_meta(const at::Tensor& input, const at::Tensor&, cons
 void gated_add_rms_norm_meta(at::Tensor&, at::Tensor&, c10::optional<at::Tensor>, const at::Tensor&,
                              c10::optional<at::Tensor>, const at::Tensor&, c10::optional<at::Tensor>,
                              double, double) {}
+void gated_add_rms_norm_sum_meta(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                 c10::optional<at::Tensor>, const at::Tensor&, c10::optional<at::Tensor>,
+                                 double, double) {}
 void rms_norm_int8_meta(at::Tensor&, at::Tensor&, const at::Tensor&, c10::optional<at::Tensor>,
                         c10::optional<at::Tensor>, c10::optional<at::Tensor>, double) {}
 void linear_int8_meta(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
@@ -1110,6 +1132,9 @@ TORCH_LIBRARY(hp_rms_norm, m) {
         "Tensor input, Tensor weight, Tensor? grad_residual, float eps) -> ()");
   m.def("gated_add_rms_norm(Tensor(a!) out, Tensor(b!) residual, Tensor(c!)? residual_out, Tensor input, "
         "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
+  // The .sum forms leave residual as it is, so that a traced graph orders no write to it.
+  m.def("gated_add_rms_norm.sum(Tensor(a!) out, Tensor(b!) residual_out, Tensor input, Tensor residual, "
+        "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
   // (Gradients of what is absent come back without elements, as do alternatives with top 0.)
   m.def("gated_add_rms_norm_backward(Tensor grad_out, Tensor? grad_residual_out, Tensor input, "
         "Tensor residual_out, Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, "
@@ -1123,6 +1148,8 @@ TORCH_LIBRARY(hp_rms_norm, m) {
         "(Tensor grad_input, Tensor grad_weight)");
   // Extensions: 8-bit integers.
   m.def("rms_norm_int8(Tensor input, Tensor? weight, Tensor(a!)? residual, Tensor(b!)? residual_out, "
+        "float eps) -> (Tensor codes, Tensor scales)");
+  m.def("rms_norm_int8.sum(Tensor input, Tensor? weight, Tensor residual, Tensor(a!) residual_out, "
         "float eps) -> (Tensor codes, Tensor scales)");
   m.def("rms_norm_int8.out(Tensor(a!) out, Tensor(b!) scales, Tensor input, Tensor? weight, "
         "Tensor(c!)? residual, Tensor(d!)? residual_out, float eps) -> ()");
@@ -1152,10 +1179,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("grad_norm", &grad_norm);
   m.impl("clip_grad_norm", &clip_grad_norm);
   m.impl("gated_add_rms_norm", &gated_add_rms_norm);
+  m.impl("gated_add_rms_norm.sum", &gated_add_rms_norm_sum);
   m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_new);
   m.impl("linear_log_probs", &linear_log_probs_new);
   m.impl("linear_log_probs_backward", &linear_log_probs_backward_new);
   m.impl("rms_norm_int8", &rms_norm_int8_new);
+  m.impl("rms_norm_int8.sum", &rms_norm_int8_sum);
   m.impl("rms_norm_int8.out", &rms_norm_int8);
   m.impl("linear_int8", &linear_int8_new);
   m.impl("linear_int8.out", &linear_int8);
@@ -1179,10 +1208,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("grad_norm", &grad_norm_meta);
   m.impl("clip_grad_norm", &clip_grad_norm_meta);
   m.impl("gated_add_rms_norm", &gated_add_rms_norm_meta);
+  m.impl("gated_add_rms_norm.sum", &gated_add_rms_norm_sum_meta);
   m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_new_meta);
   m.impl("linear_log_probs", &linear_log_probs_new_meta);
   m.impl("linear_log_probs_backward", &linear_log_probs_backward_new_meta);
   m.impl("rms_norm_int8", &rms_norm_int8_new_meta);
+  m.impl("rms_norm_int8.sum", &rms_norm_int8_sum_meta);
   m.impl("rms_norm_int8.out", &rms_norm_int8_meta);
   m.impl("linear_int8", &linear_int8_new_meta);
   m.impl("linear_int8.out", &linear_int8_meta);
@@ -1195,5 +1226,6 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Autograd, m) {
   m.impl("linear_log_probs", torch::CppFunction::makeFallthrough());
   m.impl("linear_log_probs_backward", torch::CppFunction::makeFallthrough());
   m.impl("rms_norm_int8", torch::CppFunction::makeFallthrough());
+  m.impl("rms_norm_int8.sum", torch::CppFunction::makeFallthrough());
   m.impl("linear_int8", torch::CppFunction::makeFallthrough());
 }

@@ -236,7 +236,11 @@ def gated_add_rms_norm(input, residual, post_weight, weight, eps, gate=None, res
     of 1.  The sums are fp32 and ``out`` comes from the unrounded new residual.  Returns ``out``."""
     if out is None:
         out = torch.empty_like(input)
-    _ops.gated_add_rms_norm.default(out, residual, residual_out, input, post_weight, weight, gate,
+    if residual_out is None or residual_out is residual:
+        _ops.gated_add_rms_norm.default(out, residual, None, input, post_weight, weight, gate,
+                                        residual_scale, eps)
+    else:
+        _ops.gated_add_rms_norm.sum(out, residual_out, input, residual, post_weight, weight, gate,
                                     residual_scale, eps)
     return out
 
@@ -290,7 +294,9 @@ def rms_norm_int8(input, weight, eps, residual=None, residual_out=None):
     ``residual`` itself without one) with an int8 output and one scale a row: returns (codes,
     scales), codes int8 of input's shape, scales float32 [...] = max|y| / 127, y ~ codes *
     scale.  ``linear_int8`` takes both."""
-    return _ops.rms_norm_int8.default(input, weight, residual, residual_out, eps)
+    if residual is None or residual_out is None or residual_out is residual:
+        return _ops.rms_norm_int8.default(input, weight, residual, residual_out, eps)
+    return _ops.rms_norm_int8.sum(input, weight, residual, residual_out, eps)
 
 
 def quantize_int8(input):

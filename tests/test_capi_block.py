@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import hp_rms_norm_b200 as hp
 from hp_rms_norm_b200 import capi
@@ -171,6 +172,30 @@ def test_outputs_are_tensors_of_their_own():
         grads = torch.ops.hp_rms_norm.gated_add_rms_norm_backward.default(x, None, x, x, post, w, gate, 1.0, 1e-6)
         assert len({id(g) for g in grads}) == 5
         assert [g.numel() for g in grads] == [256, 256, 0 if post is None else 64, 64, 0 if gate is None else 64]
+
+
+def test_only_what_is_written_is_declared_written():
+    """A traced graph orders and copies for the writes that the schemas declare."""
+    class Written(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            for declared, given in zip(func._schema.arguments, args):
+                if declared.alias_info is not None and declared.alias_info.is_write and isinstance(given, torch.Tensor):
+                    found.append(given)
+            return func(*args, **(kwargs or {}))
+
+    x, w = torch.empty(4, 64, device="meta", dtype=torch.bfloat16), torch.empty(64, device="meta", dtype=torch.bfloat16)
+    r, out, total = x.clone(), x.clone(), x.clone()
+    for call, want in ((lambda: hp.gated_add_rms_norm(x, r, w, w, 1e-6, out=out, residual_out=total), [out, total]),
+                       (lambda: hp.gated_add_rms_norm(x, r, w, w, 1e-6, out=out), [out, r]),
+                       (lambda: hp.gated_add_rms_norm(x, r, w, w, 1e-6, out=out, residual_out=r), [out, r]),
+                       (lambda: hp.rms_norm_int8(x, w, 1e-6, residual=r, residual_out=total), [total]),
+                       (lambda: hp.rms_norm_int8(x, w, 1e-6, residual=r), [r]),
+                       (lambda: hp.rms_norm_int8(x, w, 1e-6, residual=r, residual_out=r), [r]),
+                       (lambda: hp.rms_norm_int8(x, w, 1e-6), [])):
+        found = []
+        with Written():
+            call()
+        assert {id(t) for t in found} == {id(t) for t in want}
 
 
 def test_no_cpu_kernels():
