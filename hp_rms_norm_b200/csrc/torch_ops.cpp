@@ -926,6 +926,19 @@ struct Tensors {
   }
 };
 
+// The operators below fall through Autograd, whose own bookkeeping costs each call host
+// time, so that the dispatcher does not tell a caller who asks for gradients: they do.
+inline bool asks(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+inline bool asks(const c10::optional<at::Tensor>& t) { return t.has_value() && asks(*t); }
+template <typename... Ts>
+bool any_asks(const Ts&... t) {
+  return c10::GradMode::is_enabled() && (asks(t) || ...);
+}
+#define HPRN_NOTE_NO_HISTORY(name, differentiable, ...)                                                        \
+  if (any_asks(__VA_ARGS__))                                                                                   \
+  TORCH_WARN_ONCE("hp_rms_norm::" name ": an input asks for gradients, but the outputs have no history and what " \
+                  "is updated in place keeps none of it; " differentiable)
+
 // Absent gradients are tensors without elements.
 using BlockGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 
@@ -945,6 +958,8 @@ BlockGrads gated_add_rms_norm_backward_new(const at::Tensor& grad_out, c10::opti
                                            c10::optional<at::Tensor> post_weight, const at::Tensor& weight,
                                            c10::optional<at::Tensor> gate, double residual_scale, double eps) {
   TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  HPRN_NOTE_NO_HISTORY("gated_add_rms_norm_backward", "there are no second derivatives", grad_out, grad_residual_out, input, residual_out,
+                       post_weight, weight, gate);
   BlockGrads grads = block_grads_like<Tensors>(input, post_weight, weight, gate);
   auto& [gi, gr, gp, gw, gg] = grads;
   if (gate.has_value() && input.numel() == 0) gg.zero_();  // a gate without rows
@@ -977,6 +992,7 @@ LogProbOutputs log_prob_outputs(const at::Tensor& input, int64_t top) {
 LogProbOutputs linear_log_probs_new(const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
                                     int64_t top, double temperature, int64_t ignore_index) {
   TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  HPRN_NOTE_NO_HISTORY("linear_log_probs", "hp_rms_norm_b200.autograd has the differentiable form", input, weight);
   LogProbOutputs outputs = log_prob_outputs<Tensors>(input, top);
   auto& [log_prob, entropy, lse, values, indices] = outputs;
   c10::optional<at::Tensor> v, k;
@@ -995,6 +1011,8 @@ std::tuple<at::Tensor, at::Tensor> linear_log_probs_backward_new(
     const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse, c10::optional<at::Tensor> entropy,
     double temperature, int64_t ignore_index) {
   TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  HPRN_NOTE_NO_HISTORY("linear_log_probs_backward", "there are no second derivatives", grad_log_prob, grad_entropy, input, weight, lse,
+                       entropy);
   at::Tensor gi = Tensors::dense_like(input, input.scalar_type());
   at::Tensor gw = Tensors::dense_like(weight, weight.scalar_type());
   linear_log_probs_backward(gi, gw, grad_log_prob, grad_entropy, input, weight, target, lse, entropy, temperature,
@@ -1018,6 +1036,7 @@ std::tuple<at::Tensor, at::Tensor> rms_norm_int8_new(const at::Tensor& input, c1
                                                      c10::optional<at::Tensor> residual,
                                                      c10::optional<at::Tensor> residual_out, double eps) {
   TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  HPRN_NOTE_NO_HISTORY("rms_norm_int8", "8-bit integers have no gradients", input, weight, residual, residual_out);
   auto outputs = int8_outputs<Tensors>(input);
   rms_norm_int8(std::get<0>(outputs), std::get<1>(outputs), input, weight, residual, residual_out, eps);
   return outputs;
@@ -1050,6 +1069,7 @@ at::Tensor int8_product_like(const at::Tensor& input, const at::Tensor& weight, 
 at::Tensor linear_int8_new(const at::Tensor& input, const at::Tensor& input_scale, const at::Tensor& weight,
                            const at::Tensor& weight_scale, c10::optional<at::Tensor> bias, at::ScalarType dtype) {
   TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  HPRN_NOTE_NO_HISTORY("linear_int8", "8-bit integers have no gradients", input_scale, weight_scale, bias);
   at::Tensor out = int8_product_like<Tensors>(input, weight, dtype);
   linear_int8(out, input, input_scale, weight, weight_scale, bias);
   return out;
@@ -1220,7 +1240,8 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
 }
 
 // No gradients of their own (hp_rms_norm_b200.autograd has the differentiable forms):
-// outputs of these have no history, whatever their inputs ask for.
+// outputs of these have no history, whatever their inputs ask for, and a call that such
+// an input reaches says so once (HPRN_NOTE_NO_HISTORY).
 TORCH_LIBRARY_IMPL(hp_rms_norm, Autograd, m) {
   m.impl("gated_add_rms_norm_backward", torch::CppFunction::makeFallthrough());
   m.impl("linear_log_probs", torch::CppFunction::makeFallthrough());
