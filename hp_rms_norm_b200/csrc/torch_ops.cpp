@@ -894,6 +894,7 @@ struct Shapes {
   static at::Tensor dense_like(const at::Tensor& t, at::ScalarType type) {
     return at::empty_like(t, t.options().dtype(type), at::MemoryFormat::Contiguous);
   }
+  static at::Tensor none(const at::Tensor& input) { return at::empty({0}, input.options()); }
   // The leading dimensions of `input`, and `last` after them where it is not negative.
   static at::Tensor rows_like(const at::Tensor& input, at::ScalarType type, int64_t last) {
     c10::SymDimVector sizes(input.sym_sizes().begin(), input.sym_sizes().end() - (input.dim() > 0));
@@ -916,6 +917,7 @@ struct Tensors {
     // (What is on the host is refused where the arguments are checked.)
     return t.is_cuda() ? make(t.sizes(), type, t.device()) : Shapes::dense_like(t, type);
   }
+  static at::Tensor none(const at::Tensor& input) { return make({0}, input.scalar_type(), input.device()); }
   static at::Tensor rows_like(const at::Tensor& input, at::ScalarType type, int64_t last) {
     c10::DimVector sizes(input.sizes().begin(), input.sizes().end() - (input.dim() > 0));
     if (last >= 0) sizes.push_back(last);
@@ -948,7 +950,7 @@ BlockGrads block_grads_like(const at::Tensor& input, const c10::optional<at::Ten
   auto like = [](const at::Tensor& t) { return M::dense_like(t, t.scalar_type()); };
   // (One each: outputs of an operator are not the same tensor.)
   auto like_or_none = [&](const c10::optional<at::Tensor>& t) {
-    return t.has_value() ? like(*t) : at::empty({0}, input.options());
+    return t.has_value() ? like(*t) : M::none(input);
   };
   return {like(input), like(input), like_or_none(post_weight), like(weight), like_or_none(gate)};
 }
