@@ -6,6 +6,10 @@
 //   dr = a dt,  dg = sum of dt m p over what shares the gate,
 //   dx = inv_x (p g dt - m mean(p g dt m)),  dp = sum over rows of g dt m,
 //   dw = sum over rows of D n
+// t is read as the forward call wrote it, rounded to 16 bits: the unrounded sum would
+// have to be kept in 32 bits, 4 bytes an element more to write and read, or made again
+// from the old residual, which an update in place has overwritten.  In bf16 the gradients
+// are 2.3e-3 from 64 bits for it, where 1.7e-3 is their own rounding.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -73,7 +77,7 @@ struct BlockGradArgs {
 //   kVectors: every row of every tensor starts on a 16-byte boundary and hidden is
 // a multiple of 8.  Else a row is copied with the 16-byte granules it lies in
 // (elements in granules that reach out of the tensor one by one), and a vector put
-// together from two (12 x 257 rows of 1001, fp16: 33 us).
+// together from two (12 x 257 rows of 1001, fp16: 34 us).
 //
 // A wait that runs out (mbar_wait_bounded) ends its group after the copies in
 // flight, and says so (report_give_up).
@@ -627,7 +631,10 @@ __global__ void __launch_bounds__(32 * kRunWarps) block_grad_runs(BlockGradArgs 
 }
 
 // ---------------------------------------------------------------------------
-// Rows too long for that, read twice, element by element.
+// Rows that block_grad_rows has no variant for, read twice, element by element: from
+// 16897 elements, from 8449 where they start anywhere, from 14081 with a gate for every
+// element, of which two buffers have no room (us: 4096 x 9001 384, x 10001 411, x 16383
+// 718; 4096 x 16384 with a full gate 813, where one row for all takes 239 in the ring).
 
 // The values of one element of row i that the sums and outputs are made of.
 template <typename T>
@@ -775,7 +782,7 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
                  aligned(a.w, 16) && aligned(a.p, 16) &&
                  (!a.gate_each || (tma_rows(a.dg, a.rows, a.dg_stride) && tma_rows(a.g, a.rows, a.g_stride))) &&
                  (!a.gate_row || a.gate_each || tma_rows(a.g, a.gates, a.g_stride));
-  if (a.rows <= 0 || a.hidden <= 0 || a.hidden > 32768) return plan;
+  if (a.rows <= 0 || a.hidden <= 0) return plan;
   const int64_t nvec = (a.hidden + 7) / 8;
   // Two buffers at least: a row's last pass waits for the next one's first.  Where E
   // leaves no room for them it stays outside.
@@ -813,6 +820,7 @@ BlockGradPlan plan_block_grad(BlockGradArgs& a) {
       const int64_t ring = a.ring_at + slots * groups * slot, joined = groups > 1 ? words * threads * groups * 8 : 0;
       plan.smem = static_cast<int>(ring > joined ? ring : joined);
       const int64_t need = (a.rows + groups - 1) / groups;
+      // (A B200's SMs, as in the tilings: workspaces are sized without a device.)
       a.ctas = need < 148 ? need : 148;
       a.runs = a.ctas;
       a.own_runs = a.gate_row && !a.gate_each && a.gates > 2 * a.ctas;

@@ -5,6 +5,10 @@
 //   out_ij = (sum_k q_ik v_jk) scale_i channel_j + bias_j
 // The sum is an exact 32-bit integer from the tensor cores; it is rounded to
 // fp32 once, and the result to 16 bits once.
+//   Of a norm y_ij = (t_ij w_j) inv_i: its largest is known before inv is.  That order
+// and 1 / scale in place of a division each cost y / scale one fp32 rounding, at most
+// 127 2^-24 of a step: a code within 2^-16 of a tie may be its neighbour, half a step off
+// like the other one.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -20,6 +24,8 @@ namespace hprn {
 // ---------------------------------------------------------------------------
 // Quantised rows: y = RMSNorm(t) w with t = x [+ r], or y = x without a weight.
 
+// (quantize_int8, nothing in L2: 4096 x 4096 9.9 us, x 8192 19.8, 0.78 of the copy rate;
+// x 16384 54.3, one row of 1024 threads an SM; 3084 x 1001 5.6; one row 1.4.)
 struct QuantArgs {
   int8_t* q;
   float* scales;
