@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import hp_rms_norm_b200 as hp
+from hp_rms_norm_b200 import capi
 from tests.test_gpu_gated_norm import EPS, GATES, check, make
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +76,29 @@ def test_more_wide_rows_than_CTAs(cuda, gate):
     check(make((2, 230), 12288, torch.bfloat16, cuda, gate=gate), 1.0, f"460 x 12288 {gate}")
     check(make((5, 64), 8200, torch.float16, cuda, gate=gate), 1.0, f"320 x 8200 {gate}")
     check(make((4, 41), 9001, torch.float16, cuda, gate=gate), 1.0, f"164 x 9001 {gate}")
+
+
+def test_a_wait_that_runs_out_in_a_run_of_its_own(cuda):
+    """The hook leaves out all loads: the launch ends, the count tells, later calls are refused until it
+    is reset, and nothing is left behind."""
+    s = make((2500, 2), 512, torch.bfloat16, cuda, gate="sequence")
+
+    def call():
+        return hp.gated_add_rms_norm_backward(s["d"], s["x"], s["r"], s["p"], s["w"], EPS, gate=s["gate"], grad_residual=s["e"])
+
+    want = call()
+    torch.cuda.synchronize()
+    assert capi.wait_timeouts(reset=True) == 0
+    try:
+        capi.test_stall_loads(True, 5_000_000)
+        call()
+        torch.cuda.synchronize()
+    finally:
+        capi.test_stall_loads(False)
+    assert capi.wait_timeouts() > 0
+    with pytest.raises(RuntimeError, match="ran out"):
+        call()
+    assert capi.wait_timeouts(reset=True) > 0
+    got = call()
+    torch.cuda.synchronize()
+    assert capi.wait_timeouts() == 0 and all(torch.equal(a, b) for a, b in zip(want, got))
