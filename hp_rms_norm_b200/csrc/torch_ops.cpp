@@ -1154,8 +1154,9 @@ TORCH_LIBRARY(hp_rms_norm, m) {
         "Tensor input, Tensor weight, Tensor? grad_residual, float eps) -> ()");
   m.def("gated_add_rms_norm(Tensor(a!) out, Tensor(b!) residual, Tensor(c!)? residual_out, Tensor input, "
         "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
-  // The .sum forms leave residual as it is, so that a traced graph orders no write to it.
-  m.def("gated_add_rms_norm.sum(Tensor(a!) out, Tensor(b!) residual_out, Tensor input, Tensor residual, "
+  // The _sum forms leave residual as it is, so that a traced graph orders no write to it.
+  // (Names of their own: overloads would fit the same calls by position.)
+  m.def("gated_add_rms_norm_sum(Tensor(a!) out, Tensor(b!) residual_out, Tensor input, Tensor residual, "
         "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
   // (Gradients of what is absent come back without elements, as do alternatives with top 0.)
   m.def("gated_add_rms_norm_backward(Tensor grad_out, Tensor? grad_residual_out, Tensor input, "
@@ -1171,7 +1172,7 @@ TORCH_LIBRARY(hp_rms_norm, m) {
   // Extensions: 8-bit integers.
   m.def("rms_norm_int8(Tensor input, Tensor? weight, Tensor(a!)? residual, Tensor(b!)? residual_out, "
         "float eps) -> (Tensor codes, Tensor scales)");
-  m.def("rms_norm_int8.sum(Tensor input, Tensor? weight, Tensor residual, Tensor(a!) residual_out, "
+  m.def("rms_norm_int8_sum(Tensor input, Tensor? weight, Tensor residual, Tensor(a!) residual_out, "
         "float eps) -> (Tensor codes, Tensor scales)");
   m.def("rms_norm_int8.out(Tensor(a!) out, Tensor(b!) scales, Tensor input, Tensor? weight, "
         "Tensor(c!)? residual, Tensor(d!)? residual_out, float eps) -> ()");
@@ -1201,12 +1202,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("grad_norm", &grad_norm);
   m.impl("clip_grad_norm", &clip_grad_norm);
   m.impl("gated_add_rms_norm", &gated_add_rms_norm);
-  m.impl("gated_add_rms_norm.sum", &gated_add_rms_norm_sum);
+  m.impl("gated_add_rms_norm_sum", &gated_add_rms_norm_sum);
   m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_new);
   m.impl("linear_log_probs", &linear_log_probs_new);
   m.impl("linear_log_probs_backward", &linear_log_probs_backward_new);
   m.impl("rms_norm_int8", &rms_norm_int8_new);
-  m.impl("rms_norm_int8.sum", &rms_norm_int8_sum);
+  m.impl("rms_norm_int8_sum", &rms_norm_int8_sum);
   m.impl("rms_norm_int8.out", &rms_norm_int8);
   m.impl("linear_int8", &linear_int8_new);
   m.impl("linear_int8.out", &linear_int8);
@@ -1230,12 +1231,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("grad_norm", &grad_norm_meta);
   m.impl("clip_grad_norm", &clip_grad_norm_meta);
   m.impl("gated_add_rms_norm", &gated_add_rms_norm_meta);
-  m.impl("gated_add_rms_norm.sum", &gated_add_rms_norm_sum_meta);
+  m.impl("gated_add_rms_norm_sum", &gated_add_rms_norm_sum_meta);
   m.impl("gated_add_rms_norm_backward", &gated_add_rms_norm_backward_new_meta);
   m.impl("linear_log_probs", &linear_log_probs_new_meta);
   m.impl("linear_log_probs_backward", &linear_log_probs_backward_new_meta);
   m.impl("rms_norm_int8", &rms_norm_int8_new_meta);
-  m.impl("rms_norm_int8.sum", &rms_norm_int8_sum_meta);
+  m.impl("rms_norm_int8_sum", &rms_norm_int8_sum_meta);
   m.impl("rms_norm_int8.out", &rms_norm_int8_meta);
   m.impl("linear_int8", &linear_int8_new_meta);
   m.impl("linear_int8.out", &linear_int8_meta);
@@ -1249,6 +1250,6 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Autograd, m) {
   m.impl("linear_log_probs", torch::CppFunction::makeFallthrough());
   m.impl("linear_log_probs_backward", torch::CppFunction::makeFallthrough());
   m.impl("rms_norm_int8", torch::CppFunction::makeFallthrough());
-  m.impl("rms_norm_int8.sum", torch::CppFunction::makeFallthrough());
+  m.impl("rms_norm_int8_sum", torch::CppFunction::makeFallthrough());
   m.impl("linear_int8", torch::CppFunction::makeFallthrough());
 }

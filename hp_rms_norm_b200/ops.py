@@ -240,8 +240,8 @@ def gated_add_rms_norm(input, residual, post_weight, weight, eps, gate=None, res
         _ops.gated_add_rms_norm.default(out, residual, None, input, post_weight, weight, gate,
                                         residual_scale, eps)
     else:
-        _ops.gated_add_rms_norm.sum(out, residual_out, input, residual, post_weight, weight, gate,
-                                    residual_scale, eps)
+        _ops.gated_add_rms_norm_sum.default(out, residual_out, input, residual, post_weight, weight,
+                                            gate, residual_scale, eps)
     return out
 
 
@@ -296,7 +296,7 @@ def rms_norm_int8(input, weight, eps, residual=None, residual_out=None):
     scale.  ``linear_int8`` takes both."""
     if residual is None or residual_out is None or residual_out is residual:
         return _ops.rms_norm_int8.default(input, weight, residual, residual_out, eps)
-    return _ops.rms_norm_int8.sum(input, weight, residual, residual_out, eps)
+    return _ops.rms_norm_int8_sum.default(input, weight, residual, residual_out, eps)
 
 
 def quantize_int8(input):

@@ -178,7 +178,10 @@ def test_only_what_is_written_is_declared_written():
     """A traced graph orders and copies for the writes that the schemas declare."""
     class Written(TorchDispatchMode):
         def __torch_dispatch__(self, func, types, args=(), kwargs=None):
-            for declared, given in zip(func._schema.arguments, args):
+            called.append(func)
+            given_by = dict(zip((a.name for a in func._schema.arguments), args)) | (kwargs or {})
+            for declared in func._schema.arguments:
+                given = given_by.get(declared.name)
                 if declared.alias_info is not None and declared.alias_info.is_write and isinstance(given, torch.Tensor):
                     found.append(given)
             return func(*args, **(kwargs or {}))
@@ -192,10 +195,20 @@ def test_only_what_is_written_is_declared_written():
                        (lambda: hp.rms_norm_int8(x, w, 1e-6, residual=r), [r]),
                        (lambda: hp.rms_norm_int8(x, w, 1e-6, residual=r, residual_out=r), [r]),
                        (lambda: hp.rms_norm_int8(x, w, 1e-6), [])):
-        found = []
+        found, called = [], []
         with Written():
             call()
         assert {id(t) for t in found} == {id(t) for t in want}
+
+
+    # By position an operator's name means the form that it always meant.
+    ops = torch.ops.hp_rms_norm
+    for call, want in ((lambda: ops.gated_add_rms_norm(out, r, total, x, w, w, None, 1.0, 1e-6), ops.gated_add_rms_norm.default),
+                       (lambda: ops.rms_norm_int8(x, w, r, total, 1e-6), ops.rms_norm_int8.default)):
+        found, called = [], []
+        with Written():
+            call()
+        assert called == [want]
 
 
 def test_no_cpu_kernels():
